@@ -449,6 +449,33 @@ int zk_ce_finish(const int64_t* row_label, int64_t rows, float* run_max,
                  const float* run_sum, const float* target_logit, const int64_t* stats,
                  float* lse, float* loss, zk_stream_t stream);
 
+/* -------------------------------------------------------- Token embedding --
+ * Replaces nn.Embedding as the models hold it (embed_tokens of
+ * models/llama_simple.py:524-585; tok_embeddings of models/llama_v2.py:
+ * 402-543) and its gradient:
+ *     y[t]  = round(scale * w[ids[t]])           NaN where ids[t] is not in
+ *                                                 [0, vocab)
+ *     dw[r] = round(scale * sum of dy[t] over t with ids[t] = r)
+ *                     (+ the old dw[r] inside the rounding when accumulate != 0)
+ * ids: [tokens], int64 (ids_64 != 0) or int32; w, dw: [vocab, hidden] and
+ * y, dy: [tokens, hidden], contiguous, any of the three types each.  Without
+ * accumulate every row of dw is written (zero for ids that no token names);
+ * with it only rows that tokens name are touched.  Tokens whose id is
+ * padding_idx (-1: none) or outside [0, vocab) have no gradient.  The sums are
+ * fp32, in an order that the ids alone decide: equal calls give equal bits.
+ * Sizes: tokens < 2^29, vocab < 2^28, hidden < 2^23 (ZK_EINVAL). */
+int zk_embedding_fwd(const void* ids, int ids_64, int64_t tokens, const void* w,
+                     int64_t vocab, int64_t hidden, void* y, float scale,
+                     int w_dtype, int y_dtype, zk_stream_t stream);
+/* Bytes of workspace (16-byte aligned) of the gradient; negative for sizes
+ * that it refuses. */
+int64_t zk_embedding_bwd_workspace(int64_t tokens, int64_t vocab, int64_t hidden);
+int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, const void* dy,
+                     int dy_dtype, void* dw, int dw_dtype, int64_t vocab,
+                     int64_t hidden, float scale, int64_t padding_idx,
+                     int accumulate, void* workspace, int64_t workspace_bytes,
+                     zk_stream_t stream);
+
 /* ------------------------------------------------------------- Utilities --
  * Dtype conversion of a contiguous buffer (the autocast weight cast and the
  * grad cast of utils/patch.py:115-119 when done outside the AdamW kernel).

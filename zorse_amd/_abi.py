@@ -135,6 +135,11 @@ SIGNATURES = {
     "zk_ce_labels": (_int, [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "zk_ce_finish": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "zk_ce_bwd_chunk": (_int, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _f32, _int, _ptr]),
+    "zk_embedding_fwd": (_int, [_ptr, _int, _i64, _ptr, _i64, _i64, _ptr, _f32, _int, _int,
+                                _ptr]),
+    "zk_embedding_bwd_workspace": (_i64, [_i64, _i64, _i64]),
+    "zk_embedding_bwd": (_int, [_ptr, _int, _i64, _ptr, _int, _ptr, _int, _i64, _i64, _f32, _i64,
+                                _int, _ptr, _i64, _ptr]),
     "zk_transpose": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "zk_copy_to_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),
     "zk_copy_from_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),

@@ -1,5 +1,5 @@
 """Autograd functions over the HIP kernels (RMSNorm, RoPE + flash attention,
-SwiGLU), usable on their own; the fused decoder layer lives in ``layer.py``.
+SwiGLU, token embedding), usable on their own; the fused decoder layer lives in ``layer.py``.
 
 RoPE tables are built once per (S, d, theta, pairing, dtype, device) with the
 reference's formula (models/llama_simple.py:75-81, 115-137: inv_freq and the
@@ -98,6 +98,40 @@ class SwiGLUFunction(torch.autograd.Function):
 
 def swiglu(g, u):
     return SwiGLUFunction.apply(g, u)
+
+
+# -------------------------------------------------------- Token embedding --
+
+class EmbeddingFunction(torch.autograd.Function):
+    """y = round(scale * weight[ids]); the whole table's gradient."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx, dtype):
+        ids = ids.contiguous()
+        ctx.save_for_backward(ids)
+        ctx.cfg = (scale, padding_idx, weight.shape[0], weight.dtype)
+        return K.embedding_fwd(ids, weight.contiguous(), scale=scale, dtype=dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        scale, padding_idx, vocab, w_dtype = ctx.cfg
+        dw = K.embedding_bwd(ids, dy.contiguous(), vocab, scale=scale, padding_idx=padding_idx,
+                             dw_dtype=w_dtype)
+        return None, dw, None, None, None
+
+
+def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
+    """Rows of a token table: scale * weight[ids] as [*ids.shape, hidden] in
+    ``dtype`` (default the table's).  ids int32 / int64; an id outside
+    [0, vocab) gives a row of NaN and no gradient (nothing is read back to the
+    host to check it).  ``padding_idx`` (negative: from the end, as nn.Embedding
+    takes it): the row whose tokens have no gradient."""
+    if padding_idx is not None:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
+        padding_idx %= weight.shape[0]
+    return EmbeddingFunction.apply(ids, weight, float(scale), padding_idx, dtype)
 
 
 # -------------------------------------------------------------- Attention --

@@ -39,7 +39,7 @@ import torch.nn as nn
 
 from . import kernels as K
 from .lm_head import lm_head_cross_entropy
-from .llama_simple import LlamaDecoderLayer, LlamaRMSNorm, llama_config
+from .llama_simple import LlamaDecoderLayer, LlamaRMSNorm, TokenEmbedding, llama_config
 from .mistral_simple import mistral_config
 
 # models/llama.py:12-47: hidden size, layers, attention heads
@@ -73,7 +73,8 @@ class DecoderModel(nn.Module):
         self.config = config
         self.padding_idx = config.pad_token_id
         self.vocab_size = config.vocab_size
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, self.padding_idx)
+        self.embed_tokens = TokenEmbedding(config.vocab_size, config.hidden_size,
+                                           self.padding_idx)
         nn.init.normal_(self.embed_tokens.weight, 0.0, INIT_STD)
         self.layers = nn.ModuleList(
             LlamaDecoderLayer(config, i, sliding_window=sliding_window, **layer_kw)

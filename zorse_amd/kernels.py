@@ -9,6 +9,7 @@ GPU tensor these functions raise.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import math
 
@@ -18,6 +19,7 @@ from . import _abi
 from ._abi import check, dtype_code, lib, ptr, stream_handle
 
 _LOWP = (torch.bfloat16, torch.float16)
+FLOAT_DTYPES = (torch.float32, *_LOWP)  # what the kernels compute in and store
 
 
 def _require_gpu(*tensors: torch.Tensor | None) -> torch.device:
@@ -39,6 +41,13 @@ def _require_gpu(*tensors: torch.Tensor | None) -> torch.device:
 def _require_contig(name: str, t: torch.Tensor) -> None:
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _on(dev: torch.device):
+    """Launches go to ``dev``, also while another device is the current one."""
+    if torch.cuda.current_device() == dev.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 # --------------------------------------------------------------- RMSNorm ---
@@ -707,6 +716,86 @@ def _check_transposed(transposed, q, k):
     if Sq % 8 != 0 or Skv % 8 != 0:
         raise ValueError("transposed outputs need sequence lengths that are multiples of 8")
     return ld
+
+
+# -------------------------------------------------------------- Embedding --
+
+def _embedding_ids(ids: torch.Tensor) -> int:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"token ids must be int32 or int64 (got {ids.dtype})")
+    _require_contig("ids", ids)
+    return int(ids.dtype == torch.int64)
+
+
+def _float_dtype(name: str, dtype: torch.dtype) -> int:
+    if dtype not in FLOAT_DTYPES:
+        raise ValueError(f"unsupported {name} dtype {dtype}")
+    return dtype_code(dtype)
+
+
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+                  dtype: torch.dtype | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """round(scale * weight[ids]) in ``dtype`` (default the table's): ids
+    int32 / int64 of any shape, weight [vocab, hidden], both contiguous.  A row
+    whose id is outside [0, vocab) is NaN.  ``out``: [*ids.shape, hidden]."""
+    dev = _require_gpu(ids, weight, out)
+    is64 = _embedding_ids(ids)
+    if weight.dim() != 2 or not weight.numel():
+        raise ValueError(f"weight must be a [vocab, hidden] table, got {tuple(weight.shape)}")
+    _require_contig("weight", weight)
+    w_code = _float_dtype("weight", weight.dtype)
+    V, h = weight.shape
+    if out is None:
+        out = torch.empty(*ids.shape, h, device=dev, dtype=dtype or weight.dtype)
+    elif out.shape != (*ids.shape, h) or not out.is_contiguous() \
+            or out.dtype != (dtype or out.dtype):
+        raise ValueError(f"out must be contiguous {(*ids.shape, h)} of the output's dtype")
+    y_code = _float_dtype("output", out.dtype)
+    with _on(dev):
+        check(lib().zk_embedding_fwd(ptr(ids), is64, ids.numel(), ptr(weight), V, h, ptr(out),
+                                     float(scale), w_code, y_code, stream_handle(dev)),
+              "zk_embedding_fwd")
+    return out
+
+
+def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: float = 1.0,
+                  padding_idx: int | None = None, dw: torch.Tensor | None = None,
+                  accumulate: bool = False, dw_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The table's gradient, dw[r] = scale * the sum of dy over the tokens with
+    id r: dy [*ids.shape, hidden] contiguous; tokens of ``padding_idx`` (and ids
+    outside [0, vocab)) have none.  ``dw`` [vocab, hidden] contiguous is
+    overwritten, or with ``accumulate`` added to, which touches only the rows
+    that tokens name; without it a new tensor of ``dw_dtype`` (default dy's).
+    fp32 sums in an order that the ids alone decide (no atomics)."""
+    dev = _require_gpu(ids, dy, dw)
+    is64 = _embedding_ids(ids)
+    _require_contig("dy", dy)
+    dy_code = _float_dtype("dy", dy.dtype)
+    if dy.dim() < 1 or dy.shape[:-1] != ids.shape or not dy.shape[-1]:
+        raise ValueError(f"dy must be [*ids.shape, hidden], got {tuple(dy.shape)} for ids "
+                         f"{tuple(ids.shape)}")
+    h = dy.shape[-1]
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab})")
+    if dw is None:
+        if accumulate:
+            raise ValueError("accumulate needs the dw to add to")
+        dw = torch.empty(vocab, h, device=dev, dtype=dw_dtype or dy.dtype)
+    elif dw.shape != (vocab, h) or not dw.is_contiguous() or dw.dtype != (dw_dtype or dw.dtype):
+        raise ValueError(f"dw must be contiguous [{vocab}, {h}] of dw_dtype")
+    dw_code = _float_dtype("dw", dw.dtype)
+    nbytes = lib().zk_embedding_bwd_workspace(ids.numel(), vocab, h)
+    if nbytes < 0:
+        raise ValueError(f"embedding_bwd: {ids.numel()} tokens of a [{vocab}, {h}] table are out "
+                         f"of range")
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        check(lib().zk_embedding_bwd(ptr(ids), is64, ids.numel(), ptr(dy), dy_code, ptr(dw),
+                                     dw_code, vocab, h, float(scale),
+                                     -1 if padding_idx is None else padding_idx, int(accumulate),
+                                     ptr(ws), nbytes, stream_handle(dev)), "zk_embedding_bwd")
+    return dw
 
 
 # ------------------------------------------------------------------ AdamW --

@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as Fn
+from . import kernels as K
 from .layer import DecoderLayerFunction, LayerSpec
 
 
@@ -112,6 +113,19 @@ class LlamaRMSNorm(nn.Module):
 
     def forward(self, x):
         return Fn.rms_norm(x, self.weight, self.variance_epsilon)
+
+
+class TokenEmbedding(nn.Embedding):
+    """nn.Embedding whose lookup and gradient run on the embedding kernels
+    (functional.embedding).  A table on the CPU, of another type than the
+    kernels' three, or with options that they do not have (max_norm,
+    scale_grad_by_freq, sparse) is nn.Embedding's."""
+
+    def forward(self, input):
+        if not self.weight.is_cuda or self.max_norm is not None or self.scale_grad_by_freq \
+                or self.sparse or self.weight.dtype not in K.FLOAT_DTYPES:
+            return super().forward(input)
+        return Fn.embedding(input, self.weight, padding_idx=self.padding_idx)
 
 
 class LlamaAttention(nn.Module):
@@ -337,7 +351,8 @@ class DeepspeedLlama(nn.Module):
         self.config = config
         self.padding_idx = config.pad_token_id
         self.vocab_size = config.vocab_size
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, self.padding_idx)
+        self.embed_tokens = TokenEmbedding(config.vocab_size, config.hidden_size,
+                                           self.padding_idx)
         layers = []
         for i in range(config.num_hidden_layers):
             layers.append(Block(config, i, dtype, sliding_window=sliding_window, **layer_kw))

@@ -24,7 +24,8 @@ import torch
 import torch.nn as nn
 
 from .layer import LayerSpec
-from .llama_simple import FlatDecoderLayer, FlatLinear, FlatRMSNorm, LlamaRMSNorm
+from .llama_simple import (FlatDecoderLayer, FlatLinear, FlatRMSNorm, LlamaRMSNorm,
+                           TokenEmbedding)
 
 
 @dataclass
@@ -144,7 +145,7 @@ class Transformer(nn.Module):
         self.model_args = model_args
         self.vocab_size = model_args.vocab_size
         self.n_layers = model_args.n_layers
-        self.tok_embeddings = nn.Embedding(model_args.vocab_size, model_args.dim)
+        self.tok_embeddings = TokenEmbedding(model_args.vocab_size, model_args.dim)
         self.layers = nn.ModuleList([TransformerBlock(i, model_args, None, **block_kw)
                                      for i in range(model_args.n_layers)])
         self.norm = LlamaRMSNorm(model_args.dim, eps=model_args.norm_eps)

@@ -12,7 +12,7 @@ import torch
 import torch.nn as nn
 
 from .llama_simple import Block as _LlamaBlock
-from .llama_simple import LlamaRMSNorm, NoOp, llama_config
+from .llama_simple import LlamaRMSNorm, NoOp, TokenEmbedding, llama_config
 
 
 def mistral_config(**kw):
@@ -49,7 +49,8 @@ class DeepspeedMistral(nn.Module):
         self.config = config
         self.padding_idx = config.pad_token_id
         self.vocab_size = config.vocab_size
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, self.padding_idx)
+        self.embed_tokens = TokenEmbedding(config.vocab_size, config.hidden_size,
+                                           self.padding_idx)
         layers = []
         for i in range(config.num_hidden_layers):
             layers.append(Block(config, i, **layer_kw))
