@@ -449,6 +449,43 @@ int zk_ce_finish(const int64_t* row_label, int64_t rows, float* run_max,
                  const float* run_sum, const float* target_logit, const int64_t* stats,
                  float* lse, float* loss, zk_stream_t stream);
 
+/* ------------------------------------- Norm of q and k heads, with rotation --
+ * RMS norm of every query and key head over its d elements and the rotary
+ * embedding in one pass (no counterpart in the reference, whose attention
+ * rotates unnormed heads, models/llama_simple.py:34-58).  For a row x of d
+ * elements at position pos, weights w [d] (one vector for the query heads, one
+ * for the key heads):
+ *     r = 1 / sqrt(mean(x^2) + eps)      y = R(pos) (w x r)
+ * and backward from dy: dn = R(pos)^T dy, dw = sum over rows of dn x r,
+ * dx = r (dn w - x r mean(dn w x r)).  fp32 inside, one rounding of y, dx, dw.
+ * q, k: [B, S, H, d] views (element strides, unit stride along d; Hkv 0: no k).
+ * o*: strides of the outputs (y forward, dx backward), which may be the inputs
+ * themselves; dy*: strides of dy (backward only).  cos / sin: fp32
+ * [n_pos, d/2]; positions: int64, row b's at b * pos_sb (0: shared by the
+ * batch), or NULL for 0 .. S-1.  A row whose position is outside [0, n_pos) is
+ * NaN, and so are its dx and then dw.  Any even d up to 1024
+ * (ZK_EUNSUPPORTED above), rows at any element. */
+typedef struct zk_qk_desc {
+  int64_t B, S, Hq, Hkv, d;
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh;
+  int64_t oq_sb, oq_ss, oq_sh, ok_sb, ok_ss, ok_sh;
+  int64_t dyq_sb, dyq_ss, dyq_sh, dyk_sb, dyk_ss, dyk_sh;
+  int64_t n_pos, pos_sb;
+  float eps;
+  int pairing, dtype, w_dtype;
+} zk_qk_desc;
+int zk_qk_norm_rope_fwd(const zk_qk_desc* desc, const void* q, const void* k,
+                        const void* wq, const void* wk, void* q_out, void* k_out,
+                        const float* cos, const float* sin, const int64_t* positions,
+                        zk_stream_t stream);
+/* Bytes of workspace of the backward (dw's partial sums). */
+int64_t zk_qk_norm_rope_bwd_workspace(int64_t d);
+int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const void* k,
+                        const void* wq, const void* wk, const void* dq_out,
+                        const void* dk_out, void* dq, void* dk, void* dwq, void* dwk,
+                        const float* cos, const float* sin, const int64_t* positions,
+                        void* workspace, int64_t workspace_bytes, zk_stream_t stream);
+
 /* -------------------------------------------------------- Token embedding --
  * Replaces nn.Embedding as the models hold it (embed_tokens of
  * models/llama_simple.py:524-585; tok_embeddings of models/llama_v2.py:

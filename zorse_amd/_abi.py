@@ -58,6 +58,24 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class QkDesc(ctypes.Structure):
+    """Mirror of ``zk_qk_desc``."""
+
+    _fields_ = [
+        (name, _i64)
+        for name in (
+            "B", "S", "Hq", "Hkv", "d",
+            "q_sb", "q_ss", "q_sh",
+            "k_sb", "k_ss", "k_sh",
+            "oq_sb", "oq_ss", "oq_sh",
+            "ok_sb", "ok_ss", "ok_sh",
+            "dyq_sb", "dyq_ss", "dyq_sh",
+            "dyk_sb", "dyk_ss", "dyk_sh",
+            "n_pos", "pos_sb",
+        )
+    ] + [("eps", _f32), ("pairing", _int), ("dtype", _int), ("w_dtype", _int)]
+
+
 class AdamwRegion(ctypes.Structure):
     """Mirror of ``zk_adamw_region``."""
 
@@ -140,6 +158,11 @@ SIGNATURES = {
     "zk_embedding_bwd_workspace": (_i64, [_i64, _i64, _i64]),
     "zk_embedding_bwd": (_int, [_ptr, _int, _i64, _ptr, _int, _ptr, _int, _i64, _i64, _f32, _i64,
                                 _int, _ptr, _i64, _ptr]),
+    "zk_qk_norm_rope_fwd": (_int, [ctypes.POINTER(QkDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _ptr, _ptr, _ptr, _ptr]),
+    "zk_qk_norm_rope_bwd_workspace": (_i64, [_i64]),
+    "zk_qk_norm_rope_bwd": (_int, [ctypes.POINTER(QkDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "zk_transpose": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "zk_copy_to_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),
     "zk_copy_from_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),

@@ -1,5 +1,5 @@
 """Autograd functions over the HIP kernels (RMSNorm, RoPE + flash attention,
-SwiGLU, token embedding), usable on their own; the fused decoder layer lives in ``layer.py``.
+SwiGLU, token embedding, the norm of query and key heads), usable on their own; the fused decoder layer lives in ``layer.py``.
 
 RoPE tables are built once per (S, d, theta, pairing, dtype, device) with the
 reference's formula (models/llama_simple.py:75-81, 115-137: inv_freq and the
@@ -132,6 +132,46 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
             raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
         padding_idx %= weight.shape[0]
     return EmbeddingFunction.apply(ids, weight, float(scale), padding_idx, dtype)
+
+
+# ----------------------------------------- Norm of q and k heads, rotation --
+
+def _unit_rows(t):
+    """t with unit stride along its last dim (an expanded gradient has none)."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+class QkNormRopeFunction(torch.autograd.Function):
+    """RMS norm and rotation of every q and k head; saves its inputs only."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        q, k = _unit_rows(q), _unit_rows(k)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.cfg = (eps, interleaved)
+        return K.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, positions=positions,
+                                  eps=eps, interleaved=interleaved)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        eps, interleaved = ctx.cfg
+        grads = K.qk_norm_rope_bwd(_unit_rows(dq_out), _unit_rows(dk_out), q, k, q_weight,
+                                   k_weight, cos, sin, positions=positions, eps=eps,
+                                   interleaved=interleaved)
+        return (*grads, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6,
+                 interleaved=False):
+    """(q', k') for attention without rope_theta: RMS norm of every head of q
+    [B,S,Hq,d] and k [B,S,Hkv,d] over its d elements with the weights [d], then
+    the rotation, in one pass with one rounding.  cos / sin: fp32 [n_pos, d/2]
+    tables (rope_tables(..., torch.float32, ...)); ``positions`` int64 [S] or
+    [B, S], default 0 .. S-1; a position outside the tables gives NaN.  Any even
+    d up to 1024; q and k may be views of one q|k|v buffer."""
+    return QkNormRopeFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps),
+                                    bool(interleaved))
 
 
 # -------------------------------------------------------------- Attention --

@@ -527,6 +527,108 @@ def rope_copy(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     return q, k
 
 
+# ----------------------------------------- Norm of q and k heads, rotation --
+
+def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs, grads):
+    """The checks of both directions; (device, zk_qk_desc).  ``outs`` are y or
+    dx, ``grads`` dy of q and k."""
+    if q.dim() != 4:
+        raise ValueError("q must be [B, S, H, d]")
+    B, S, Hq, d = q.shape
+    if (k is None) != (k_weight is None):
+        raise ValueError("k and k_weight belong together")
+    sides = [("q", q, q_weight)] + ([("k", k, k_weight)] if k is not None else [])
+    dev = _require_gpu(q, k, q_weight, k_weight, cos, sin, positions, *outs, *grads)
+    code, w_code = _float_dtype("q", q.dtype), _float_dtype("q_weight", q_weight.dtype)
+    strides = []
+    for i, (name, t, w) in enumerate(sides):
+        if t.dim() != 4 or t.shape[:2] != (B, S) or t.shape[3] != d or t.dtype != q.dtype:
+            raise ValueError(f"{name} must be [B, S, H, d] matching q")
+        if w.shape != (d,) or w.dtype != q_weight.dtype or not w.is_contiguous():
+            raise ValueError(f"{name}_weight must be contiguous [{d}] of q_weight's dtype")
+        for other, x in (("", t), (" output", outs[i] if outs else None),
+                         (" gradient", grads[i] if grads else None)):
+            if x is not None and (x.shape != t.shape or x.dtype != t.dtype
+                                  or (x.stride(3) != 1 and d > 1 and x.numel())):
+                raise ValueError(f"{name}{other} must match {name} and have unit stride along d")
+        if outs and 0 in [st for st, n in zip(outs[i].stride(), t.shape) if n > 1]:
+            raise ValueError(f"{name} output overlaps itself (an expanded tensor)")
+    if not Hq:
+        raise ValueError("q has no heads")
+    if d % 2 or not 0 < d <= 1024:
+        raise ValueError(f"head dims are even and up to 1024 (got {d})")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != d // 2 \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous fp32 [n_pos, {d // 2}] table")
+    if cos.shape != sin.shape:
+        raise ValueError("cos and sin tables differ in shape")
+    n_pos, pos_sb = cos.shape[0], 0
+    if positions is not None:
+        if positions.dtype != torch.int64 or positions.shape not in ((S,), (B, S)) \
+                or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int64 [S] or [B, S] tensor")
+        pos_sb = S if positions.dim() == 2 else 0
+    elif n_pos < S:
+        raise ValueError(f"table holds {n_pos} positions < S={S}")
+    if not n_pos:
+        raise ValueError("the tables hold no positions")
+    none = (0, 0, 0)
+    for group in ((q, k), outs or (None, None), grads or (None, None)):
+        strides += [t.stride()[:3] if t is not None else none for t in group]
+    return dev, _abi.QkDesc(B, S, Hq, k.shape[2] if k is not None else 0, d,
+                            *(v for st in strides for v in st), n_pos, pos_sb, float(eps),
+                            _abi.ZK_ROPE_INTERLEAVED if interleaved else _abi.ZK_ROPE_HALF, code,
+                            w_code)
+
+
+def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: float = 1e-6,
+                     interleaved: bool = False, out=None):
+    """RMS norm of every head of q [B,S,Hq,d] and k [B,S,Hkv,d] over its d
+    elements (weights [d]) and the rotation, in one pass: returns contiguous
+    (q', k'), or ``out`` = (q', k') views with unit stride along d, which may be
+    q and k themselves.  k and k_weight may both be None (then k' is).  cos /
+    sin: fp32 [n_pos, d/2] tables; ``positions`` int64 [S] or [B, S] (default
+    0 .. S-1), those outside the tables giving rows of NaN.  fp32 inside, one
+    rounding."""
+    if out is None:
+        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
+               None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
+    dev, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out, ())
+    with _on(dev):
+        check(lib().zk_qk_norm_rope_fwd(desc, ptr(q), ptr(k), ptr(q_weight), ptr(k_weight),
+                                        ptr(out[0]), ptr(out[1]), ptr(cos), ptr(sin),
+                                        ptr(positions), stream_handle(dev)),
+              "zk_qk_norm_rope_fwd")
+    return out[0], out[1]
+
+
+def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, positions=None,
+                     eps: float = 1e-6, interleaved: bool = False, out=None):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope_fwd from the gradients of
+    its outputs; nothing of the forward but its inputs is needed.  ``out`` =
+    (dq, dk) views with unit stride along d, which may be dq_out and dk_out
+    themselves.  The weights' gradients are summed in fp32 in one order."""
+    if out is None:
+        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
+               None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
+    if dq_out is None or (dk_out is None) != (k is None):
+        raise ValueError("a gradient for each of q and k is needed")
+    dev, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
+                         (dq_out, dk_out))
+    dwq = torch.empty_like(q_weight)
+    dwk = None if k is None else torch.empty_like(k_weight)
+    nbytes = lib().zk_qk_norm_rope_bwd_workspace(q.shape[3])
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        check(lib().zk_qk_norm_rope_bwd(desc, ptr(q), ptr(k), ptr(q_weight), ptr(k_weight),
+                                        ptr(dq_out), ptr(dk_out), ptr(out[0]), ptr(out[1]),
+                                        ptr(dwq), ptr(dwk), ptr(cos), ptr(sin), ptr(positions),
+                                        ptr(ws), nbytes, stream_handle(dev)),
+              "zk_qk_norm_rope_bwd")
+    return out[0], out[1], dwq, dwk
+
+
 # -------------------------------------------------------------- Attention --
 
 def _attn_desc(q, k, v, o, scale, causal, window, dq=None, dk=None, dv=None):
