@@ -411,6 +411,61 @@ int zk_adamw_step_t(float* param, const void* grad, int grad_dtype,
                     int64_t n, double lr, double beta1, double beta2, double eps,
                     double weight_decay, int64_t step, zk_stream_t stream);
 
+/* zk_adamw_step over a list of tensors, in as few launches as their table
+ * allows (56 tensors each, 44 with 8-bit moments); the same bits as a call for each.  Hyper-parameters
+ * are shared, the step counts are not.  lowp NULL: no compute copy.  The table
+ * is host memory, read before the call returns. */
+typedef struct zk_adamw_tensor {
+  float* param;
+  const void* grad;
+  float* exp_avg;
+  float* exp_avg_sq;
+  void* lowp;
+  int64_t n, step, grad_dtype, lowp_dtype;
+} zk_adamw_tensor;
+int zk_adamw_multi(const zk_adamw_tensor* tensors, int64_t count, double lr,
+                   double beta1, double beta2, double eps, double weight_decay,
+                   zk_stream_t stream);
+
+/* The same step with both moments held in 8 bits.  Let r(x) be the top 12 bits
+ * below the sign of a float (8 of exponent, 3 of mantissa: x rounded to 4
+ * significant bits), an integer that grows with |x|.  256 neighbouring
+ * elements share base[block] = {of exp_avg, of exp_avg_sq}, and a code c > 0
+ * stands for the float whose r is c + base (c = 0: zero):
+ *   exp_avg     bit 7 the sign, c = r - base in bits 0-6, r rounded to nearest,
+ *               base = max(0, largest r - 127); r <= base becomes zero
+ *   exp_avg_sq  c = r - base in 8 bits, base = max(0, largest r - 255); r is
+ *               rounded up with the probability of the fraction cut off (20
+ *               bits from a hash of seed and element index), so that a moment
+ *               that moves by less than a step keeps its mean; c >= 1 unless
+ *               the moment is zero
+ * The update itself uses the new moments in fp32, before they are rounded.
+ * Infinities and NaN take the largest code and do not move the base.
+ * exp_avg, exp_avg_sq: n bytes; base: int16 [ceil(n / 256)][2]. */
+typedef struct zk_adamw8_tensor {
+  float* param;
+  const void* grad;
+  uint8_t* exp_avg;
+  uint8_t* exp_avg_sq;
+  int16_t* base;
+  void* lowp;
+  int64_t n, step, seed, grad_dtype, lowp_dtype;
+} zk_adamw8_tensor;
+int zk_adamw8_multi(const zk_adamw8_tensor* tensors, int64_t count, double lr,
+                    double beta1, double beta2, double eps, double weight_decay,
+                    zk_stream_t stream);
+/* The moments' values, fp32 or bf16 (which holds every code's value exactly). */
+typedef struct zk_adamw8_view {
+  const uint8_t* exp_avg;
+  const uint8_t* exp_avg_sq;
+  const int16_t* base;
+  void* m_out;
+  void* v_out;
+  int64_t n;
+} zk_adamw8_view;
+int zk_adamw8_values(const zk_adamw8_view* tensors, int64_t count, int out_dtype,
+                     zk_stream_t stream);
+
 /* ------------------------------------------------- LM head cross-entropy --
  * Replaces the last stage's loss, F.cross_entropy(out.flatten(0, 1),
  * target.flatten(0, 1)) (zorse_utils/pipeline_schedule_v2.py:181-184) over

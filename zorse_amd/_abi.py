@@ -145,6 +145,9 @@ SIGNATURES = {
                              _f64, _f64, _f64, _f64, _f64, _i64, _ptr]),
     "zk_adamw_step_t": (_int, [_ptr, _ptr, _int, _ptr, _ptr, _ptr, _int, _ptr, _int, _i64,
                                 _f64, _f64, _f64, _f64, _f64, _i64, _ptr]),
+    "zk_adamw_multi": (_int, [_ptr, _i64, _f64, _f64, _f64, _f64, _f64, _ptr]),
+    "zk_adamw8_multi": (_int, [_ptr, _i64, _f64, _f64, _f64, _f64, _f64, _ptr]),
+    "zk_adamw8_values": (_int, [_ptr, _i64, _int, _ptr]),
     "zk_cast": (_int, [_ptr, _int, _ptr, _int, _i64, _int, _ptr]),
     "zk_ce_fwd_chunk": (_int, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _int,
                                _ptr]),

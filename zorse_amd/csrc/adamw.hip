@@ -13,20 +13,9 @@
 // keeps 16-byte accesses: its one-element-per-lane form was slower alone
 // (63-64 %) and, run beside the attention backward as the stage runs it,
 // cost 2.3 ms per 8-layer step.
-#include <cmath>
-
-#include "zk_common.h"
+#include "adamw_math.h"
 
 namespace zk {
-
-struct AdamScalars {
-  float decay;         // 1 - lr * weight_decay
-  float one_minus_b1;  // lerp weight of the first moment
-  float b2, one_minus_b2;
-  float step_size;     // lr / (1 - b1^t)
-  float bc2_sqrt;      // sqrt(1 - b2^t)
-  float eps;
-};
 
 template <typename G>
 __device__ __forceinline__ void load_grad4(const G* g, int64_t i, float (&o)[4]) {
@@ -76,16 +65,6 @@ __device__ __forceinline__ void store4<f16>(f16* dst, const float4& v) {
 template <>
 __device__ __forceinline__ void store4<float>(float* dst, const float4& v) {
   *reinterpret_cast<float4*>(dst) = v;
-}
-
-__device__ __forceinline__ float adam_one(float& p, float g, float& m, float& v,
-                                          const AdamScalars& s) {
-  p = p * s.decay;
-  m = fmaf(s.one_minus_b1, g - m, m);
-  v = fmaf(s.one_minus_b2, g * g, v * s.b2);
-  const float denom = sqrtf(v) / s.bc2_sqrt + s.eps;
-  p = p - s.step_size * (m / denom);
-  return p;
 }
 
 // 8 elements per thread (the region kernel): p, m, v as two 16-byte accesses
@@ -290,21 +269,6 @@ static void launch_flat(float* p, const void* g, float* m, float* v, void* lowp,
   else if (ldt == ZK_BF16) launch_elem<G, bf16, true>(p, g, m, v, lowp, n, s, st);
   else if (ldt == ZK_F16) launch_elem<G, f16, true>(p, g, m, v, lowp, n, s, st);
   else launch_elem<G, float, true>(p, g, m, v, lowp, n, s, st);
-}
-
-static AdamScalars adam_scalars(double lr, double beta1, double beta2, double eps,
-                                double weight_decay, int64_t step) {
-  AdamScalars s;
-  s.decay = static_cast<float>(1.0 - lr * weight_decay);
-  s.one_minus_b1 = static_cast<float>(1.0 - beta1);
-  s.b2 = static_cast<float>(beta2);
-  s.one_minus_b2 = static_cast<float>(1.0 - beta2);
-  const double bc1 = 1.0 - std::pow(beta1, static_cast<double>(step));
-  const double bc2 = 1.0 - std::pow(beta2, static_cast<double>(step));
-  s.step_size = static_cast<float>(lr / bc1);
-  s.bc2_sqrt = static_cast<float>(std::sqrt(bc2));
-  s.eps = static_cast<float>(eps);
-  return s;
 }
 
 }  // namespace zk

@@ -960,6 +960,150 @@ def adamw_step_t(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tensor,
                                 int(step), stream_handle(dev)), "zk_adamw_step_t")
 
 
+def _tensor_table(who: str, named, steps, grads, params, lowp_outs):
+    """The device of a step over lists of tensors (None: empty lists), after
+    its checks.  ``named``: (name, list, dtype, elements for n) of what must have one dtype;
+    every list is as long as ``params`` and every tensor contiguous on the
+    first parameter's device."""
+    count = len(params)
+    lists = [t for _, t, _, _ in named] + [grads] + ([lowp_outs] if lowp_outs is not None else [])
+    if any(len(t) != count for t in lists) or (steps is not None and len(steps) != count):
+        raise ValueError(f"{who}: the lists differ in length")
+    if not count:
+        return None
+    dev = params[0].device
+    if dev.type != "cuda":
+        raise ValueError("zorse_amd kernels need GPU tensors (got a CPU tensor)")
+    index = dev.index
+    for i, p in enumerate(params):
+        n = p.numel()
+        for name, ts, dtype, elems in named:
+            t = ts[i]
+            if t.dtype != dtype or t.numel() != (elems(n) if elems else n) \
+                    or not t.is_contiguous() or t.get_device() != index:
+                raise ValueError(f"{who}: {name} {i} must be contiguous {dtype} with "
+                                 f"{elems(n) if elems else n} elements on {dev}")
+        g = grads[i]
+        if g.numel() != n or not g.is_contiguous() or g.get_device() != index \
+                or g.dtype not in _DTYPE_CODES:
+            raise ValueError(f"{who}: grad {i} must be contiguous {list(_DTYPE_CODES)} with {n} "
+                             f"elements on {dev}")
+        low = lowp_outs[i] if lowp_outs is not None else None
+        if low is not None and (low.numel() != n or not low.is_contiguous()
+                                or low.get_device() != index or low.dtype not in _DTYPE_CODES):
+            raise ValueError(f"{who}: lowp_out {i} must be contiguous {list(_DTYPE_CODES)} with "
+                             f"{n} elements on {dev}")
+    return dev
+
+
+_DTYPE_CODES = {dt: dtype_code(dt) for dt in FLOAT_DTYPES}
+
+
+def _step_table(cols, params, grads, steps, lowp_outs, seeds=None):
+    """The rows of zk_adamw_tensor / zk_adamw8_tensor (every field 8 bytes)."""
+    flat, seen = [], set()
+    lows = lowp_outs if lowp_outs is not None else [None] * len(params)
+    for i, (p, g, low, step) in enumerate(zip(params, grads, lows, steps)):
+        n, at = p.numel(), p.data_ptr()
+        if n and at in seen:
+            raise ValueError(f"parameter {i} is in the list twice")
+        seen.add(at)
+        flat += (at, g.data_ptr())
+        flat += [c[i].data_ptr() for c in cols]
+        flat += (0 if low is None else low.data_ptr(), n, int(step))
+        if seeds is not None:
+            flat.append(int(seeds[i]) & 0xFFFFFFFF)
+        flat += (_DTYPE_CODES[g.dtype], 0 if low is None else _DTYPE_CODES[low.dtype])
+    return (_abi._i64 * len(flat))(*flat)
+
+
+def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1: float,
+                beta2: float, eps: float, weight_decay: float, lowp_outs=None) -> None:
+    """adamw_step over lists of tensors (any shapes, all contiguous and on one
+    device) in one launch for every 56, with the same bits: fp32 ``params``
+    and moments, ``grads`` in any of the three types, ``steps`` the step count
+    of each, ``lowp_outs`` a 16- or 32-bit copy of each parameter or None."""
+    f32 = torch.float32
+    dev = _tensor_table("adamw_multi", (("param", params, f32, None),
+                                        ("exp_avg", exp_avgs, f32, None),
+                                        ("exp_avg_sq", exp_avg_sqs, f32, None)),
+                        steps, grads, params, lowp_outs)
+    if dev is None:
+        return
+    table = _step_table((exp_avgs, exp_avg_sqs), params, grads, steps, lowp_outs)
+    with _on(dev):
+        check(lib().zk_adamw_multi(table, len(params), float(lr), float(beta1), float(beta2),
+                                   float(eps), float(weight_decay), stream_handle(dev)),
+              "zk_adamw_multi")
+
+
+ADAMW8_BLOCK = 256  # elements whose 8-bit codes are counted from one base
+
+
+def _adamw8_base_elems(n: int) -> int:
+    return 2 * (-(-n // ADAMW8_BLOCK))
+
+
+def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, lr: float,
+                 beta1: float, beta2: float, eps: float, weight_decay: float,
+                 lowp_outs=None) -> None:
+    """adamw_multi with both moments held in 8 bits: ``exp_avgs`` and
+    ``exp_avg_sqs`` uint8 codes with as many elements as the parameter,
+    ``bases`` int16 [ceil(n / 256), 2], all zero at the start (the format:
+    zk_adamw8_multi in zorse_amd.h; adamw8_values reads it).  The update uses
+    the new moments in fp32; rounded to 4 significant bits, they are kept: the
+    first to nearest, the second up or down at random with the right mean.
+    ``seeds``: an integer for each tensor (mod 2^32) that the random bits come
+    from, another for each step."""
+    if len(seeds) != len(params):
+        raise ValueError("adamw8_multi: the lists differ in length")
+    u8 = torch.uint8
+    dev = _tensor_table("adamw8_multi", (("param", params, torch.float32, None),
+                                         ("exp_avg", exp_avgs, u8, None),
+                                         ("exp_avg_sq", exp_avg_sqs, u8, None),
+                                         ("base", bases, torch.int16, _adamw8_base_elems)),
+                        steps, grads, params, lowp_outs)
+    if dev is None:
+        return
+    table = _step_table((exp_avgs, exp_avg_sqs, bases), params, grads, steps, lowp_outs, seeds)
+    with _on(dev):
+        check(lib().zk_adamw8_multi(table, len(params), float(lr), float(beta1), float(beta2),
+                                    float(eps), float(weight_decay), stream_handle(dev)),
+              "zk_adamw8_multi")
+
+
+def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.float32, outs=None):
+    """The values that adamw8_multi's codes stand for: (first moments, second
+    moments), lists of tensors of the codes' shapes in fp32 or bf16, either of
+    which holds every value exactly; ``outs``: the two lists to fill."""
+    if outs is None:
+        outs = tuple([torch.empty(t.shape, device=t.device, dtype=dtype) for t in ts]
+                     for ts in (exp_avgs, exp_avg_sqs))
+    elif len(outs[0]):
+        dtype = outs[0][0].dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"adamw8_values: values are fp32 or bf16 (got {dtype})")
+    u8 = torch.uint8
+    dev = _tensor_table("adamw8_values", (("exp_avg", exp_avgs, u8, None),
+                                          ("exp_avg_sq", exp_avg_sqs, u8, None),
+                                          ("base", bases, torch.int16, _adamw8_base_elems),
+                                          ("first moment", outs[0], dtype, None)),
+                        None, outs[1], exp_avgs, None)
+    if dev is None:
+        return outs
+    if any(t.dtype != dtype for t in outs[1]):
+        raise ValueError(f"adamw8_values: every output must be {dtype}")
+    flat = []
+    for row in zip(exp_avgs, exp_avg_sqs, bases, *outs):
+        flat += [t.data_ptr() for t in row]
+        flat.append(row[0].numel())
+    table = (_abi._i64 * len(flat))(*flat)
+    with _on(dev):
+        check(lib().zk_adamw8_values(table, len(exp_avgs), dtype_code(dtype), stream_handle(dev)),
+              "zk_adamw8_values")
+    return outs
+
+
 def cast_(src: torch.Tensor, dst: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
     """dst = round(src) (or dst = round(dst + src)); contiguous, same numel."""
     dev = _require_gpu(src, dst)

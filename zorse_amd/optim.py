@@ -1,4 +1,4 @@
-"""Fused AdamW on flat parameter shards (one kernel pass per shard).
+"""Fused AdamW on flat parameter shards and on lists of tensors.
 
 Replaces ``torch.optim.Adam(fused=True)`` as the reference builds it for each
 FSDP module's flat shard (zorse_utils/pipeline.py:150-181) and steps it from
@@ -11,11 +11,18 @@ runs on), the optimizer keeps an fp32 master copy in its state, updates the
 master, m and v, and writes the rounded parameter back -- all in the same
 pass.  With an fp32 parameter the update is in place.
 
+``step()`` steps all of a group's parameters on a GPU in one launch (for every
+56), ``step_param`` one of them.  ``state_bits=8`` holds both moments in 8 bits
+a value (kernels.adamw8_multi): 2 bytes an element of state beside the master
+where 32 bits take 8.
+
 ``weight_decay`` is decoupled (AdamW); ``FusedAdam`` is the same optimizer
 with weight decay fixed at 0, which is exactly ``torch.optim.Adam`` with its
 defaults -- the reference's optimizer.
 """
 from __future__ import annotations
+
+import itertools
 
 import torch
 
@@ -23,11 +30,15 @@ from . import kernels as K
 
 
 class FusedAdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 state_bits=32):
         if lr < 0 or eps < 0 or weight_decay < 0:
             raise ValueError("lr, eps and weight_decay must be non-negative")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"invalid betas {betas}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32 (got {state_bits})")
+        self.state_bits = state_bits
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay))
         self._step_hooks = {}   # param -> [callable(param)]
@@ -39,9 +50,13 @@ class FusedAdamW(torch.optim.Optimizer):
     def _init_state(self, p: torch.Tensor) -> dict:
         st = self.state[p]
         if not st:
+            n, kw = p.numel(), {"device": p.device}
             st["step"] = 0
-            st["exp_avg"] = torch.zeros(p.numel(), device=p.device, dtype=torch.float32)
-            st["exp_avg_sq"] = torch.zeros(p.numel(), device=p.device, dtype=torch.float32)
+            moment = torch.uint8 if self.state_bits == 8 else torch.float32
+            st["exp_avg"] = torch.zeros(n, dtype=moment, **kw)
+            st["exp_avg_sq"] = torch.zeros(n, dtype=moment, **kw)
+            if self.state_bits == 8:
+                st["exp_base"] = torch.zeros(-(-n // K.ADAMW8_BLOCK), 2, dtype=torch.int16, **kw)
             if p.dtype != torch.float32:
                 st["master"] = p.detach().reshape(-1).to(torch.float32)
         return st
@@ -53,9 +68,16 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
+            by_device = {}
             for p in group["params"]:
                 if p.grad is not None:
-                    self._step_one(group, p)
+                    by_device.setdefault(p.device, []).append(p)
+            for dev, params in by_device.items():
+                if dev.type == "cuda":
+                    self._step_list(group, params)
+                else:
+                    for p in params:
+                        self._step_one(group, p)
         return loss
 
     @torch.no_grad()
@@ -72,24 +94,20 @@ class FusedAdamW(torch.optim.Optimizer):
                     return
         raise ValueError("step_param: the tensor is not a parameter of this optimizer")
 
-    def _step_one(self, group: dict, p: torch.Tensor) -> None:
-        b1, b2 = group["betas"]
+    def _checked(self, p: torch.Tensor) -> dict:
+        """p's state, on p's device, after the checks of p and its gradient."""
         if p.grad.is_sparse:
             raise RuntimeError("FusedAdamW does not support sparse gradients")
         if not p.is_contiguous() or not p.grad.is_contiguous():
             raise ValueError("FusedAdamW needs contiguous parameters and gradients")
         st = self._init_state(p)
         if st["exp_avg"].device != p.device:
-            for k in ("exp_avg", "exp_avg_sq", "master"):
+            for k in ("exp_avg", "exp_avg_sq", "exp_base", "master"):
                 if k in st:
                     st[k] = st[k].to(p.device)
-        st["step"] += 1
-        master = st.get("master")
-        hyper = dict(lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"],
-                     weight_decay=group["weight_decay"], step=st["step"])
-        K.adamw_step(master if master is not None else p.view(-1),
-                     p.grad.view(-1), st["exp_avg"], st["exp_avg_sq"],
-                     lowp_out=p.view(-1) if master is not None else None, **hyper)
+        return st
+
+    def _stepped(self, p: torch.Tensor) -> None:
         # the kernel wrote p through a raw pointer: advance its version
         # counter as an in-place torch op would, so caches keyed on it
         # (compute-dtype weight copies, attention caches) see the update
@@ -97,18 +115,102 @@ class FusedAdamW(torch.optim.Optimizer):
         for fn in self._step_hooks.get(p, ()):
             fn(p)
 
+    @staticmethod
+    def _hyper(group: dict) -> dict:
+        b1, b2 = group["betas"]
+        return dict(lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"],
+                    weight_decay=group["weight_decay"])
+
+    def _seeds(self, params: list, steps: list) -> list:
+        """Of the random bits of each second moment at its step: from the
+        parameter's place in the optimizer and the step, so that a resumed run
+        repeats them."""
+        place = {id(p): i for i, p in enumerate(itertools.chain.from_iterable(
+            g["params"] for g in self.param_groups))}
+        return [(t * 0xC2B2AE3D + place[id(p)] * 0x27D4EB2F) & 0xFFFFFFFF
+                for p, t in zip(params, steps)]
+
+    def _step_one(self, group: dict, p: torch.Tensor) -> None:
+        if self.state_bits == 8:
+            self._step_list(group, [p])
+            return
+        st = self._checked(p)
+        st["step"] += 1
+        master = st.get("master")
+        K.adamw_step(master if master is not None else p.view(-1),
+                     p.grad.view(-1), st["exp_avg"], st["exp_avg_sq"],
+                     lowp_out=p.view(-1) if master is not None else None,
+                     step=st["step"], **self._hyper(group))
+        self._stepped(p)
+
+    def _step_list(self, group: dict, params: list) -> None:
+        # one parameter, or parameters that share their memory: one by one
+        shared = len({p.data_ptr() for p in params}) < len(params)
+        if (len(params) == 1 or shared) and self.state_bits == 32:
+            for p in params:
+                self._step_one(group, p)
+            return
+        if shared:
+            for p in params:
+                self._step_list(group, [p])
+            return
+        states = [self._checked(p) for p in params]
+        for st in states:
+            st["step"] += 1
+        masters = [st.get("master") for st in states]
+        args = ([p if m is None else m for p, m in zip(params, masters)],
+                [p.grad for p in params], [st["exp_avg"] for st in states],
+                [st["exp_avg_sq"] for st in states])
+        steps = [st["step"] for st in states]
+        lows = [None if m is None else p for p, m in zip(params, masters)]
+        if self.state_bits == 8:
+            K.adamw8_multi(*args, [st["exp_base"] for st in states], steps, lowp_outs=lows,
+                           seeds=self._seeds(params, steps), **self._hyper(group))
+        else:
+            K.adamw_multi(*args, steps, lowp_outs=lows, **self._hyper(group))
+        for p in params:
+            self._stepped(p)
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch.optim.Optimizer's, but every state tensor keeps its own
+        type (fp32 masters and moments of 16-bit parameters, 8-bit codes)."""
+        saved = state_dict["state"]
+        want = torch.uint8 if self.state_bits == 8 else torch.float32
+        for st in saved.values():
+            if "exp_avg" in st and st["exp_avg"].dtype != want:
+                raise ValueError(f"the saved moments are {st['exp_avg'].dtype}, those of "
+                                 f"state_bits={self.state_bits} are {want}")
+        super().load_state_dict(state_dict)
+        keys = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for key, p in zip(keys, params):
+            for name, t in saved.get(key, {}).items():
+                if torch.is_tensor(t):
+                    self.state[p][name] = t.detach().to(device=p.device, copy=True)
+
     def master_param(self, p: torch.Tensor) -> torch.Tensor:
         """fp32 master of ``p`` (``p`` itself when it is fp32)."""
         st = self._init_state(p)
         return st.get("master", p.view(-1))
+
+    def moments(self, p: torch.Tensor):
+        """(exp_avg, exp_avg_sq) of ``p`` as fp32 values [numel] (of 8-bit
+        states: new tensors with the values that the codes stand for)."""
+        st = self._init_state(p)
+        if self.state_bits == 32:
+            return st["exp_avg"], st["exp_avg_sq"]
+        m, v = K.adamw8_values([st["exp_avg"]], [st["exp_avg_sq"]], [st["exp_base"]])
+        return m[0], v[0]
 
 
 class FusedAdam(FusedAdamW):
     """torch.optim.Adam's defaults (lr 1e-3, betas (0.9, 0.999), eps 1e-8,
     no weight decay) -- the optimizer the reference builds per flat shard."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
+                 state_bits=32):
         if weight_decay != 0:
             raise ValueError("FusedAdam applies no weight decay; use FusedAdamW for "
                              "decoupled weight decay")
-        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=0.0)
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=0.0,
+                         state_bits=state_bits)

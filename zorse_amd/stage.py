@@ -45,7 +45,8 @@ def _call(layer: nn.Module, x: torch.Tensor) -> torch.Tensor:
 class StageRunner:
     def __init__(self, layers: Sequence[nn.Module], lr=1e-4, betas=(0.9, 0.95), eps=1e-8,
                  weight_decay=0.1, optimizer_in_backwards=True, recompute=False,
-                 cache_attention=True, optimizer_overlap="attention", offload_inputs=False):
+                 cache_attention=True, optimizer_overlap="attention", offload_inputs=False,
+                 state_bits=32):
         if optimizer_overlap not in ("attention", "immediate"):
             raise ValueError(f"optimizer_overlap {optimizer_overlap!r}: 'attention' or 'immediate'")
         if offload_inputs and not recompute:
@@ -89,7 +90,8 @@ class StageRunner:
         self._step_no = 0
         for layer in self.layers:
             params = [p for p in layer.parameters() if p.requires_grad]
-            opt = FusedAdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+            opt = FusedAdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                             state_bits=state_bits)
             self.optimizers.append(opt)
             if optimizer_in_backwards:
                 for p in params:
