@@ -412,9 +412,10 @@ int zk_adamw_step_t(float* param, const void* grad, int grad_dtype,
                     double weight_decay, int64_t step, zk_stream_t stream);
 
 /* zk_adamw_step over a list of tensors, in as few launches as their table
- * allows (56 tensors each, 44 with 8-bit moments); the same bits as a call for each.  Hyper-parameters
- * are shared, the step counts are not.  lowp NULL: no compute copy.  The table
- * is host memory, read before the call returns. */
+ * allows (56 tensors each, 44 with 8-bit moments; large ones alone); the same
+ * bits as a call for each.  Hyper-parameters are shared, the step counts are
+ * not.  lowp NULL: no compute copy.  The table is host memory, read before the
+ * call returns. */
 typedef struct zk_adamw_tensor {
   float* param;
   const void* grad;

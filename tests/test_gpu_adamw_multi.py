@@ -287,3 +287,34 @@ def test_optimizer_steps_lists(dev):
             oa.step()
             oc.step()
             assert all(torch.equal(x, z) for x, z in zip(a, c))
+
+
+def test_large_tensors_among_small_ones(dev):
+    """Tensors above the size that is launched alone, and elements past 2^31 of
+    an 8-bit state, whose random bits go by the whole index."""
+    from zorse_amd import kernels
+    sizes = [(6 << 20) + 5, 7, 6 << 20]
+    p, gr, m, v, low = _lists(dev, sizes, BF, BF)
+    want = [[t.clone() for t in ts] for ts in (p, m, v)]
+    for i in range(3):
+        kernels.adamw_step(want[0][i], gr[i].clone(), want[1][i], want[2][i], step=2, **H)
+    kernels.adamw_multi(p, gr, m, v, [2, 2, 2], lowp_outs=low, **H)
+    for got, ref in zip((p, m, v), want):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    del p, gr, m, v, low, want
+    n, tail = (1 << 31) + 700, 700
+    p = torch.zeros(n, device=dev)
+    g = torch.zeros(n, device=dev, dtype=BF)
+    g[-tail:] = torch.linspace(-1, 1, tail)
+    cm, cv, base = _state(dev, [n])
+    kernels.adamw8_multi([p], [g], cm, cv, base, [1], seeds=[17], **H)
+    gt = g[-tail:].float().cpu().numpy()
+    z = np.zeros(tail, np.uint8)
+    with np.errstate(over="ignore"):  # what 2^31 adds to the index's product
+        seed = int(np.uint32(17) + np.uint32(1 << 31) * np.uint32(0x9E3779B1))
+    _, _, wm, wv, wb = _expected(z, z, np.zeros((3, 2), np.int16), gt, seed)
+    assert np.array_equal(cm[0][-tail:].cpu().numpy(), wm)
+    assert np.array_equal(cv[0][-tail:].cpu().numpy(), wv)
+    assert np.array_equal(base[0][-3:].cpu().numpy(), wb)
+    assert not bool(cm[0][:-tail].any()) and not bool(cv[0][:-tail].any())
+    assert not bool(p[:-tail].any()) and bool(p[-tail:].all())

@@ -26,6 +26,12 @@ static constexpr int kTile = 1024;        // elements a workgroup steps
 static constexpr int kMax32 = 56, kMax8 = 44;  // tensors a launch: 4 KB of arguments
 static constexpr int64_t kPiece = int64_t(1) << 31;       // elements of a tensor a launch
 static constexpr int64_t kMaxGrid = int64_t(1) << 23;     // workgroups a launch
+// Larger tensors with 32-bit moments are launched alone (adamw.hip's kernel, an
+// element a thread): it streams 6.5 TB/s where a workgroup that first looks its
+// tensor up reaches 6.0, and a launch costs 3 us.  us for equal tensors, alone
+// / in one launch: 48 of 2^20 elements 317 / 238, 24 of 2^22 507 / 504, 12 of
+// 2^23 460 / 498, 4 of 2^25 567 / 612.
+static constexpr int64_t kAlone = 6 << 20;
 
 struct AdamCommon {
   float decay, one_minus_b1, b2, one_minus_b2, eps;
@@ -49,7 +55,7 @@ struct Tensor8 {
   int16_t* base;
   void* low;
   int64_t n, index0;  // index0: of the piece's first element in its tensor
-  float step_size, bc2_sqrt;
+  float step_size, bc2_sqrt, inv_bc2;
   uint32_t seed;
   short g_dt, low_dt;
 };
@@ -137,31 +143,34 @@ __global__ __launch_bounds__(256) void adamw_list(const Table<Tensor32, kMax32> 
 }
 
 // ------------------------------------------------------------ 8-bit moments --
-// 4 neighbouring elements, the first n of them, at any alignment.
-template <typename T>
-struct Part4 {
-  typedef T V4 __attribute__((ext_vector_type(4)));
-  typedef V4 V4u __attribute__((aligned(sizeof(T))));
-  V4 u;
+// N neighbouring elements, the first n of them, at any alignment.
+template <typename T, int N>
+struct PartN {
+  typedef T VN __attribute__((ext_vector_type(N)));
+  typedef VN VNu __attribute__((aligned(sizeof(T))));
+  VN u;
   __device__ __forceinline__ void load(const T* p, int n) {
-    if (n >= 4) {
-      u = *reinterpret_cast<const V4u*>(p);
+    if (n >= N) {
+      u = __builtin_nontemporal_load(reinterpret_cast<const VNu*>(p));
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = i < n ? p[i] : static_cast<T>(0);
+    for (int i = 0; i < N; ++i) u[i] = i < n ? p[i] : static_cast<T>(0);
   }
   __device__ __forceinline__ void store(T* p, int n) const {
-    if (n >= 4) {
-      *reinterpret_cast<V4u*>(p) = u;
+    if (n >= N) {
+      __builtin_nontemporal_store(u, reinterpret_cast<VNu*>(p));
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
       if (i < n) p[i] = u[i];
   }
 };
 
+static constexpr int kLane = 4;    // neighbouring elements a lane: a block a wave
+static constexpr int kTile8 = 256 * kLane;
+static constexpr int kLaneR = 8, kTileR = 256 * kLaneR;  // of the reading kernel
 static constexpr int kTopM = 127, kTopV = 255;     // largest codes
 static constexpr uint32_t kMaxR = 0x7f7;           // r of the largest finite float
 static constexpr uint32_t kInf = 0x7f800000u;
@@ -174,11 +183,17 @@ __device__ __forceinline__ float code_value_m(uint32_t c, int base) {
   return c & 128 ? -v : v;
 }
 
-// 20 random bits of element i: index and seed through two products with odd
-// constants (the fractions of the roots of 2 and 3 times 2^32) and shifts.
-__device__ __forceinline__ uint32_t random20(uint32_t seed, int64_t i) {
-  uint32_t x = static_cast<uint32_t>(i) * 0x9E3779B1u +
-               static_cast<uint32_t>(static_cast<uint64_t>(i) >> 32) * 0x85157AF5u + seed;
+// 20 random bits of element i + k: index and seed through two products with
+// odd constants (the fractions of the roots of 2 and 3 times 2^32) and shifts.
+// `mixed` is mix_index(seed, i), whose products (quarter rate) a lane takes
+// once; i is a multiple of kLane, so i + k carries nothing over.
+static constexpr uint32_t kIndexMul = 0x9E3779B1u;
+__device__ __forceinline__ uint32_t mix_index(uint32_t seed, int64_t i) {
+  return static_cast<uint32_t>(i) * kIndexMul +
+         static_cast<uint32_t>(static_cast<uint64_t>(i) >> 32) * 0x85157AF5u + seed;
+}
+__device__ __forceinline__ uint32_t random20(uint32_t mixed, int k) {
+  uint32_t x = mixed + static_cast<uint32_t>(k) * kIndexMul;
   x = (x ^ (x >> 16)) * 0x6A09E667u;
   x = (x ^ (x >> 15)) * 0xBB67AE85u;
   return (x ^ (x >> 16)) >> 12;
@@ -186,69 +201,142 @@ __device__ __forceinline__ uint32_t random20(uint32_t seed, int64_t i) {
 
 // r of a float (its bits below the sign), rounded to nearest, ties to even.
 __device__ __forceinline__ uint32_t r_nearest(uint32_t b) {
-  const uint32_t r = (b + 0x7ffff + ((b >> 20) & 1)) >> 20;
-  return r < kMaxR ? r : kMaxR;
-}
-__device__ __forceinline__ uint32_t r_random(uint32_t b, uint32_t bits) {
-  const uint32_t r = (b + bits) >> 20;
-  return r < kMaxR ? r : kMaxR;
+  return (b + 0x7ffff + ((b >> 20) & 1)) >> 20;
 }
 
-// One block of 256 elements a wave, four neighbours a lane.
-template <typename G, typename L, bool kCopy>
-__device__ __forceinline__ void step8(const Tensor8& t, const AdamScalars& s, int64_t i,
-                                      int64_t block) {
-  const int n = i < t.n ? (t.n - i < 4 ? static_cast<int>(t.n - i) : 4) : 0;
-  Part4<float> p;
-  Part4<G> g;
-  Part4<uint8_t> mc, vc;
+// The update with the hardware's reciprocal and root (1 ulp each) in place of
+// the IEEE sequences, for moments whose roots and squares neither overflow nor
+// reach the numbers that those flush; 30 operations fewer an element, without
+// which the vector units and not HBM would bound the step.
+__device__ __forceinline__ void adam_one_fast(float& p, float g, float& m, float& v,
+                                              const AdamScalars& s, float inv_bc2) {
+  m = fmaf(s.one_minus_b1, g - m, m);
+  v = fmaf(s.one_minus_b2, g * g, v * s.b2);
+  const float denom = fmaf(__builtin_amdgcn_sqrtf(v), inv_bc2, s.eps);
+  p = fmaf(-s.step_size * m, __builtin_amdgcn_rcpf(denom), p * s.decay);
+}
+
+// One lane's elements after the update.
+struct Rounded {
+  uint32_t bm[kLane];            // the first moment's bits
+  uint32_t rm[kLane], rv[kLane];
+  bool zero[kLane], odd[kLane];  // second moment 0; not finite
+};
+
+template <bool kFast, typename G>
+__device__ __forceinline__ bool update8(PartN<float, kLane>& p, const PartN<G, kLane>& g,
+                                        const PartN<uint8_t, kLane>& mc,
+                                        const PartN<uint8_t, kLane>& vc, int mb, int vb,
+                                        const AdamScalars& s, float inv_bc2, uint32_t mixed,
+                                        Rounded& R) {
+  bool fast = true;
+#pragma unroll
+  for (int k = 0; k < kLane; ++k) {
+    float m = code_value_m(mc.u[k], mb), v = code_value(vc.u[k], vb), q = p.u[k];
+    if (kFast) adam_one_fast(q, static_cast<float>(g.u[k]), m, v, s, inv_bc2);
+    else adam_one(q, static_cast<float>(g.u[k]), m, v, s);
+    p.u[k] = q;
+    const uint32_t bm = __float_as_uint(m), bv = __float_as_uint(v);
+    R.bm[k] = bm;
+    R.zero[k] = bv == 0;
+    R.rm[k] = r_nearest(bm & 0x7fffffffu);
+    R.rv[k] = (bv + random20(mixed, k)) >> 20;
+    R.odd[k] = false;
+    if (kFast) {
+      // 2^-96 .. 2^120, or 0: finite, and so is m
+      fast = fast && (R.zero[k] || bv - (31u << 23) <= (216u << 23));
+    } else {
+      R.odd[k] = (bm & 0x7fffffffu) >= kInf || (bv & 0x7fffffffu) >= kInf;
+      R.rm[k] = R.odd[k] ? 0 : R.rm[k] < kMaxR ? R.rm[k] : kMaxR;
+      R.rv[k] = R.odd[k] ? 0 : R.rv[k] < kMaxR ? R.rv[k] : kMaxR;
+    }
+  }
+  return fast;
+}
+
+// The largest r of both moments in a wave's block, 16 bits each: the lanes of
+// 16 by rotations among them, the four sixteens by the two broadcasts, and the
+// last lane's for all (elements behind the tensor's last have only zeros for
+// inputs, and r = 0).
+typedef uint16_t Largest __attribute__((ext_vector_type(2)));
+template <int kCtrl, int kRows>
+__device__ __forceinline__ Largest max_with(Largest x) {
+  const int y = __builtin_bit_cast(int, x);
+  return __builtin_elementwise_max(
+      x, __builtin_bit_cast(Largest, __builtin_amdgcn_update_dpp(y, y, kCtrl, kRows, 0xf, false)));
+}
+__device__ __forceinline__ Largest block_largest(const Rounded& R) {
+  uint32_t a = R.rm[0], b = R.rv[0];
+#pragma unroll
+  for (int k = 1; k < kLane; ++k) {
+    a = R.rm[k] > a ? R.rm[k] : a;
+    b = R.rv[k] > b ? R.rv[k] : b;
+  }
+  Largest most = __builtin_bit_cast(Largest, b << 16 | a);
+  most = max_with<0x121, 0xf>(most);  // row_ror:1, 2, 4, 8
+  most = max_with<0x122, 0xf>(most);
+  most = max_with<0x124, 0xf>(most);
+  most = max_with<0x128, 0xf>(most);
+  most = max_with<0x142, 0xa>(most);  // row_bcast:15 into rows 1 and 3
+  most = max_with<0x143, 0xc>(most);  // row_bcast:31 into rows 2 and 3
+  return __builtin_bit_cast(Largest, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most), 63));
+}
+
+__device__ __forceinline__ uint32_t four_bytes(const uint32_t (&b)[4]) {
+  return (b[3] << 8 | b[2]) << 16 | (b[1] << 8 | b[0]);
+}
+
+// One block of 256 elements a wave, from element i of this lane on; kFull: all
+// of them are there.
+template <typename G, typename L, bool kCopy, bool kFull>
+__device__ __forceinline__ void step8(const Tensor8& t, const AdamScalars& s, int64_t i) {
+  const int n = kFull ? kLane : i < t.n ? (t.n - i < kLane ? static_cast<int>(t.n - i) : kLane) : 0;
+  PartN<float, kLane> p;
+  PartN<G, kLane> g;
+  PartN<uint8_t, kLane> mc, vc;
   p.load(t.p + i, n);
   g.load(static_cast<const G*>(t.g) + i, n);
   mc.load(t.m + i, n);
   vc.load(t.v + i, n);
-  int16_t* bp = t.base + 2 * block;
+  const int64_t block = __builtin_amdgcn_readfirstlane(static_cast<int>(i >> 8));
+  int16_t* bp = t.base + block * 2;
   const int mb = bp[0], vb = bp[1];
-  uint32_t rm[4], rv[4], sign[4], most_m = 0, most_v = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float m = code_value_m(mc.u[k], mb), v = code_value(vc.u[k], vb), q = p.u[k];
-    adam_one(q, static_cast<float>(g.u[k]), m, v, s);
-    p.u[k] = q;
-    const uint32_t bm = __float_as_uint(m) & 0x7fffffffu, bv = __float_as_uint(v) & 0x7fffffffu;
-    sign[k] = __float_as_uint(m) >> 24 & 128;
-    // not finite: ~0, which counts for no largest value
-    rm[k] = k < n ? bm < kInf ? r_nearest(bm) : ~0u : 0;
-    rv[k] = k < n && bv != 0 ? bv < kInf ? r_random(bv, random20(t.seed, t.index0 + i + k)) + 1 : ~0u : 0;
-    if (rm[k] != ~0u && rm[k] > most_m) most_m = rm[k];
-    if (rv[k] != ~0u && rv[k] > most_v) most_v = rv[k];
+  Rounded R;
+  const uint32_t mixed = mix_index(t.seed, t.index0 + i);
+  bool fast = s.eps == 0.f || s.eps >= 1e-30f;
+  fast = update8<true>(p, g, mc, vc, mb, vb, s, t.inv_bc2, mixed, R) && fast;
+  const bool slow = __ballot(!fast) != 0;
+  if (slow) {  // the IEEE sequences, and codes of what is not finite
+    p.load(t.p + i, n);
+    update8<false>(p, g, mc, vc, mb, vb, s, 0.f, mixed, R);
   }
   p.store(t.p + i, n);
   if (kCopy) {
-    Part4<L> low;
+    PartN<L, kLane> low;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kLane; ++k) {
       float q = p.u[k];
       asm volatile("" : "+v"(q));  // round the stored fp32 value (see adamw.hip)
       low.u[k] = static_cast<L>(q);
     }
     low.store(static_cast<L*>(t.low) + i, n);
   }
+  const Largest most = block_largest(R);
+  const uint32_t nm = most[0] > kTopM ? most[0] - kTopM : 0, nv = most[1] > kTopV ? most[1] - kTopV : 0;
+  uint32_t cm[kLane], cv[kLane];
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const uint32_t a = __shfl_xor(most_m, off, 64), b = __shfl_xor(most_v, off, 64);
-    most_m = a > most_m ? a : most_m;
-    most_v = b > most_v ? b : most_v;
+  for (int k = 0; k < kLane; ++k) {
+    const uint32_t a = __builtin_elementwise_sub_sat(R.rm[k], nm);
+    const uint32_t b = __builtin_elementwise_sub_sat(R.rv[k], nv);
+    cm[k] = a != 0 ? a | (R.bm[k] >> 24 & 128) : 0;
+    cv[k] = R.zero[k] ? 0 : b > 1 ? b : 1;
+    if (slow && R.odd[k]) {
+      cm[k] = kTopM | (R.bm[k] >> 24 & 128);
+      cv[k] = kTopV;
+    }
   }
-  // rv is r + 1, or 0 for a moment of 0
-  const int nm = static_cast<int>(most_m) > kTopM ? static_cast<int>(most_m) - kTopM : 0;
-  const int nv = static_cast<int>(most_v) - 1 > kTopV ? static_cast<int>(most_v) - 1 - kTopV : 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    int c = rm[k] == ~0u ? kTopM : static_cast<int>(rm[k]) - nm;
-    mc.u[k] = static_cast<uint8_t>(c > 0 ? c | static_cast<int>(sign[k]) : 0);
-    c = rv[k] == ~0u ? kTopV : static_cast<int>(rv[k]) - 1 - nv;
-    vc.u[k] = static_cast<uint8_t>(rv[k] == 0 ? 0 : c > 1 ? c : 1);
-  }
+  mc.u = __builtin_bit_cast(decltype(mc.u), four_bytes(cm));
+  vc.u = __builtin_bit_cast(decltype(vc.u), four_bytes(cv));
   mc.store(t.m + i, n);
   vc.store(t.v + i, n);
   if ((threadIdx.x & 63) == 0) {
@@ -257,44 +345,48 @@ __device__ __forceinline__ void step8(const Tensor8& t, const AdamScalars& s, in
   }
 }
 
+template <typename G, typename L, bool kCopy>
+__device__ __forceinline__ void block8(const Tensor8& t, const AdamScalars& s, int64_t i) {
+  const int64_t first = i - (threadIdx.x & 63) * kLane;
+  if (first >= t.n) return;
+  if (first + 256 <= t.n) step8<G, L, kCopy, true>(t, s, i);
+  else step8<G, L, kCopy, false>(t, s, i);
+}
+
 template <typename G>
-__device__ __forceinline__ void step8_low(const Tensor8& t, const AdamScalars& s, int64_t i,
-                                          int64_t block) {
-  if (t.low_dt < 0) step8<G, float, false>(t, s, i, block);
-  else if (t.low_dt == ZK_BF16) step8<G, bf16, true>(t, s, i, block);
-  else if (t.low_dt == ZK_F16) step8<G, f16, true>(t, s, i, block);
-  else step8<G, float, true>(t, s, i, block);
+__device__ __forceinline__ void block8_low(const Tensor8& t, const AdamScalars& s, int64_t i) {
+  if (t.low_dt < 0) block8<G, float, false>(t, s, i);
+  else if (t.low_dt == ZK_BF16) block8<G, bf16, true>(t, s, i);
+  else if (t.low_dt == ZK_F16) block8<G, f16, true>(t, s, i);
+  else block8<G, float, true>(t, s, i);
 }
 
 __global__ __launch_bounds__(256) void adamw8_list(const Table<Tensor8, kMax8> tab) {
   const int k = find_tensor(tab);
   const Tensor8 t = tab.e[k];
   const AdamScalars s = scalars(tab.c, t.step_size, t.bc2_sqrt);
-  const int64_t block = static_cast<int64_t>(static_cast<int>(blockIdx.x) - tab.first[k]) *
-                            (kTile / 256) + (threadIdx.x >> 6);
-  const int64_t i = block * 256 + (threadIdx.x & 63) * 4;
-  if (block * 256 >= t.n) return;  // a whole wave
-  if (t.g_dt == ZK_BF16) step8_low<bf16>(t, s, i, block);
-  else if (t.g_dt == ZK_F16) step8_low<f16>(t, s, i, block);
-  else step8_low<float>(t, s, i, block);
+  const int64_t i = static_cast<int64_t>(static_cast<int>(blockIdx.x) - tab.first[k]) * kTile8 +
+                    threadIdx.x * kLane;
+  if (t.g_dt == ZK_BF16) block8_low<bf16>(t, s, i);
+  else if (t.g_dt == ZK_F16) block8_low<f16>(t, s, i);
+  else block8_low<float>(t, s, i);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8_read(const Table<View8, kMax32> tab) {
   const int k = find_tensor(tab);
   const View8 t = tab.e[k];
-  const int64_t block = static_cast<int64_t>(static_cast<int>(blockIdx.x) - tab.first[k]) *
-                            (kTile / 256) + (threadIdx.x >> 6);
-  const int64_t i = block * 256 + (threadIdx.x & 63) * 4;
+  const int64_t i = static_cast<int64_t>(static_cast<int>(blockIdx.x) - tab.first[k]) * kTileR +
+                    threadIdx.x * kLaneR;
   if (i >= t.n) return;
-  const int n = t.n - i < 4 ? static_cast<int>(t.n - i) : 4;
-  const int mb = t.base[2 * block], vb = t.base[2 * block + 1];
-  Part4<uint8_t> mc, vc;
+  const int n = t.n - i < kLaneR ? static_cast<int>(t.n - i) : kLaneR;
+  const int mb = t.base[i / 256 * 2], vb = t.base[i / 256 * 2 + 1];
+  PartN<uint8_t, kLaneR> mc, vc;
   mc.load(t.m + i, n);
   vc.load(t.v + i, n);
-  Part4<T> mo, vo;
+  PartN<T, kLaneR> mo, vo;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < kLaneR; ++q) {
     mo.u[q] = static_cast<T>(code_value_m(mc.u[q], mb));
     vo.u[q] = static_cast<T>(code_value(vc.u[q], vb));
   }
@@ -304,7 +396,7 @@ __global__ __launch_bounds__(256) void adamw8_read(const Table<View8, kMax32> ta
 
 // ------------------------------------------------------------------- host ---
 // Fills tables and launches them as they fill up.
-template <typename E, int N, typename F>
+template <typename E, int N, int kTileOf, typename F>
 struct Launcher {
   Table<E, N> t;
   int64_t grid = 0;
@@ -312,7 +404,7 @@ struct Launcher {
   F launch;
   explicit Launcher(F f) : launch(f) { t.count = 0; }
   void add(const E& e) {
-    const int64_t wgs = (e.n + kTile - 1) / kTile;
+    const int64_t wgs = (e.n + kTileOf - 1) / kTileOf;
     if (wgs == 0) return;
     if (t.count == N || grid + wgs > kMaxGrid) flush();
     t.e[t.count] = e;
@@ -389,16 +481,24 @@ extern "C" int zk_adamw_multi(const zk_adamw_tensor* tensors, int64_t count, dou
   auto launch = [st](const Table<Tensor32, kMax32>& t, dim3 grid) {
     hipLaunchKernelGGL(adamw_list, grid, dim3(256), 0, st, t);
   };
-  Launcher<Tensor32, kMax32, decltype(launch)> L(launch);
+  Launcher<Tensor32, kMax32, kTile, decltype(launch)> L(launch);
   L.t.c = common(lr, beta1, beta2, eps, weight_decay);
   for (int64_t i = 0; i < count; ++i) {
     const zk_adamw_tensor& r = tensors[i];
     const AdamScalars s = adam_scalars(lr, beta1, beta2, eps, weight_decay, r.step);
     const int gdt = static_cast<int>(r.grad_dtype), ldt = static_cast<int>(r.lowp_dtype);
-    for (int64_t at = 0; at < r.n; at += kPiece)
-      L.add(Tensor32{r.param + at, ahead_dt(r.grad, at, gdt), r.exp_avg + at, r.exp_avg_sq + at,
-                     const_cast<void*>(ahead_dt(r.lowp, at, ldt)), r.n - at < kPiece ? r.n - at : kPiece,
-                     s.step_size, s.bc2_sqrt, gdt, r.lowp ? ldt : -1});
+    if (r.n > kAlone) {
+      for (int64_t at = 0; at < r.n; at += kPiece) {
+        rc = zk_adamw_step(r.param + at, ahead_dt(r.grad, at, gdt), gdt, r.exp_avg + at,
+                           r.exp_avg_sq + at, const_cast<void*>(ahead_dt(r.lowp, at, ldt)), ldt,
+                           r.n - at < kPiece ? r.n - at : kPiece, lr, beta1, beta2, eps, weight_decay,
+                           r.step, stream);
+        if (rc != ZK_OK) return rc;
+      }
+      continue;
+    }
+    L.add(Tensor32{r.param, r.grad, r.exp_avg, r.exp_avg_sq, r.lowp, r.n, s.step_size, s.bc2_sqrt,
+                   gdt, r.lowp ? ldt : -1});
   }
   return L.status(who);
 }
@@ -422,7 +522,7 @@ extern "C" int zk_adamw8_multi(const zk_adamw8_tensor* tensors, int64_t count, d
   auto launch = [st](const Table<Tensor8, kMax8>& t, dim3 grid) {
     hipLaunchKernelGGL(adamw8_list, grid, dim3(256), 0, st, t);
   };
-  Launcher<Tensor8, kMax8, decltype(launch)> L(launch);
+  Launcher<Tensor8, kMax8, kTile8, decltype(launch)> L(launch);
   L.t.c = common(lr, beta1, beta2, eps, weight_decay);
   for (int64_t i = 0; i < count; ++i) {
     const zk_adamw8_tensor& r = tensors[i];
@@ -432,7 +532,7 @@ extern "C" int zk_adamw8_multi(const zk_adamw8_tensor* tensors, int64_t count, d
       L.add(Tensor8{r.param + at, ahead_dt(r.grad, at, gdt), r.exp_avg + at, r.exp_avg_sq + at,
                     r.base + at / 256 * 2, const_cast<void*>(ahead_dt(r.lowp, at, ldt)),
                     r.n - at < kPiece ? r.n - at : kPiece, at, s.step_size, s.bc2_sqrt,
-                    static_cast<uint32_t>(r.seed), static_cast<short>(gdt),
+                    1.f / s.bc2_sqrt, static_cast<uint32_t>(r.seed), static_cast<short>(gdt),
                     static_cast<short>(r.lowp ? ldt : -1)});
   }
   return L.status(who);
@@ -457,7 +557,7 @@ extern "C" int zk_adamw8_values(const zk_adamw8_view* tensors, int64_t count, in
     if (out_dtype == ZK_F32) hipLaunchKernelGGL(adamw8_read<float>, grid, dim3(256), 0, st, t);
     else hipLaunchKernelGGL(adamw8_read<bf16>, grid, dim3(256), 0, st, t);
   };
-  Launcher<View8, kMax32, decltype(launch)> L(launch);
+  Launcher<View8, kMax32, kTileR, decltype(launch)> L(launch);
   L.t.c = AdamCommon{};
   for (int64_t i = 0; i < count; ++i) {
     const zk_adamw8_view& r = tensors[i];
