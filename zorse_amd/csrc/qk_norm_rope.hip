@@ -9,10 +9,14 @@
 // again (x is read for dw and dx anyway), so nothing but the inputs is kept.
 //
 // A lane holds 8 pairs of a row (16 elements: two 16-byte accesses of 2-byte
-// types), 2^log_g lanes a row, so a row's sums take log_g shuffles and a wave
-// holds 64 >> log_g rows of one or more positions at a time.  A wave stays
-// with its positions and goes through their heads: cos, sin and w are read
-// once for all of them.  HBM bounds both directions: x and y, or x, dy and dx.
+// types), 2^log_g lanes a row, so a row's sums take log_g steps among lanes and
+// a wave holds 64 >> log_g rows at a time: those of one position, or of several
+// where heads are few.  A wave goes through the heads of its positions, query
+// and key heads being different waves' work, so that cos, sin and the weight
+// are read once for all of them.  HBM bounds both directions: x and y, or x, dy
+// and dx.
+#include <type_traits>
+
 #include "part8.h"
 
 namespace zk {
@@ -76,23 +80,63 @@ struct Pairs {
   }
 };
 
-template <int kPairing>
-__device__ __forceinline__ int first_of(int i, int half) {
-  return kPairing == ZK_ROPE_HALF ? i : 2 * i;
+// The sums of two values over a row's lanes, in every lane of the row: among
+// 16 lanes by permutations within them, then across.
+template <int kCtrl>
+__device__ __forceinline__ float lanes_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                           0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
 }
-template <int kPairing>
-__device__ __forceinline__ int second_of(int i, int half) {
-  return kPairing == ZK_ROPE_HALF ? i + half : 2 * i + 1;
+template <bool kBoth>
+__device__ __forceinline__ void row_sums(float& a, float& b, int lanes) {
+  if (lanes > 1) {
+    a = lanes_add<0xb1>(a);  // quad_perm: 1 0 3 2
+    if (kBoth) b = lanes_add<0xb1>(b);
+  }
+  if (lanes > 2) {
+    a = lanes_add<0x4e>(a);  // quad_perm: 2 3 0 1
+    if (kBoth) b = lanes_add<0x4e>(b);
+  }
+  if (lanes > 4) {
+    a = lanes_add<0x141>(a);  // row_half_mirror: the other four of 8
+    if (kBoth) b = lanes_add<0x141>(b);
+  }
+  if (lanes > 8) {
+    a = lanes_add<0x140>(a);  // row_mirror: the other 8 of 16
+    if (kBoth) b = lanes_add<0x140>(b);
+  }
+  if (lanes > 16) {
+    a += __shfl_xor(a, 16, 64);
+    if (kBoth) b += __shfl_xor(b, 16, 64);
+  }
+  if (lanes > 32) {
+    a += __shfl_xor(a, 32, 64);
+    if (kBoth) b += __shfl_xor(b, 32, 64);
+  }
 }
 
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+template <int kPairing>
+__device__ __forceinline__ void load_weight(const void* w, int dt, int i0, int half, int n,
+                                            float (&a)[8], float (&b)[8]) {
+  auto take = [&](auto* p) {
+    typedef typename std::remove_const<typename std::remove_pointer<decltype(p)>::type>::type W;
+    Pairs<W, kPairing> x;
+    x.load(p, i0, half, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = x.first(i);
+      b[i] = x.second(i);
+    }
+  };
+  if (dt == ZK_F32) take(static_cast<const float*>(w));
+  else if (dt == ZK_BF16) take(static_cast<const bf16*>(w));
+  else take(static_cast<const f16*>(w));
 }
 
 template <typename T, int kPairing, bool kBwd>
-__global__ __launch_bounds__(256) void qk_kernel(QkArgs A, int log_g) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool is_q = blockIdx.x < A.q.wgs;
   const QkSide& X = is_q ? A.q : A.k;
   const int64_t wg = is_q ? blockIdx.x : blockIdx.x - A.q.wgs;
@@ -103,14 +147,12 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs A, int log_g) {
   const int log_ppw = 6 - log_g - X.log_hpw;           // positions a wave holds
   const int h0 = slot & ((1 << X.log_hpw) - 1), p_in = slot >> X.log_hpw;
   float wa[8], wb[8], da[8], db[8];
+  load_weight<kPairing>(X.w, A.w_dt, i0, half, n, wa, wb);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    wa[i] = i < n ? load_dt(X.w, first_of<kPairing>(i0 + i, half), A.w_dt) : 0.f;
-    wb[i] = i < n ? load_dt(X.w, second_of<kPairing>(i0 + i, half), A.w_dt) : 0.f;
-    da[i] = db[i] = 0.f;
-  }
+  for (int i = 0; i < 8; ++i) da[i] = db[i] = 0.f;
   const int64_t groups = (A.rows + (1 << log_ppw) - 1) >> log_ppw;
   const int64_t items = groups * X.splits;
+  const int step = X.splits << X.log_hpw;              // heads from one step to the next
   const float inv_d = 1.f / static_cast<float>(A.d);
   for (int64_t item = wg * 4 + wave; item < items; item += X.wgs * 4) {
     const int64_t group = X.splits == 1 ? item : item / X.splits;
@@ -118,6 +160,14 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs A, int log_g) {
     const int64_t p = (group << log_ppw) + p_in;
     const bool in = p < A.rows && n > 0;
     const int64_t b = in ? p / A.S : 0, s = in ? p - b * A.S : 0;
+    int h = (split << X.log_hpw) + h0;
+    const T* xr = static_cast<const T*>(X.x) + b * X.x_sb + s * X.x_ss + h * X.x_sh;
+    const T* gr = static_cast<const T*>(X.dy) + (kBwd ? b * X.dy_sb + s * X.dy_ss + h * X.dy_sh : 0);
+    T* yr = static_cast<T*>(X.out) + b * X.o_sb + s * X.o_ss + h * X.o_sh;
+    bool on = in && h < X.heads;
+    Pairs<T, kPairing> x, g;
+    x.load(xr, i0, half, on ? n : 0);
+    if (kBwd) g.load(gr, i0, half, on ? n : 0);
     int64_t pos = s;
     if (A.positions != nullptr && in) pos = A.positions[b * A.pos_sb + s];
     const bool known = pos >= 0 && pos < A.n_pos;  // rows off the table are NaN
@@ -127,43 +177,47 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs A, int log_g) {
     float c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = known ? cs[i] : __builtin_nanf("");
-    const T* xr = static_cast<const T*>(X.x) + b * X.x_sb + s * X.x_ss;
-    const T* gr = static_cast<const T*>(X.dy) + (kBwd ? b * X.dy_sb + s * X.dy_ss : 0);
-    T* yr = static_cast<T*>(X.out) + b * X.o_sb + s * X.o_ss;
-    for (int hb = split << X.log_hpw; hb < X.heads; hb += X.splits << X.log_hpw) {
-      const int h = hb + h0;
-      const bool on = in && h < X.heads;
-      Pairs<T, kPairing> x, g;
-      x.load(xr + h * X.x_sh, i0, half, on ? n : 0);
-      if (kBwd) g.load(gr + h * X.dy_sh, i0, half, on ? n : 0);
+    for (int hb = split << X.log_hpw; hb < X.heads; hb += step) {
+      const bool now = on;
+      Pairs<T, kPairing> x1 = x, g1 = g;
+      h += step;
+      on = in && h < X.heads;
+      if (hb + step < X.heads) {  // the next step's rows, ahead of this one's work
+        xr += step * X.x_sh;
+        x.load(xr, i0, half, on ? n : 0);
+        if (kBwd) {
+          gr += step * X.dy_sh;
+          g.load(gr, i0, half, on ? n : 0);
+        }
+      }
       float ss = 0.f, t = 0.f, ga[8], gb[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float u = x.first(i), v = x.second(i);
+        const float u = x1.first(i), v = x1.second(i);
         ss = fmaf(u, u, fmaf(v, v, ss));
         if (kBwd) {  // dn = R^T dy
-          const float e = g.first(i), f = g.second(i);
+          const float e = g1.first(i), f = g1.second(i);
           ga[i] = fmaf(e, c[i], f * sn[i]);
           gb[i] = fmaf(f, c[i], -(e * sn[i]));
           t = fmaf(ga[i] * wa[i], u, fmaf(gb[i] * wb[i], v, t));
         }
       }
-      ss = group_sum(ss, lanes);
+      row_sums<kBwd>(ss, t, lanes);
       const float r = 1.f / sqrtf(ss * inv_d + A.eps);
       float oa[8], ob[8];
       if (!kBwd) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float u = x.first(i) * r * wa[i], v = x.second(i) * r * wb[i];
+          const float u = x1.first(i) * r * wa[i], v = x1.second(i) * r * wb[i];
           oa[i] = fmaf(u, c[i], -(v * sn[i]));
           ob[i] = fmaf(v, c[i], u * sn[i]);
         }
       } else {
-        t = group_sum(t, lanes) * r * r * inv_d;  // r mean(g x r)
+        t *= r * r * inv_d;  // r mean(g x r)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float u = x.first(i), v = x.second(i);
-          if (on) {
+          const float u = x1.first(i), v = x1.second(i);
+          if (now) {
             da[i] = fmaf(ga[i], u * r, da[i]);
             db[i] = fmaf(gb[i], v * r, db[i]);
           }
@@ -171,50 +225,52 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs A, int log_g) {
           ob[i] = r * fmaf(-t, v, gb[i] * wb[i]);
         }
       }
-      if (on) Pairs<T, kPairing>::store(yr + h * X.o_sh, oa, ob, i0, half, n);
+      if (now) Pairs<T, kPairing>::store(yr, oa, ob, i0, half, n);
+      yr += step * X.o_sh;
     }
   }
   if (!kBwd) return;
-  // dw: this workgroup's row of partial sums
+  // dw: this workgroup's row of partial sums, of 4 waves' row slots in order.
+  // A slot's 16 * lanes values in LDS: the pairs' first elements, the second.
   __shared__ float sums[4][1024];
+  float* mine = sums[wave] + slot * 16 * lanes + i0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    for (int off = lanes; off < 64; off <<= 1) {
-      da[i] += __shfl_xor(da[i], off, 64);
-      db[i] += __shfl_xor(db[i], off, 64);
-    }
-    if (slot == 0 && i < n) {
-      sums[wave][first_of<kPairing>(i0 + i, half)] = da[i];
-      sums[wave][second_of<kPairing>(i0 + i, half)] = db[i];
-    }
+    mine[i] = da[i];
+    mine[8 * lanes + i] = db[i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < A.d; i += 256)
-    A.part[static_cast<int64_t>(blockIdx.x) * A.d + i] =
-        (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+  for (int i = threadIdx.x; i < A.d; i += 256) {
+    int at;
+    if (kPairing == ZK_ROPE_HALF) at = i < half ? i : i - half + 8 * lanes;
+    else at = (i & 1) * 8 * lanes + (i >> 1);
+    float v = 0.f;
+    for (int w = 0; w < 4; ++w)
+      for (int k = 0; k < 64 / lanes; ++k) v += sums[w][k * 16 * lanes + at];
+    A.part[static_cast<int64_t>(blockIdx.x) * A.d + i] = v;
+  }
 }
 
-// dw [d] from the partial rows: 64 columns a workgroup, 16 waves a share of
-// the rows each, in order.
+// dw [d] from the partial rows: 16 columns a workgroup, of whose 64 times 16
+// threads each 16 take a share of the rows, in order.
 __global__ __launch_bounds__(1024) void qk_dw(const float* __restrict__ part, int64_t q_rows,
                                               int64_t k_rows, int d, void* dwq, void* dwk,
                                               int w_dt) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + lane;
+  __shared__ float sums[64][16];
+  const int c = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
   const int64_t first = blockIdx.y == 0 ? 0 : q_rows;
   const int64_t rows = blockIdx.y == 0 ? q_rows : k_rows;
-  const int64_t a = rows * wave / 16, b = rows * (wave + 1) / 16;
+  const int64_t a = rows * share / 64, b = rows * (share + 1) / 64;
   float v = 0.f;
   if (col < d) {
 #pragma unroll 8
     for (int64_t i = a; i < b; ++i) v += part[(first + i) * d + col];
   }
-  sums[wave][lane] = v;
+  sums[share][c] = v;
   __syncthreads();
-  if (wave != 0 || col >= d) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) v += sums[i][lane];
+  if (share != 0 || col >= d) return;
+  for (int i = 1; i < 64; ++i) v += sums[i][c];
   store_dt(blockIdx.y == 0 ? dwq : dwk, col, w_dt, v);
 }
 
@@ -225,19 +281,55 @@ static int log_lanes(int64_t d) {
 }
 
 static constexpr int64_t kMaxWgs = int64_t(1) << 22;  // below 2^32 threads a launch
-static constexpr int64_t kBwdWgs = 1024;              // partial rows of dw for each side
+// The backward's workgroups, which are dw's partial rows: what three a CU hold
+// at once.  us at 768 / 1024 / 2048: 32 and 32 heads of 128, 4096 positions
+// 42.5 / 50.2 / 48.3, 32 and 8 heads, 30035 positions 181 / 219 / 200.
+static constexpr int64_t kBwdWgs = 768;
+// What a group's positions, cos and sin cost a wave, in steps through heads.
+static constexpr int64_t kStart = 2;
 
-static void plan(QkSide& s, int64_t rows, int64_t heads, int log_g, bool bwd) {
-  s.heads = static_cast<int>(heads);
-  s.log_hpw = 0;
-  while (s.log_hpw < 6 - log_g && (int64_t(1) << s.log_hpw) < heads) ++s.log_hpw;
-  const int log_ppw = 6 - log_g - s.log_hpw;
-  const int64_t groups = (rows + (int64_t(1) << log_ppw) - 1) >> log_ppw;
-  const int64_t passes = (heads + (int64_t(1) << s.log_hpw) - 1) >> s.log_hpw;
-  // few positions: a wave for every pass over the heads
-  s.splits = groups < 2048 ? static_cast<int>(passes) : 1;
-  const int64_t wgs = (groups * s.splits + 3) / 4, cap = bwd ? kBwdWgs : kMaxWgs;
-  s.wgs = heads == 0 ? 0 : wgs < cap ? wgs : cap;
+// A wave's row slots hold as many heads of a position at a time as leave the
+// fewest slots without a row over all of them (32 or 8 heads in 8 slots: 8; 5:
+// 1, of eight positions), the most where several do.
+static int heads_a_wave(int64_t heads, int slots_log) {
+  auto used = [&](int lh) { return (heads + (int64_t(1) << lh) - 1) >> lh << lh; };
+  int best = 0;
+  for (int lh = 1; lh <= slots_log; ++lh)
+    if (used(lh) <= used(best)) best = lh;
+  return best;
+}
+
+// Steps of a wave through one group of positions, and the groups.
+static int64_t steps_of(const QkSide& s) {
+  return (s.heads + (int64_t(1) << s.log_hpw) - 1) >> s.log_hpw;
+}
+
+static void plan(QkArgs& A, int64_t Hq, int64_t Hkv, int log_g, bool bwd) {
+  int64_t work[2] = {0, 0};
+  QkSide* sides[2] = {&A.q, &A.k};
+  const int64_t heads[2] = {Hq, Hkv};
+  for (int i = 0; i < 2; ++i) {
+    QkSide& s = *sides[i];
+    s.heads = static_cast<int>(heads[i]);
+    s.log_hpw = heads_a_wave(heads[i], 6 - log_g);
+    s.splits = 1;
+    s.wgs = 0;
+    if (heads[i] == 0) continue;
+    const int log_ppw = 6 - log_g - s.log_hpw;
+    const int64_t groups = (A.rows + (int64_t(1) << log_ppw) - 1) >> log_ppw;
+    // few positions: a wave for every step
+    if (groups < 2048) s.splits = static_cast<int>(steps_of(s));
+    s.wgs = (groups * s.splits + 3) / 4;
+    // a group's positions, cos and sin cost a wave as much as kStart steps
+    work[i] = groups * (steps_of(s) + kStart * s.splits);
+  }
+  // few enough workgroups for the partial rows of dw, shared by the work
+  const int64_t cap = bwd ? kBwdWgs : 2 * kMaxWgs;
+  for (int i = 0; i < 2; ++i) {
+    const double share = work[i] > 0 ? static_cast<double>(work[i]) / (work[0] + work[1]) : 0.0;
+    const int64_t most = static_cast<int64_t>(share * cap) > 1 ? static_cast<int64_t>(share * cap) : 1;
+    if (sides[i]->wgs > most) sides[i]->wgs = most;
+  }
 }
 
 template <bool kBwd>
@@ -295,8 +387,7 @@ static int qk_args(const char* who, const zk_qk_desc* D, const void* q, const vo
   A.n_pos = D->n_pos; A.S = D->S; A.rows = D->B * D->S;
   A.d = static_cast<int>(D->d); A.w_dt = D->w_dtype; A.eps = D->eps;
   const int lg = log_lanes(D->d);
-  plan(A.q, A.rows, D->Hq, lg, bwd);
-  plan(A.k, A.rows, D->Hkv, lg, bwd);
+  plan(A, D->Hq, D->Hkv, lg, bwd);
   return ZK_OK;
 }
 
@@ -322,7 +413,7 @@ extern "C" int zk_qk_norm_rope_fwd(const zk_qk_desc* desc, const void* q, const 
 }
 
 extern "C" int64_t zk_qk_norm_rope_bwd_workspace(int64_t d) {
-  return d > 0 && d <= 1024 ? 2 * kBwdWgs * d * 4 : -1;
+  return d > 0 && d <= 1024 ? (kBwdWgs + 2) * d * 4 : -1;
 }
 
 extern "C" int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const void* k,
@@ -350,7 +441,7 @@ extern "C" int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const 
   hipStream_t st = as_stream(stream);
   if (A.rows > 0) launch_qk<true>(A, desc->dtype, desc->pairing, log_lanes(desc->d), st);
   // without rows there are no partial rows: dw is zero
-  hipLaunchKernelGGL(qk_dw, dim3(static_cast<unsigned>((A.d + 63) / 64), desc->Hkv > 0 ? 2 : 1),
+  hipLaunchKernelGGL(qk_dw, dim3(static_cast<unsigned>((A.d + 15) / 16), desc->Hkv > 0 ? 2 : 1),
                      dim3(1024), 0, st, A.part, A.q.wgs, A.k.wgs, A.d, dwq, dwk, A.w_dt);
   return launch_status("zk_qk_norm_rope_bwd");
 }

@@ -107,17 +107,15 @@ class EmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, dtype):
-        ids = ids.contiguous()
         ctx.save_for_backward(ids)
-        ctx.cfg = (scale, padding_idx, weight.shape[0], weight.dtype)
-        return K.embedding_fwd(ids, weight.contiguous(), scale=scale, dtype=dtype)
+        ctx.cfg = (weight.shape[0], scale, padding_idx, weight.dtype)
+        return K.embedding_fwd(ids, weight, scale=scale, dtype=dtype)
 
     @staticmethod
     def backward(ctx, dy):
-        ids, = ctx.saved_tensors
-        scale, padding_idx, vocab, w_dtype = ctx.cfg
-        dw = K.embedding_bwd(ids, dy.contiguous(), vocab, scale=scale, padding_idx=padding_idx,
-                             dw_dtype=w_dtype)
+        # autograd hands on a gradient of y's shape, type and device, with that
+        # device current
+        dw = K._embedding_bwd(dy.get_device(), ctx.saved_tensors[0], dy.contiguous(), *ctx.cfg)
         return None, dw, None, None, None
 
 
@@ -131,7 +129,10 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
         if not -weight.shape[0] <= padding_idx < weight.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
         padding_idx %= weight.shape[0]
-    return EmbeddingFunction.apply(ids, weight, float(scale), padding_idx, dtype)
+    ids, scale = ids.contiguous(), float(scale)
+    if not (weight.requires_grad and torch.is_grad_enabled()):
+        return K.embedding_fwd(ids, weight.contiguous(), scale=scale, dtype=dtype)
+    return EmbeddingFunction.apply(ids, weight.contiguous(), scale, padding_idx, dtype)
 
 
 # ----------------------------------------- Norm of q and k heads, rotation --
@@ -146,19 +147,27 @@ class QkNormRopeFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        q, k = _unit_rows(q), _unit_rows(k)
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.cfg = (eps, interleaved)
-        return K.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, positions=positions,
-                                  eps=eps, interleaved=interleaved)
+        qo, ko, desc = K._qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        # the backward's descriptor for contiguous gradients: they, dq and dk
+        # lie as the outputs do
+        desc.dyq_sb, desc.dyq_ss, desc.dyq_sh = desc.oq_sb, desc.oq_ss, desc.oq_sh
+        desc.dyk_sb, desc.dyk_ss, desc.dyk_sh = desc.ok_sb, desc.ok_ss, desc.ok_sh
+        ctx.desc = desc
+        return qo, ko
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        eps, interleaved = ctx.cfg
-        grads = K.qk_norm_rope_bwd(_unit_rows(dq_out), _unit_rows(dk_out), q, k, q_weight,
-                                   k_weight, cos, sin, positions=positions, eps=eps,
-                                   interleaved=interleaved)
+        if dq_out.is_contiguous() and (k is None or dk_out.is_contiguous()):
+            grads = K._qk_bwd(ctx.desc, q.get_device(), dq_out, dk_out, q, k, q_weight, k_weight,
+                              cos, sin, positions, K._empty_qk(q, k))
+        else:
+            eps, interleaved = ctx.cfg
+            grads = K.qk_norm_rope_bwd(_unit_rows(dq_out), _unit_rows(dk_out), q, k, q_weight,
+                                       k_weight, cos, sin, positions=positions, eps=eps,
+                                       interleaved=interleaved)
         return (*grads, None, None, None, None, None)
 
 
@@ -170,8 +179,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6
     tables (rope_tables(..., torch.float32, ...)); ``positions`` int64 [S] or
     [B, S], default 0 .. S-1; a position outside the tables gives NaN.  Any even
     d up to 1024; q and k may be views of one q|k|v buffer."""
-    return QkNormRopeFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps),
-                                    bool(interleaved))
+    args = (_unit_rows(q), _unit_rows(k), q_weight, k_weight, cos, sin, positions, float(eps),
+            bool(interleaved))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return QkNormRopeFunction.apply(*args)
+    return K._qk_fwd(*args)[:2]
 
 
 # -------------------------------------------------------------- Attention --

@@ -43,11 +43,42 @@ def _require_contig(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
-def _on(dev: torch.device):
-    """Launches go to ``dev``, also while another device is the current one."""
-    if torch.cuda.current_device() == dev.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _on(index: int):
+    """Launches go to this device, also while another is the current one."""
+    if torch.cuda.current_device() == index:
+        return _NO_CONTEXT
+    return torch.cuda.device(index)
+
+
+def _stream(index: int) -> int:
+    """stream_handle of the device with this index."""
+    return stream_handle(torch.device("cuda", index)) if _abi._raw_stream is None \
+        else _abi._raw_stream(index)
+
+
+_DTYPE_CODES = {dt: dtype_code(dt) for dt in FLOAT_DTYPES}
+
+
+def _float_code(name: str, dtype: torch.dtype) -> int:
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported {name} dtype {dtype}")
+    return code
+
+
+def _device_index(first: torch.Tensor, others) -> int:
+    """The index of the GPU that all of these tensors (None: skipped) are on."""
+    index = first.get_device()
+    if index >= 0:
+        for t in others:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return index
+    return _require_gpu(first, *others).index  # says what is wrong
 
 
 # --------------------------------------------------------------- RMSNorm ---
@@ -529,41 +560,56 @@ def rope_copy(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
 # ----------------------------------------- Norm of q and k heads, rotation --
 
-def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs, grads):
-    """The checks of both directions; (device, zk_qk_desc).  ``outs`` are y or
-    dx, ``grads`` dy of q and k."""
+def _qk_side(name, t, w, q, q_weight, out, grad):
+    """The checks of the q or the k heads; t, out and grad (or None) and their
+    strides."""
+    shape, d = t.shape, q.shape[-1]
+    if len(shape) != 4 or shape[:2] != q.shape[:2] or shape[3] != d or t.dtype != q.dtype:
+        raise ValueError(f"{name} must be [B, S, H, d] matching q")
+    if w.shape != (d,) or w.dtype != q_weight.dtype or not w.is_contiguous():
+        raise ValueError(f"{name}_weight must be contiguous [{d}] of q_weight's dtype")
+    strides = []
+    for what, x in (("", t), (" output", out), (" gradient", grad)):
+        if x is None:
+            strides.append((0, 0, 0))
+            continue
+        if x.shape != shape or x.dtype != t.dtype:
+            raise ValueError(f"{name}{what} must match {name}")
+        *st, unit = x.stride()
+        if unit != 1 and x.numel():
+            raise ValueError(f"{name}{what} needs unit stride along d")
+        if what == " output" and 0 in st and any(a == 0 and n > 1 for a, n in zip(st, shape)):
+            raise ValueError(f"{name} output overlaps itself (an expanded tensor)")
+        strides.append(st)
+    return strides
+
+
+def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs,
+             grads=(None, None)):
+    """The checks of both directions; (device index, zk_qk_desc).  ``outs`` are
+    y or dx, ``grads`` dy of q and k."""
     if q.dim() != 4:
         raise ValueError("q must be [B, S, H, d]")
     B, S, Hq, d = q.shape
     if (k is None) != (k_weight is None):
         raise ValueError("k and k_weight belong together")
-    sides = [("q", q, q_weight)] + ([("k", k, k_weight)] if k is not None else [])
-    dev = _require_gpu(q, k, q_weight, k_weight, cos, sin, positions, *outs, *grads)
-    code, w_code = _float_dtype("q", q.dtype), _float_dtype("q_weight", q_weight.dtype)
-    strides = []
-    for i, (name, t, w) in enumerate(sides):
-        if t.dim() != 4 or t.shape[:2] != (B, S) or t.shape[3] != d or t.dtype != q.dtype:
-            raise ValueError(f"{name} must be [B, S, H, d] matching q")
-        if w.shape != (d,) or w.dtype != q_weight.dtype or not w.is_contiguous():
-            raise ValueError(f"{name}_weight must be contiguous [{d}] of q_weight's dtype")
-        for other, x in (("", t), (" output", outs[i] if outs else None),
-                         (" gradient", grads[i] if grads else None)):
-            if x is not None and (x.shape != t.shape or x.dtype != t.dtype
-                                  or (x.stride(3) != 1 and d > 1 and x.numel())):
-                raise ValueError(f"{name}{other} must match {name} and have unit stride along d")
-        if outs and 0 in [st for st, n in zip(outs[i].stride(), t.shape) if n > 1]:
-            raise ValueError(f"{name} output overlaps itself (an expanded tensor)")
+    index = _device_index(q, (k, q_weight, k_weight, cos, sin, positions, *outs, *grads))
+    code, w_code = _float_code("q", q.dtype), _float_code("q_weight", q_weight.dtype)
     if not Hq:
         raise ValueError("q has no heads")
     if d % 2 or not 0 < d <= 1024:
         raise ValueError(f"head dims are even and up to 1024 (got {d})")
+    (q_st, oq, gq), Hkv = _qk_side("q", q, q_weight, q, q_weight, outs[0], grads[0]), 0
+    k_st = ok = gk = (0, 0, 0)
+    if k is not None:
+        k_st, ok, gk = _qk_side("k", k, k_weight, q, q_weight, outs[1], grads[1])
+        Hkv = k.shape[2]
+    n_pos = cos.shape[0]
     for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != d // 2 \
-                or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous fp32 [n_pos, {d // 2}] table")
-    if cos.shape != sin.shape:
-        raise ValueError("cos and sin tables differ in shape")
-    n_pos, pos_sb = cos.shape[0], 0
+        if t.dtype != torch.float32 or t.shape != (n_pos, d // 2) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous fp32 [n_pos, {d // 2}] table, both of "
+                             f"as many positions")
+    pos_sb = 0
     if positions is not None:
         if positions.dtype != torch.int64 or positions.shape not in ((S,), (B, S)) \
                 or not positions.is_contiguous():
@@ -573,13 +619,14 @@ def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, ou
         raise ValueError(f"table holds {n_pos} positions < S={S}")
     if not n_pos:
         raise ValueError("the tables hold no positions")
-    none = (0, 0, 0)
-    for group in ((q, k), outs or (None, None), grads or (None, None)):
-        strides += [t.stride()[:3] if t is not None else none for t in group]
-    return dev, _abi.QkDesc(B, S, Hq, k.shape[2] if k is not None else 0, d,
-                            *(v for st in strides for v in st), n_pos, pos_sb, float(eps),
-                            _abi.ZK_ROPE_INTERLEAVED if interleaved else _abi.ZK_ROPE_HALF, code,
-                            w_code)
+    return index, _abi.QkDesc(B, S, Hq, Hkv, d, *q_st, *k_st, *oq, *ok, *gq, *gk, n_pos, pos_sb,
+                              eps, _abi.ZK_ROPE_INTERLEAVED if interleaved else _abi.ZK_ROPE_HALF,
+                              code, w_code)
+
+
+def _empty_qk(q, k):
+    return (torch.empty(q.shape, device=q.device, dtype=q.dtype),
+            None if k is None else torch.empty(k.shape, device=k.device, dtype=k.dtype))
 
 
 def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: float = 1e-6,
@@ -591,16 +638,19 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps:
     sin: fp32 [n_pos, d/2] tables; ``positions`` int64 [S] or [B, S] (default
     0 .. S-1), those outside the tables giving rows of NaN.  fp32 inside, one
     rounding."""
-    if out is None:
-        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
-               None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
-    dev, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out, ())
-    with _on(dev):
-        check(lib().zk_qk_norm_rope_fwd(desc, ptr(q), ptr(k), ptr(q_weight), ptr(k_weight),
-                                        ptr(out[0]), ptr(out[1]), ptr(cos), ptr(sin),
-                                        ptr(positions), stream_handle(dev)),
+    return _qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)[:2]
+
+
+def _qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out=None):
+    """(q', k', the descriptor)."""
+    qo, ko = out = _empty_qk(q, k) if out is None else out
+    index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
+    with _on(index):
+        check(lib().zk_qk_norm_rope_fwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
+                                        ptr(k_weight), qo.data_ptr(), ptr(ko), cos.data_ptr(),
+                                        sin.data_ptr(), ptr(positions), _stream(index)),
               "zk_qk_norm_rope_fwd")
-    return out[0], out[1]
+    return qo, ko, desc
 
 
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, positions=None,
@@ -609,24 +659,34 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, posi
     its outputs; nothing of the forward but its inputs is needed.  ``out`` =
     (dq, dk) views with unit stride along d, which may be dq_out and dk_out
     themselves.  The weights' gradients are summed in fp32 in one order."""
-    if out is None:
-        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
-               None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
     if dq_out is None or (dk_out is None) != (k is None):
         raise ValueError("a gradient for each of q and k is needed")
-    dev, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
-                         (dq_out, dk_out))
-    dwq = torch.empty_like(q_weight)
-    dwk = None if k is None else torch.empty_like(k_weight)
-    nbytes = lib().zk_qk_norm_rope_bwd_workspace(q.shape[3])
+    out = _empty_qk(q, k) if out is None else out
+    index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
+                           (dq_out, dk_out))
+    with _on(index):
+        return _qk_bwd(desc, index, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions,
+                       out)
+
+
+@functools.lru_cache(maxsize=1024)
+def _qk_workspace(d: int) -> int:
+    return lib().zk_qk_norm_rope_bwd_workspace(d)
+
+
+def _qk_bwd(desc, index, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, out):
+    """The launches, for checked arguments, on the current device."""
+    dq, dk = out
+    dev, nbytes = q.device, _qk_workspace(desc.d)
+    dwq = torch.empty(desc.d, device=dev, dtype=q_weight.dtype)
+    dwk = None if k is None else torch.empty(desc.d, device=dev, dtype=q_weight.dtype)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    with _on(dev):
-        check(lib().zk_qk_norm_rope_bwd(desc, ptr(q), ptr(k), ptr(q_weight), ptr(k_weight),
-                                        ptr(dq_out), ptr(dk_out), ptr(out[0]), ptr(out[1]),
-                                        ptr(dwq), ptr(dwk), ptr(cos), ptr(sin), ptr(positions),
-                                        ptr(ws), nbytes, stream_handle(dev)),
-              "zk_qk_norm_rope_bwd")
-    return out[0], out[1], dwq, dwk
+    check(lib().zk_qk_norm_rope_bwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(), ptr(k_weight),
+                                    dq_out.data_ptr(), ptr(dk_out), dq.data_ptr(), ptr(dk),
+                                    dwq.data_ptr(), ptr(dwk), cos.data_ptr(), sin.data_ptr(),
+                                    ptr(positions), ws.data_ptr(), nbytes, _stream(index)),
+          "zk_qk_norm_rope_bwd")
+    return dq, dk, dwq, dwk
 
 
 # -------------------------------------------------------------- Attention --
@@ -829,36 +889,39 @@ def _embedding_ids(ids: torch.Tensor) -> int:
     return int(ids.dtype == torch.int64)
 
 
-def _float_dtype(name: str, dtype: torch.dtype) -> int:
-    if dtype not in FLOAT_DTYPES:
-        raise ValueError(f"unsupported {name} dtype {dtype}")
-    return dtype_code(dtype)
-
-
 def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
                   dtype: torch.dtype | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """round(scale * weight[ids]) in ``dtype`` (default the table's): ids
     int32 / int64 of any shape, weight [vocab, hidden], both contiguous.  A row
     whose id is outside [0, vocab) is NaN.  ``out``: [*ids.shape, hidden]."""
-    dev = _require_gpu(ids, weight, out)
+    index = _device_index(ids, (weight, out))
     is64 = _embedding_ids(ids)
     if weight.dim() != 2 or not weight.numel():
         raise ValueError(f"weight must be a [vocab, hidden] table, got {tuple(weight.shape)}")
     _require_contig("weight", weight)
-    w_code = _float_dtype("weight", weight.dtype)
+    w_code = _float_code("weight", weight.dtype)
     V, h = weight.shape
     if out is None:
-        out = torch.empty(*ids.shape, h, device=dev, dtype=dtype or weight.dtype)
+        out = torch.empty((*ids.shape, h), device=ids.device, dtype=dtype or weight.dtype)
     elif out.shape != (*ids.shape, h) or not out.is_contiguous() \
             or out.dtype != (dtype or out.dtype):
         raise ValueError(f"out must be contiguous {(*ids.shape, h)} of the output's dtype")
-    y_code = _float_dtype("output", out.dtype)
-    with _on(dev):
-        check(lib().zk_embedding_fwd(ptr(ids), is64, ids.numel(), ptr(weight), V, h, ptr(out),
-                                     float(scale), w_code, y_code, stream_handle(dev)),
+    y_code = _float_code("output", out.dtype)
+    with _on(index):
+        check(lib().zk_embedding_fwd(ids.data_ptr(), is64, ids.numel(), weight.data_ptr(), V, h,
+                                     out.data_ptr(), scale, w_code, y_code, _stream(index)),
               "zk_embedding_fwd")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _embedding_workspace(tokens: int, vocab: int, hidden: int) -> int:
+    nbytes = lib().zk_embedding_bwd_workspace(tokens, vocab, hidden)
+    if nbytes < 0:
+        raise ValueError(f"embedding_bwd: {tokens} tokens of a [{vocab}, {hidden}] table are out "
+                         f"of range")
+    return nbytes
 
 
 def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: float = 1.0,
@@ -870,10 +933,9 @@ def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: flo
     overwritten, or with ``accumulate`` added to, which touches only the rows
     that tokens name; without it a new tensor of ``dw_dtype`` (default dy's).
     fp32 sums in an order that the ids alone decide (no atomics)."""
-    dev = _require_gpu(ids, dy, dw)
-    is64 = _embedding_ids(ids)
+    index = _device_index(ids, (dy, dw))
+    _embedding_ids(ids)
     _require_contig("dy", dy)
-    dy_code = _float_dtype("dy", dy.dtype)
     if dy.dim() < 1 or dy.shape[:-1] != ids.shape or not dy.shape[-1]:
         raise ValueError(f"dy must be [*ids.shape, hidden], got {tuple(dy.shape)} for ids "
                          f"{tuple(ids.shape)}")
@@ -883,20 +945,27 @@ def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: flo
     if dw is None:
         if accumulate:
             raise ValueError("accumulate needs the dw to add to")
-        dw = torch.empty(vocab, h, device=dev, dtype=dw_dtype or dy.dtype)
     elif dw.shape != (vocab, h) or not dw.is_contiguous() or dw.dtype != (dw_dtype or dw.dtype):
         raise ValueError(f"dw must be contiguous [{vocab}, {h}] of dw_dtype")
-    dw_code = _float_dtype("dw", dw.dtype)
-    nbytes = lib().zk_embedding_bwd_workspace(ids.numel(), vocab, h)
-    if nbytes < 0:
-        raise ValueError(f"embedding_bwd: {ids.numel()} tokens of a [{vocab}, {h}] table are out "
-                         f"of range")
+    w_dtype = dw.dtype if dw is not None else dw_dtype or dy.dtype
+    _float_code("dw", w_dtype)
+    _float_code("dy", dy.dtype)
+    with _on(index):
+        return _embedding_bwd(index, ids, dy, vocab, scale, padding_idx, w_dtype, dw, accumulate)
+
+
+def _embedding_bwd(index, ids, dy, vocab, scale, padding_idx, w_dtype, dw=None, accumulate=False):
+    """The launches, for checked arguments, on the current device."""
+    tokens, h, dev = ids.numel(), dy.shape[-1], dy.device
+    nbytes = _embedding_workspace(tokens, vocab, h)
+    if dw is None:
+        dw = torch.empty((vocab, h), device=dev, dtype=w_dtype)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    with _on(dev):
-        check(lib().zk_embedding_bwd(ptr(ids), is64, ids.numel(), ptr(dy), dy_code, ptr(dw),
-                                     dw_code, vocab, h, float(scale),
-                                     -1 if padding_idx is None else padding_idx, int(accumulate),
-                                     ptr(ws), nbytes, stream_handle(dev)), "zk_embedding_bwd")
+    check(lib().zk_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, tokens, dy.data_ptr(),
+                                 _DTYPE_CODES[dy.dtype], dw.data_ptr(), _DTYPE_CODES[w_dtype],
+                                 vocab, h, scale, -1 if padding_idx is None else padding_idx,
+                                 accumulate, ws.data_ptr(), nbytes, _stream(index)),
+          "zk_embedding_bwd")
     return dw
 
 
@@ -996,9 +1065,6 @@ def _tensor_table(who: str, named, steps, grads, params, lowp_outs):
     return dev
 
 
-_DTYPE_CODES = {dt: dtype_code(dt) for dt in FLOAT_DTYPES}
-
-
 def _step_table(cols, params, grads, steps, lowp_outs, seeds=None):
     """The rows of zk_adamw_tensor / zk_adamw8_tensor (every field 8 bytes)."""
     flat, seen = [], set()
@@ -1031,7 +1097,7 @@ def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1
     if dev is None:
         return
     table = _step_table((exp_avgs, exp_avg_sqs), params, grads, steps, lowp_outs)
-    with _on(dev):
+    with _on(dev.index):
         check(lib().zk_adamw_multi(table, len(params), float(lr), float(beta1), float(beta2),
                                    float(eps), float(weight_decay), stream_handle(dev)),
               "zk_adamw_multi")
@@ -1066,7 +1132,7 @@ def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, l
     if dev is None:
         return
     table = _step_table((exp_avgs, exp_avg_sqs, bases), params, grads, steps, lowp_outs, seeds)
-    with _on(dev):
+    with _on(dev.index):
         check(lib().zk_adamw8_multi(table, len(params), float(lr), float(beta1), float(beta2),
                                     float(eps), float(weight_decay), stream_handle(dev)),
               "zk_adamw8_multi")
@@ -1098,7 +1164,7 @@ def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.fl
         flat += [t.data_ptr() for t in row]
         flat.append(row[0].numel())
     table = (_abi._i64 * len(flat))(*flat)
-    with _on(dev):
+    with _on(dev.index):
         check(lib().zk_adamw8_values(table, len(exp_avgs), dtype_code(dtype), stream_handle(dev)),
               "zk_adamw8_values")
     return outs
