@@ -6,17 +6,18 @@
 // repeated pass gives the same bits.  Three launches:
 //   1. embed_sort: the tokens grouped by id (stable), and each id's count.
 //      Workgroup g of G (a power of two) owns the ids with id mod G = g, so
-//      that the frequent low ids of a text spread over all of them.  It reads
-//      every id twice: once to count its own ids and the tokens of the groups
-//      before it -- its offset, so no workgroup waits for another -- and once
-//      to place its tokens.  For the stable order each of 16 waves owns a
-//      sixteenth of the tokens and a row of counters in LDS.
-//   2. embed_grad: the grouped tokens in blocks of kBlock, one wave for each
-//      block and 512 columns, whatever the ids: a token that fills half the
-//      batch costs no more than many single ones.  An id whose tokens lie in
-//      one block is finished there; of one that crosses blocks, each block
-//      leaves a partial sum (at most two a block: the id it begins with and
-//      the id it ends in).  Waves after those write the rows of unused ids.
+//      that the frequent low ids of a text spread over all of them.  Every
+//      workgroup reads all ids, to count its own and the tokens of the groups
+//      before it -- its offset, so none waits for another.  For the stable
+//      order each of 16 waves owns a sixteenth of the tokens, a row of counters
+//      and a list of the tokens it found; what a full list does not hold (a
+//      token that fills much of a batch) is looked for again.
+//   2. embed_grad: the grouped tokens in blocks, one wave for each block and
+//      512 columns, whatever the ids: a token that fills half the batch costs
+//      no more than many single ones.  An id whose tokens lie in one block is
+//      finished there; of one that crosses blocks, each block leaves a partial
+//      sum (at most two a block: the id it begins with and the id it ends in).
+//      Waves after those write the rows of unused ids.
 //   3. embed_join: the partial sums of ids that cross blocks.
 #include "part8.h"
 
@@ -24,11 +25,14 @@ namespace zk {
 
 static constexpr int kSortWaves = 16;
 static constexpr int kMaxSlots = 512;   // ids a sort workgroup owns: 32 KB of counters
-static constexpr int kBlock = 64;       // grouped tokens a gradient wave sums (one a lane)
+static constexpr int kList = 448;       // found tokens a wave remembers: 28 KB
 static constexpr int kFillRows = 8;     // table rows a filling wave looks at
 
 struct Token {
   int t, id;
+};
+struct Span {  // the id that crosses out of the block where it begins (-1: none)
+  int id, parts;
 };
 
 // ---------------------------------------------------------------- forward ---
@@ -60,34 +64,90 @@ __global__ __launch_bounds__(256) void embed_fwd(const I* __restrict__ ids, int6
 }
 
 // ------------------------------------------------------------------- sort ---
-template <typename I>
-__global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
-    const I* __restrict__ ids, int T, int64_t V, int log_g, int slots, int64_t pad,
-    Token* __restrict__ out, int* __restrict__ count, int* __restrict__ total) {
-  extern __shared__ int cnt[];  // [kSortWaves][slots]
-  __shared__ int red[kSortWaves], run[kSortWaves];
-  const int g = blockIdx.x, groups = 1 << log_g;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < kSortWaves * slots; i += 64 * kSortWaves) cnt[i] = 0;
-  __syncthreads();
-  const int per = (T + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;
-  const int64_t t0 = static_cast<int64_t>(wave) * per;
-  const int t1 = static_cast<int>(t0 + per < T ? t0 + per : T);
-  int* mine = cnt + wave * slots;
-  // the group of a token, or `groups` for one that has no gradient
-  auto group = [&](int64_t id) {
-    return id >= 0 && id < V && id != pad ? static_cast<int>(id & (groups - 1)) : groups;
-  };
-  int before = 0;
-#pragma unroll 4
-  for (int64_t t = t0 + lane; t < t1; t += 64) {
-    const int64_t id = ids[t];
-    const int gi = group(id);
-    before += gi < g;
-    if (gi == g) atomicAdd(mine + static_cast<int>(id >> log_g), 1);
+// A token's id in 32 bits, or all ones for one that has no row of the table
+// (vocab < 2^28).
+__device__ __forceinline__ uint32_t id32(const int32_t* ids, int64_t t) {
+  return static_cast<uint32_t>(ids[t]);
+}
+__device__ __forceinline__ uint32_t id32(const int64_t* ids, int64_t t) {
+  const uint2 u = reinterpret_cast<const uint2*>(ids)[t];
+  return u.y == 0 ? u.x : ~0u;
+}
+
+// The keys of N chunks of 64 tokens from t on, one a lane and chunk: the id
+// turned right by log_g bits, so that the group stands above the slot and keys
+// order the groups; all ones where there is no token with a gradient (no key:
+// an id is below 2^28, its slot below 2^20).
+template <int N, typename I>
+__device__ __forceinline__ void load_keys(const I* ids, int64_t t, int64_t end, uint32_t V,
+                                          uint32_t pad, int log_g, uint32_t (&key)[N]) {
+  const int lane = threadIdx.x & 63;
+  if (t + N * 64 <= end) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) key[k] = id32(ids, t + k * 64 + lane);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) key[k] = t + k * 64 + lane < end ? id32(ids, t + k * 64 + lane) : ~0u;
   }
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
+  for (int k = 0; k < N; ++k)
+    key[k] = key[k] < V && key[k] != pad ? __builtin_rotateright32(key[k], log_g) : ~0u;
+}
+
+template <typename I>
+__global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
+    const I* __restrict__ ids, int T, uint32_t V, int log_g, int slots, uint32_t pad,
+    Token* __restrict__ out, int* __restrict__ count, int* __restrict__ total) {
+  extern __shared__ int cnt[];  // [kSortWaves][slots]
+  __shared__ uint32_t list[kSortWaves][kList];
+  __shared__ int red[kSortWaves], run[kSortWaves];
+  const uint32_t g = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  for (int i = threadIdx.x; i < kSortWaves * slots; i += 64 * kSortWaves) cnt[i] = 0;
+  __syncthreads();
+  // this wave's tokens: chunks of 64 from t0 on
+  const int chunks = (T + 64 * kSortWaves - 1) / (64 * kSortWaves);
+  const int64_t t0 = static_cast<int64_t>(wave) * chunks * 64;
+  const int64_t end = t0 + chunks * 64 < T ? t0 + chunks * 64 : T;
+  const uint32_t first = g << (32 - log_g), last = first | (slots - 1);  // this group's keys
+  int* mine = cnt + wave * slots;
+  const uint64_t below = (1ull << lane) - 1;
+  int before = 0, found = 0, again = -1;  // again: the first chunk that the list does not hold
+  constexpr int kAhead = 8;
+  for (int c0 = 0; c0 < chunks; c0 += kAhead) {
+    uint32_t key[kAhead];
+    load_keys(ids, t0 + c0 * 64, end, V, pad, log_g, key);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      before += __popcll(__ballot(key[k] < first));
+      const uint64_t m = __ballot(key[k] >= first && key[k] <= last);
+      if (m == 0) continue;
+      const int slot = static_cast<int>(key[k] - first);
+      const bool is = (m >> lane) & 1;
+      const int n = __popcll(m);
+      if (n <= 8) {
+        if (is) atomicAdd(mine + slot, 1);
+      } else {  // mostly one id: one lane adds for all of an id's
+        for (uint64_t left = m; left != 0;) {
+          const int lead = __builtin_ctzll(left);
+          const uint64_t same = __ballot(is && slot == __builtin_amdgcn_readlane(slot, lead));
+          if (lane == lead) atomicAdd(mine + slot, __popcll(same));
+          left &= ~same;
+        }
+      }
+      if (again < 0) {
+        // an entry: 17 bits of chunk, 6 of lane, 9 of slot
+        if (found + n <= kList && c0 + k < 1 << 17) {
+          if (is) list[wave][found + __popcll(m & below)] =
+              static_cast<uint32_t>(c0 + k) << 15 | lane << 9 | slot;
+          found += n;
+        } else {
+          again = c0 + k;
+        }
+      }
+    }
+  }
+  if (again < 0) again = chunks;
   if (lane == 0) red[wave] = before;
   __syncthreads();
   int base = 0;
@@ -112,7 +172,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
     if (k < wave) prior += run[k];
     all += run[k];
   }
-  if (g == groups - 1 && i == 0) *total = base + all;
+  if (g == gridDim.x - 1 && i == 0) *total = base + all;
   if (i < slots) {
     int at = base + prior + incl - n;
     for (int k = 0; k < kSortWaves; ++k) {
@@ -120,48 +180,41 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
       cnt[k * slots + i] = at;
       at += c;
     }
-    const int64_t id = (static_cast<int64_t>(i) << log_g) + g;
+    const uint32_t id = (static_cast<uint32_t>(i) << log_g) + g;
     if (id < V) count[id] = n;
   }
   __syncthreads();
-  // place: 64 tokens at a time, the lanes of one id after another; a wave's
-  // counters are its own, and its LDS accesses (volatile) are in order
+  // place: up to 64 tokens at a time, the lanes of one id after another; a
+  // wave's counters are its own, and its LDS accesses (volatile) are in order
   volatile int* next = mine;
-  for (int64_t tb = t0; tb < t1; tb += 64) {
-    const int64_t t = tb + lane;
-    const int64_t id = t < t1 ? static_cast<int64_t>(ids[t]) : -1;
-    unsigned long long left = __ballot(group(id) == g);
+  auto place = [&](int slot, int t, uint64_t left) {
     while (left != 0) {
       const int lead = __builtin_ctzll(left);
-      const int key = __builtin_amdgcn_readlane(static_cast<int>(id), lead);
-      const bool same = ((left >> lane) & 1) != 0 && static_cast<int>(id) == key;
-      const unsigned long long m = __ballot(same);
-      const int slot = key >> log_g;
-      const int at = next[slot];
-      if (same) out[at + __popcll(m & ((1ull << lane) - 1))] = Token{static_cast<int>(t), key};
-      if (lane == lead) next[slot] = at + __popcll(m);
+      const int key = __builtin_amdgcn_readlane(slot, lead);
+      const bool same = ((left >> lane) & 1) != 0 && slot == key;
+      const uint64_t m = __ballot(same);
+      const int at = next[key];
+      if (same) out[at + __popcll(m & below)] = Token{t, static_cast<int>((key << log_g) + g)};
+      if (lane == lead) next[key] = at + __popcll(m);
       left &= ~m;
     }
+  };
+  for (int i0 = 0; i0 < found; i0 += 64) {
+    const bool is = i0 + lane < found;
+    const uint32_t e = is ? list[wave][i0 + lane] : 0;
+    place(e & 511, static_cast<int>(t0 + (e >> 15) * 64 + (e >> 9 & 63)), __ballot(is));
+  }
+  for (int c0 = again; c0 < chunks; c0 += kAhead) {
+    uint32_t key[kAhead];
+    load_keys(ids, t0 + c0 * 64, end, V, pad, log_g, key);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      place(static_cast<int>(key[k] - first), static_cast<int>(t0 + (c0 + k) * 64 + lane),
+            __ballot(key[k] >= first && key[k] <= last));
   }
 }
 
 // --------------------------------------------------------------- gradient ---
-template <typename W>
-__device__ __forceinline__ void put_row(W* p, const float (&acc)[8], int n, float scale,
-                                        bool accumulate) {
-  float o[8];
-  if (accumulate) {
-    Part8<W> old;
-    old.load(p, n);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = old[i] + scale * acc[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = scale * acc[i];
-  }
-  Part8<W>::store(p, o, n);
-}
-
 __device__ __forceinline__ void put_part(float* p, const float (&acc)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -169,114 +222,193 @@ __device__ __forceinline__ void put_part(float* p, const float (&acc)[8]) {
 
 // part: [blocks][2][hp] fp32 (hp = h rounded up to 8): the sum of the id that
 // a block begins with and of the one that it ends in, where they reach over
-// its border (an id that does both: the first).
-template <typename D, typename W>
+// its border (an id that does both: the first).  blk: tokens a block, up to 64
+// (a lane holds one).  kStream: dy is larger than the last-level cache, and its
+// rows take no place there.
+template <typename D, typename W, bool kAdd, bool kStream>
 __global__ __launch_bounds__(256) void embed_grad(
     const D* __restrict__ dy, W* __restrict__ dw, const Token* __restrict__ tok,
     const int* __restrict__ count, const int* __restrict__ total, float* __restrict__ part,
-    int64_t V, int h, int hp, int slices, int64_t sum_items, float scale, bool accumulate) {
+    Span* __restrict__ span, int64_t V, int h, int hp, int slices, int blk, int64_t sum_items,
+    float scale) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= sum_items) {  // rows of ids without tokens
-    if (accumulate) return;  // (a wave that rounds the last workgroup up)
+    if (kAdd) return;       // (a wave that rounds the last workgroup up)
     const int64_t r0 = (item - sum_items) * kFillRows;
-    const float zero[8] = {};
     for (int64_t r = r0; r < r0 + kFillRows && r < V; ++r) {
       if (count[r] != 0) continue;
-      for (int c = lane * 8; c < h; c += 512) Part8<W>::store(dw + r * h + c, zero, h - c);
+      for (int c = lane * 8; c < h; c += 512) Part8<W>::store_zero_nt(dw + r * h + c, h - c);
     }
     return;
   }
   const int64_t j = item / slices;
   const int c = static_cast<int>(item - j * slices) * 512 + lane * 8;
   const int n_all = *total;
-  const int64_t p0 = j * kBlock;
-  if (p0 >= n_all) return;
-  const int n = n_all - p0 < kBlock ? static_cast<int>(n_all - p0) : kBlock;
+  const int64_t p0 = j * blk;
+  if (p0 >= n_all) {
+    if (c == 0) span[j] = Span{-1, 0};
+    return;
+  }
+  const int n = n_all - p0 < blk ? static_cast<int>(n_all - p0) : blk;
   const Token e = lane < n ? tok[p0 + lane] : Token{0, -1};
   const int prev = p0 > 0 ? tok[p0 - 1].id : -1;
   const int next = p0 + n < n_all ? tok[p0 + n].id : -1;
-  const int nc = h - c;  // columns from here on
-  float acc[8] = {};
-  int cur = __builtin_amdgcn_readlane(e.id, 0);
-  bool head = cur == prev;
+  // bit i: token i is the last of its id here; the first of them ends an id
+  // that began before this block, the last one may reach into the next
+  const int after = __shfl_down(e.id, 1, 64);
+  const uint64_t ends = __ballot(lane < n && (lane == n - 1 || after != e.id));
+  const bool head = __builtin_amdgcn_readfirstlane(e.id) == prev;
+  const int first_end = __builtin_ctzll(ends);
+  const int last_id = __builtin_amdgcn_readlane(e.id, n - 1);
+  const int nc = h - c < 0 ? 0 : h - c;  // columns from here on (lanes without any stay: they
+                                         // hold tokens that the others read)
+  if (c == 0) {  // one lane: what embed_join has to add up from this block on
+    Span sp = {-1, 0};
+    const uint64_t before = ends & ~(1ull << (n - 1));  // where the last id begins
+    const int first = before != 0 ? 64 - __builtin_clzll(before) : 0;
+    if (last_id == next && !(head && first == 0))
+      sp = Span{last_id, static_cast<int>((p0 + first + count[last_id] - 1) / blk - j) + 1};
+    span[j] = sp;
+  }
   float* pj = part + j * 2 * hp + c;
-  constexpr int kAhead = 8;
-  for (int i0 = 0; i0 < n; i0 += kAhead) {
-    Part8<D> x[kAhead];
+  float acc[8] = {};
+  // rows in flight; with kAdd also the old rows of the ids that end among them
+  constexpr int kAhead = 8, kSame = 16;
+  for (int i0 = 0; i0 < n;) {
+    if (i0 + kSame <= n && (ends >> i0 & ((1u << kSame) - 1)) == 0) {
+      Part8<D> x[kSame];  // rows of one id that goes on after them
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t t = __builtin_amdgcn_readlane(e.t, (i0 + k) & 63);
-      if (i0 + k < n && nc > 0) x[k].load(dy + t * h + c, nc);
-    }
+      for (int k = 0; k < kSame; ++k)
+        x[k].template get<kStream>(
+            dy + static_cast<int64_t>(__builtin_amdgcn_readlane(e.t, i0 + k)) * h + c, nc);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k >= n) break;
-      const int id = __builtin_amdgcn_readlane(e.id, (i0 + k) & 63);
-      if (id != cur) {
-        if (nc > 0) {
-          if (head) put_part(pj, acc);
-          else put_row(dw + static_cast<int64_t>(cur) * h + c, acc, nc, scale, accumulate);
-        }
-        head = false;
-        cur = id;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] = 0.f;
-      }
-      if (nc > 0) {
+      for (int k = 0; k < kSame; ++k) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc[q] += x[k][q];
       }
+      i0 += kSame;
+      continue;
     }
+    Part8<D> x[kAhead];
+    Part8<W> old[kAdd ? kAhead : 1];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k;
+      if (i >= n) break;
+      const int64_t t = __builtin_amdgcn_readlane(e.t, i);
+      x[k].template get<kStream>(dy + t * h + c, nc);
+      if (kAdd && (ends >> i & 1)) {
+        const int64_t id = __builtin_amdgcn_readlane(e.id, i);
+        old[kAdd ? k : 0].load(dw + id * h + c, nc);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k;
+      if (i >= n) break;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] += x[k][q];
+      if (!(ends >> i & 1)) continue;
+      const bool begun = head && i == first_end;
+      if (begun || (i == n - 1 && last_id == next)) {
+        if (nc > 0) put_part(begun ? pj : pj + hp, acc);
+      } else {
+        float o[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          o[q] = kAdd ? old[kAdd ? k : 0][q] + scale * acc[q] : scale * acc[q];
+        const int64_t id = __builtin_amdgcn_readlane(e.id, i);
+        Part8<W>::store(dw + id * h + c, o, nc);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] = 0.f;
+    }
+    i0 += kAhead;
   }
-  if (nc <= 0) return;
-  if (head) put_part(pj, acc);
-  else if (cur == next) put_part(pj + hp, acc);
-  else put_row(dw + static_cast<int64_t>(cur) * h + c, acc, nc, scale, accumulate);
 }
 
-// Block j's last id, if it begins there and crosses into the next block: its
-// partial sums of all blocks, in order, 256 columns a workgroup.  Four waves
-// take a quarter of the blocks each.
-template <typename W>
-__global__ __launch_bounds__(256) void embed_join(
-    W* __restrict__ dw, const Token* __restrict__ tok, const int* __restrict__ count,
-    const int* __restrict__ total, const float* __restrict__ part, int h, int hp, float scale,
-    bool accumulate) {
-  const int64_t j = blockIdx.x, p1 = (j + 1) * kBlock;
-  if (p1 >= *total) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int id = tok[p1].id;
-  const int mine = tok[p1 - kBlock + lane].id;
-  const unsigned long long same = __ballot(mine == id);
-  if (same == 0) return;  // no id crosses this border
-  const int64_t start = p1 - __popcll(same);  // grouped: the lanes of an id are the last ones
-  if (start == p1 - kBlock && start > 0 && tok[start - 1].id == id) return;  // began earlier
-  const int64_t last = (start + count[id] - 1) / kBlock;
-  const int64_t parts = last - j + 1;  // the first from block j's end, the others' beginnings
-  const int c = blockIdx.y * 256 + lane * 4;
-  const int64_t a = parts * wave / 4, b = parts * (wave + 1) / 4;
+// The partial sums of each id that crosses blocks, in order, 256 columns a
+// workgroup.  Each of 4 waves looks at a block and adds a few parts alone; the
+// parts of an id that spans many blocks are shared by the four.
+static constexpr int kJoinWaves = 4, kAloneParts = 16;
+
+__device__ __forceinline__ float4 add_parts(const float* part, int64_t j, int64_t a, int64_t b,
+                                            int hp, int c) {
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c < hp) {
-#pragma unroll 8
-    for (int64_t k = a; k < b; ++k) {
-      const float* p = part + (j + k) * 2 * hp + (k == 0 ? hp : 0) + c;
-      const float4 x = *reinterpret_cast<const float4*>(p);
-      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  if (c >= hp) return acc;
+  // part 0 at block j's end, the others at their blocks' beginnings
+  const float* base = part + j * 2 * hp + c;
+  constexpr int kAhead = 16;
+  int64_t k = a;
+  for (; k + kAhead <= b; k += kAhead) {
+    float4 x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      x[u] = *reinterpret_cast<const float4*>(base + (k + u == 0 ? hp : (k + u) * 2 * hp));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      acc.x += x[u].x; acc.y += x[u].y; acc.z += x[u].z; acc.w += x[u].w;
     }
   }
-  __shared__ float4 sums[4][64];
-  sums[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0 || c >= h) return;
-#pragma unroll
-  for (int k = 1; k < 4; ++k) {
-    const float4 x = sums[k][lane];
+#pragma unroll 4
+  for (; k < b; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(base + (k == 0 ? hp : k * 2 * hp));
     acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
   }
-  const float v[8] = {acc.x, acc.y, acc.z, acc.w, 0.f, 0.f, 0.f, 0.f};
-  put_row(dw + static_cast<int64_t>(id) * h + c, v, h - c < 4 ? h - c : 4, scale, accumulate);
+  return acc;
+}
+
+template <typename W, bool kAdd>
+__device__ __forceinline__ void put_sum(W* p, const float4& acc, int n, float scale) {
+  float o[8] = {scale * acc.x, scale * acc.y, scale * acc.z, scale * acc.w, 0.f, 0.f, 0.f, 0.f};
+  if (kAdd) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < n) o[q] += to_f32(p[q]);
+  }
+  Part8<W>::store(p, o, n < 4 ? n : 4);
+}
+
+template <typename W, bool kAdd>
+__global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
+    W* __restrict__ dw, const Span* __restrict__ span, const float* __restrict__ part, int64_t blocks,
+    int h, int hp, float scale) {
+  __shared__ int many[kJoinWaves], many_id[kJoinWaves];
+  __shared__ float4 sums[kJoinWaves][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * kJoinWaves + wave;
+  const int c = blockIdx.y * 256 + lane * 4;
+  const Span sp = j < blocks ? span[j] : Span{-1, 0};
+  const int parts = sp.parts, id = sp.id;
+  if (lane == 0) {
+    many[wave] = parts > kAloneParts ? parts : 0;
+    many_id[wave] = id;
+  }
+  if (parts > 0 && parts <= kAloneParts) {
+    const float4 acc = add_parts(part, j, 0, parts, hp, c);
+    if (c < h) put_sum<W, kAdd>(dw + static_cast<int64_t>(id) * h + c, acc, h - c, scale);
+  }
+  __syncthreads();
+  for (int w = 0; w < kJoinWaves; ++w) {
+    const int64_t all = many[w];
+    if (all == 0) continue;  // the same for every wave
+    sums[wave][lane] = add_parts(part, static_cast<int64_t>(blockIdx.x) * kJoinWaves + w,
+                                 all * wave / kJoinWaves, all * (wave + 1) / kJoinWaves, hp, c);
+    __syncthreads();
+    if (wave == 0 && c < h) {
+      float4 acc = sums[0][lane];
+#pragma unroll
+      for (int k = 1; k < kJoinWaves; ++k) {
+        const float4 x = sums[k][lane];
+        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+      }
+      put_sum<W, kAdd>(dw + static_cast<int64_t>(many_id[w]) * h + c, acc, h - c, scale);
+    }
+    __syncthreads();
+  }
 }
 
 // The groups of embed_sort: at least 256 workgroups, at most kMaxSlots ids each.
@@ -286,12 +418,23 @@ static int sort_log_groups(int64_t V) {
   return lg;
 }
 
-static int64_t embed_blocks(int64_t T) { return (T + kBlock - 1) / kBlock; }
+// Tokens a block of embed_grad: 64, or fewer while there would be less than 4096
+// waves of 512 columns (16 a CU).
+static int embed_block(int64_t T, int64_t h) {
+  int blk = 64;
+  while (blk > 8 && (T + blk - 1) / blk * ((h + 511) / 512) < 4096) blk >>= 1;
+  return blk;
+}
+static int64_t embed_blocks(int64_t T, int64_t h) {
+  const int blk = embed_block(T, h);
+  return (T + blk - 1) / blk;
+}
 static int64_t pad_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// Workspace: the partial sums, the grouped tokens, the counts, the total.
+// Workspace: the partial sums, the spans, the grouped tokens, the counts, the total.
 static int64_t embed_ws_bytes(int64_t T, int64_t V, int64_t h) {
-  return embed_blocks(T) * 2 * pad_to(h, 8) * 4 + pad_to(T * 8, 16) + pad_to(V * 4, 16) + 16;
+  return embed_blocks(T, h) * (2 * pad_to(h, 8) * 4 + 16) + pad_to(T * 8, 16) +
+         pad_to(V * 4, 16) + 16;
 }
 
 static bool embed_sizes_ok(int64_t T, int64_t V, int64_t h) {
@@ -324,22 +467,33 @@ static void launch_fwd_w(const void* ids, int64_t T, const void* w, int wdt, int
   else launch_fwd<I, f16>(ids, T, w, V, h, y, ydt, scale, st);
 }
 
-template <typename D, typename W>
+template <typename D, typename W, bool kAdd>
 static void launch_grad(const void* dy, void* dw, const Token* tok, const int* count,
-                        const int* total, float* part, int64_t T, int64_t V, int64_t h,
-                        float scale, bool accumulate, hipStream_t st) {
+                        const int* total, float* part, Span* span, int64_t T, int64_t V,
+                        int64_t h, float scale, hipStream_t st) {
   const int hp = static_cast<int>(pad_to(h, 8)), slices = static_cast<int>((h + 511) / 512);
-  const int64_t blocks = embed_blocks(T), sums = blocks * slices;
-  const int64_t items = sums + (accumulate ? 0 : (V + kFillRows - 1) / kFillRows);
-  if (items > 0)
-    hipLaunchKernelGGL((embed_grad<D, W>), dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256),
-                       0, st, (const D*)dy, (W*)dw, tok, count, total, part, V,
-                       static_cast<int>(h), hp, slices, sums, scale, accumulate);
+  const int blk = embed_block(T, h);
+  const int64_t blocks = embed_blocks(T, h), sums = blocks * slices;
+  const int64_t items = sums + (kAdd ? 0 : (V + kFillRows - 1) / kFillRows);
+  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+#define ZK_GRAD(S)                                                                            \
+  hipLaunchKernelGGL((embed_grad<D, W, kAdd, S>), grid, dim3(256), 0, st, (const D*)dy, (W*)dw, \
+                     tok, count, total, part, span, V, static_cast<int>(h), hp, slices, blk, sums, scale)
+  // dy within the 256 MB of last-level cache may still be there from the kernel
+  // that wrote it.  us with streaming loads / ordinary ones: 65536 tokens of
+  // 5120 (671 MB), a text's ids 337 / 348, nine tenths one id 361 / 427; 8192 of
+  // 1000 (16 MB, fresh) 35 / 31, 4096 of 4096 (34 MB) 94 / 92
+  const bool stream = T * h * static_cast<int64_t>(sizeof(D)) > (int64_t(1) << 28);
+  if (items > 0) {
+    if (stream) ZK_GRAD(true); else ZK_GRAD(false);
+  }
+#undef ZK_GRAD
   if (blocks > 1)
-    hipLaunchKernelGGL((embed_join<W>),
-                       dim3(static_cast<unsigned>(blocks - 1), static_cast<unsigned>((h + 255) / 256)),
-                       dim3(256), 0, st, (W*)dw, tok, count, total, part, static_cast<int>(h), hp,
-                       scale, accumulate);
+    hipLaunchKernelGGL((embed_join<W, kAdd>),
+                       dim3(static_cast<unsigned>((blocks - 1 + kJoinWaves - 1) / kJoinWaves),
+                            static_cast<unsigned>((h + 255) / 256)),
+                       dim3(64 * kJoinWaves), 0, st, (W*)dw, span, part, blocks - 1,
+                       static_cast<int>(h), hp, scale);
 }
 
 }  // namespace zk
@@ -391,7 +545,9 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
              (long long)embed_ws_bytes(tokens, vocab, hidden));
   char* ws = static_cast<char*>(workspace);
   float* part = reinterpret_cast<float*>(ws);
-  ws += embed_blocks(tokens) * 2 * pad_to(hidden, 8) * 4;
+  ws += embed_blocks(tokens, hidden) * 2 * pad_to(hidden, 8) * 4;
+  Span* span = reinterpret_cast<Span*>(ws);
+  ws += embed_blocks(tokens, hidden) * 16;
   Token* tok = reinterpret_cast<Token*>(ws);
   ws += pad_to(tokens * 8, 16);
   int* count = reinterpret_cast<int*>(ws);
@@ -402,14 +558,20 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
   hipStream_t st = as_stream(stream);
   const dim3 grid(1u << lg), block(64 * kSortWaves);
   const size_t lds = sizeof(int) * kSortWaves * slots;
+  const uint32_t pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<uint32_t>(padding_idx) : ~0u;
   if (ids_64)
     hipLaunchKernelGGL((embed_sort<int64_t>), grid, block, lds, st, (const int64_t*)ids,
-                       static_cast<int>(tokens), vocab, lg, slots, padding_idx, tok, count, total);
+                       static_cast<int>(tokens), static_cast<uint32_t>(vocab), lg, slots, pad, tok,
+                       count, total);
   else
     hipLaunchKernelGGL((embed_sort<int32_t>), grid, block, lds, st, (const int32_t*)ids,
-                       static_cast<int>(tokens), vocab, lg, slots, padding_idx, tok, count, total);
-#define ZK_G(D, W) \
-  launch_grad<D, W>(dy, dw, tok, count, total, part, tokens, vocab, hidden, scale, accumulate != 0, st)
+                       static_cast<int>(tokens), static_cast<uint32_t>(vocab), lg, slots, pad, tok,
+                       count, total);
+#define ZK_G(D, W)                                                                               \
+  do {                                                                                           \
+    if (accumulate) launch_grad<D, W, true>(dy, dw, tok, count, total, part, span, tokens, vocab, hidden, scale, st); \
+    else launch_grad<D, W, false>(dy, dw, tok, count, total, part, span, tokens, vocab, hidden, scale, st); \
+  } while (0)
 #define ZK_GW(D)                             \
   do {                                       \
     if (dw_dtype == ZK_F32) ZK_G(D, float);  \

@@ -14,6 +14,11 @@ struct Part8 {
   typedef T V8 __attribute__((ext_vector_type(8)));
   typedef V8 V8u __attribute__((aligned(sizeof(T))));
   V8 u;
+  template <bool kOnce>  // kOnce: read once, not worth a place in the caches
+  __device__ __forceinline__ void get(const T* p, int n) {
+    if (kOnce && n >= 8) u = __builtin_nontemporal_load(reinterpret_cast<const V8u*>(p));
+    else load(p, n);
+  }
   // the first n (<= 8) elements at p; the others are zero
   __device__ __forceinline__ void load(const T* p, int n) {
     if (n >= 8) {
@@ -24,6 +29,14 @@ struct Part8 {
     for (int i = 0; i < 8; ++i) u[i] = i < n ? p[i] : static_cast<T>(0.f);
   }
   __device__ __forceinline__ float operator[](int i) const { return static_cast<float>(u[i]); }
+  // zeros that nothing reads soon
+  static __device__ __forceinline__ void store_zero_nt(T* p, int n) {
+    if (n >= 8) {
+      __builtin_nontemporal_store(V8{}, reinterpret_cast<V8u*>(p));
+      return;
+    }
+    for (int i = 0; i < n; ++i) __builtin_nontemporal_store(static_cast<T>(0.f), p + i);
+  }
   static __device__ __forceinline__ void store(T* p, const float (&v)[8], int n) {
     if (n >= 8) {
       V8 w;
