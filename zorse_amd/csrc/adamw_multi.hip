@@ -213,7 +213,7 @@ __device__ __forceinline__ void adam_one_fast(float& p, float g, float& m, float
   m = fmaf(s.one_minus_b1, g - m, m);
   v = fmaf(s.one_minus_b2, g * g, v * s.b2);
   const float denom = fmaf(__builtin_amdgcn_sqrtf(v), inv_bc2, s.eps);
-  p = fmaf(-s.step_size * m, __builtin_amdgcn_rcpf(denom), p * s.decay);
+  p = fmaf(-s.step_size, m * __builtin_amdgcn_rcpf(denom), p * s.decay);
 }
 
 // One lane's elements after the update.

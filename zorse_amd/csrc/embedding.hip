@@ -220,7 +220,7 @@ __device__ __forceinline__ void put_part(float* p, const float (&acc)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
 
-// part: [blocks][2][hp] fp32 (hp = h rounded up to 8): the sum of the id that
+// part: [blocks][2][hp] fp32 (hp: part_row(h)): the sum of the id that
 // a block begins with and of the one that it ends in, where they reach over
 // its border (an id that does both: the first).  blk: tokens a block, up to 64
 // (a lane holds one).  kStream: dy is larger than the last-level cache, and its
@@ -330,45 +330,74 @@ __global__ __launch_bounds__(256) void embed_grad(
 }
 
 // The partial sums of each id that crosses blocks, in order, 256 columns a
-// workgroup.  Each of 4 waves looks at a block and adds a few parts alone; the
-// parts of an id that spans many blocks are shared by the four.
-static constexpr int kJoinWaves = 4, kAloneParts = 16;
+// workgroup.  Each of 8 waves looks at a block and adds a few parts alone; the
+// parts of an id that spans many blocks are shared by the eight.  Latency
+// bounds it, not bytes: 16 parts are in flight at a time, and 65536 tokens of
+// 5120 columns, nine tenths of them one id, take 282 us in all where four waves
+// a workgroup took 320.
+static constexpr int kJoinWaves = 8, kAloneParts = 16;
 
 __device__ __forceinline__ float4 add_parts(const float* part, int64_t j, int64_t a, int64_t b,
-                                            int hp, int c) {
+                                            int h, int hp, int c) {
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c >= hp) return acc;
+  if (c >= h) return acc;
   // part 0 at block j's end, the others at their blocks' beginnings
   const float* base = part + j * 2 * hp + c;
   constexpr int kAhead = 16;
-  int64_t k = a;
-  for (; k + kAhead <= b; k += kAhead) {
+  for (int64_t k = a; k < b; k += kAhead) {
     float4 x[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      x[u] = *reinterpret_cast<const float4*>(base + (k + u == 0 ? hp : (k + u) * 2 * hp));
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t q = k + u < b ? k + u : b - 1;
+      x[u] = *reinterpret_cast<const float4*>(base + (q == 0 ? hp : q * 2 * hp));
+    }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      acc.x += x[u].x; acc.y += x[u].y; acc.z += x[u].z; acc.w += x[u].w;
+      const bool on = k + u < b;
+      acc.x += on ? x[u].x : 0.f;
+      acc.y += on ? x[u].y : 0.f;
+      acc.z += on ? x[u].z : 0.f;
+      acc.w += on ? x[u].w : 0.f;
     }
-  }
-#pragma unroll 4
-  for (; k < b; ++k) {
-    const float4 x = *reinterpret_cast<const float4*>(base + (k == 0 ? hp : k * 2 * hp));
-    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
   }
   return acc;
 }
 
+// The old elements of a row's 4 columns, fetched before the parts they add to.
 template <typename W, bool kAdd>
-__device__ __forceinline__ void put_sum(W* p, const float4& acc, int n, float scale) {
-  float o[8] = {scale * acc.x, scale * acc.y, scale * acc.z, scale * acc.w, 0.f, 0.f, 0.f, 0.f};
-  if (kAdd) {
+__device__ __forceinline__ void get_old(const W* p, int n, float (&old)[4]) {
+  typedef W W4 __attribute__((ext_vector_type(4)));
+  typedef W4 W4u __attribute__((aligned(sizeof(W))));
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < n) o[q] += to_f32(p[q]);
+  for (int q = 0; q < 4; ++q) old[q] = 0.f;
+  if (!kAdd) return;
+  if (n >= 4) {
+    const W4 u = *reinterpret_cast<const W4u*>(p);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) old[q] = to_f32(static_cast<W>(u[q]));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      if (q < n) old[q] = to_f32(p[q]);
   }
-  Part8<W>::store(p, o, n < 4 ? n : 4);
+}
+
+template <typename W, bool kAdd>
+__device__ __forceinline__ void put_sum(W* p, const float4& acc, const float (&old)[4], int n,
+                                        float scale) {
+  typedef W W4 __attribute__((ext_vector_type(4)));
+  typedef W4 W4u __attribute__((aligned(sizeof(W))));
+  const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+  W4 u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) u[q] = static_cast<W>(kAdd ? old[q] + scale * a[q] : scale * a[q]);
+  if (n >= 4) {
+    *reinterpret_cast<W4u*>(p) = u;
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+    if (q < n) p[q] = u[q];
 }
 
 template <typename W, bool kAdd>
@@ -388,15 +417,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
     many_id[wave] = id;
   }
   if (parts > 0 && parts <= kAloneParts) {
-    const float4 acc = add_parts(part, j, 0, parts, hp, c);
-    if (c < h) put_sum<W, kAdd>(dw + static_cast<int64_t>(id) * h + c, acc, h - c, scale);
+    W* p = dw + static_cast<int64_t>(id) * h + c;
+    float old[4];
+    get_old<W, kAdd>(p, h - c, old);
+    put_sum<W, kAdd>(p, add_parts(part, j, 0, parts, h, hp, c), old, h - c, scale);
   }
   __syncthreads();
   for (int w = 0; w < kJoinWaves; ++w) {
     const int64_t all = many[w];
     if (all == 0) continue;  // the same for every wave
     sums[wave][lane] = add_parts(part, static_cast<int64_t>(blockIdx.x) * kJoinWaves + w,
-                                 all * wave / kJoinWaves, all * (wave + 1) / kJoinWaves, hp, c);
+                                 all * wave / kJoinWaves, all * (wave + 1) / kJoinWaves, h, hp, c);
     __syncthreads();
     if (wave == 0 && c < h) {
       float4 acc = sums[0][lane];
@@ -405,7 +436,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
         const float4 x = sums[k][lane];
         acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
       }
-      put_sum<W, kAdd>(dw + static_cast<int64_t>(many_id[w]) * h + c, acc, h - c, scale);
+      W* p = dw + static_cast<int64_t>(many_id[w]) * h + c;
+      float old[4];
+      get_old<W, kAdd>(p, h - c, old);
+      put_sum<W, kAdd>(p, acc, old, h - c, scale);
     }
     __syncthreads();
   }
@@ -430,10 +464,14 @@ static int64_t embed_blocks(int64_t T, int64_t h) {
   return (T + blk - 1) / blk;
 }
 static int64_t pad_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+// Floats of a partial row: two of them are an odd number of 256-byte units, so
+// that the parts of one column, which embed_join reads together, lie in all of
+// the memory's channels.
+static int64_t part_row(int64_t h) { return ((h + 31) / 32 | 1) * 32; }
 
 // Workspace: the partial sums, the spans, the grouped tokens, the counts, the total.
 static int64_t embed_ws_bytes(int64_t T, int64_t V, int64_t h) {
-  return embed_blocks(T, h) * (2 * pad_to(h, 8) * 4 + 16) + pad_to(T * 8, 16) +
+  return embed_blocks(T, h) * (2 * part_row(h) * 4 + 16) + pad_to(T * 8, 16) +
          pad_to(V * 4, 16) + 16;
 }
 
@@ -471,7 +509,7 @@ template <typename D, typename W, bool kAdd>
 static void launch_grad(const void* dy, void* dw, const Token* tok, const int* count,
                         const int* total, float* part, Span* span, int64_t T, int64_t V,
                         int64_t h, float scale, hipStream_t st) {
-  const int hp = static_cast<int>(pad_to(h, 8)), slices = static_cast<int>((h + 511) / 512);
+  const int hp = static_cast<int>(part_row(h)), slices = static_cast<int>((h + 511) / 512);
   const int blk = embed_block(T, h);
   const int64_t blocks = embed_blocks(T, h), sums = blocks * slices;
   const int64_t items = sums + (kAdd ? 0 : (V + kFillRows - 1) / kFillRows);
@@ -545,7 +583,7 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
              (long long)embed_ws_bytes(tokens, vocab, hidden));
   char* ws = static_cast<char*>(workspace);
   float* part = reinterpret_cast<float*>(ws);
-  ws += embed_blocks(tokens, hidden) * 2 * pad_to(hidden, 8) * 4;
+  ws += embed_blocks(tokens, hidden) * 2 * part_row(hidden) * 4;
   Span* span = reinterpret_cast<Span*>(ws);
   ws += embed_blocks(tokens, hidden) * 16;
   Token* tok = reinterpret_cast<Token*>(ws);

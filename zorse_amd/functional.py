@@ -149,12 +149,9 @@ class QkNormRopeFunction(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.cfg = (eps, interleaved)
-        qo, ko, desc = K._qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-        # the backward's descriptor for contiguous gradients: they, dq and dk
-        # lie as the outputs do
-        desc.dyq_sb, desc.dyq_ss, desc.dyq_sh = desc.oq_sb, desc.oq_ss, desc.oq_sh
-        desc.dyk_sb, desc.dyk_ss, desc.dyk_sh = desc.ok_sb, desc.ok_ss, desc.ok_sh
-        ctx.desc = desc
+        # the descriptor is the backward's too where the gradients are contiguous
+        qo, ko, ctx.desc = K._qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                     interleaved)
         return qo, ko
 
     @staticmethod

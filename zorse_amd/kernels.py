@@ -9,6 +9,7 @@ GPU tensor these functions raise.
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import functools
 import math
@@ -560,55 +561,66 @@ def rope_copy(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
 # ----------------------------------------- Norm of q and k heads, rotation --
 
-def _qk_side(name, t, w, q, q_weight, out, grad):
-    """The checks of the q or the k heads; t, out and grad (or None) and their
-    strides."""
-    shape, d = t.shape, q.shape[-1]
-    if len(shape) != 4 or shape[:2] != q.shape[:2] or shape[3] != d or t.dtype != q.dtype:
-        raise ValueError(f"{name} must be [B, S, H, d] matching q")
-    if w.shape != (d,) or w.dtype != q_weight.dtype or not w.is_contiguous():
-        raise ValueError(f"{name}_weight must be contiguous [{d}] of q_weight's dtype")
-    strides = []
-    for what, x in (("", t), (" output", out), (" gradient", grad)):
-        if x is None:
-            strides.append((0, 0, 0))
-            continue
-        if x.shape != shape or x.dtype != t.dtype:
-            raise ValueError(f"{name}{what} must match {name}")
-        *st, unit = x.stride()
-        if unit != 1 and x.numel():
-            raise ValueError(f"{name}{what} needs unit stride along d")
-        if what == " output" and 0 in st and any(a == 0 and n > 1 for a, n in zip(st, shape)):
-            raise ValueError(f"{name} output overlaps itself (an expanded tensor)")
-        strides.append(st)
-    return strides
+def _qk_strides(name, x, t):
+    """The strides of an output or gradient of the heads t, after its checks."""
+    if x.shape != t.shape or x.dtype != t.dtype:
+        raise ValueError(f"{name} must have the shape and type of its heads")
+    *st, unit = x.stride()
+    if unit != 1 and x.numel():
+        raise ValueError(f"{name} needs unit stride along d")
+    return st
 
 
-def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs,
+def _qk_out(name, x, t):
+    st = _qk_strides(name, x, t)
+    if 0 in st and any(a == 0 and n > 1 for a, n in zip(st, x.shape)):
+        raise ValueError(f"{name} overlaps itself (an expanded tensor)")
+    return st
+
+
+def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs=None,
              grads=(None, None)):
     """The checks of both directions; (device index, zk_qk_desc).  ``outs`` are
-    y or dx, ``grads`` dy of q and k."""
+    y or dx (None: new contiguous tensors), ``grads`` dy of q and k."""
     if q.dim() != 4:
         raise ValueError("q must be [B, S, H, d]")
     B, S, Hq, d = q.shape
     if (k is None) != (k_weight is None):
         raise ValueError("k and k_weight belong together")
-    index = _device_index(q, (k, q_weight, k_weight, cos, sin, positions, *outs, *grads))
+    index = _device_index(q, (k, q_weight, k_weight, cos, sin, positions, *(outs or ()), *grads))
     code, w_code = _float_code("q", q.dtype), _float_code("q_weight", q_weight.dtype)
     if not Hq:
         raise ValueError("q has no heads")
     if d % 2 or not 0 < d <= 1024:
         raise ValueError(f"head dims are even and up to 1024 (got {d})")
-    (q_st, oq, gq), Hkv = _qk_side("q", q, q_weight, q, q_weight, outs[0], grads[0]), 0
-    k_st = ok = gk = (0, 0, 0)
+    if q_weight.shape != (d,) or not q_weight.is_contiguous():
+        raise ValueError(f"q_weight must be contiguous [{d}]")
+    q_st, Hkv = _qk_strides("q", q, q), 0
+    k_st = ok = gq = gk = (0, 0, 0)
     if k is not None:
-        k_st, ok, gk = _qk_side("k", k, k_weight, q, q_weight, outs[1], grads[1])
-        Hkv = k.shape[2]
-    n_pos = cos.shape[0]
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype != torch.float32 or t.shape != (n_pos, d // 2) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous fp32 [n_pos, {d // 2}] table, both of "
-                             f"as many positions")
+        if k.dim() != 4 or k.shape[:2] != (B, S) or k.shape[3] != d or k.dtype != q.dtype:
+            raise ValueError("k must be [B, S, H, d] matching q")
+        if k_weight.shape != (d,) or k_weight.dtype != q_weight.dtype \
+                or not k_weight.is_contiguous():
+            raise ValueError(f"k_weight must be contiguous [{d}] of q_weight's dtype")
+        k_st, Hkv = _qk_strides("k", k, k), k.shape[2]
+    if outs is None:
+        # and the gradients of such outputs lie as they do
+        oq = gq = (S * Hq * d, Hq * d, d)
+        ok = gk = (S * Hkv * d, Hkv * d, d)
+    else:
+        oq = _qk_out("q output", outs[0], q)
+        if k is not None:
+            ok = _qk_out("k output", outs[1], k)
+    if grads[0] is not None:
+        gq = _qk_strides("q gradient", grads[0], q)
+    if grads[1] is not None:
+        gk = _qk_strides("k gradient", grads[1], k)
+    n_pos, half = cos.shape[0], d // 2
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != (n_pos, half) \
+            or sin.shape != (n_pos, half) or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError(f"cos and sin must be contiguous fp32 [n_pos, {half}] tables of as many "
+                         f"positions")
     pos_sb = 0
     if positions is not None:
         if positions.dtype != torch.int64 or positions.shape not in ((S,), (B, S)) \
@@ -643,8 +655,8 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps:
 
 def _qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out=None):
     """(q', k', the descriptor)."""
-    qo, ko = out = _empty_qk(q, k) if out is None else out
     index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
+    qo, ko = _empty_qk(q, k) if out is None else out
     with _on(index):
         check(lib().zk_qk_norm_rope_fwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
                                         ptr(k_weight), qo.data_ptr(), ptr(ko), cos.data_ptr(),
@@ -661,9 +673,9 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, posi
     themselves.  The weights' gradients are summed in fp32 in one order."""
     if dq_out is None or (dk_out is None) != (k is None):
         raise ValueError("a gradient for each of q and k is needed")
-    out = _empty_qk(q, k) if out is None else out
     index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
                            (dq_out, dk_out))
+    out = _empty_qk(q, k) if out is None else out
     with _on(index):
         return _qk_bwd(desc, index, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions,
                        out)
@@ -1029,58 +1041,80 @@ def adamw_step_t(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tensor,
                                 int(step), stream_handle(dev)), "zk_adamw_step_t")
 
 
-def _tensor_table(who: str, named, steps, grads, params, lowp_outs):
-    """The device of a step over lists of tensors (None: empty lists), after
-    its checks.  ``named``: (name, list, dtype, elements for n) of what must have one dtype;
-    every list is as long as ``params`` and every tensor contiguous on the
-    first parameter's device."""
+_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
+_is_contiguous, _get_device = torch.Tensor.is_contiguous, torch.Tensor.get_device
+
+
+def _gpu_index(t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("zorse_amd kernels need GPU tensors (got a CPU tensor)")
+    return index
+
+
+def _check_lists(who: str, sizes, index: int, columns) -> None:
+    """Every tensor of each column (name, tensors, allowed dtypes, elements for
+    n or None) is contiguous, on GPU ``index``, of an allowed dtype and as large
+    as ``sizes`` say.  A list at a time, in calls that loop inside the
+    interpreter: 150 tensors of five kinds are 750 checks a step."""
+    for name, tensors, dtypes, elems in columns:
+        want = sizes if elems is None else list(map(elems, sizes))
+        if {t.dtype for t in tensors} <= dtypes and list(map(_numel, tensors)) == want \
+                and all(map(_is_contiguous, tensors)) \
+                and set(map(_get_device, tensors)) == {index}:
+            continue
+        for i, t in enumerate(tensors):
+            _gpu_index(t)
+            if t.dtype not in dtypes or t.numel() != want[i] or not t.is_contiguous() \
+                    or t.get_device() != index:
+                raise ValueError(f"{who}: {name} {i} must be contiguous {sorted(map(str, dtypes))} "
+                                 f"with {want[i]} elements on cuda:{index}")
+
+
+def _rows(columns) -> array.array:
+    """The columns (lists of integers) as rows of 64-bit fields."""
+    n = len(columns)
+    table = array.array("q", bytes(8 * n * len(columns[0])))
+    for i, c in enumerate(columns):
+        table[i::n] = array.array("q", c)
+    return table
+
+
+_F32, _U8, _I16 = {torch.float32}, {torch.uint8}, {torch.int16}
+_FLOATS = set(FLOAT_DTYPES)
+
+
+def _step_rows(who, columns, params, grads, steps, lowp_outs, seeds=None):
+    """(device index, rows of zk_adamw_tensor / zk_adamw8_tensor) after the
+    checks of a step; ``columns``: the states as _check_lists takes them."""
     count = len(params)
-    lists = [t for _, t, _, _ in named] + [grads] + ([lowp_outs] if lowp_outs is not None else [])
-    if any(len(t) != count for t in lists) or (steps is not None and len(steps) != count):
+    if len(grads) != count or len(steps) != count or any(len(c[1]) != count for c in columns) \
+            or (lowp_outs is not None and len(lowp_outs) != count) \
+            or (seeds is not None and len(seeds) != count):
         raise ValueError(f"{who}: the lists differ in length")
     if not count:
-        return None
-    dev = params[0].device
-    if dev.type != "cuda":
-        raise ValueError("zorse_amd kernels need GPU tensors (got a CPU tensor)")
-    index = dev.index
-    for i, p in enumerate(params):
-        n = p.numel()
-        for name, ts, dtype, elems in named:
-            t = ts[i]
-            if t.dtype != dtype or t.numel() != (elems(n) if elems else n) \
-                    or not t.is_contiguous() or t.get_device() != index:
-                raise ValueError(f"{who}: {name} {i} must be contiguous {dtype} with "
-                                 f"{elems(n) if elems else n} elements on {dev}")
-        g = grads[i]
-        if g.numel() != n or not g.is_contiguous() or g.get_device() != index \
-                or g.dtype not in _DTYPE_CODES:
-            raise ValueError(f"{who}: grad {i} must be contiguous {list(_DTYPE_CODES)} with {n} "
-                             f"elements on {dev}")
-        low = lowp_outs[i] if lowp_outs is not None else None
-        if low is not None and (low.numel() != n or not low.is_contiguous()
-                                or low.get_device() != index or low.dtype not in _DTYPE_CODES):
-            raise ValueError(f"{who}: lowp_out {i} must be contiguous {list(_DTYPE_CODES)} with "
-                             f"{n} elements on {dev}")
-    return dev
-
-
-def _step_table(cols, params, grads, steps, lowp_outs, seeds=None):
-    """The rows of zk_adamw_tensor / zk_adamw8_tensor (every field 8 bytes)."""
-    flat, seen = [], set()
-    lows = lowp_outs if lowp_outs is not None else [None] * len(params)
-    for i, (p, g, low, step) in enumerate(zip(params, grads, lows, steps)):
-        n, at = p.numel(), p.data_ptr()
-        if n and at in seen:
-            raise ValueError(f"parameter {i} is in the list twice")
-        seen.add(at)
-        flat += (at, g.data_ptr())
-        flat += [c[i].data_ptr() for c in cols]
-        flat += (0 if low is None else low.data_ptr(), n, int(step))
-        if seeds is not None:
-            flat.append(int(seeds[i]) & 0xFFFFFFFF)
-        flat += (_DTYPE_CODES[g.dtype], 0 if low is None else _DTYPE_CODES[low.dtype])
-    return (_abi._i64 * len(flat))(*flat)
+        return None, None
+    sizes, index = list(map(_numel, params)), _gpu_index(params[0])
+    _check_lists(who, sizes, index, [("param", params, _F32, None), ("grad", grads, _FLOATS, None),
+                                     *columns])
+    at = list(map(_data_ptr, params))
+    if len(set(at)) < count:
+        held = [a for a, n in zip(at, sizes) if n]
+        if len(set(held)) < len(held):
+            raise ValueError(f"{who}: a parameter is in the list twice")
+    low_at = low_dt = [0] * count
+    if lowp_outs is not None:
+        have = [(low, n) for low, n in zip(lowp_outs, sizes) if low is not None]
+        if have:
+            _check_lists(who, [n for _, n in have], index,
+                         [("lowp_out", [low for low, _ in have], _FLOATS, None)])
+            low_at = [0 if low is None else low.data_ptr() for low in lowp_outs]
+            low_dt = [0 if low is None else _DTYPE_CODES[low.dtype] for low in lowp_outs]
+    fields = [at, list(map(_data_ptr, grads)), *(list(map(_data_ptr, c[1])) for c in columns),
+              low_at, sizes, list(map(int, steps))]
+    if seeds is not None:
+        fields.append([int(s) & 0xFFFFFFFF for s in seeds])
+    return index, _rows([*fields, [_DTYPE_CODES[g.dtype] for g in grads], low_dt])
 
 
 def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1: float,
@@ -1089,18 +1123,14 @@ def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1
     device) in one launch for every 56, with the same bits: fp32 ``params``
     and moments, ``grads`` in any of the three types, ``steps`` the step count
     of each, ``lowp_outs`` a 16- or 32-bit copy of each parameter or None."""
-    f32 = torch.float32
-    dev = _tensor_table("adamw_multi", (("param", params, f32, None),
-                                        ("exp_avg", exp_avgs, f32, None),
-                                        ("exp_avg_sq", exp_avg_sqs, f32, None)),
-                        steps, grads, params, lowp_outs)
-    if dev is None:
+    index, table = _step_rows("adamw_multi", [("exp_avg", exp_avgs, _F32, None),
+                                              ("exp_avg_sq", exp_avg_sqs, _F32, None)],
+                              params, grads, steps, lowp_outs)
+    if table is None:
         return
-    table = _step_table((exp_avgs, exp_avg_sqs), params, grads, steps, lowp_outs)
-    with _on(dev.index):
-        check(lib().zk_adamw_multi(table, len(params), float(lr), float(beta1), float(beta2),
-                                   float(eps), float(weight_decay), stream_handle(dev)),
-              "zk_adamw_multi")
+    with _on(index):
+        check(lib().zk_adamw_multi(table.buffer_info()[0], len(params), lr, beta1, beta2, eps,
+                                   weight_decay, _stream(index)), "zk_adamw_multi")
 
 
 ADAMW8_BLOCK = 256  # elements whose 8-bit codes are counted from one base
@@ -1121,21 +1151,15 @@ def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, l
     first to nearest, the second up or down at random with the right mean.
     ``seeds``: an integer for each tensor (mod 2^32) that the random bits come
     from, another for each step."""
-    if len(seeds) != len(params):
-        raise ValueError("adamw8_multi: the lists differ in length")
-    u8 = torch.uint8
-    dev = _tensor_table("adamw8_multi", (("param", params, torch.float32, None),
-                                         ("exp_avg", exp_avgs, u8, None),
-                                         ("exp_avg_sq", exp_avg_sqs, u8, None),
-                                         ("base", bases, torch.int16, _adamw8_base_elems)),
-                        steps, grads, params, lowp_outs)
-    if dev is None:
+    index, table = _step_rows("adamw8_multi", [("exp_avg", exp_avgs, _U8, None),
+                                               ("exp_avg_sq", exp_avg_sqs, _U8, None),
+                                               ("base", bases, _I16, _adamw8_base_elems)],
+                              params, grads, steps, lowp_outs, seeds)
+    if table is None:
         return
-    table = _step_table((exp_avgs, exp_avg_sqs, bases), params, grads, steps, lowp_outs, seeds)
-    with _on(dev.index):
-        check(lib().zk_adamw8_multi(table, len(params), float(lr), float(beta1), float(beta2),
-                                    float(eps), float(weight_decay), stream_handle(dev)),
-              "zk_adamw8_multi")
+    with _on(index):
+        check(lib().zk_adamw8_multi(table.buffer_info()[0], len(params), lr, beta1, beta2, eps,
+                                    weight_decay, _stream(index)), "zk_adamw8_multi")
 
 
 def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.float32, outs=None):
@@ -1149,24 +1173,20 @@ def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.fl
         dtype = outs[0][0].dtype
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"adamw8_values: values are fp32 or bf16 (got {dtype})")
-    u8 = torch.uint8
-    dev = _tensor_table("adamw8_values", (("exp_avg", exp_avgs, u8, None),
-                                          ("exp_avg_sq", exp_avg_sqs, u8, None),
-                                          ("base", bases, torch.int16, _adamw8_base_elems),
-                                          ("first moment", outs[0], dtype, None)),
-                        None, outs[1], exp_avgs, None)
-    if dev is None:
+    count = len(exp_avgs)
+    if any(len(ts) != count for ts in (exp_avg_sqs, bases, *outs)):
+        raise ValueError("adamw8_values: the lists differ in length")
+    if not count:
         return outs
-    if any(t.dtype != dtype for t in outs[1]):
-        raise ValueError(f"adamw8_values: every output must be {dtype}")
-    flat = []
-    for row in zip(exp_avgs, exp_avg_sqs, bases, *outs):
-        flat += [t.data_ptr() for t in row]
-        flat.append(row[0].numel())
-    table = (_abi._i64 * len(flat))(*flat)
-    with _on(dev.index):
-        check(lib().zk_adamw8_values(table, len(exp_avgs), dtype_code(dtype), stream_handle(dev)),
-              "zk_adamw8_values")
+    sizes, index = list(map(_numel, exp_avgs)), _gpu_index(exp_avgs[0])
+    columns = [("exp_avg", exp_avgs, _U8, None), ("exp_avg_sq", exp_avg_sqs, _U8, None),
+               ("base", bases, _I16, _adamw8_base_elems),
+               ("first moment", outs[0], {dtype}, None), ("second moment", outs[1], {dtype}, None)]
+    _check_lists("adamw8_values", sizes, index, columns)
+    table = _rows([*(list(map(_data_ptr, c[1])) for c in columns), sizes])
+    with _on(index):
+        check(lib().zk_adamw8_values(table.buffer_info()[0], count, dtype_code(dtype),
+                                     _stream(index)), "zk_adamw8_values")
     return outs
 
 
