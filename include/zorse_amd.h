@@ -560,8 +560,8 @@ int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const void* k,
 int zk_embedding_fwd(const void* ids, int ids_64, int64_t tokens, const void* w,
                      int64_t vocab, int64_t hidden, void* y, float scale,
                      int w_dtype, int y_dtype, zk_stream_t stream);
-/* Bytes of workspace (16-byte aligned) of the gradient; negative for sizes
- * that it refuses. */
+/* Bytes of workspace (16-byte aligned) of the gradient, 0 where few tokens need
+ * none; negative for sizes that it refuses. */
 int64_t zk_embedding_bwd_workspace(int64_t tokens, int64_t vocab, int64_t hidden);
 int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, const void* dy,
                      int dy_dtype, void* dw, int dw_dtype, int64_t vocab,

@@ -21,13 +21,14 @@ def test_entry_points_refuse():
     assert fwd(None, 1, 4, p, 8, 16, p, 1.0, 0, 0, None) == -1
     assert fwd(p, 1, 4, odd, 8, 16, p, 1.0, 2, 0, None) == -3
     assert fwd(None, 1, 0, None, 8, 16, None, 1.0, 0, 0, None) == 0  # no tokens
-    ws = lib.zk_embedding_bwd_workspace(4, 8, 16)
+    ws = lib.zk_embedding_bwd_workspace(400, 8, 16)
     assert ws > 0 and lib.zk_embedding_bwd_workspace(4, 0, 16) < 0
     assert lib.zk_embedding_bwd_workspace(1 << 29, 8, 16) < 0
-    args = (p, 1, 4, p, 0, p, 0, 8, 16, 1.0, -1, 0)
+    args = (p, 1, 400, p, 0, p, 0, 8, 16, 1.0, -1, 0)
     assert bwd(*args, p, ws - 1, None) == -5
     assert bwd(*args, None, ws, None) == -1
     assert bwd(*args, ctypes.c_void_p(264), ws, None) == -3
+    assert lib.zk_embedding_bwd_workspace(4, 8, 16) == 0  # few tokens need none
     assert bwd(p, 1, 4, None, 0, p, 0, 8, 16, 1.0, -1, 0, p, ws, None) == -1
     assert bwd(p, 1, 4, p, 5, p, 0, 8, 16, 1.0, -1, 0, p, ws, None) == -2
     # nothing to add: no launch

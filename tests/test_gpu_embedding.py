@@ -59,6 +59,8 @@ CASES = [
     ((64,), 512, 7, "one", BF, BF, 1.0, None),
     ((65,), 520, 3, "one", FP, FP, 0.5, None),
     ((5, 77), 100, 257, "uniform", F4, F4, 10.0, None),
+    ((128,), 1030, 61, "zipf", F4, FP, 3.0, None),  # the most that one launch takes
+    ((100,), 24, 5, "outside", FP, FP, 1.0, 4),
     ((129,), 7, 1000, "zipf", BF, F4, 1.0, 0),
     ((3, 43), 1033, 50, "zipf", F4, BF, -2.0, 49),
     ((4097,), 264, 128, "runs", BF, BF, 1.0, None),

@@ -19,6 +19,8 @@
 //      sum (at most two a block: the id it begins with and the id it ends in).
 //      Waves after those write the rows of unused ids.
 //   3. embed_join: the partial sums of ids that cross blocks.
+// Up to kFew tokens take one launch instead, embed_few: every wave holds all
+// ids, two a lane, and finds a row's tokens by comparing.
 #include "part8.h"
 
 namespace zk {
@@ -445,6 +447,74 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
   }
 }
 
+// ------------------------------------------------------------- few tokens ---
+static constexpr int kFew = 128;
+
+// A wave's 512 columns of kFillRows rows or, with kAdd, of the row that a
+// token names first.
+template <typename I, typename D, typename W, bool kAdd>
+__global__ __launch_bounds__(256) void embed_few(
+    const I* __restrict__ ids, int T, const D* __restrict__ dy, W* __restrict__ dw, uint32_t V, int h,
+    int slices, int64_t items, float scale, uint32_t pad) {
+  const int lane = threadIdx.x & 63;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= items) return;
+  const int64_t group = item / slices;
+  const int c = static_cast<int>(item - group * slices) * 512 + lane * 8;
+  const int nc = h - c < 0 ? 0 : h - c;
+  uint32_t key[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int t = k * 64 + lane;
+    key[k] = t < T ? id32(ids, t) : ~0u;
+    key[k] = key[k] < V && key[k] != pad ? key[k] : ~0u;
+  }
+  auto row = [&](uint32_t r, uint64_t m0, uint64_t m1) {
+    W* p = dw + static_cast<int64_t>(r) * h + c;
+    if ((m0 | m1) == 0) {
+      Part8<W>::store_zero_nt(p, nc);
+      return;
+    }
+    Part8<W> old;
+    if (kAdd) old.load(p, nc);
+    float acc[8] = {};
+    constexpr int kAhead = 8;
+    while ((m0 | m1) != 0) {  // the tokens in order
+      Part8<D> x[kAhead];
+      bool on[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        on[k] = (m0 | m1) != 0;
+        const int t = m0 != 0 ? __builtin_ctzll(m0) : 64 + (m1 != 0 ? __builtin_ctzll(m1) : 0);
+        if (m0 != 0) m0 &= m0 - 1;
+        else m1 &= m1 - 1;
+        x[k].load(dy + static_cast<int64_t>(t) * h + c, on[k] ? nc : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += on[k] ? x[k][q] : 0.f;
+      }
+    }
+    float o[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = kAdd ? old[q] + scale * acc[q] : scale * acc[q];
+    Part8<W>::store(p, o, nc);
+  };
+  if (kAdd) {
+    const int t = static_cast<int>(group);
+    const uint32_t r = __builtin_amdgcn_readlane(t < 64 ? key[0] : key[1], t & 63);
+    const uint64_t m0 = __ballot(key[0] == r), m1 = __ballot(key[1] == r);
+    const int first = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
+    if (r != ~0u && first == t) row(r, m0, m1);
+    return;
+  }
+  const uint32_t r0 = static_cast<uint32_t>(group) * kFillRows;
+  for (uint32_t r = r0; r < r0 + kFillRows && r < V; ++r)
+    row(r, __ballot(key[0] == r), __ballot(key[1] == r));
+}
+
 // The groups of embed_sort: at least 256 workgroups, at most kMaxSlots ids each.
 static int sort_log_groups(int64_t V) {
   int lg = 8;
@@ -471,6 +541,7 @@ static int64_t part_row(int64_t h) { return ((h + 31) / 32 | 1) * 32; }
 
 // Workspace: the partial sums, the spans, the grouped tokens, the counts, the total.
 static int64_t embed_ws_bytes(int64_t T, int64_t V, int64_t h) {
+  if (T <= kFew) return 0;
   return embed_blocks(T, h) * (2 * part_row(h) * 4 + 16) + pad_to(T * 8, 16) +
          pad_to(V * 4, 16) + 16;
 }
@@ -503,6 +574,20 @@ static void launch_fwd_w(const void* ids, int64_t T, const void* w, int wdt, int
   if (wdt == ZK_F32) launch_fwd<I, float>(ids, T, w, V, h, y, ydt, scale, st);
   else if (wdt == ZK_BF16) launch_fwd<I, bf16>(ids, T, w, V, h, y, ydt, scale, st);
   else launch_fwd<I, f16>(ids, T, w, V, h, y, ydt, scale, st);
+}
+
+template <typename D, typename W, bool kAdd>
+static void launch_few(const void* ids, int ids_64, int64_t T, const void* dy, void* dw, int64_t V,
+                       int64_t h, float scale, uint32_t pad, hipStream_t st) {
+  const int slices = static_cast<int>((h + 511) / 512);
+  const int64_t items = (kAdd ? T : (V + kFillRows - 1) / kFillRows) * slices;
+  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+#define ZK_FEW(I)                                                                                \
+  hipLaunchKernelGGL((embed_few<I, D, W, kAdd>), grid, dim3(256), 0, st, (const I*)ids,          \
+                     static_cast<int>(T), (const D*)dy, (W*)dw, static_cast<uint32_t>(V),        \
+                     static_cast<int>(h), slices, items, scale, pad)
+  if (ids_64) ZK_FEW(int64_t); else ZK_FEW(int32_t);
+#undef ZK_FEW
 }
 
 template <typename D, typename W, bool kAdd>
@@ -572,15 +657,40 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
              "zk_embedding_bwd: bad size (%lld tokens, table %lld x %lld)", (long long)tokens,
              (long long)vocab, (long long)hidden);
   if (tokens == 0 && accumulate) return ZK_OK;
-  ZK_REQUIRE((tokens == 0 || (ids && dy)) && dw && workspace, ZK_EINVAL,
+  const int64_t needed = embed_ws_bytes(tokens, vocab, hidden);
+  ZK_REQUIRE((tokens == 0 || (ids && dy)) && dw && (needed == 0 || workspace), ZK_EINVAL,
              "zk_embedding_bwd: null pointer");
   ZK_REQUIRE(aligned(ids, ids_64 ? 8 : 4) && aligned(dy, dtype_bytes(dy_dtype)) &&
                  aligned(dw, dtype_bytes(dw_dtype)) && aligned(workspace, 16),
              ZK_EALIGN, "zk_embedding_bwd: tensors must be aligned to their element size, the "
              "workspace to 16 bytes");
-  ZK_REQUIRE(workspace_bytes >= embed_ws_bytes(tokens, vocab, hidden), ZK_EWORKSPACE,
+  ZK_REQUIRE(workspace_bytes >= needed, ZK_EWORKSPACE,
              "zk_embedding_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-             (long long)embed_ws_bytes(tokens, vocab, hidden));
+             (long long)needed);
+  hipStream_t st = as_stream(stream);
+  const uint32_t pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<uint32_t>(padding_idx) : ~0u;
+#define ZK_DTYPES(ZK_G)                            \
+  do {                                             \
+    if (dy_dtype == ZK_F32) ZK_DW(ZK_G, float);    \
+    else if (dy_dtype == ZK_BF16) ZK_DW(ZK_G, bf16); \
+    else ZK_DW(ZK_G, f16);                         \
+  } while (0)
+#define ZK_DW(ZK_G, D)                             \
+  do {                                             \
+    if (dw_dtype == ZK_F32) ZK_G(D, float);        \
+    else if (dw_dtype == ZK_BF16) ZK_G(D, bf16);   \
+    else ZK_G(D, f16);                             \
+  } while (0)
+  if (tokens <= kFew) {
+#define ZK_G(D, W)                                                                               \
+  do {                                                                                           \
+    if (accumulate) launch_few<D, W, true>(ids, ids_64, tokens, dy, dw, vocab, hidden, scale, pad, st); \
+    else launch_few<D, W, false>(ids, ids_64, tokens, dy, dw, vocab, hidden, scale, pad, st);    \
+  } while (0)
+    ZK_DTYPES(ZK_G);
+#undef ZK_G
+    return launch_status("zk_embedding_bwd");
+  }
   char* ws = static_cast<char*>(workspace);
   float* part = reinterpret_cast<float*>(ws);
   ws += embed_blocks(tokens, hidden) * 2 * part_row(hidden) * 4;
@@ -593,10 +703,8 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
   int* total = reinterpret_cast<int*>(ws);
   const int lg = sort_log_groups(vocab);
   const int slots = static_cast<int>((vocab + (int64_t(1) << lg) - 1) >> lg);
-  hipStream_t st = as_stream(stream);
   const dim3 grid(1u << lg), block(64 * kSortWaves);
   const size_t lds = sizeof(int) * kSortWaves * slots;
-  const uint32_t pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<uint32_t>(padding_idx) : ~0u;
   if (ids_64)
     hipLaunchKernelGGL((embed_sort<int64_t>), grid, block, lds, st, (const int64_t*)ids,
                        static_cast<int>(tokens), static_cast<uint32_t>(vocab), lg, slots, pad, tok,
@@ -610,16 +718,9 @@ extern "C" int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, con
     if (accumulate) launch_grad<D, W, true>(dy, dw, tok, count, total, part, span, tokens, vocab, hidden, scale, st); \
     else launch_grad<D, W, false>(dy, dw, tok, count, total, part, span, tokens, vocab, hidden, scale, st); \
   } while (0)
-#define ZK_GW(D)                             \
-  do {                                       \
-    if (dw_dtype == ZK_F32) ZK_G(D, float);  \
-    else if (dw_dtype == ZK_BF16) ZK_G(D, bf16); \
-    else ZK_G(D, f16);                       \
-  } while (0)
-  if (dy_dtype == ZK_F32) ZK_GW(float);
-  else if (dy_dtype == ZK_BF16) ZK_GW(bf16);
-  else ZK_GW(f16);
-#undef ZK_GW
+  ZK_DTYPES(ZK_G);
 #undef ZK_G
+#undef ZK_DW
+#undef ZK_DTYPES
   return launch_status("zk_embedding_bwd");
 }

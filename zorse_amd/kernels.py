@@ -972,11 +972,11 @@ def _embedding_bwd(index, ids, dy, vocab, scale, padding_idx, w_dtype, dw=None, 
     nbytes = _embedding_workspace(tokens, vocab, h)
     if dw is None:
         dw = torch.empty((vocab, h), device=dev, dtype=w_dtype)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     check(lib().zk_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, tokens, dy.data_ptr(),
                                  _DTYPE_CODES[dy.dtype], dw.data_ptr(), _DTYPE_CODES[w_dtype],
                                  vocab, h, scale, -1 if padding_idx is None else padding_idx,
-                                 accumulate, ws.data_ptr(), nbytes, _stream(index)),
+                                 accumulate, ptr(ws), nbytes, _stream(index)),
           "zk_embedding_bwd")
     return dw
 
