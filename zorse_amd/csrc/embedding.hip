@@ -217,9 +217,18 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
 }
 
 // --------------------------------------------------------------- gradient ---
-__device__ __forceinline__ void put_part(float* p, const float (&acc)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+// A wave's columns of a row: `lanes` chunks of 8 a slice.  The row's last chunk
+// ends with the row and may overlap the one before it, lanes behind it repeat
+// it: they read, compute and store the same values in the same instructions.
+// Rows of less than 8 columns are one chunk of h.
+struct Columns {
+  int lanes, slices;  // chosen so that a slice has more than an overlapping chunk:
+                      // two waves may not add to the same column
+};
+__device__ __forceinline__ int my_column(const Columns& cols, int slice, int h) {
+  const int lane = threadIdx.x & 63;
+  const int c = (slice * cols.lanes + (lane < cols.lanes ? lane : cols.lanes - 1)) * 8;
+  return h < 8 ? 0 : c < h - 8 ? c : h - 8;
 }
 
 // part: [blocks][2][hp] fp32 (hp: part_row(h)): the sum of the id that
@@ -231,7 +240,7 @@ template <typename D, typename W, bool kAdd, bool kStream>
 __global__ __launch_bounds__(256) void embed_grad(
     const D* __restrict__ dy, W* __restrict__ dw, const Token* __restrict__ tok,
     const int* __restrict__ count, const int* __restrict__ total, float* __restrict__ part,
-    Span* __restrict__ span, int64_t V, int h, int hp, int slices, int blk, int64_t sum_items,
+    Span* __restrict__ span, int64_t V, int h, int hp, Columns cols, int blk, int64_t sum_items,
     float scale) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
@@ -245,8 +254,8 @@ __global__ __launch_bounds__(256) void embed_grad(
     }
     return;
   }
-  const int64_t j = item / slices;
-  const int c = static_cast<int>(item - j * slices) * 512 + lane * 8;
+  const int64_t j = item / cols.slices;
+  const int c = my_column(cols, static_cast<int>(item - j * cols.slices), h), nc = h < 8 ? h : 8;
   const int n_all = *total;
   const int64_t p0 = j * blk;
   if (p0 >= n_all) {
@@ -264,8 +273,6 @@ __global__ __launch_bounds__(256) void embed_grad(
   const bool head = __builtin_amdgcn_readfirstlane(e.id) == prev;
   const int first_end = __builtin_ctzll(ends);
   const int last_id = __builtin_amdgcn_readlane(e.id, n - 1);
-  const int nc = h - c < 0 ? 0 : h - c;  // columns from here on (lanes without any stay: they
-                                         // hold tokens that the others read)
   if (c == 0) {  // one lane: what embed_join has to add up from this block on
     Span sp = {-1, 0};
     const uint64_t before = ends & ~(1ull << (n - 1));  // where the last id begins
@@ -315,7 +322,7 @@ __global__ __launch_bounds__(256) void embed_grad(
       if (!(ends >> i & 1)) continue;
       const bool begun = head && i == first_end;
       if (begun || (i == n - 1 && last_id == next)) {
-        if (nc > 0) put_part(begun ? pj : pj + hp, acc);
+        Part8<float>::store(begun ? pj : pj + hp, acc, nc);
       } else {
         float o[8];
 #pragma unroll
@@ -455,14 +462,13 @@ static constexpr int kFew = 128;
 template <typename I, typename D, typename W, bool kAdd>
 __global__ __launch_bounds__(256) void embed_few(
     const I* __restrict__ ids, int T, const D* __restrict__ dy, W* __restrict__ dw, uint32_t V, int h,
-    int slices, int64_t items, float scale, uint32_t pad) {
+    Columns cols, int64_t items, float scale, uint32_t pad) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= items) return;
-  const int64_t group = item / slices;
-  const int c = static_cast<int>(item - group * slices) * 512 + lane * 8;
-  const int nc = h - c < 0 ? 0 : h - c;
+  const int64_t group = item / cols.slices;
+  const int c = my_column(cols, static_cast<int>(item - group * cols.slices), h), nc = h < 8 ? h : 8;
   uint32_t key[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(256) void embed_few(
     Part8<W> old;
     if (kAdd) old.load(p, nc);
     float acc[8] = {};
-    constexpr int kAhead = 8;
+    constexpr int kAhead = sizeof(D) == 2 ? 16 : 8;
     while ((m0 | m1) != 0) {  // the tokens in order
       Part8<D> x[kAhead];
       bool on[kAhead];
@@ -489,7 +495,7 @@ __global__ __launch_bounds__(256) void embed_few(
         const int t = m0 != 0 ? __builtin_ctzll(m0) : 64 + (m1 != 0 ? __builtin_ctzll(m1) : 0);
         if (m0 != 0) m0 &= m0 - 1;
         else m1 &= m1 - 1;
-        x[k].load(dy + static_cast<int64_t>(t) * h + c, on[k] ? nc : 0);
+        x[k].load(dy + static_cast<int64_t>(on[k] ? t : 0) * h + c, nc);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
@@ -532,6 +538,13 @@ static int embed_block(int64_t T, int64_t h) {
 static int64_t embed_blocks(int64_t T, int64_t h) {
   const int blk = embed_block(T, h);
   return (T + blk - 1) / blk;
+}
+static Columns columns(int64_t h) {
+  const int64_t chunks = (h + 7) / 8;
+  int lanes = 64;
+  if (h % 8 != 0)
+    while (chunks > lanes && chunks % lanes == 1) --lanes;
+  return Columns{lanes, static_cast<int>((chunks + lanes - 1) / lanes)};
 }
 static int64_t pad_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // Floats of a partial row: two of them are an odd number of 256-byte units, so
@@ -579,13 +592,13 @@ static void launch_fwd_w(const void* ids, int64_t T, const void* w, int wdt, int
 template <typename D, typename W, bool kAdd>
 static void launch_few(const void* ids, int ids_64, int64_t T, const void* dy, void* dw, int64_t V,
                        int64_t h, float scale, uint32_t pad, hipStream_t st) {
-  const int slices = static_cast<int>((h + 511) / 512);
-  const int64_t items = (kAdd ? T : (V + kFillRows - 1) / kFillRows) * slices;
+  const Columns cols = columns(h);
+  const int64_t items = (kAdd ? T : (V + kFillRows - 1) / kFillRows) * cols.slices;
   const dim3 grid(static_cast<unsigned>((items + 3) / 4));
 #define ZK_FEW(I)                                                                                \
   hipLaunchKernelGGL((embed_few<I, D, W, kAdd>), grid, dim3(256), 0, st, (const I*)ids,          \
                      static_cast<int>(T), (const D*)dy, (W*)dw, static_cast<uint32_t>(V),        \
-                     static_cast<int>(h), slices, items, scale, pad)
+                     static_cast<int>(h), cols, items, scale, pad)
   if (ids_64) ZK_FEW(int64_t); else ZK_FEW(int32_t);
 #undef ZK_FEW
 }
@@ -594,14 +607,15 @@ template <typename D, typename W, bool kAdd>
 static void launch_grad(const void* dy, void* dw, const Token* tok, const int* count,
                         const int* total, float* part, Span* span, int64_t T, int64_t V,
                         int64_t h, float scale, hipStream_t st) {
-  const int hp = static_cast<int>(part_row(h)), slices = static_cast<int>((h + 511) / 512);
+  const int hp = static_cast<int>(part_row(h));
+  const Columns cols = columns(h);
   const int blk = embed_block(T, h);
-  const int64_t blocks = embed_blocks(T, h), sums = blocks * slices;
+  const int64_t blocks = embed_blocks(T, h), sums = blocks * cols.slices;
   const int64_t items = sums + (kAdd ? 0 : (V + kFillRows - 1) / kFillRows);
   const dim3 grid(static_cast<unsigned>((items + 3) / 4));
 #define ZK_GRAD(S)                                                                            \
   hipLaunchKernelGGL((embed_grad<D, W, kAdd, S>), grid, dim3(256), 0, st, (const D*)dy, (W*)dw, \
-                     tok, count, total, part, span, V, static_cast<int>(h), hp, slices, blk, sums, scale)
+                     tok, count, total, part, span, V, static_cast<int>(h), hp, cols, blk, sums, scale)
   // dy within the 256 MB of last-level cache may still be there from the kernel
   // that wrote it.  us with streaming loads / ordinary ones: 65536 tokens of
   // 5120 (671 MB), a text's ids 337 / 348, nine tenths one id 361 / 427; 8192 of

@@ -1,9 +1,13 @@
-// Up to 8 neighbouring elements of a row that may start at any element: one
-// 16-byte access (two for fp32) where all 8 are there, element accesses at a
-// row's ragged end.  The vector types carry the alignment of one element, so
-// the compiler may use wide accesses only as the target allows them unaligned
-// (gfx950's global memory does), and rows of odd widths need no kernel of
-// their own.
+// 8 neighbouring elements of a row that may start at any element, or the first n
+// of them.  The vector types carry the alignment of one element, so the compiler
+// may use wide accesses only as the target allows them unaligned (gfx950's
+// global memory does), and rows of odd widths need no kernel of their own.
+//
+// A row's ragged end: where lanes of one wave take different paths in load(),
+// the element path writes registers that the other lanes' wide load still has
+// to fill, and the wave waits for it -- one load in flight instead of many.  So
+// n should be the same for all lanes: kernels let the last chunk of a row
+// overlap the one before it instead (ragged rows of 8 and more).
 #pragma once
 #include "zk_common.h"
 

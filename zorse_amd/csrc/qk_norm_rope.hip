@@ -45,8 +45,11 @@ struct QkArgs {
   float eps;
 };
 
-// One lane's 8 pairs of a row: elements i and i + half of the half-split
-// pairing, 2i and 2i + 1 of the interleaved one; n of them exist.
+// One lane's 8 pairs of a row from pair i0 on: elements i and i + half of the
+// half-split pairing, 2i and 2i + 1 of the interleaved one.  Every lane loads 8
+// pairs that exist (n of them where a row has fewer, in all lanes): a row's last
+// lane takes its last 8 and leaves the first `skip` of them, which are another
+// lane's, out of the sums and the stores; a lane behind it leaves all out.
 template <typename T, int kPairing>
 struct Pairs {
   Part8<T> a, b;
@@ -59,6 +62,22 @@ struct Pairs {
       b.load(row + 2 * i0 + 8, 2 * n - 8);
     }
   }
+  __device__ __forceinline__ void drop(int skip) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool out = i < skip;
+      if (kPairing == ZK_ROPE_HALF) {
+        a.u[i] = out ? static_cast<T>(0.f) : a.u[i];
+        b.u[i] = out ? static_cast<T>(0.f) : b.u[i];
+      } else if (i < 4) {
+        a.u[2 * i] = out ? static_cast<T>(0.f) : a.u[2 * i];
+        a.u[2 * i + 1] = out ? static_cast<T>(0.f) : a.u[2 * i + 1];
+      } else {
+        b.u[2 * i - 8] = out ? static_cast<T>(0.f) : b.u[2 * i - 8];
+        b.u[2 * i - 7] = out ? static_cast<T>(0.f) : b.u[2 * i - 7];
+      }
+    }
+  }
   // the pairs' first and second elements
   __device__ __forceinline__ float first(int i) const {
     return kPairing == ZK_ROPE_HALF ? a[i] : i < 4 ? a[2 * i] : b[2 * i - 8];
@@ -67,16 +86,25 @@ struct Pairs {
     return kPairing == ZK_ROPE_HALF ? b[i] : i < 4 ? a[2 * i + 1] : b[2 * i - 7];
   }
   static __device__ __forceinline__ void store(T* row, const float (&u)[8], const float (&v)[8],
-                                               int i0, int half, int n) {
-    if (kPairing == ZK_ROPE_HALF) {
-      Part8<T>::store(row + i0, u, n);
-      Part8<T>::store(row + half + i0, v, n);
-    } else {
-      const float lo[8] = {u[0], v[0], u[1], v[1], u[2], v[2], u[3], v[3]};
-      const float hi[8] = {u[4], v[4], u[5], v[5], u[6], v[6], u[7], v[7]};
-      Part8<T>::store(row + 2 * i0, lo, 2 * n);
-      Part8<T>::store(row + 2 * i0 + 8, hi, 2 * n - 8);
+                                               int i0, int half, int skip, int n) {
+    if (skip == 0 && n == 8) {
+      if (kPairing == ZK_ROPE_HALF) {
+        Part8<T>::store(row + i0, u, 8);
+        Part8<T>::store(row + half + i0, v, 8);
+      } else {
+        const float lo[8] = {u[0], v[0], u[1], v[1], u[2], v[2], u[3], v[3]};
+        const float hi[8] = {u[4], v[4], u[5], v[5], u[6], v[6], u[7], v[7]};
+        Part8<T>::store(row + 2 * i0, lo, 8);
+        Part8<T>::store(row + 2 * i0 + 8, hi, 8);
+      }
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i >= skip && i < n) {
+        row[kPairing == ZK_ROPE_HALF ? i0 + i : 2 * (i0 + i)] = static_cast<T>(u[i]);
+        row[kPairing == ZK_ROPE_HALF ? half + i0 + i : 2 * (i0 + i) + 1] = static_cast<T>(v[i]);
+      }
   }
 };
 
@@ -141,8 +169,11 @@ __global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
   const QkSide& X = is_q ? A.q : A.k;
   const int64_t wg = is_q ? blockIdx.x : blockIdx.x - A.q.wgs;
   const int half = A.d / 2, lanes = 1 << log_g;
-  const int i0 = (lane & (lanes - 1)) * 8;
-  const int n = half - i0 < 0 ? 0 : half - i0 < 8 ? half - i0 : 8;
+  const int my0 = (lane & (lanes - 1)) * 8;            // this lane's first pair, if all were there
+  const int n = half < 8 ? half : 8;
+  const int i0 = half < 8 ? 0 : my0 < half - 8 ? my0 : half - 8;
+  const int skip = my0 - i0 < 8 ? my0 - i0 : 8;
+  const bool ragged = (half & 7) != 0 || lanes * 8 != half;
   const int slot = lane >> log_g;                      // row slot of this lane
   const int log_ppw = 6 - log_g - X.log_hpw;           // positions a wave holds
   const int h0 = slot & ((1 << X.log_hpw) - 1), p_in = slot >> X.log_hpw;
@@ -158,37 +189,39 @@ __global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
     const int64_t group = X.splits == 1 ? item : item / X.splits;
     const int split = X.splits == 1 ? 0 : static_cast<int>(item - group * X.splits);
     const int64_t p = (group << log_ppw) + p_in;
-    const bool in = p < A.rows && n > 0;
+    const bool in = p < A.rows;
     const int64_t b = in ? p / A.S : 0, s = in ? p - b * A.S : 0;
-    int h = (split << X.log_hpw) + h0;
+    // a slot without a position reads the first one's rows; every slot has a
+    // head (2^log_hpw divides their number)
+    const int h = (split << X.log_hpw) + h0;
     const T* xr = static_cast<const T*>(X.x) + b * X.x_sb + s * X.x_ss + h * X.x_sh;
     const T* gr = static_cast<const T*>(X.dy) + (kBwd ? b * X.dy_sb + s * X.dy_ss + h * X.dy_sh : 0);
     T* yr = static_cast<T*>(X.out) + b * X.o_sb + s * X.o_ss + h * X.o_sh;
-    bool on = in && h < X.heads;
     Pairs<T, kPairing> x, g;
-    x.load(xr, i0, half, on ? n : 0);
-    if (kBwd) g.load(gr, i0, half, on ? n : 0);
+    x.load(xr, i0, half, n);
+    if (kBwd) g.load(gr, i0, half, n);
     int64_t pos = s;
     if (A.positions != nullptr && in) pos = A.positions[b * A.pos_sb + s];
     const bool known = pos >= 0 && pos < A.n_pos;  // rows off the table are NaN
     Part8<float> cs, sn;
-    cs.load(A.cosT + (known ? pos : 0) * half + i0, in ? n : 0);
-    sn.load(A.sinT + (known ? pos : 0) * half + i0, in ? n : 0);
+    cs.load(A.cosT + (known ? pos : 0) * half + i0, n);
+    sn.load(A.sinT + (known ? pos : 0) * half + i0, n);
     float c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = known ? cs[i] : __builtin_nanf("");
     for (int hb = split << X.log_hpw; hb < X.heads; hb += step) {
-      const bool now = on;
       Pairs<T, kPairing> x1 = x, g1 = g;
-      h += step;
-      on = in && h < X.heads;
       if (hb + step < X.heads) {  // the next step's rows, ahead of this one's work
         xr += step * X.x_sh;
-        x.load(xr, i0, half, on ? n : 0);
+        x.load(xr, i0, half, n);
         if (kBwd) {
           gr += step * X.dy_sh;
-          g.load(gr, i0, half, on ? n : 0);
+          g.load(gr, i0, half, n);
         }
+      }
+      if (ragged) {
+        x1.drop(skip);
+        if (kBwd) g1.drop(skip);
       }
       float ss = 0.f, t = 0.f, ga[8], gb[8];
 #pragma unroll
@@ -217,7 +250,7 @@ __global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float u = x1.first(i), v = x1.second(i);
-          if (now) {
+          if (in) {
             da[i] = fmaf(ga[i], u * r, da[i]);
             db[i] = fmaf(gb[i], v * r, db[i]);
           }
@@ -225,7 +258,7 @@ __global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
           ob[i] = r * fmaf(-t, v, gb[i] * wb[i]);
         }
       }
-      if (now) Pairs<T, kPairing>::store(yr, oa, ob, i0, half, n);
+      if (in) Pairs<T, kPairing>::store(yr, oa, ob, i0, half, skip, n);
       yr += step * X.o_sh;
     }
   }
@@ -233,12 +266,13 @@ __global__ __launch_bounds__(256, 3) void qk_kernel(QkArgs A, int log_g) {
   // dw: this workgroup's row of partial sums, of 4 waves' row slots in order.
   // A slot's 16 * lanes values in LDS: the pairs' first elements, the second.
   __shared__ float sums[4][1024];
-  float* mine = sums[wave] + slot * 16 * lanes + i0;
+  float* mine = sums[wave] + slot * 16 * lanes;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    mine[i] = da[i];
-    mine[8 * lanes + i] = db[i];
-  }
+  for (int i = 0; i < 8; ++i)
+    if (i >= skip) {  // pair i0 + i < 8 lanes
+      mine[i0 + i] = da[i];
+      mine[8 * lanes + i0 + i] = db[i];
+    }
   __syncthreads();
   for (int i = threadIdx.x; i < A.d; i += 256) {
     int at;
@@ -288,21 +322,17 @@ static constexpr int64_t kBwdWgs = 768;
 // What a group's positions, cos and sin cost a wave, in steps through heads.
 static constexpr int64_t kStart = 2;
 
-// A wave's row slots hold as many heads of a position at a time as leave the
-// fewest slots without a row over all of them (32 or 8 heads in 8 slots: 8; 5:
-// 1, of eight positions), the most where several do.
+// A wave's row slots hold 2^log_hpw heads of a position at a time: the largest
+// power of two that divides the heads (32 and 8 heads in 8 slots: 8; 12: 4, of
+// two positions; 5: 1, of eight), so that no slot is without a row.
 static int heads_a_wave(int64_t heads, int slots_log) {
-  auto used = [&](int lh) { return (heads + (int64_t(1) << lh) - 1) >> lh << lh; };
-  int best = 0;
-  for (int lh = 1; lh <= slots_log; ++lh)
-    if (used(lh) <= used(best)) best = lh;
-  return best;
+  int lh = 0;
+  while (lh < slots_log && heads % (int64_t(2) << lh) == 0) ++lh;
+  return lh;
 }
 
 // Steps of a wave through one group of positions, and the groups.
-static int64_t steps_of(const QkSide& s) {
-  return (s.heads + (int64_t(1) << s.log_hpw) - 1) >> s.log_hpw;
-}
+static int64_t steps_of(const QkSide& s) { return s.heads >> s.log_hpw; }
 
 static void plan(QkArgs& A, int64_t Hq, int64_t Hkv, int log_g, bool bwd) {
   int64_t work[2] = {0, 0};
