@@ -102,3 +102,23 @@ def test_states_keep_their_types_through_a_checkpoint():
             wrong.load_state_dict(opt.state_dict())
     with pytest.raises(ValueError, match="state_bits"):
         optim.FusedAdamW([p], state_bits=16)
+
+
+def test_spans_that_meet():
+    meet = kernels.spans_meet
+    assert not meet([], [], 4) and not meet([0, 0, 0], [0, 0, 0], 4) and not meet([64], [8], 4)
+    assert not meet([64, 32, 96], [8, 8, 1], 4) and not meet([64, 64], [8, 0], 4)
+    assert meet([64, 64], [8, 8], 4) and meet([64, 32], [8, 9], 4) and meet([96, 0, 64], [1, 1, 9], 4)
+    assert meet([0, 4, 100], [100, 0, 1], 4)
+
+
+def test_step_counts_load_as_torch_loads_them():
+    """torch.optim.Adam's, whose step count is a tensor (left to torch to place)."""
+    p = torch.nn.Parameter(torch.randn(6))
+    opt = torch.optim.Adam([p])
+    p.grad = torch.ones(6)
+    opt.step()
+    ours = optim.FusedAdamW([p])
+    ours.load_state_dict(opt.state_dict())
+    assert int(ours.state[p]["step"]) == 1
+    assert torch.equal(ours.state[p]["exp_avg"], opt.state[p]["exp_avg"])

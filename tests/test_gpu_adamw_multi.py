@@ -318,3 +318,37 @@ def test_large_tensors_among_small_ones(dev):
     assert np.array_equal(base[0][-3:].cpu().numpy(), wb)
     assert not bool(cm[0][:-tail].any()) and not bool(cv[0][:-tail].any())
     assert not bool(p[:-tail].any()) and bool(p[-tail:].all())
+
+
+def test_parameters_that_share_memory(dev):
+    """Overlapping parameters: refused in a list, stepped one after another by
+    the optimizer, as by steps of each; neighbours that only touch are a list.
+    A list that is refused leaves the step counts."""
+    from zorse_amd import kernels
+    from zorse_amd.optim import FusedAdamW
+    flat = torch.linspace(-1, 1, 64, device=dev)
+    p, gr, m, v, _ = _lists(dev, [40, 40], F4, None)
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.adamw_multi([flat[:40], flat[24:]], gr, m, v, [1, 1], **H)
+    kernels.adamw_multi([flat[:24], flat[24:]], [gr[0][:24], gr[1]], [m[0][:24], m[1]],
+                        [v[0][:24], v[1]], [1, 1], **H)
+    for bits in (32, 8):
+        got, want = flat.clone(), flat.clone()
+        a, b = ([torch.nn.Parameter(t[:40]), torch.nn.Parameter(t[24:])] for t in (got, want))
+        oa, ob = (FusedAdamW(x, lr=1e-2, state_bits=bits) for x in (a, b))
+        for x, y in zip(a, b):
+            assert x.data_ptr() in (got.data_ptr(), got[24:].data_ptr())
+            x.grad = torch.randn_like(x)
+            y.grad = x.grad.clone()
+        oa.step()
+        for y in b:
+            ob.step_param(y)
+        assert torch.equal(got, want)
+        c = [torch.nn.Parameter(torch.zeros(8, device=dev)) for _ in range(2)]
+        oc = FusedAdamW(c, state_bits=bits)
+        for x in c:
+            x.grad = torch.ones_like(x)
+        oc.param_groups[0]["lr"] = float("nan")
+        with pytest.raises(RuntimeError, match="range"):
+            oc.step()
+        assert [oc.state[x]["step"] for x in c] == [0, 0] and not bool(c[0].any())

@@ -1071,6 +1071,18 @@ def _check_lists(who: str, sizes, index: int, columns) -> None:
                                  f"with {want[i]} elements on cuda:{index}")
 
 
+def spans_meet(at, sizes, itemsize: int) -> bool:
+    """Whether any two of the tensors with these addresses and numbers of
+    elements share memory: they can't be stepped in one launch."""
+    end = 0
+    for a, n in sorted(zip(at, sizes)):
+        if n:
+            if a < end:
+                return True
+            end = a + n * itemsize
+    return False
+
+
 def _rows(columns) -> array.array:
     """The columns (lists of integers) as rows of 64-bit fields."""
     n = len(columns)
@@ -1098,10 +1110,8 @@ def _step_rows(who, columns, params, grads, steps, lowp_outs, seeds=None):
     _check_lists(who, sizes, index, [("param", params, _F32, None), ("grad", grads, _FLOATS, None),
                                      *columns])
     at = list(map(_data_ptr, params))
-    if len(set(at)) < count:
-        held = [a for a, n in zip(at, sizes) if n]
-        if len(set(held)) < len(held):
-            raise ValueError(f"{who}: a parameter is in the list twice")
+    if spans_meet(at, sizes, 4):
+        raise ValueError(f"{who}: a parameter is in the list twice, or parameters overlap")
     low_at = low_dt = [0] * count
     if lowp_outs is not None:
         have = [(low, n) for low, n in zip(lowp_outs, sizes) if low is not None]

@@ -144,8 +144,9 @@ class FusedAdamW(torch.optim.Optimizer):
         self._stepped(p)
 
     def _step_list(self, group: dict, params: list) -> None:
-        # one parameter, or parameters that share their memory: one by one
-        shared = len({p.data_ptr() for p in params}) < len(params)
+        # one parameter, or parameters that share memory: one by one
+        shared = len(params) > 1 and K.spans_meet(
+            [p.data_ptr() for p in params], [p.numel() * p.element_size() for p in params], 1)
         if (len(params) == 1 or shared) and self.state_bits == 32:
             for p in params:
                 self._step_one(group, p)
@@ -155,19 +156,19 @@ class FusedAdamW(torch.optim.Optimizer):
                 self._step_list(group, [p])
             return
         states = [self._checked(p) for p in params]
-        for st in states:
-            st["step"] += 1
         masters = [st.get("master") for st in states]
         args = ([p if m is None else m for p, m in zip(params, masters)],
                 [p.grad for p in params], [st["exp_avg"] for st in states],
                 [st["exp_avg_sq"] for st in states])
-        steps = [st["step"] for st in states]
+        steps = [st["step"] + 1 for st in states]
         lows = [None if m is None else p for p, m in zip(params, masters)]
         if self.state_bits == 8:
             K.adamw8_multi(*args, [st["exp_base"] for st in states], steps, lowp_outs=lows,
                            seeds=self._seeds(params, steps), **self._hyper(group))
         else:
             K.adamw_multi(*args, steps, lowp_outs=lows, **self._hyper(group))
+        for st, t in zip(states, steps):  # a refused list has not been stepped
+            st["step"] = t
         for p in params:
             self._stepped(p)
 
@@ -185,7 +186,7 @@ class FusedAdamW(torch.optim.Optimizer):
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for key, p in zip(keys, params):
             for name, t in saved.get(key, {}).items():
-                if torch.is_tensor(t):
+                if torch.is_tensor(t) and name != "step":
                     self.state[p][name] = t.detach().to(device=p.device, copy=True)
 
     def master_param(self, p: torch.Tensor) -> torch.Tensor:
