@@ -207,3 +207,27 @@ def test_model_embedding_module(dev):
     y.backward(dy)
     ref, terms, _ = _reference(ids.cpu(), dy.cpu(), 64, 1.0, 3)
     assert bool(((m.weight.grad.cpu().double() - ref).abs() <= _bound(ref, terms, F4)).all())
+
+
+def test_gradient_is_differentiable(dev):
+    """A second differentiation (create_graph): the table's gradient is linear
+    in dy, its own gradient the lookup, and zero for tokens without one."""
+    from zorse_amd import functional
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(-2, 14, (5, 40), generator=g).to(dev)
+    w = torch.randn(12, 24, generator=g).to(dev).requires_grad_()
+    dy = torch.randn(5, 40, 24, generator=g).to(dev).requires_grad_()
+    a = torch.randn(12, 24, generator=g).to(dev).requires_grad_()
+    for scale, pad in ((1.0, None), (0.5, 4)):
+        y = functional.embedding(ids, w, scale=scale, padding_idx=pad)
+        plain, = torch.autograd.grad(y, w, dy.detach(), retain_graph=True)
+        dw, = torch.autograd.grad(y, w, dy, create_graph=True)
+        assert torch.equal(dw, plain)
+        ddy, = torch.autograd.grad(dw, dy, a, create_graph=True)
+        ok = (ids >= 0) & (ids < 12)
+        if pad is not None:
+            ok &= ids != pad
+        want = torch.where(ok.unsqueeze(-1), scale * a[ids.clamp(0, 11)], 0.0)
+        assert torch.equal(ddy, want)
+        da, = torch.autograd.grad(ddy, a, dy.detach())  # linear in a: dw again
+        assert torch.equal(da, plain)

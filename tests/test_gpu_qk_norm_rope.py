@@ -253,3 +253,14 @@ def test_captured_pass_replays_with_new_values(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_second_differentiation_is_refused(dev):
+    from zorse_amd import functional
+    q = torch.randn(1, 3, 2, 16, device=dev, requires_grad=True)
+    w = torch.ones(16, device=dev, requires_grad=True)
+    cos, sin = (t.to(dev) for t in _tables(3, 16))
+    y, _ = functional.qk_norm_rope(q, None, w, None, cos, sin)
+    dq, = torch.autograd.grad(y, q, torch.ones_like(y, requires_grad=True), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        dq.sum().backward()

@@ -9,6 +9,7 @@ there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 
@@ -16,6 +17,7 @@ import torch  # noqa: F401  (must precede the library load: shared HIP runtime)
 
 LIB_NAME = "libzorse_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
+NODES_PATH = os.path.join(os.path.dirname(LIB_PATH), "_nodes.so")
 
 ZK_F32, ZK_F16, ZK_BF16 = 0, 1, 2
 ZK_ROPE_HALF, ZK_ROPE_INTERLEAVED = 0, 1
@@ -194,6 +196,24 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+_nodes = None
+
+
+def nodes():
+    """Load (once) and return the module of csrc/nodes.cpp: autograd nodes and
+    tables for torch's C++ side, over the same library."""
+    global _nodes
+    if _nodes is None:
+        lib()
+        if not os.path.exists(NODES_PATH):
+            raise RuntimeError(
+                f"{NODES_PATH} is missing: build it with "
+                "`python -m zorse_amd.build` (or __graft_entry__.build())"
+            )
+        _nodes = importlib.import_module("._nodes", __package__)
+    return _nodes
 
 
 def exported_symbols() -> list[str]:

@@ -1,10 +1,13 @@
-"""Build recipe for libzorse_amd.so (gfx950).
+"""Build recipe for libzorse_amd.so (gfx950) and the torch module beside it.
 
 Each ``csrc/*.hip`` file is compiled to an object with hipcc (in parallel),
 then linked into ``zorse_amd/libzorse_amd.so``.  The library depends only on
 the HIP runtime; when it is loaded after ``import torch`` the dynamic loader
 binds it to the HIP runtime torch already mapped (same SONAME), so torch's
 streams and allocations are shared with the kernels.
+
+``csrc/nodes.cpp`` is host code against torch's headers and becomes
+``zorse_amd/_nodes.so``, which is linked to the library beside it.
 
 Usage: ``python -m zorse_amd.build`` or ``zorse_amd.build.build()``.
 """
@@ -15,11 +18,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libzorse_amd.so")
+NODES_PATH = os.path.join(PKG_DIR, "_nodes.so")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -76,9 +81,23 @@ def sources() -> list[str]:
     )
 
 
+def _nodes_commands(obj: str, out: str) -> tuple[list[str], list[str]]:
+    """Compiling csrc/nodes.cpp, and linking it to torch and the library."""
+    from torch.utils import cpp_extension as ext
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    includes = [*ext.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include"]
+    compile_ = [cxx, "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                *(f for p in includes for f in ("-isystem", p)), "-c",
+                os.path.join(CSRC, "nodes.cpp"), "-o", obj]
+    link = [cxx, "-shared", "-o", out, obj, *(f"-L{p}" for p in ext.library_paths()), "-lc10",
+            "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{PKG_DIR}",
+            f"-l:{os.path.basename(LIB_PATH)}", "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile every kernel source and link the shared library.  Always
-    rebuilds (the driver's build check compiles from source each time)."""
+    """Compile every kernel source and link the shared library, then the torch
+    module.  Always rebuilds."""
     hipcc = _hipcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
@@ -94,14 +113,20 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         _run(cmd)
         return obj
 
+    nodes_obj = os.path.join(OBJ_DIR, "nodes.o")
+    nodes_compile, nodes_link = _nodes_commands(nodes_obj, NODES_PATH + ".tmp")
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        nodes = ex.submit(_run, nodes_compile)
         list(ex.map(compile_one, zip(srcs, objs)))
+        nodes.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     _run(cmd)
     os.replace(tmp, LIB_PATH)
+    _run(nodes_link)
+    os.replace(NODES_PATH + ".tmp", NODES_PATH)
     return LIB_PATH
 
 

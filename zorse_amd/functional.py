@@ -1,5 +1,6 @@
 """Autograd functions over the HIP kernels (RMSNorm, RoPE + flash attention,
-SwiGLU, token embedding, the norm of query and key heads), usable on their own; the fused decoder layer lives in ``layer.py``.
+SwiGLU, token embedding, the norm of query and key heads), usable on their own;
+the fused decoder layer lives in ``layer.py``.
 
 RoPE tables are built once per (S, d, theta, pairing, dtype, device) with the
 reference's formula (models/llama_simple.py:75-81, 115-137: inv_freq and the
@@ -9,12 +10,14 @@ which stays fp32) and handed to the kernel as fp32 [S, d/2] tables.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import threading
 
 import torch
 
 from . import kernels as K
+from ._abi import nodes
 
 
 # ------------------------------------------------------------- RoPE tables --
@@ -102,23 +105,6 @@ def swiglu(g, u):
 
 # -------------------------------------------------------- Token embedding --
 
-class EmbeddingFunction(torch.autograd.Function):
-    """y = round(scale * weight[ids]); the whole table's gradient."""
-
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx, dtype):
-        ctx.save_for_backward(ids)
-        ctx.cfg = (weight.shape[0], scale, padding_idx, weight.dtype)
-        return K.embedding_fwd(ids, weight, scale=scale, dtype=dtype)
-
-    @staticmethod
-    def backward(ctx, dy):
-        # autograd hands on a gradient of y's shape, type and device, with that
-        # device current
-        dw = K._embedding_bwd(dy.get_device(), ctx.saved_tensors[0], dy.contiguous(), *ctx.cfg)
-        return None, dw, None, None, None
-
-
 def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     """Rows of a token table: scale * weight[ids] as [*ids.shape, hidden] in
     ``dtype`` (default the table's).  ids int32 / int64; an id outside
@@ -130,42 +116,18 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
             raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
         padding_idx %= weight.shape[0]
     ids, scale = ids.contiguous(), float(scale)
+    weight = weight.contiguous()
     if not (weight.requires_grad and torch.is_grad_enabled()):
-        return K.embedding_fwd(ids, weight.contiguous(), scale=scale, dtype=dtype)
-    return EmbeddingFunction.apply(ids, weight.contiguous(), scale, padding_idx, dtype)
+        return K.embedding_fwd(ids, weight, scale=scale, dtype=dtype)
+    _, _, y_code = K.embedding_checked(ids, weight, dtype or weight.dtype)
+    return nodes().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx, y_code)
 
 
 # ----------------------------------------- Norm of q and k heads, rotation --
 
 def _unit_rows(t):
-    """t with unit stride along its last dim (an expanded gradient has none)."""
+    """t with unit stride along its last dim (expanded heads have none)."""
     return t if t is None or t.stride(-1) == 1 else t.contiguous()
-
-
-class QkNormRopeFunction(torch.autograd.Function):
-    """RMS norm and rotation of every q and k head; saves its inputs only."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.cfg = (eps, interleaved)
-        # the descriptor is the backward's too where the gradients are contiguous
-        qo, ko, ctx.desc = K._qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps,
-                                     interleaved)
-        return qo, ko
-
-    @staticmethod
-    def backward(ctx, dq_out, dk_out):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        if dq_out.is_contiguous() and (k is None or dk_out.is_contiguous()):
-            grads = K._qk_bwd(ctx.desc, q.get_device(), dq_out, dk_out, q, k, q_weight, k_weight,
-                              cos, sin, positions, K._empty_qk(q, k))
-        else:
-            eps, interleaved = ctx.cfg
-            grads = K.qk_norm_rope_bwd(_unit_rows(dq_out), _unit_rows(dk_out), q, k, q_weight,
-                                       k_weight, cos, sin, positions=positions, eps=eps,
-                                       interleaved=interleaved)
-        return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6,
@@ -176,11 +138,15 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6
     tables (rope_tables(..., torch.float32, ...)); ``positions`` int64 [S] or
     [B, S], default 0 .. S-1; a position outside the tables gives NaN.  Any even
     d up to 1024; q and k may be views of one q|k|v buffer."""
-    args = (_unit_rows(q), _unit_rows(k), q_weight, k_weight, cos, sin, positions, float(eps),
-            bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
-        return QkNormRopeFunction.apply(*args)
-    return K._qk_fwd(*args)[:2]
+    q, k = _unit_rows(q), _unit_rows(k)
+    heads = (q, k, q_weight, k_weight)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in heads)):
+        return K.qk_norm_rope_fwd(*heads, cos, sin, positions=positions, eps=eps,
+                                  interleaved=interleaved)
+    # the node saves its inputs only, and takes the norm from them again
+    _, desc = K.qk_checked(*heads, cos, sin, positions, eps, interleaved)
+    out = nodes().qk_norm_rope(*heads, cos, sin, positions, ctypes.addressof(desc))
+    return (out[0], None) if k is None else tuple(out)
 
 
 # -------------------------------------------------------------- Attention --

@@ -9,7 +9,6 @@ GPU tensor these functions raise.
 """
 from __future__ import annotations
 
-import array
 import contextlib
 import functools
 import math
@@ -578,8 +577,8 @@ def _qk_out(name, x, t):
     return st
 
 
-def _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs=None,
-             grads=(None, None)):
+def qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs=None,
+               grads=(None, None)):
     """The checks of both directions; (device index, zk_qk_desc).  ``outs`` are
     y or dx (None: new contiguous tensors), ``grads`` dy of q and k."""
     if q.dim() != 4:
@@ -650,19 +649,14 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps:
     sin: fp32 [n_pos, d/2] tables; ``positions`` int64 [S] or [B, S] (default
     0 .. S-1), those outside the tables giving rows of NaN.  fp32 inside, one
     rounding."""
-    return _qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)[:2]
-
-
-def _qk_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out=None):
-    """(q', k', the descriptor)."""
-    index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
+    index, desc = qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
     qo, ko = _empty_qk(q, k) if out is None else out
     with _on(index):
         check(lib().zk_qk_norm_rope_fwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
                                         ptr(k_weight), qo.data_ptr(), ptr(ko), cos.data_ptr(),
                                         sin.data_ptr(), ptr(positions), _stream(index)),
               "zk_qk_norm_rope_fwd")
-    return qo, ko, desc
+    return qo, ko
 
 
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, positions=None,
@@ -673,31 +667,20 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, posi
     themselves.  The weights' gradients are summed in fp32 in one order."""
     if dq_out is None or (dk_out is None) != (k is None):
         raise ValueError("a gradient for each of q and k is needed")
-    index, desc = _qk_desc(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
+    index, desc = qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
                            (dq_out, dk_out))
-    out = _empty_qk(q, k) if out is None else out
+    dq, dk = _empty_qk(q, k) if out is None else out
+    nbytes = lib().zk_qk_norm_rope_bwd_workspace(desc.d)
+    dwq = torch.empty_like(q_weight)
+    dwk = None if k is None else torch.empty_like(k_weight)
     with _on(index):
-        return _qk_bwd(desc, index, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions,
-                       out)
-
-
-@functools.lru_cache(maxsize=1024)
-def _qk_workspace(d: int) -> int:
-    return lib().zk_qk_norm_rope_bwd_workspace(d)
-
-
-def _qk_bwd(desc, index, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, out):
-    """The launches, for checked arguments, on the current device."""
-    dq, dk = out
-    dev, nbytes = q.device, _qk_workspace(desc.d)
-    dwq = torch.empty(desc.d, device=dev, dtype=q_weight.dtype)
-    dwk = None if k is None else torch.empty(desc.d, device=dev, dtype=q_weight.dtype)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    check(lib().zk_qk_norm_rope_bwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(), ptr(k_weight),
-                                    dq_out.data_ptr(), ptr(dk_out), dq.data_ptr(), ptr(dk),
-                                    dwq.data_ptr(), ptr(dwk), cos.data_ptr(), sin.data_ptr(),
-                                    ptr(positions), ws.data_ptr(), nbytes, _stream(index)),
-          "zk_qk_norm_rope_bwd")
+        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+        check(lib().zk_qk_norm_rope_bwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
+                                        ptr(k_weight), dq_out.data_ptr(), ptr(dk_out),
+                                        dq.data_ptr(), ptr(dk), dwq.data_ptr(), ptr(dwk),
+                                        cos.data_ptr(), sin.data_ptr(), ptr(positions),
+                                        ws.data_ptr(), nbytes, _stream(index)),
+              "zk_qk_norm_rope_bwd")
     return dq, dk, dwq, dwk
 
 
@@ -894,11 +877,21 @@ def _check_transposed(transposed, q, k):
 
 # -------------------------------------------------------------- Embedding --
 
-def _embedding_ids(ids: torch.Tensor) -> int:
+def _embedding_ids(ids: torch.Tensor) -> None:
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"token ids must be int32 or int64 (got {ids.dtype})")
     _require_contig("ids", ids)
-    return int(ids.dtype == torch.int64)
+
+
+def embedding_checked(ids, weight, dtype, out=None):
+    """The forward's checks; (device index, the codes of the table's type and of
+    ``dtype``)."""
+    index = _device_index(ids, (weight, out))
+    _embedding_ids(ids)
+    if weight.dim() != 2 or not weight.numel():
+        raise ValueError(f"weight must be a [vocab, hidden] table, got {tuple(weight.shape)}")
+    _require_contig("weight", weight)
+    return index, _float_code("weight", weight.dtype), _float_code("output", dtype)
 
 
 def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
@@ -907,33 +900,19 @@ def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0
     """round(scale * weight[ids]) in ``dtype`` (default the table's): ids
     int32 / int64 of any shape, weight [vocab, hidden], both contiguous.  A row
     whose id is outside [0, vocab) is NaN.  ``out``: [*ids.shape, hidden]."""
-    index = _device_index(ids, (weight, out))
-    is64 = _embedding_ids(ids)
-    if weight.dim() != 2 or not weight.numel():
-        raise ValueError(f"weight must be a [vocab, hidden] table, got {tuple(weight.shape)}")
-    _require_contig("weight", weight)
-    w_code = _float_code("weight", weight.dtype)
+    dtype = dtype or (weight.dtype if out is None else out.dtype)
+    index, w_code, y_code = embedding_checked(ids, weight, dtype, out)
     V, h = weight.shape
     if out is None:
-        out = torch.empty((*ids.shape, h), device=ids.device, dtype=dtype or weight.dtype)
-    elif out.shape != (*ids.shape, h) or not out.is_contiguous() \
-            or out.dtype != (dtype or out.dtype):
+        out = torch.empty((*ids.shape, h), device=ids.device, dtype=dtype)
+    elif out.shape != (*ids.shape, h) or not out.is_contiguous() or out.dtype != dtype:
         raise ValueError(f"out must be contiguous {(*ids.shape, h)} of the output's dtype")
-    y_code = _float_code("output", out.dtype)
     with _on(index):
-        check(lib().zk_embedding_fwd(ids.data_ptr(), is64, ids.numel(), weight.data_ptr(), V, h,
-                                     out.data_ptr(), scale, w_code, y_code, _stream(index)),
+        check(lib().zk_embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(),
+                                     weight.data_ptr(), V, h, out.data_ptr(), scale, w_code, y_code,
+                                     _stream(index)),
               "zk_embedding_fwd")
     return out
-
-
-@functools.lru_cache(maxsize=1024)
-def _embedding_workspace(tokens: int, vocab: int, hidden: int) -> int:
-    nbytes = lib().zk_embedding_bwd_workspace(tokens, vocab, hidden)
-    if nbytes < 0:
-        raise ValueError(f"embedding_bwd: {tokens} tokens of a [{vocab}, {hidden}] table are out "
-                         f"of range")
-    return nbytes
 
 
 def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: float = 1.0,
@@ -960,24 +939,19 @@ def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: flo
     elif dw.shape != (vocab, h) or not dw.is_contiguous() or dw.dtype != (dw_dtype or dw.dtype):
         raise ValueError(f"dw must be contiguous [{vocab}, {h}] of dw_dtype")
     w_dtype = dw.dtype if dw is not None else dw_dtype or dy.dtype
-    _float_code("dw", w_dtype)
-    _float_code("dy", dy.dtype)
-    with _on(index):
-        return _embedding_bwd(index, ids, dy, vocab, scale, padding_idx, w_dtype, dw, accumulate)
-
-
-def _embedding_bwd(index, ids, dy, vocab, scale, padding_idx, w_dtype, dw=None, accumulate=False):
-    """The launches, for checked arguments, on the current device."""
-    tokens, h, dev = ids.numel(), dy.shape[-1], dy.device
-    nbytes = _embedding_workspace(tokens, vocab, h)
+    w_code, dy_code = _float_code("dw", w_dtype), _float_code("dy", dy.dtype)
+    nbytes = lib().zk_embedding_bwd_workspace(ids.numel(), vocab, h)
+    if nbytes < 0:
+        raise ValueError(f"embedding_bwd: {ids.numel()} tokens of a [{vocab}, {h}] table are out of "
+                         f"range")
     if dw is None:
-        dw = torch.empty((vocab, h), device=dev, dtype=w_dtype)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    check(lib().zk_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, tokens, dy.data_ptr(),
-                                 _DTYPE_CODES[dy.dtype], dw.data_ptr(), _DTYPE_CODES[w_dtype],
-                                 vocab, h, scale, -1 if padding_idx is None else padding_idx,
-                                 accumulate, ptr(ws), nbytes, _stream(index)),
-          "zk_embedding_bwd")
+        dw = torch.empty((vocab, h), device=dy.device, dtype=w_dtype)
+    with _on(index):
+        ws = torch.empty(nbytes, device=dy.device, dtype=torch.uint8) if nbytes else None
+        check(lib().zk_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(),
+                                     dy.data_ptr(), dy_code, dw.data_ptr(), w_code, vocab, h, scale,
+                                     -1 if padding_idx is None else padding_idx, accumulate, ptr(ws),
+                                     nbytes, _stream(index)), "zk_embedding_bwd")
     return dw
 
 
@@ -1041,36 +1015,6 @@ def adamw_step_t(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tensor,
                                 int(step), stream_handle(dev)), "zk_adamw_step_t")
 
 
-_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
-_is_contiguous, _get_device = torch.Tensor.is_contiguous, torch.Tensor.get_device
-
-
-def _gpu_index(t: torch.Tensor) -> int:
-    index = t.get_device()
-    if index < 0:
-        raise ValueError("zorse_amd kernels need GPU tensors (got a CPU tensor)")
-    return index
-
-
-def _check_lists(who: str, sizes, index: int, columns) -> None:
-    """Every tensor of each column (name, tensors, allowed dtypes, elements for
-    n or None) is contiguous, on GPU ``index``, of an allowed dtype and as large
-    as ``sizes`` say.  A list at a time, in calls that loop inside the
-    interpreter: 150 tensors of five kinds are 750 checks a step."""
-    for name, tensors, dtypes, elems in columns:
-        want = sizes if elems is None else list(map(elems, sizes))
-        if {t.dtype for t in tensors} <= dtypes and list(map(_numel, tensors)) == want \
-                and all(map(_is_contiguous, tensors)) \
-                and set(map(_get_device, tensors)) == {index}:
-            continue
-        for i, t in enumerate(tensors):
-            _gpu_index(t)
-            if t.dtype not in dtypes or t.numel() != want[i] or not t.is_contiguous() \
-                    or t.get_device() != index:
-                raise ValueError(f"{who}: {name} {i} must be contiguous {sorted(map(str, dtypes))} "
-                                 f"with {want[i]} elements on cuda:{index}")
-
-
 def spans_meet(at, sizes, itemsize: int) -> bool:
     """Whether any two of the tensors with these addresses and numbers of
     elements share memory: they can't be stepped in one launch."""
@@ -1083,48 +1027,21 @@ def spans_meet(at, sizes, itemsize: int) -> bool:
     return False
 
 
-def _rows(columns) -> array.array:
-    """The columns (lists of integers) as rows of 64-bit fields."""
-    n = len(columns)
-    table = array.array("q", bytes(8 * n * len(columns[0])))
-    for i, c in enumerate(columns):
-        table[i::n] = array.array("q", c)
-    return table
+# Types that a column of a list may have, as bits (csrc/nodes.cpp), and what
+# its tensors are beside the first column's: as large, or None, or a base.
+_F32, _U8, _I16 = 1 << _abi.ZK_F32, 1 << 3, 1 << 4
+_FLOATS = sum(1 << code for code in _DTYPE_CODES.values())
+_SAME, _OR_NONE, _BASE = 0, 1, 2
 
 
-_F32, _U8, _I16 = {torch.float32}, {torch.uint8}, {torch.int16}
-_FLOATS = set(FLOAT_DTYPES)
-
-
-def _step_rows(who, columns, params, grads, steps, lowp_outs, seeds=None):
+def _step_table(who, states, params, grads, steps, lowp_outs, *seeds):
     """(device index, rows of zk_adamw_tensor / zk_adamw8_tensor) after the
-    checks of a step; ``columns``: the states as _check_lists takes them."""
-    count = len(params)
-    if len(grads) != count or len(steps) != count or any(len(c[1]) != count for c in columns) \
-            or (lowp_outs is not None and len(lowp_outs) != count) \
-            or (seeds is not None and len(seeds) != count):
-        raise ValueError(f"{who}: the lists differ in length")
-    if not count:
-        return None, None
-    sizes, index = list(map(_numel, params)), _gpu_index(params[0])
-    _check_lists(who, sizes, index, [("param", params, _F32, None), ("grad", grads, _FLOATS, None),
-                                     *columns])
-    at = list(map(_data_ptr, params))
-    if spans_meet(at, sizes, 4):
-        raise ValueError(f"{who}: a parameter is in the list twice, or parameters overlap")
-    low_at = low_dt = [0] * count
-    if lowp_outs is not None:
-        have = [(low, n) for low, n in zip(lowp_outs, sizes) if low is not None]
-        if have:
-            _check_lists(who, [n for _, n in have], index,
-                         [("lowp_out", [low for low, _ in have], _FLOATS, None)])
-            low_at = [0 if low is None else low.data_ptr() for low in lowp_outs]
-            low_dt = [0 if low is None else _DTYPE_CODES[low.dtype] for low in lowp_outs]
-    fields = [at, list(map(_data_ptr, grads)), *(list(map(_data_ptr, c[1])) for c in columns),
-              low_at, sizes, list(map(int, steps))]
-    if seeds is not None:
-        fields.append([int(s) & 0xFFFFFFFF for s in seeds])
-    return index, _rows([*fields, [_DTYPE_CODES[g.dtype] for g in grads], low_dt])
+    checks of a step; ``states``: its columns between gradients and copies."""
+    if lowp_outs is None:
+        lowp_outs = [None] * len(params)
+    columns = (("param", params, _F32, _SAME), ("grad", grads, _FLOATS, _SAME), *states,
+               ("lowp_out", lowp_outs, _FLOATS, _OR_NONE))
+    return _abi.nodes().rows(who, columns, (steps, *seeds), (1, len(columns) - 1), True)
 
 
 def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1: float,
@@ -1133,21 +1050,17 @@ def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1
     device) in one launch for every 56, with the same bits: fp32 ``params``
     and moments, ``grads`` in any of the three types, ``steps`` the step count
     of each, ``lowp_outs`` a 16- or 32-bit copy of each parameter or None."""
-    index, table = _step_rows("adamw_multi", [("exp_avg", exp_avgs, _F32, None),
-                                              ("exp_avg_sq", exp_avg_sqs, _F32, None)],
-                              params, grads, steps, lowp_outs)
-    if table is None:
+    index, table = _step_table("adamw_multi", (("exp_avg", exp_avgs, _F32, _SAME),
+                                               ("exp_avg_sq", exp_avg_sqs, _F32, _SAME)),
+                               params, grads, steps, lowp_outs)
+    if not table:
         return
     with _on(index):
-        check(lib().zk_adamw_multi(table.buffer_info()[0], len(params), lr, beta1, beta2, eps,
+        check(lib().zk_adamw_multi(table, len(params), lr, beta1, beta2, eps,
                                    weight_decay, _stream(index)), "zk_adamw_multi")
 
 
 ADAMW8_BLOCK = 256  # elements whose 8-bit codes are counted from one base
-
-
-def _adamw8_base_elems(n: int) -> int:
-    return 2 * (-(-n // ADAMW8_BLOCK))
 
 
 def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, lr: float,
@@ -1161,14 +1074,14 @@ def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, l
     first to nearest, the second up or down at random with the right mean.
     ``seeds``: an integer for each tensor (mod 2^32) that the random bits come
     from, another for each step."""
-    index, table = _step_rows("adamw8_multi", [("exp_avg", exp_avgs, _U8, None),
-                                               ("exp_avg_sq", exp_avg_sqs, _U8, None),
-                                               ("base", bases, _I16, _adamw8_base_elems)],
-                              params, grads, steps, lowp_outs, seeds)
-    if table is None:
+    index, table = _step_table("adamw8_multi", (("exp_avg", exp_avgs, _U8, _SAME),
+                                                ("exp_avg_sq", exp_avg_sqs, _U8, _SAME),
+                                                ("base", bases, _I16, _BASE)),
+                               params, grads, steps, lowp_outs, [s & 0xFFFFFFFF for s in seeds])
+    if not table:
         return
     with _on(index):
-        check(lib().zk_adamw8_multi(table.buffer_info()[0], len(params), lr, beta1, beta2, eps,
+        check(lib().zk_adamw8_multi(table, len(params), lr, beta1, beta2, eps,
                                     weight_decay, _stream(index)), "zk_adamw8_multi")
 
 
@@ -1183,20 +1096,15 @@ def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.fl
         dtype = outs[0][0].dtype
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"adamw8_values: values are fp32 or bf16 (got {dtype})")
-    count = len(exp_avgs)
-    if any(len(ts) != count for ts in (exp_avg_sqs, bases, *outs)):
-        raise ValueError("adamw8_values: the lists differ in length")
-    if not count:
-        return outs
-    sizes, index = list(map(_numel, exp_avgs)), _gpu_index(exp_avgs[0])
-    columns = [("exp_avg", exp_avgs, _U8, None), ("exp_avg_sq", exp_avg_sqs, _U8, None),
-               ("base", bases, _I16, _adamw8_base_elems),
-               ("first moment", outs[0], {dtype}, None), ("second moment", outs[1], {dtype}, None)]
-    _check_lists("adamw8_values", sizes, index, columns)
-    table = _rows([*(list(map(_data_ptr, c[1])) for c in columns), sizes])
-    with _on(index):
-        check(lib().zk_adamw8_values(table.buffer_info()[0], count, dtype_code(dtype),
-                                     _stream(index)), "zk_adamw8_values")
+    values = 1 << dtype_code(dtype)
+    index, table = _abi.nodes().rows("adamw8_values", (
+        ("exp_avg", exp_avgs, _U8, _SAME), ("exp_avg_sq", exp_avg_sqs, _U8, _SAME),
+        ("base", bases, _I16, _BASE), ("first moment", outs[0], values, _SAME),
+        ("second moment", outs[1], values, _SAME)), (), (), False)
+    if table:
+        with _on(index):
+            check(lib().zk_adamw8_values(table, len(exp_avgs), dtype_code(dtype), _stream(index)),
+                  "zk_adamw8_values")
     return outs
 
 
