@@ -1,14 +1,13 @@
-// Autograd nodes of the token embedding and of the norm of query and key heads,
-// and the tables of the steps over lists of tensors, for torch's C++ side.
+// The token embedding, the norm of query and key heads and the tables of the
+// steps over lists of tensors on torch's C++ side: checks, autograd nodes, and
+// the launches through the C ABI.
 //
-// torch runs a backward pass in a thread of its own, which finds every Python
-// object of a node written in Python in another core's caches: a training pass
-// of few tokens took 85 us where torch's own lookup takes 54, of which the
-// kernels are 10.  A node in C++ touches no Python object.  The tables of 150
-// tensors are 750 checks and 1500 numbers, 350 us of Python and 20 us here.
-//
-// The arguments of the nodes are checked by the Python functions that call
-// them; the kernels are called through the C ABI, as from Python.
+// Small calls are bound by the host.  torch runs a backward pass in a thread of
+// its own, which finds every Python object of a node written in Python in
+// another core's caches: a training pass of few tokens took 85 us where torch's
+// own lookup takes 54, of which the kernels are 10.  A node in C++ touches no
+// Python object.  The tables of 150 tensors are 750 checks and 1500 numbers,
+// 350 us of Python and 20 us here.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -34,8 +33,16 @@ typedef std::optional<Tensor> MaybeTensor;
 
 namespace {
 
+[[noreturn]] void bad(const std::string& what) { throw py::value_error(what); }
+
 void check(int status, const char* who) {
-  TORCH_CHECK(status == 0, who, " failed with status ", status, ": ", zk_last_error());
+  if (status == 0) return;
+  static const char* const names[] = {"ZK_EINVAL", "ZK_EDTYPE", "ZK_EALIGN", "ZK_EUNSUPPORTED",
+                                      "ZK_EWORKSPACE"};
+  throw std::runtime_error(std::string(who) + " failed with " +
+                           (status < 0 && status >= -5 ? names[-1 - status]
+                                                       : "hipError " + std::to_string(status)) +
+                           ": " + zk_last_error());
 }
 
 zk_stream_t stream_of(const Tensor& t) {
@@ -48,26 +55,103 @@ at::ScalarType type_of(int64_t code) {
 int code_of(at::ScalarType t) {
   return t == at::kFloat ? ZK_F32 : t == at::kHalf ? ZK_F16 : t == at::kBFloat16 ? ZK_BF16 : -1;
 }
+int float_code(const char* name, at::ScalarType t) {
+  const int code = code_of(t);
+  if (code < 0) bad(c10::str("unsupported ", name, " dtype ", t));
+  return code;
+}
+
+constexpr const char* kNeedGpu = "zorse_amd kernels need GPU tensors (got a CPU tensor)";
+
+void one_gpu(std::initializer_list<const Tensor*> tensors) {
+  const Tensor& first = **tensors.begin();
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    if (!t->is_cuda()) bad(kNeedGpu);
+    if (t->get_device() != first.get_device()) bad("tensors are on different devices");
+  }
+}
 
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 Tensor workspace(int64_t bytes, const Tensor& like) {
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
 // -------------------------------------------------------- token embedding ---
-Tensor embedding_grad(const Tensor& ids, const Tensor& dy, int64_t vocab, double scale, int64_t pad,
-                      int64_t w_code) {
+void check_ids(const Tensor& ids) {
+  if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong)
+    bad(c10::str("token ids must be int32 or int64 (got ", ids.scalar_type(), ")"));
+  if (!ids.is_contiguous()) bad("ids must be contiguous");
+}
+
+Tensor embedding_fwd(const Tensor& ids, const Tensor& weight, double scale,
+                     std::optional<at::ScalarType> dtype, const MaybeTensor& given_out) {
+  Tensor out = given(given_out);
+  one_gpu({&ids, &weight, &out});
+  check_ids(ids);
+  if (weight.dim() != 2 || weight.numel() == 0)
+    bad(c10::str("weight must be a [vocab, hidden] table, got ", weight.sizes()));
+  if (!weight.is_contiguous()) bad("weight must be contiguous");
+  const at::ScalarType type =
+      dtype ? *dtype : out.defined() ? out.scalar_type() : weight.scalar_type();
+  const int w_code = float_code("weight", weight.scalar_type()), y_code = float_code("output", type);
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(weight.size(1));
+  const c10::DeviceGuard on(weight.device());
+  if (!out.defined())
+    out = at::empty(shape, weight.options().dtype(type));
+  else if (out.sizes() != shape || !out.is_contiguous() || out.scalar_type() != type)
+    bad(c10::str("out must be contiguous ", shape, " of the output's dtype"));
+  check(zk_embedding_fwd(ids.data_ptr(), ids.scalar_type() == at::kLong, ids.numel(),
+                         weight.data_ptr(), weight.size(0), weight.size(1), out.data_ptr(),
+                         static_cast<float>(scale), w_code, y_code, stream_of(weight)),
+        "zk_embedding_fwd");
+  return out;
+}
+
+// The launches of the gradient, for checked arguments; pad -1: none.
+void embedding_grad(const Tensor& ids, const Tensor& dy, const Tensor& dw, double scale, int64_t pad,
+                    bool accumulate) {
   const c10::DeviceGuard on(dy.device());
-  const int64_t h = dy.size(-1), bytes = zk_embedding_bwd_workspace(ids.numel(), vocab, h);
-  TORCH_CHECK_VALUE(bytes >= 0, "embedding: ", ids.numel(), " tokens of a [", vocab, ", ", h,
-                    "] table are out of range");
-  Tensor dw = at::empty({vocab, h}, dy.options().dtype(type_of(w_code)));
+  const int64_t vocab = dw.size(0), h = dw.size(1);
+  const int64_t bytes = zk_embedding_bwd_workspace(ids.numel(), vocab, h);
+  if (bytes < 0)
+    bad(c10::str("embedding_bwd: ", ids.numel(), " tokens of a ", dw.sizes(), " table are out of range"));
   const Tensor ws = workspace(bytes, dy);
   check(zk_embedding_bwd(ids.data_ptr(), ids.scalar_type() == at::kLong, ids.numel(), dy.data_ptr(),
-                         code_of(dy.scalar_type()), dw.data_ptr(), static_cast<int>(w_code), vocab, h,
-                         static_cast<float>(scale), pad, 0, address(ws), bytes, stream_of(dy)),
+                         code_of(dy.scalar_type()), dw.data_ptr(), code_of(dw.scalar_type()), vocab, h,
+                         static_cast<float>(scale), pad, accumulate, address(ws), bytes, stream_of(dy)),
         "zk_embedding_bwd");
+}
+
+Tensor embedding_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, double scale,
+                     std::optional<int64_t> pad, const MaybeTensor& given_dw, bool accumulate,
+                     std::optional<at::ScalarType> dw_dtype) {
+  Tensor dw = given(given_dw);
+  one_gpu({&ids, &dy, &dw});
+  check_ids(ids);
+  if (!dy.is_contiguous()) bad("dy must be contiguous");
+  if (dy.dim() < 1 || dy.sizes().slice(0, dy.dim() - 1) != ids.sizes() || dy.size(-1) == 0)
+    bad(c10::str("dy must be [*ids.shape, hidden], got ", dy.sizes(), " for ids ", ids.sizes()));
+  const int64_t h = dy.size(-1);
+  if (vocab <= 0) bad(c10::str("a table has rows (got vocab ", vocab, ")"));
+  if (pad && !(*pad >= 0 && *pad < vocab))
+    bad(c10::str("padding_idx ", *pad, " outside [0, ", vocab, ")"));
+  float_code("dy", dy.scalar_type());
+  const at::ScalarType type =
+      dw_dtype ? *dw_dtype : dw.defined() ? dw.scalar_type() : dy.scalar_type();
+  float_code("dw", type);
+  if (!dw.defined()) {
+    if (accumulate) bad("accumulate needs the dw to add to");
+    dw = at::empty({vocab, h}, dy.options().dtype(type));
+  } else if (dw.dim() != 2 || dw.size(0) != vocab || dw.size(1) != h || !dw.is_contiguous() ||
+             dw.scalar_type() != type) {
+    bad(c10::str("dw must be contiguous [", vocab, ", ", h, "] of dw_dtype"));
+  }
+  embedding_grad(ids, dy, dw, scale, pad.value_or(-1), accumulate);
   return dw;
 }
 
@@ -85,7 +169,9 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
     ctx->save_for_backward({ids});
     ctx->saved_data["cfg"] = std::vector<int64_t>{vocab, pad, code_of(dy.scalar_type())};
     ctx->saved_data["scale"] = scale;
-    return embedding_grad(ids, dy, vocab, scale, pad, w_code);
+    const Tensor dw = at::empty({vocab, dy.size(-1)}, dy.options().dtype(type_of(w_code)));
+    embedding_grad(ids, dy, dw, scale, pad, false);
+    return dw;
   }
   static variable_list backward(AutogradContext* ctx, variable_list ddw) {
     const Tensor ids = ctx->get_saved_variables()[0];
@@ -100,19 +186,10 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
 
 Tensor Embedding::forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale,
                           int64_t pad, int64_t y_code) {
-  const c10::DeviceGuard on(weight.device());
-  const int64_t vocab = weight.size(0), h = weight.size(1), w_code = code_of(weight.scalar_type());
   ctx->save_for_backward({ids});
-  ctx->saved_data["cfg"] = std::vector<int64_t>{vocab, pad, w_code};
+  ctx->saved_data["cfg"] = std::vector<int64_t>{weight.size(0), pad, code_of(weight.scalar_type())};
   ctx->saved_data["scale"] = scale;
-  std::vector<int64_t> shape = ids.sizes().vec();
-  shape.push_back(h);
-  Tensor y = at::empty(shape, weight.options().dtype(type_of(y_code)));
-  check(zk_embedding_fwd(ids.data_ptr(), ids.scalar_type() == at::kLong, ids.numel(),
-                         weight.data_ptr(), vocab, h, y.data_ptr(), static_cast<float>(scale),
-                         static_cast<int>(w_code), static_cast<int>(y_code), stream_of(weight)),
-        "zk_embedding_fwd");
-  return y;
+  return embedding_fwd(ids, weight, scale, type_of(y_code), MaybeTensor());
 }
 
 variable_list Embedding::backward(AutogradContext* ctx, variable_list dy) {
@@ -120,62 +197,182 @@ variable_list Embedding::backward(AutogradContext* ctx, variable_list dy) {
   const auto cfg = ctx->saved_data["cfg"].toIntVector();
   const double scale = ctx->saved_data["scale"].toDouble();
   const Tensor g = dy[0].contiguous();
-  const Tensor dw = at::GradMode::is_enabled() && g.requires_grad()
-                        ? EmbeddingGrad::apply(ids, g, cfg[0], scale, cfg[1], cfg[2])
-                        : embedding_grad(ids, g, cfg[0], scale, cfg[1], cfg[2]);
+  Tensor dw;
+  if (at::GradMode::is_enabled() && g.requires_grad()) {  // create_graph
+    dw = EmbeddingGrad::apply(ids, g, cfg[0], scale, cfg[1], cfg[2]);
+  } else {
+    dw = at::empty({cfg[0], g.size(-1)}, g.options().dtype(type_of(cfg[2])));
+    embedding_grad(ids, g, dw, scale, cfg[1], false);
+  }
   return {Tensor(), dw, Tensor(), Tensor(), Tensor()};
 }
 
-// ---------------------------------------- norm of q and k heads, rotation ---
-Tensor rows_of(const Tensor& t) {  // unit stride along d (an expanded gradient has none)
-  return !t.defined() || t.stride(-1) == 1 ? t : t.contiguous();
+// functional.embedding
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding,
+                 std::optional<at::ScalarType> dtype) {
+  int64_t pad = -1;
+  if (padding) {
+    const int64_t rows = weight.dim() > 0 ? weight.size(0) : 0;
+    if (*padding < -rows || *padding >= rows)
+      bad(c10::str("padding_idx ", *padding, " outside a table of ", rows, " rows"));
+    pad = *padding < 0 ? *padding + rows : *padding;
+  }
+  const Tensor i = ids.contiguous(), w = weight.contiguous();
+  if (!at::GradMode::is_enabled() || !w.requires_grad())
+    return embedding_fwd(i, w, scale, dtype, MaybeTensor());
+  return Embedding::apply(i, w, scale, pad, float_code("output", dtype.value_or(w.scalar_type())));
 }
 
+// ---------------------------------------- norm of q and k heads, rotation ---
+struct Qk {  // operands; k, wk and positions may be undefined
+  Tensor q, k, wq, wk, cos, sin, positions;
+};
+
+// Unit stride along d (expanded heads and gradients have none).
+Tensor rows_of(const Tensor& t) {
+  return !t.defined() || t.dim() == 0 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+struct Strides {
+  int64_t b = 0, s = 0, h = 0;
+};
+Strides contiguous_strides(const Tensor& t) {
+  return Strides{t.size(1) * t.size(2) * t.size(3), t.size(2) * t.size(3), t.size(3)};
+}
+// Of x, which lies over the heads t; `out`: and is written.
+Strides strides_over(const char* name, const Tensor& x, const Tensor& t, bool out) {
+  if (x.sizes() != t.sizes() || x.scalar_type() != t.scalar_type())
+    bad(std::string(name) + " must have the shape and type of its heads");
+  if (x.stride(3) != 1 && x.numel() != 0) bad(std::string(name) + " needs unit stride along d");
+  for (int i = 0; out && i < 3; ++i)
+    if (x.stride(i) == 0 && x.size(i) > 1)
+      bad(std::string(name) + " overlaps itself (an expanded tensor)");
+  return Strides{x.stride(0), x.stride(1), x.stride(2)};
+}
+
+// The checks of both directions.  qo, ko: y or dx (undefined: new contiguous
+// tensors); gq, gk: dy, of the backward.
+zk_qk_desc qk_checked(const Qk& A, double eps, bool interleaved, const Tensor& qo, const Tensor& ko,
+                      const Tensor& gq, const Tensor& gk) {
+  const Tensor &q = A.q, &k = A.k;
+  if (q.dim() != 4) bad("q must be [B, S, H, d]");
+  if (k.defined() != A.wk.defined()) bad("k and k_weight belong together");
+  one_gpu({&q, &k, &A.wq, &A.wk, &A.cos, &A.sin, &A.positions, &qo, &ko, &gq, &gk});
+  zk_qk_desc D{};
+  D.B = q.size(0), D.S = q.size(1), D.Hq = q.size(2), D.d = q.size(3);
+  D.dtype = float_code("q", q.scalar_type());
+  D.w_dtype = float_code("q_weight", A.wq.scalar_type());
+  if (D.Hq == 0) bad("q has no heads");
+  if (D.d % 2 != 0 || D.d <= 0 || D.d > 1024)
+    bad(c10::str("head dims are even and up to 1024 (got ", D.d, ")"));
+  if (A.wq.dim() != 1 || A.wq.size(0) != D.d || !A.wq.is_contiguous())
+    bad(c10::str("q_weight must be contiguous [", D.d, "]"));
+  if (k.defined()) {
+    if (k.dim() != 4 || k.size(0) != D.B || k.size(1) != D.S || k.size(3) != D.d ||
+        k.scalar_type() != q.scalar_type())
+      bad("k must be [B, S, H, d] matching q");
+    if (A.wk.dim() != 1 || A.wk.size(0) != D.d || A.wk.scalar_type() != A.wq.scalar_type() ||
+        !A.wk.is_contiguous())
+      bad(c10::str("k_weight must be contiguous [", D.d, "] of q_weight's dtype"));
+    D.Hkv = k.size(2);
+  }
+  if (k.defined() != ko.defined() && qo.defined()) bad("an output for each of q and k is needed");
+  Strides s = strides_over("q", q, q, false);
+  D.q_sb = s.b, D.q_ss = s.s, D.q_sh = s.h;
+  s = qo.defined() ? strides_over("q output", qo, q, true) : contiguous_strides(q);
+  D.oq_sb = s.b, D.oq_ss = s.s, D.oq_sh = s.h;
+  if (gq.defined()) s = strides_over("q gradient", gq, q, false);
+  D.dyq_sb = s.b, D.dyq_ss = s.s, D.dyq_sh = s.h;
+  if (k.defined()) {
+    s = strides_over("k", k, k, false);
+    D.k_sb = s.b, D.k_ss = s.s, D.k_sh = s.h;
+    s = ko.defined() ? strides_over("k output", ko, k, true) : contiguous_strides(k);
+    D.ok_sb = s.b, D.ok_ss = s.s, D.ok_sh = s.h;
+    if (gk.defined()) s = strides_over("k gradient", gk, k, false);
+    D.dyk_sb = s.b, D.dyk_ss = s.s, D.dyk_sh = s.h;
+  }
+  const int64_t half = D.d / 2;
+  if (A.cos.scalar_type() != at::kFloat || A.sin.scalar_type() != at::kFloat || A.cos.dim() != 2 ||
+      A.cos.size(1) != half || A.sin.sizes() != A.cos.sizes() || !A.cos.is_contiguous() ||
+      !A.sin.is_contiguous())
+    bad(c10::str("cos and sin must be contiguous fp32 [n_pos, ", half,
+                 "] tables of as many positions"));
+  D.n_pos = A.cos.size(0);
+  if (A.positions.defined()) {
+    const Tensor& p = A.positions;
+    const bool shared = p.dim() == 1 && p.size(0) == D.S;
+    const bool own = p.dim() == 2 && p.size(0) == D.B && p.size(1) == D.S;
+    if (p.scalar_type() != at::kLong || !(shared || own) || !p.is_contiguous())
+      bad("positions must be a contiguous int64 [S] or [B, S] tensor");
+    D.pos_sb = own ? D.S : 0;
+  } else if (D.n_pos < D.S) {
+    bad(c10::str("table holds ", D.n_pos, " positions < S=", D.S));
+  }
+  if (D.n_pos == 0) bad("the tables hold no positions");
+  D.eps = static_cast<float>(eps);
+  D.pairing = interleaved ? ZK_ROPE_INTERLEAVED : ZK_ROPE_HALF;
+  return D;
+}
+
+// The launches, for checked arguments; outputs that are undefined are made.
+void qk_fwd(const Qk& A, const zk_qk_desc& D, Tensor& qo, Tensor& ko) {
+  const c10::DeviceGuard on(A.q.device());
+  if (!qo.defined()) {
+    qo = at::empty(A.q.sizes(), A.q.options());
+    if (A.k.defined()) ko = at::empty(A.k.sizes(), A.k.options());
+  }
+  check(zk_qk_norm_rope_fwd(&D, A.q.data_ptr(), address(A.k), A.wq.data_ptr(), address(A.wk),
+                            qo.data_ptr(), address(ko), static_cast<const float*>(A.cos.data_ptr()),
+                            static_cast<const float*>(A.sin.data_ptr()),
+                            static_cast<const int64_t*>(address(A.positions)), stream_of(A.q)),
+        "zk_qk_norm_rope_fwd");
+}
+
+variable_list qk_bwd(const Qk& A, const zk_qk_desc& D, const Tensor& gq, const Tensor& gk, Tensor dq,
+                     Tensor dk) {
+  const c10::DeviceGuard on(A.q.device());
+  if (!dq.defined()) {
+    dq = at::empty(A.q.sizes(), A.q.options());
+    if (A.k.defined()) dk = at::empty(A.k.sizes(), A.k.options());
+  }
+  const Tensor dwq = at::empty({D.d}, A.wq.options());
+  const Tensor dwk = A.k.defined() ? at::empty({D.d}, A.wk.options()) : Tensor();
+  const int64_t bytes = zk_qk_norm_rope_bwd_workspace(D.d);
+  const Tensor ws = workspace(bytes, A.q);
+  check(zk_qk_norm_rope_bwd(&D, A.q.data_ptr(), address(A.k), A.wq.data_ptr(), address(A.wk),
+                            gq.data_ptr(), address(gk), dq.data_ptr(), address(dk), dwq.data_ptr(),
+                            address(dwk), static_cast<const float*>(A.cos.data_ptr()),
+                            static_cast<const float*>(A.sin.data_ptr()),
+                            static_cast<const int64_t*>(address(A.positions)), address(ws), bytes,
+                            stream_of(A.q)),
+        "zk_qk_norm_rope_bwd");
+  return {dq, dk, dwq, dwk};
+}
+
+// Saves its inputs only, and takes the norm from them again.
 struct QkNormRope : torch::autograd::Function<QkNormRope> {
-  // desc: of contiguous outputs, whose gradients' strides backward() fills in
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const MaybeTensor& k,
                                const Tensor& wq, const MaybeTensor& wk, const Tensor& cos,
                                const Tensor& sin, const MaybeTensor& positions,
                                const zk_qk_desc& desc) {
-    const c10::DeviceGuard on(q.device());
-    const Tensor key = k.value_or(Tensor()), key_w = wk.value_or(Tensor()),
-                 pos = positions.value_or(Tensor());
-    ctx->save_for_backward({q, key, wq, key_w, cos, sin, pos});
+    const Qk A{q, given(k), wq, given(wk), cos, sin, given(positions)};
+    ctx->save_for_backward({A.q, A.k, A.wq, A.wk, A.cos, A.sin, A.positions});
     ctx->saved_data["desc"] = std::string(reinterpret_cast<const char*>(&desc), sizeof(desc));
-    variable_list out = {at::empty(q.sizes(), q.options())};
-    if (key.defined()) out.push_back(at::empty(key.sizes(), q.options()));
-    check(zk_qk_norm_rope_fwd(&desc, q.data_ptr(), address(key), wq.data_ptr(), address(key_w),
-                              out[0].data_ptr(), key.defined() ? out[1].data_ptr() : nullptr,
-                              static_cast<const float*>(cos.data_ptr()),
-                              static_cast<const float*>(sin.data_ptr()),
-                              static_cast<const int64_t*>(address(pos)), stream_of(q)),
-          "zk_qk_norm_rope_fwd");
-    return out;
+    Tensor qo, ko;
+    qk_fwd(A, desc, qo, ko);
+    return A.k.defined() ? variable_list{qo, ko} : variable_list{qo};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
-    const variable_list saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &cos = saved[4],
-                 &sin = saved[5], &pos = saved[6];
-    const c10::DeviceGuard on(q.device());
-    zk_qk_desc desc;
-    std::memcpy(&desc, ctx->saved_data["desc"].toStringRef().data(), sizeof(desc));
-    const Tensor gq = rows_of(dy[0]), gk = k.defined() ? rows_of(dy[1]) : Tensor();
-    desc.dyq_sb = gq.stride(0), desc.dyq_ss = gq.stride(1), desc.dyq_sh = gq.stride(2);
-    if (k.defined()) desc.dyk_sb = gk.stride(0), desc.dyk_ss = gk.stride(1), desc.dyk_sh = gk.stride(2);
-    const int64_t bytes = zk_qk_norm_rope_bwd_workspace(desc.d);
-    const Tensor dq = at::empty(q.sizes(), q.options()), dwq = at::empty({desc.d}, wq.options());
-    const Tensor dk = k.defined() ? at::empty(k.sizes(), k.options()) : Tensor();
-    const Tensor dwk = k.defined() ? at::empty({desc.d}, wk.options()) : Tensor();
-    const Tensor ws = workspace(bytes, q);
-    check(zk_qk_norm_rope_bwd(&desc, q.data_ptr(), address(k), wq.data_ptr(), address(wk),
-                              gq.data_ptr(), address(gk), dq.data_ptr(), address(dk), dwq.data_ptr(),
-                              address(dwk), static_cast<const float*>(cos.data_ptr()),
-                              static_cast<const float*>(sin.data_ptr()),
-                              static_cast<const int64_t*>(address(pos)), address(ws), bytes,
-                              stream_of(q)),
-          "zk_qk_norm_rope_bwd");
-    variable_list out = {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    const Qk A{s[0], s[1], s[2], s[3], s[4], s[5], s[6]};
+    zk_qk_desc D;
+    std::memcpy(&D, ctx->saved_data["desc"].toStringRef().data(), sizeof(D));
+    const Tensor gq = rows_of(dy[0]), gk = A.k.defined() ? rows_of(dy[1]) : Tensor();
+    D.dyq_sb = gq.stride(0), D.dyq_ss = gq.stride(1), D.dyq_sh = gq.stride(2);
+    if (gk.defined()) D.dyk_sb = gk.stride(0), D.dyk_ss = gk.stride(1), D.dyk_sh = gk.stride(2);
+    variable_list out = qk_bwd(A, D, gq, gk, Tensor(), Tensor());
+    out.resize(8);
     if (!at::GradMode::is_enabled() || !(gq.requires_grad() || (gk.defined() && gk.requires_grad())))
       return out;
     // create_graph: what is differentiated once more says so
@@ -184,6 +381,51 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     return torch::autograd::DelayedError("qk_norm_rope can be differentiated once", 8)(std::move(out));
   }
 };
+
+typedef std::pair<Tensor, MaybeTensor> QkPair;
+MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+
+// functional.qk_norm_rope
+QkPair qk_norm_rope(const Tensor& q, const MaybeTensor& k, const Tensor& wq, const MaybeTensor& wk,
+                    const Tensor& cos, const Tensor& sin, const MaybeTensor& positions, double eps,
+                    bool interleaved) {
+  const Qk A{rows_of(q), rows_of(given(k)), wq, given(wk), cos, sin, given(positions)};
+  const zk_qk_desc D = qk_checked(A, eps, interleaved, Tensor(), Tensor(), Tensor(), Tensor());
+  bool grad = false;
+  for (const Tensor* t : {&A.q, &A.k, &A.wq, &A.wk}) grad = grad || (t->defined() && t->requires_grad());
+  if (!grad || !at::GradMode::is_enabled()) {
+    Tensor qo, ko;
+    qk_fwd(A, D, qo, ko);
+    return {qo, maybe(ko)};
+  }
+  const variable_list out = QkNormRope::apply(A.q, maybe(A.k), wq, wk, cos, sin, positions, D);
+  return {out[0], A.k.defined() ? MaybeTensor(out[1]) : MaybeTensor()};
+}
+
+QkPair qk_norm_rope_fwd(const Tensor& q, const MaybeTensor& k, const Tensor& wq, const MaybeTensor& wk,
+                        const Tensor& cos, const Tensor& sin, const MaybeTensor& positions, double eps,
+                        bool interleaved, const MaybeTensor& q_out, const MaybeTensor& k_out) {
+  const Qk A{q, given(k), wq, given(wk), cos, sin, given(positions)};
+  Tensor qo = given(q_out), ko = given(k_out);
+  const zk_qk_desc D = qk_checked(A, eps, interleaved, qo, ko, Tensor(), Tensor());
+  qk_fwd(A, D, qo, ko);
+  return {qo, maybe(ko)};
+}
+
+std::vector<MaybeTensor> qk_norm_rope_bwd(const MaybeTensor& dq_out, const MaybeTensor& dk_out,
+                                          const Tensor& q, const MaybeTensor& k, const Tensor& wq,
+                                          const MaybeTensor& wk, const Tensor& cos, const Tensor& sin,
+                                          const MaybeTensor& positions, double eps, bool interleaved,
+                                          const MaybeTensor& dq, const MaybeTensor& dk) {
+  const Qk A{q, given(k), wq, given(wk), cos, sin, given(positions)};
+  if (!dq_out || dk_out.has_value() != k.has_value()) bad("a gradient for each of q and k is needed");
+  const zk_qk_desc D =
+      qk_checked(A, eps, interleaved, given(dq), given(dk), given(dq_out), given(dk_out));
+  std::vector<MaybeTensor> out;
+  for (const Tensor& t : qk_bwd(A, D, given(dq_out), given(dk_out), given(dq), given(dk)))
+    out.push_back(maybe(t));
+  return out;
+}
 
 // ------------------------------------------------- lists of tensors: tables ---
 constexpr int kByteBit = 3, kShortBit = 4;  // beside the three types' codes
@@ -250,7 +492,7 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
       }
       if (!THPVariable_Check(o)) throw py::type_error(who + ": lists of tensors are needed");
       const Tensor& t = THPVariable_Unpack(o);
-      if (!t.is_cuda()) throw py::value_error("zorse_amd kernels need GPU tensors (got a CPU tensor)");
+      if (!t.is_cuda()) throw py::value_error(kNeedGpu);
       if (c == 0) numel[i] = t.numel();
       if (index < 0) index = t.get_device();
       const int64_t want = kind == 2 ? (numel[i] + kBlock - 1) / kBlock * 2 : numel[i];
@@ -288,17 +530,12 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
 }  // namespace
 
 PYBIND11_MODULE(_nodes, m) {
-  m.def("embedding",
-        [](const Tensor& ids, const Tensor& weight, double scale, int64_t pad, int64_t y_code) {
-          return Embedding::apply(ids, weight, scale, pad, y_code);
-        },
-        py::call_guard<py::gil_scoped_release>());
-  m.def("qk_norm_rope",
-        [](const Tensor& q, const MaybeTensor& k, const Tensor& wq, const MaybeTensor& wk,
-           const Tensor& cos, const Tensor& sin, const MaybeTensor& positions, int64_t desc) {
-          return QkNormRope::apply(q, k, wq, wk, cos, sin, positions,
-                                   *reinterpret_cast<const zk_qk_desc*>(desc));
-        },
-        py::call_guard<py::gil_scoped_release>());
+  const py::call_guard<py::gil_scoped_release> free_gil;
+  m.def("embedding", &embedding, free_gil);
+  m.def("embedding_fwd", &embedding_fwd, free_gil);
+  m.def("embedding_bwd", &embedding_bwd, free_gil);
+  m.def("qk_norm_rope", &qk_norm_rope, free_gil);
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, free_gil);
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, free_gil);
   m.def("rows", &rows);
 }

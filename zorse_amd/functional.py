@@ -10,7 +10,6 @@ which stays fp32) and handed to the kernel as fp32 [S, d/2] tables.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 import threading
 
@@ -111,24 +110,10 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     [0, vocab) gives a row of NaN and no gradient (nothing is read back to the
     host to check it).  ``padding_idx`` (negative: from the end, as nn.Embedding
     takes it): the row whose tokens have no gradient."""
-    if padding_idx is not None:
-        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
-            raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
-        padding_idx %= weight.shape[0]
-    ids, scale = ids.contiguous(), float(scale)
-    weight = weight.contiguous()
-    if not (weight.requires_grad and torch.is_grad_enabled()):
-        return K.embedding_fwd(ids, weight, scale=scale, dtype=dtype)
-    _, _, y_code = K.embedding_checked(ids, weight, dtype or weight.dtype)
-    return nodes().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx, y_code)
+    return nodes().embedding(ids, weight, scale, padding_idx, dtype)
 
 
 # ----------------------------------------- Norm of q and k heads, rotation --
-
-def _unit_rows(t):
-    """t with unit stride along its last dim (expanded heads have none)."""
-    return t if t is None or t.stride(-1) == 1 else t.contiguous()
-
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6,
                  interleaved=False):
@@ -138,15 +123,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6
     tables (rope_tables(..., torch.float32, ...)); ``positions`` int64 [S] or
     [B, S], default 0 .. S-1; a position outside the tables gives NaN.  Any even
     d up to 1024; q and k may be views of one q|k|v buffer."""
-    q, k = _unit_rows(q), _unit_rows(k)
-    heads = (q, k, q_weight, k_weight)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in heads)):
-        return K.qk_norm_rope_fwd(*heads, cos, sin, positions=positions, eps=eps,
-                                  interleaved=interleaved)
-    # the node saves its inputs only, and takes the norm from them again
-    _, desc = K.qk_checked(*heads, cos, sin, positions, eps, interleaved)
-    out = nodes().qk_norm_rope(*heads, cos, sin, positions, ctypes.addressof(desc))
-    return (out[0], None) if k is None else tuple(out)
+    return nodes().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 # -------------------------------------------------------------- Attention --

@@ -59,28 +59,6 @@ def _stream(index: int) -> int:
         else _abi._raw_stream(index)
 
 
-_DTYPE_CODES = {dt: dtype_code(dt) for dt in FLOAT_DTYPES}
-
-
-def _float_code(name: str, dtype: torch.dtype) -> int:
-    code = _DTYPE_CODES.get(dtype)
-    if code is None:
-        raise ValueError(f"unsupported {name} dtype {dtype}")
-    return code
-
-
-def _device_index(first: torch.Tensor, others) -> int:
-    """The index of the GPU that all of these tensors (None: skipped) are on."""
-    index = first.get_device()
-    if index >= 0:
-        for t in others:
-            if t is not None and t.get_device() != index:
-                break
-        else:
-            return index
-    return _require_gpu(first, *others).index  # says what is wrong
-
-
 # --------------------------------------------------------------- RMSNorm ---
 
 def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -560,86 +538,6 @@ def rope_copy(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
 # ----------------------------------------- Norm of q and k heads, rotation --
 
-def _qk_strides(name, x, t):
-    """The strides of an output or gradient of the heads t, after its checks."""
-    if x.shape != t.shape or x.dtype != t.dtype:
-        raise ValueError(f"{name} must have the shape and type of its heads")
-    *st, unit = x.stride()
-    if unit != 1 and x.numel():
-        raise ValueError(f"{name} needs unit stride along d")
-    return st
-
-
-def _qk_out(name, x, t):
-    st = _qk_strides(name, x, t)
-    if 0 in st and any(a == 0 and n > 1 for a, n in zip(st, x.shape)):
-        raise ValueError(f"{name} overlaps itself (an expanded tensor)")
-    return st
-
-
-def qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, outs=None,
-               grads=(None, None)):
-    """The checks of both directions; (device index, zk_qk_desc).  ``outs`` are
-    y or dx (None: new contiguous tensors), ``grads`` dy of q and k."""
-    if q.dim() != 4:
-        raise ValueError("q must be [B, S, H, d]")
-    B, S, Hq, d = q.shape
-    if (k is None) != (k_weight is None):
-        raise ValueError("k and k_weight belong together")
-    index = _device_index(q, (k, q_weight, k_weight, cos, sin, positions, *(outs or ()), *grads))
-    code, w_code = _float_code("q", q.dtype), _float_code("q_weight", q_weight.dtype)
-    if not Hq:
-        raise ValueError("q has no heads")
-    if d % 2 or not 0 < d <= 1024:
-        raise ValueError(f"head dims are even and up to 1024 (got {d})")
-    if q_weight.shape != (d,) or not q_weight.is_contiguous():
-        raise ValueError(f"q_weight must be contiguous [{d}]")
-    q_st, Hkv = _qk_strides("q", q, q), 0
-    k_st = ok = gq = gk = (0, 0, 0)
-    if k is not None:
-        if k.dim() != 4 or k.shape[:2] != (B, S) or k.shape[3] != d or k.dtype != q.dtype:
-            raise ValueError("k must be [B, S, H, d] matching q")
-        if k_weight.shape != (d,) or k_weight.dtype != q_weight.dtype \
-                or not k_weight.is_contiguous():
-            raise ValueError(f"k_weight must be contiguous [{d}] of q_weight's dtype")
-        k_st, Hkv = _qk_strides("k", k, k), k.shape[2]
-    if outs is None:
-        # and the gradients of such outputs lie as they do
-        oq = gq = (S * Hq * d, Hq * d, d)
-        ok = gk = (S * Hkv * d, Hkv * d, d)
-    else:
-        oq = _qk_out("q output", outs[0], q)
-        if k is not None:
-            ok = _qk_out("k output", outs[1], k)
-    if grads[0] is not None:
-        gq = _qk_strides("q gradient", grads[0], q)
-    if grads[1] is not None:
-        gk = _qk_strides("k gradient", grads[1], k)
-    n_pos, half = cos.shape[0], d // 2
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != (n_pos, half) \
-            or sin.shape != (n_pos, half) or not cos.is_contiguous() or not sin.is_contiguous():
-        raise ValueError(f"cos and sin must be contiguous fp32 [n_pos, {half}] tables of as many "
-                         f"positions")
-    pos_sb = 0
-    if positions is not None:
-        if positions.dtype != torch.int64 or positions.shape not in ((S,), (B, S)) \
-                or not positions.is_contiguous():
-            raise ValueError("positions must be a contiguous int64 [S] or [B, S] tensor")
-        pos_sb = S if positions.dim() == 2 else 0
-    elif n_pos < S:
-        raise ValueError(f"table holds {n_pos} positions < S={S}")
-    if not n_pos:
-        raise ValueError("the tables hold no positions")
-    return index, _abi.QkDesc(B, S, Hq, Hkv, d, *q_st, *k_st, *oq, *ok, *gq, *gk, n_pos, pos_sb,
-                              eps, _abi.ZK_ROPE_INTERLEAVED if interleaved else _abi.ZK_ROPE_HALF,
-                              code, w_code)
-
-
-def _empty_qk(q, k):
-    return (torch.empty(q.shape, device=q.device, dtype=q.dtype),
-            None if k is None else torch.empty(k.shape, device=k.device, dtype=k.dtype))
-
-
 def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps: float = 1e-6,
                      interleaved: bool = False, out=None):
     """RMS norm of every head of q [B,S,Hq,d] and k [B,S,Hkv,d] over its d
@@ -649,14 +547,8 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps:
     sin: fp32 [n_pos, d/2] tables; ``positions`` int64 [S] or [B, S] (default
     0 .. S-1), those outside the tables giving rows of NaN.  fp32 inside, one
     rounding."""
-    index, desc = qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
-    qo, ko = _empty_qk(q, k) if out is None else out
-    with _on(index):
-        check(lib().zk_qk_norm_rope_fwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
-                                        ptr(k_weight), qo.data_ptr(), ptr(ko), cos.data_ptr(),
-                                        sin.data_ptr(), ptr(positions), _stream(index)),
-              "zk_qk_norm_rope_fwd")
-    return qo, ko
+    return _abi.nodes().qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                         interleaved, *(out or (None, None)))
 
 
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, positions=None,
@@ -665,23 +557,9 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, posi
     its outputs; nothing of the forward but its inputs is needed.  ``out`` =
     (dq, dk) views with unit stride along d, which may be dq_out and dk_out
     themselves.  The weights' gradients are summed in fp32 in one order."""
-    if dq_out is None or (dk_out is None) != (k is None):
-        raise ValueError("a gradient for each of q and k is needed")
-    index, desc = qk_checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out,
-                           (dq_out, dk_out))
-    dq, dk = _empty_qk(q, k) if out is None else out
-    nbytes = lib().zk_qk_norm_rope_bwd_workspace(desc.d)
-    dwq = torch.empty_like(q_weight)
-    dwk = None if k is None else torch.empty_like(k_weight)
-    with _on(index):
-        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        check(lib().zk_qk_norm_rope_bwd(desc, q.data_ptr(), ptr(k), q_weight.data_ptr(),
-                                        ptr(k_weight), dq_out.data_ptr(), ptr(dk_out),
-                                        dq.data_ptr(), ptr(dk), dwq.data_ptr(), ptr(dwk),
-                                        cos.data_ptr(), sin.data_ptr(), ptr(positions),
-                                        ws.data_ptr(), nbytes, _stream(index)),
-              "zk_qk_norm_rope_bwd")
-    return dq, dk, dwq, dwk
+    return tuple(_abi.nodes().qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin,
+                                               positions, eps, interleaved,
+                                               *(out or (None, None))))
 
 
 # -------------------------------------------------------------- Attention --
@@ -877,42 +755,13 @@ def _check_transposed(transposed, q, k):
 
 # -------------------------------------------------------------- Embedding --
 
-def _embedding_ids(ids: torch.Tensor) -> None:
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"token ids must be int32 or int64 (got {ids.dtype})")
-    _require_contig("ids", ids)
-
-
-def embedding_checked(ids, weight, dtype, out=None):
-    """The forward's checks; (device index, the codes of the table's type and of
-    ``dtype``)."""
-    index = _device_index(ids, (weight, out))
-    _embedding_ids(ids)
-    if weight.dim() != 2 or not weight.numel():
-        raise ValueError(f"weight must be a [vocab, hidden] table, got {tuple(weight.shape)}")
-    _require_contig("weight", weight)
-    return index, _float_code("weight", weight.dtype), _float_code("output", dtype)
-
-
 def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
                   dtype: torch.dtype | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """round(scale * weight[ids]) in ``dtype`` (default the table's): ids
     int32 / int64 of any shape, weight [vocab, hidden], both contiguous.  A row
     whose id is outside [0, vocab) is NaN.  ``out``: [*ids.shape, hidden]."""
-    dtype = dtype or (weight.dtype if out is None else out.dtype)
-    index, w_code, y_code = embedding_checked(ids, weight, dtype, out)
-    V, h = weight.shape
-    if out is None:
-        out = torch.empty((*ids.shape, h), device=ids.device, dtype=dtype)
-    elif out.shape != (*ids.shape, h) or not out.is_contiguous() or out.dtype != dtype:
-        raise ValueError(f"out must be contiguous {(*ids.shape, h)} of the output's dtype")
-    with _on(index):
-        check(lib().zk_embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(),
-                                     weight.data_ptr(), V, h, out.data_ptr(), scale, w_code, y_code,
-                                     _stream(index)),
-              "zk_embedding_fwd")
-    return out
+    return _abi.nodes().embedding_fwd(ids, weight, scale, dtype, out)
 
 
 def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: float = 1.0,
@@ -924,35 +773,7 @@ def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, *, scale: flo
     overwritten, or with ``accumulate`` added to, which touches only the rows
     that tokens name; without it a new tensor of ``dw_dtype`` (default dy's).
     fp32 sums in an order that the ids alone decide (no atomics)."""
-    index = _device_index(ids, (dy, dw))
-    _embedding_ids(ids)
-    _require_contig("dy", dy)
-    if dy.dim() < 1 or dy.shape[:-1] != ids.shape or not dy.shape[-1]:
-        raise ValueError(f"dy must be [*ids.shape, hidden], got {tuple(dy.shape)} for ids "
-                         f"{tuple(ids.shape)}")
-    h = dy.shape[-1]
-    if padding_idx is not None and not 0 <= padding_idx < vocab:
-        raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab})")
-    if dw is None:
-        if accumulate:
-            raise ValueError("accumulate needs the dw to add to")
-    elif dw.shape != (vocab, h) or not dw.is_contiguous() or dw.dtype != (dw_dtype or dw.dtype):
-        raise ValueError(f"dw must be contiguous [{vocab}, {h}] of dw_dtype")
-    w_dtype = dw.dtype if dw is not None else dw_dtype or dy.dtype
-    w_code, dy_code = _float_code("dw", w_dtype), _float_code("dy", dy.dtype)
-    nbytes = lib().zk_embedding_bwd_workspace(ids.numel(), vocab, h)
-    if nbytes < 0:
-        raise ValueError(f"embedding_bwd: {ids.numel()} tokens of a [{vocab}, {h}] table are out of "
-                         f"range")
-    if dw is None:
-        dw = torch.empty((vocab, h), device=dy.device, dtype=w_dtype)
-    with _on(index):
-        ws = torch.empty(nbytes, device=dy.device, dtype=torch.uint8) if nbytes else None
-        check(lib().zk_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(),
-                                     dy.data_ptr(), dy_code, dw.data_ptr(), w_code, vocab, h, scale,
-                                     -1 if padding_idx is None else padding_idx, accumulate, ptr(ws),
-                                     nbytes, _stream(index)), "zk_embedding_bwd")
-    return dw
+    return _abi.nodes().embedding_bwd(ids, dy, vocab, scale, padding_idx, dw, accumulate, dw_dtype)
 
 
 # ------------------------------------------------------------------ AdamW --
@@ -1030,7 +851,7 @@ def spans_meet(at, sizes, itemsize: int) -> bool:
 # Types that a column of a list may have, as bits (csrc/nodes.cpp), and what
 # its tensors are beside the first column's: as large, or None, or a base.
 _F32, _U8, _I16 = 1 << _abi.ZK_F32, 1 << 3, 1 << 4
-_FLOATS = sum(1 << code for code in _DTYPE_CODES.values())
+_FLOATS = sum(1 << dtype_code(dt) for dt in FLOAT_DTYPES)
 _SAME, _OR_NONE, _BASE = 0, 1, 2
 
 
