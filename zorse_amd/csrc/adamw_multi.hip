@@ -6,7 +6,11 @@
 // comparing its number with the tensors' first ones, a lane for each.
 //
 // HBM bounds all of it: 28 bytes an element with 32-bit moments and gradients,
-// 16 with 8-bit moments, 16-bit gradients and a 16-bit copy.
+// 16 with 8-bit moments, 16-bit gradients and a 16-bit copy.  605 M elements with
+// 8-bit moments, bf16 gradients and copies (9.7 GB) take 1540 us, 6.3 TB/s; their
+// moments read as bf16 (3.6 GB) 600 us, 6.0 TB/s; 65 tensors of 4096 with 32-bit
+// moments two launches of 5 us.  Small lists are bound by their launches: 150
+// tensors of up to 300000 elements, 5 M in all, are four launches of 6 to 10 us.
 //
 // 8-bit moments (the format is stated in zorse_amd.h): r(x), the top 12 bits
 // below the sign of a float, is an integer that grows with |x|, 8 steps an

@@ -38,7 +38,10 @@ struct Span {  // the id that crosses out of the block where it begins (-1: none
 };
 
 // ---------------------------------------------------------------- forward ---
-// tpr (a power of two up to 256) threads a row, 8 elements each at a time.
+// tpr (a power of two up to 256) threads a row, 8 elements each at a time: a
+// workgroup holds a long row or several short ones.  HBM bounds it: 16312 tokens
+// of 2048 in fp16 (134 MB at most, repeated rows come from the caches) take 16
+// us, 4096 of 4096 in bf16 (67 MB) 10.
 template <typename I, typename W, typename Y>
 __global__ __launch_bounds__(256) void embed_fwd(const I* __restrict__ ids, int64_t T,
                                                  const W* __restrict__ w, int64_t V, int h,
@@ -66,6 +69,9 @@ __global__ __launch_bounds__(256) void embed_fwd(const I* __restrict__ ids, int6
 }
 
 // ------------------------------------------------------------------- sort ---
+// Every workgroup reads all ids, from its die's L2: T 8 bytes each.  Vector
+// instructions (two ballots a chunk of 64 tokens) and the latency of those reads
+// bound it: 4096 tokens 8 us, 16312 10, 65536 31.
 // A token's id in 32 bits, or all ones for one that has no row of the table
 // (vocab < 2^28).
 __device__ __forceinline__ uint32_t id32(const int32_t* ids, int64_t t) {
@@ -219,7 +225,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
 // --------------------------------------------------------------- gradient ---
 // A wave's columns of a row: `lanes` chunks of 8 a slice.  The row's last chunk
 // ends with the row and may overlap the one before it, lanes behind it repeat
-// it: they read, compute and store the same values in the same instructions.
+// it: they read, compute and store the same values in the same instructions (why
+// not element by element: part8.h).
 // Rows of less than 8 columns are one chunk of h.
 struct Columns {
   int lanes, slices;  // chosen so that a slice has more than an overlapping chunk:
@@ -236,6 +243,11 @@ __device__ __forceinline__ int my_column(const Columns& cols, int slice, int h) 
 // its border (an id that does both: the first).  blk: tokens a block, up to 64
 // (a lane holds one).  kStream: dy is larger than the last-level cache, and its
 // rows take no place there.
+//
+// HBM bounds it: a table of 49152 x 4096 in bf16, 4096 tokens (403 MB written,
+// most of it zeros, 34 read) 80 us, 5.4 TB/s; 65536 tokens of 5120 in bf16 added
+// to an fp32 table (671 MB of dy, the named rows read and written: 1.29 GB) 267
+// us, 4.8 TB/s; 16312 tokens of 2048 in fp16, half of them padding, 30 us.
 template <typename D, typename W, bool kAdd, bool kStream>
 __global__ __launch_bounds__(256) void embed_grad(
     const D* __restrict__ dy, W* __restrict__ dw, const Token* __restrict__ tok,
@@ -341,9 +353,10 @@ __global__ __launch_bounds__(256) void embed_grad(
 // The partial sums of each id that crosses blocks, in order, 256 columns a
 // workgroup.  Each of 8 waves looks at a block and adds a few parts alone; the
 // parts of an id that spans many blocks are shared by the eight.  Latency
-// bounds it, not bytes: 16 parts are in flight at a time, and 65536 tokens of
-// 5120 columns, nine tenths of them one id, take 282 us in all where four waves
-// a workgroup took 320.
+// bounds it, not bytes: 7 us for the parts of 4096 tokens of 4096 columns, 22 for
+// 65536 of 5120.  16 parts are in flight at a time, and 65536 tokens of 5120,
+// nine tenths of them one id, take 282 us in all where four waves a workgroup
+// took 320.
 static constexpr int kJoinWaves = 8, kAloneParts = 16;
 
 __device__ __forceinline__ float4 add_parts(const float* part, int64_t j, int64_t a, int64_t b,
@@ -455,14 +468,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
 }
 
 // ------------------------------------------------------------- few tokens ---
+// Tokens that a wave holds, two a lane.  us in one launch / in three: 128 tokens
+// of 256 columns, 320 rows 5.1 / 12.5, added 5.6 / 13.5; one token 128 times 15.4
+// / 11.5 (a wave adds all rows in order, 16 at a time); 4096 columns and 49152
+// rows, mostly zeros, 73 / 81.
 static constexpr int kFew = 128;
 
-// A wave's 512 columns of kFillRows rows or, with kAdd, of the row that a
-// token names first.
+// A wave's 512 columns of `rows` rows or, with kAdd, of the row that a token
+// names first.
 template <typename I, typename D, typename W, bool kAdd>
 __global__ __launch_bounds__(256) void embed_few(
     const I* __restrict__ ids, int T, const D* __restrict__ dy, W* __restrict__ dw, uint32_t V, int h,
-    Columns cols, int64_t items, float scale, uint32_t pad) {
+    Columns cols, int rows, int64_t items, float scale, uint32_t pad) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,7 +503,23 @@ __global__ __launch_bounds__(256) void embed_few(
     if (kAdd) old.load(p, nc);
     float acc[8] = {};
     constexpr int kAhead = sizeof(D) == 2 ? 16 : 8;
-    while ((m0 | m1) != 0) {  // the tokens in order
+    // the tokens in order: those that fill rounds, then the others
+    for (int left = __popcll(m0) + __popcll(m1); left >= kAhead; left -= kAhead) {
+      Part8<D> x[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int t = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
+        if (m0 != 0) m0 &= m0 - 1;
+        else m1 &= m1 - 1;
+        x[k].load(dy + static_cast<int64_t>(t) * h + c, nc);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += x[k][q];
+      }
+    }
+    if ((m0 | m1) != 0) {
       Part8<D> x[kAhead];
       bool on[kAhead];
 #pragma unroll
@@ -516,8 +549,8 @@ __global__ __launch_bounds__(256) void embed_few(
     if (r != ~0u && first == t) row(r, m0, m1);
     return;
   }
-  const uint32_t r0 = static_cast<uint32_t>(group) * kFillRows;
-  for (uint32_t r = r0; r < r0 + kFillRows && r < V; ++r)
+  const uint32_t r0 = static_cast<uint32_t>(group) * rows;
+  for (uint32_t r = r0; r < r0 + rows && r < V; ++r)
     row(r, __ballot(key[0] == r), __ballot(key[1] == r));
 }
 
@@ -593,12 +626,15 @@ template <typename D, typename W, bool kAdd>
 static void launch_few(const void* ids, int ids_64, int64_t T, const void* dy, void* dw, int64_t V,
                        int64_t h, float scale, uint32_t pad, hipStream_t st) {
   const Columns cols = columns(h);
-  const int64_t items = (kAdd ? T : (V + kFillRows - 1) / kFillRows) * cols.slices;
+  // rows a wave, one after another: up to kFillRows while there are 4096 waves
+  int rows = kFillRows;
+  while (rows > 1 && V / rows * cols.slices < 4096) rows >>= 1;
+  const int64_t items = (kAdd ? T : (V + rows - 1) / rows) * cols.slices;
   const dim3 grid(static_cast<unsigned>((items + 3) / 4));
 #define ZK_FEW(I)                                                                                \
   hipLaunchKernelGGL((embed_few<I, D, W, kAdd>), grid, dim3(256), 0, st, (const I*)ids,          \
                      static_cast<int>(T), (const D*)dy, (W*)dw, static_cast<uint32_t>(V),        \
-                     static_cast<int>(h), cols, items, scale, pad)
+                     static_cast<int>(h), cols, rows, items, scale, pad)
   if (ids_64) ZK_FEW(int64_t); else ZK_FEW(int32_t);
 #undef ZK_FEW
 }
