@@ -28,10 +28,12 @@ namespace zk {
 static constexpr int kSortWaves = 16;
 static constexpr int kMaxSlots = 512;   // ids a sort workgroup owns: 32 KB of counters
 static constexpr int kList = 448;       // found tokens a wave remembers: 28 KB
-static constexpr int kFillRows = 8;     // table rows a filling wave looks at
 
 struct Token {
   int t, id;
+};
+struct Fill {  // the rows that a workgroup looks at, 2^log_tpr threads each
+  int rows, log_tpr;
 };
 struct Span {  // the id that crosses out of the block where it begins (-1: none)
   int id, parts;
@@ -238,6 +240,25 @@ __device__ __forceinline__ int my_column(const Columns& cols, int slice, int h) 
   return h < 8 ? 0 : c < h - 8 ? c : h - 8;
 }
 
+// Zeros for the rows r0 + i of the set bits i of `empty`, by a workgroup: each of
+// its accesses writes neighbouring 16 bytes a thread, 4 KB, of one row or of
+// several.  Lines are written whole: nontemporal stores of half lines (8 fp32 a
+// lane) took 2.4 times as long.
+template <typename W>
+__device__ __forceinline__ void fill_rows(W* dw, int64_t r0, uint64_t empty, int h, const Fill& fill) {
+  constexpr int E = 16 / sizeof(W);
+  typedef W V __attribute__((ext_vector_type(E)));
+  typedef V Vu __attribute__((aligned(sizeof(W))));
+  const int tpr = 1 << fill.log_tpr;
+  for (int i = threadIdx.x >> fill.log_tpr; i < fill.rows; i += 256 >> fill.log_tpr) {
+    if (!(empty >> i & 1)) continue;
+    W* p = dw + (r0 + i) * h;
+    int c = (threadIdx.x & (tpr - 1)) * E;
+    for (; c + E <= h; c += tpr * E) __builtin_nontemporal_store(V{}, reinterpret_cast<Vu*>(p + c));
+    for (int j = c; j < h && j < c + E; ++j) __builtin_nontemporal_store(static_cast<W>(0.f), p + j);
+  }
+}
+
 // part: [blocks][2][hp] fp32 (hp: part_row(h)): the sum of the id that
 // a block begins with and of the one that it ends in, where they reach over
 // its border (an id that does both: the first).  blk: tokens a block, up to 64
@@ -245,25 +266,23 @@ __device__ __forceinline__ int my_column(const Columns& cols, int slice, int h) 
 // rows take no place there.
 //
 // HBM bounds it: a table of 49152 x 4096 in bf16, 4096 tokens (403 MB written,
-// most of it zeros, 34 read) 80 us, 5.4 TB/s; 65536 tokens of 5120 in bf16 added
+// most of it zeros, 34 read) 68 us, 6.4 TB/s; 65536 tokens of 5120 in bf16 added
 // to an fp32 table (671 MB of dy, the named rows read and written: 1.29 GB) 267
-// us, 4.8 TB/s; 16312 tokens of 2048 in fp16, half of them padding, 30 us.
+// us, 4.8 TB/s; 16312 tokens of 2048 in fp16, half of them padding, 28 us.
 template <typename D, typename W, bool kAdd, bool kStream>
 __global__ __launch_bounds__(256) void embed_grad(
     const D* __restrict__ dy, W* __restrict__ dw, const Token* __restrict__ tok,
     const int* __restrict__ count, const int* __restrict__ total, float* __restrict__ part,
     Span* __restrict__ span, int64_t V, int h, int hp, Columns cols, int blk, int64_t sum_items,
-    float scale) {
+    Fill fill, float scale) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= sum_items) {  // rows of ids without tokens
-    if (kAdd) return;       // (a wave that rounds the last workgroup up)
-    const int64_t r0 = (item - sum_items) * kFillRows;
-    for (int64_t r = r0; r < r0 + kFillRows && r < V; ++r) {
-      if (count[r] != 0) continue;
-      for (int c = lane * 8; c < h; c += 512) Part8<W>::store_zero_nt(dw + r * h + c, h - c);
-    }
+  if (item >= sum_items) {
+    const int64_t wg = blockIdx.x - (sum_items + 3) / 4;
+    if (kAdd || wg < 0) return;  // a wave that rounds the sums' last workgroup up
+    const int64_t r0 = wg * fill.rows, r = r0 + lane;
+    fill_rows(dw, r0, __ballot(lane < fill.rows && r < V && count[r < V ? r : 0] == 0), h, fill);
     return;
   }
   const int64_t j = item / cols.slices;
@@ -471,21 +490,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join(
 // Tokens that a wave holds, two a lane.  us in one launch / in three: 128 tokens
 // of 256 columns, 320 rows 5.1 / 12.5, added 5.6 / 13.5; one token 128 times 15.4
 // / 11.5 (a wave adds all rows in order, 16 at a time); 4096 columns and 49152
-// rows, mostly zeros, 73 / 81.
+// rows, mostly zeros, 61 / 69.
 static constexpr int kFew = 128;
 
-// A wave's 512 columns of `rows` rows or, with kAdd, of the row that a token
-// names first.
+// A wave's 512 columns of the row that a token names first; waves after those
+// fill the rows that no token names.
 template <typename I, typename D, typename W, bool kAdd>
 __global__ __launch_bounds__(256) void embed_few(
     const I* __restrict__ ids, int T, const D* __restrict__ dy, W* __restrict__ dw, uint32_t V, int h,
-    Columns cols, int rows, int64_t items, float scale, uint32_t pad) {
+    Columns cols, Fill fill, float scale, uint32_t pad) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= items) return;
-  const int64_t group = item / cols.slices;
-  const int c = my_column(cols, static_cast<int>(item - group * cols.slices), h), nc = h < 8 ? h : 8;
   uint32_t key[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -493,65 +509,68 @@ __global__ __launch_bounds__(256) void embed_few(
     key[k] = t < T ? id32(ids, t) : ~0u;
     key[k] = key[k] < V && key[k] != pad ? key[k] : ~0u;
   }
-  auto row = [&](uint32_t r, uint64_t m0, uint64_t m1) {
-    W* p = dw + static_cast<int64_t>(r) * h + c;
-    if ((m0 | m1) == 0) {
-      Part8<W>::store_zero_nt(p, nc);
-      return;
+  const int64_t sums = static_cast<int64_t>(T) * cols.slices;
+  if (item >= sums) {
+    const int64_t wg = blockIdx.x - (sums + 3) / 4;
+    if (kAdd || wg < 0) return;  // a wave that rounds the sums' last workgroup up
+    const int64_t r0 = wg * fill.rows;
+    uint64_t empty = 0;
+    for (int i = 0; i < fill.rows && r0 + i < V; ++i) {
+      const uint32_t r = static_cast<uint32_t>(r0) + i;
+      if ((__ballot(key[0] == r) | __ballot(key[1] == r)) == 0) empty |= 1ull << i;
     }
-    Part8<W> old;
-    if (kAdd) old.load(p, nc);
-    float acc[8] = {};
-    constexpr int kAhead = sizeof(D) == 2 ? 16 : 8;
-    // the tokens in order: those that fill rounds, then the others
-    for (int left = __popcll(m0) + __popcll(m1); left >= kAhead; left -= kAhead) {
-      Part8<D> x[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int t = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
-        if (m0 != 0) m0 &= m0 - 1;
-        else m1 &= m1 - 1;
-        x[k].load(dy + static_cast<int64_t>(t) * h + c, nc);
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += x[k][q];
-      }
-    }
-    if ((m0 | m1) != 0) {
-      Part8<D> x[kAhead];
-      bool on[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        on[k] = (m0 | m1) != 0;
-        const int t = m0 != 0 ? __builtin_ctzll(m0) : 64 + (m1 != 0 ? __builtin_ctzll(m1) : 0);
-        if (m0 != 0) m0 &= m0 - 1;
-        else m1 &= m1 - 1;
-        x[k].load(dy + static_cast<int64_t>(on[k] ? t : 0) * h + c, nc);
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += on[k] ? x[k][q] : 0.f;
-      }
-    }
-    float o[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) o[q] = kAdd ? old[q] + scale * acc[q] : scale * acc[q];
-    Part8<W>::store(p, o, nc);
-  };
-  if (kAdd) {
-    const int t = static_cast<int>(group);
-    const uint32_t r = __builtin_amdgcn_readlane(t < 64 ? key[0] : key[1], t & 63);
-    const uint64_t m0 = __ballot(key[0] == r), m1 = __ballot(key[1] == r);
-    const int first = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
-    if (r != ~0u && first == t) row(r, m0, m1);
+    fill_rows(dw, r0, empty, h, fill);
     return;
   }
-  const uint32_t r0 = static_cast<uint32_t>(group) * rows;
-  for (uint32_t r = r0; r < r0 + rows && r < V; ++r)
-    row(r, __ballot(key[0] == r), __ballot(key[1] == r));
+  const int t = static_cast<int>(item / cols.slices);
+  const uint32_t r = __builtin_amdgcn_readlane(t < 64 ? key[0] : key[1], t & 63);
+  uint64_t m0 = __ballot(key[0] == r), m1 = __ballot(key[1] == r);
+  const int first = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
+  if (r == ~0u || first != t) return;
+  const int c = my_column(cols, static_cast<int>(item - t * static_cast<int64_t>(cols.slices)), h);
+  const int nc = h < 8 ? h : 8;
+  W* p = dw + static_cast<int64_t>(r) * h + c;
+  Part8<W> old;
+  if (kAdd) old.load(p, nc);
+  float acc[8] = {};
+  constexpr int kAhead = sizeof(D) == 2 ? 16 : 8;
+  // the tokens in order: those that fill rounds, then the others
+  for (int left = __popcll(m0) + __popcll(m1); left >= kAhead; left -= kAhead) {
+    Part8<D> x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int next = m0 != 0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
+      if (m0 != 0) m0 &= m0 - 1;
+      else m1 &= m1 - 1;
+      x[k].load(dy + static_cast<int64_t>(next) * h + c, nc);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] += x[k][q];
+    }
+  }
+  if ((m0 | m1) != 0) {
+    Part8<D> x[kAhead];
+    bool on[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      on[k] = (m0 | m1) != 0;
+      const int next = m0 != 0 ? __builtin_ctzll(m0) : 64 + (m1 != 0 ? __builtin_ctzll(m1) : 0);
+      if (m0 != 0) m0 &= m0 - 1;
+      else m1 &= m1 - 1;
+      x[k].load(dy + static_cast<int64_t>(on[k] ? next : 0) * h + c, nc);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] += on[k] ? x[k][q] : 0.f;
+    }
+  }
+  float o[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) o[q] = kAdd ? old[q] + scale * acc[q] : scale * acc[q];
+  Part8<W>::store(p, o, nc);
 }
 
 // The groups of embed_sort: at least 256 workgroups, at most kMaxSlots ids each.
@@ -598,6 +617,19 @@ static bool embed_sizes_ok(int64_t T, int64_t V, int64_t h) {
          h < (int64_t(1) << 23);
 }
 
+// Rows that a filling workgroup looks at, up to a wave's lanes: 8 KB of rows
+// above 4 KB, 16 KB of shorter ones, less while there would be less than 1024
+// workgroups.  us of the whole gradient at 8 / 16 / 64 KB: 4096 tokens, 49152 rows
+// of 8 KB 83 / 91 / 98, 16312 tokens, 32000 rows of 4 KB 60.5 / 58.3 / 60.7, 8192
+// tokens, 32000 rows of 2 KB 32.1 / 30.7 / 30.9.
+static Fill rows_to_fill(int64_t V, int64_t row_bytes) {
+  const int64_t most = row_bytes > 4096 ? 8192 : 16384;
+  Fill f{64, 0};
+  while (f.rows > 1 && (f.rows * row_bytes > most || V / f.rows < 1024)) f.rows >>= 1;
+  while (f.log_tpr < 8 && (int64_t(16) << f.log_tpr) < row_bytes) ++f.log_tpr;
+  return f;
+}
+
 template <typename I, typename W>
 static void launch_fwd(const void* ids, int64_t T, const void* w, int64_t V, int64_t h, void* y,
                        int ydt, float scale, hipStream_t st) {
@@ -626,15 +658,13 @@ template <typename D, typename W, bool kAdd>
 static void launch_few(const void* ids, int ids_64, int64_t T, const void* dy, void* dw, int64_t V,
                        int64_t h, float scale, uint32_t pad, hipStream_t st) {
   const Columns cols = columns(h);
-  // rows a wave, one after another: up to kFillRows while there are 4096 waves
-  int rows = kFillRows;
-  while (rows > 1 && V / rows * cols.slices < 4096) rows >>= 1;
-  const int64_t items = (kAdd ? T : (V + rows - 1) / rows) * cols.slices;
-  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+  const Fill fill = rows_to_fill(V, h * static_cast<int64_t>(sizeof(W)));
+  const dim3 grid(static_cast<unsigned>((T * cols.slices + 3) / 4 +
+                                        (kAdd ? 0 : (V + fill.rows - 1) / fill.rows)));
 #define ZK_FEW(I)                                                                                \
   hipLaunchKernelGGL((embed_few<I, D, W, kAdd>), grid, dim3(256), 0, st, (const I*)ids,          \
                      static_cast<int>(T), (const D*)dy, (W*)dw, static_cast<uint32_t>(V),        \
-                     static_cast<int>(h), cols, rows, items, scale, pad)
+                     static_cast<int>(h), cols, fill, scale, pad)
   if (ids_64) ZK_FEW(int64_t); else ZK_FEW(int32_t);
 #undef ZK_FEW
 }
@@ -647,17 +677,18 @@ static void launch_grad(const void* dy, void* dw, const Token* tok, const int* c
   const Columns cols = columns(h);
   const int blk = embed_block(T, h);
   const int64_t blocks = embed_blocks(T, h), sums = blocks * cols.slices;
-  const int64_t items = sums + (kAdd ? 0 : (V + kFillRows - 1) / kFillRows);
-  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+  const Fill fill = rows_to_fill(V, h * static_cast<int64_t>(sizeof(W)));
+  const dim3 grid(static_cast<unsigned>((sums + 3) / 4 + (kAdd ? 0 : (V + fill.rows - 1) / fill.rows)));
 #define ZK_GRAD(S)                                                                            \
   hipLaunchKernelGGL((embed_grad<D, W, kAdd, S>), grid, dim3(256), 0, st, (const D*)dy, (W*)dw, \
-                     tok, count, total, part, span, V, static_cast<int>(h), hp, cols, blk, sums, scale)
+                     tok, count, total, part, span, V, static_cast<int>(h), hp, cols, blk, sums, fill, \
+                     scale)
   // dy within the 256 MB of last-level cache may still be there from the kernel
   // that wrote it.  us with streaming loads / ordinary ones: 65536 tokens of
   // 5120 (671 MB), a text's ids 337 / 348, nine tenths one id 361 / 427; 8192 of
   // 1000 (16 MB, fresh) 35 / 31, 4096 of 4096 (34 MB) 94 / 92
   const bool stream = T * h * static_cast<int64_t>(sizeof(D)) > (int64_t(1) << 28);
-  if (items > 0) {
+  if (grid.x > 0) {
     if (stream) ZK_GRAD(true); else ZK_GRAD(false);
   }
 #undef ZK_GRAD

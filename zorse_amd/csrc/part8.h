@@ -33,14 +33,6 @@ struct Part8 {
     for (int i = 0; i < 8; ++i) u[i] = i < n ? p[i] : static_cast<T>(0.f);
   }
   __device__ __forceinline__ float operator[](int i) const { return static_cast<float>(u[i]); }
-  // zeros that nothing reads soon
-  static __device__ __forceinline__ void store_zero_nt(T* p, int n) {
-    if (n >= 8) {
-      __builtin_nontemporal_store(V8{}, reinterpret_cast<V8u*>(p));
-      return;
-    }
-    for (int i = 0; i < n; ++i) __builtin_nontemporal_store(static_cast<T>(0.f), p + i);
-  }
   static __device__ __forceinline__ void store(T* p, const float (&v)[8], int n) {
     if (n >= 8) {
       V8 w;
