@@ -264,3 +264,24 @@ def test_second_differentiation_is_refused(dev):
     dq, = torch.autograd.grad(y, q, torch.ones_like(y, requires_grad=True), create_graph=True)
     with pytest.raises(RuntimeError, match="differentiated once"):
         dq.sum().backward()
+
+
+def test_gradient_of_one_output(dev):
+    """A loss of q' alone: k and its weight have zero gradients, q's are those
+    without k."""
+    from zorse_amd import functional
+    g = torch.Generator().manual_seed(5)
+    q, k = (torch.randn(2, 7, h, 24, generator=g).to(dev).requires_grad_() for h in (3, 1))
+    w = [torch.randn(24, generator=g).to(dev).requires_grad_() for _ in range(2)]
+    cos, sin = (t.to(dev) for t in _tables(7, 24))
+    dy = torch.randn(2, 7, 3, 24, generator=g).to(dev)
+    y, _ = functional.qk_norm_rope(q, k, *w, cos, sin)
+    dq, dk, dwq, dwk = torch.autograd.grad(y, (q, k, *w), dy)
+    alone, none = functional.qk_norm_rope(q, None, w[0], None, cos, sin)
+    want = torch.autograd.grad(alone, (q, w[0]), dy)
+    assert none is None and torch.equal(y, alone)
+    assert torch.equal(dq, want[0]) and not bool(dk.any()) and not bool(dwk.any())
+    # dw: the same 42 products, over as many workgroups' partial sums or other
+    # ones: 42 roundings of sums below 42 max|dn x r|
+    bound = 42 * 2.0 ** -24 * 42 * float((dy.abs().max() * 2) * 24 ** 0.5)
+    assert bool(((dwq - want[1]).abs() <= bound).all())
