@@ -119,7 +119,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
   const int chunks = (T + 64 * kSortWaves - 1) / (64 * kSortWaves);
   const int64_t t0 = static_cast<int64_t>(wave) * chunks * 64;
   const int64_t end = t0 + chunks * 64 < T ? t0 + chunks * 64 : T;
-  const uint32_t first = g << (32 - log_g), last = first | (slots - 1);  // this group's keys
+  const uint32_t first = g << (32 - log_g), own = slots;  // this group's keys: first + slot
   int* mine = cnt + wave * slots;
   const uint64_t below = (1ull << lane) - 1;
   int before = 0, found = 0, again = -1;  // again: the first chunk that the list does not hold
@@ -130,17 +130,17 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       before += __popcll(__ballot(key[k] < first));
-      const uint64_t m = __ballot(key[k] >= first && key[k] <= last);
+      const uint32_t slot = key[k] - first;
+      const bool is = slot < own;
+      const uint64_t m = __ballot(is);
       if (m == 0) continue;
-      const int slot = static_cast<int>(key[k] - first);
-      const bool is = (m >> lane) & 1;
       const int n = __popcll(m);
       if (n <= 8) {
         if (is) atomicAdd(mine + slot, 1);
       } else {  // mostly one id: one lane adds for all of an id's
         for (uint64_t left = m; left != 0;) {
           const int lead = __builtin_ctzll(left);
-          const uint64_t same = __ballot(is && slot == __builtin_amdgcn_readlane(slot, lead));
+          const uint64_t same = left & __ballot(slot == __builtin_amdgcn_readlane(slot, lead));
           if (lane == lead) atomicAdd(mine + slot, __popcll(same));
           left &= ~same;
         }
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort(
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       place(static_cast<int>(key[k] - first), static_cast<int>(t0 + (c0 + k) * 64 + lane),
-            __ballot(key[k] >= first && key[k] <= last));
+            __ballot(key[k] - first < own));
   }
 }
 
