@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void embed_fwd(const I* __restrict__ ids, int6
 // ------------------------------------------------------------------- sort ---
 // Every workgroup reads all ids, from its die's L2: T 8 bytes each.  Vector
 // instructions (two ballots a chunk of 64 tokens) and the latency of those reads
-// bound it: 4096 tokens 8 us, 16312 10, 65536 31.
+// bound it: 4096 tokens 8 us, 16312 9, 65536 31.
 // A token's id in 32 bits, or all ones for one that has no row of the table
 // (vocab < 2^28).
 __device__ __forceinline__ uint32_t id32(const int32_t* ids, int64_t t) {
