@@ -257,6 +257,10 @@ zk_qk_desc qk_checked(const Qk& A, double eps, bool interleaved, const Tensor& q
   const Tensor &q = A.q, &k = A.k;
   if (q.dim() != 4) bad("q must be [B, S, H, d]");
   if (k.defined() != A.wk.defined()) bad("k and k_weight belong together");
+  // both or none: a missing one would be made new and contiguous, and written
+  // with the given one's strides
+  if ((qo.defined() || ko.defined()) && !(qo.defined() && ko.defined() == k.defined()))
+    bad("an output for each of q and k is needed");
   one_gpu({&q, &k, &A.wq, &A.wk, &A.cos, &A.sin, &A.positions, &qo, &ko, &gq, &gk});
   zk_qk_desc D{};
   D.B = q.size(0), D.S = q.size(1), D.Hq = q.size(2), D.d = q.size(3);
@@ -276,7 +280,6 @@ zk_qk_desc qk_checked(const Qk& A, double eps, bool interleaved, const Tensor& q
       bad(c10::str("k_weight must be contiguous [", D.d, "] of q_weight's dtype"));
     D.Hkv = k.size(2);
   }
-  if (k.defined() != ko.defined() && qo.defined()) bad("an output for each of q and k is needed");
   Strides s = strides_over("q", q, q, false);
   D.q_sb = s.b, D.q_ss = s.s, D.q_sh = s.h;
   s = qo.defined() ? strides_over("q output", qo, q, true) : contiguous_strides(q);
