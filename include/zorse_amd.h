@@ -534,7 +534,8 @@ int zk_qk_norm_rope_fwd(const zk_qk_desc* desc, const void* q, const void* k,
                         const void* wq, const void* wk, void* q_out, void* k_out,
                         const float* cos, const float* sin, const int64_t* positions,
                         zk_stream_t stream);
-/* Bytes of workspace of the backward (dw's partial sums). */
+/* Bytes of workspace of the backward (dw's partial sums).  dwk of Hkv 0 may be
+ * NULL; one that is given is zeroed. */
 int64_t zk_qk_norm_rope_bwd_workspace(int64_t d);
 int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const void* k,
                         const void* wq, const void* wk, const void* dq_out,

@@ -475,8 +475,8 @@ extern "C" int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const 
   A.part = static_cast<float*>(workspace);
   hipStream_t st = as_stream(stream);
   if (A.rows > 0) launch_qk<true>(A, desc->dtype, desc->pairing, log_lanes(desc->d), st);
-  // without rows there are no partial rows: dw is zero
-  hipLaunchKernelGGL(qk_dw, dim3(static_cast<unsigned>((A.d + 15) / 16), desc->Hkv > 0 ? 2 : 1),
+  // without rows, or of keys without a head, there are no partial rows: dw is zero
+  hipLaunchKernelGGL(qk_dw, dim3(static_cast<unsigned>((A.d + 15) / 16), dwk ? 2 : 1),
                      dim3(1024), 0, st, A.part, A.q.wgs, A.k.wgs, A.d, dwq, dwk, A.w_dt);
   return launch_status("zk_qk_norm_rope_bwd");
 }
