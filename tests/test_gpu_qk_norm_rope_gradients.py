@@ -35,3 +35,20 @@ def test_key_weight_without_key_heads(dev, wdt, d):
     assert y[1].shape == k.shape
     grads = torch.autograd.grad(y, leaves, (dq, k))
     assert torch.equal(grads[3], torch.zeros_like(wk)) and torch.equal(grads[2], want[2])
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_penalty_of_gradients_is_refused(dev, which):
+    """A gradient for a constant dy depends on q, k and the weights all the same:
+    with create_graph it has a node that says that it cannot be differentiated,
+    instead of counting as a constant."""
+    from zorse_amd import functional
+    *args, cos, sin = _inputs(dev, 4, 2)
+    x = args[which].requires_grad_()
+    y = functional.qk_norm_rope(*args, cos, sin)
+    total = y[0].sum() + y[1].square().sum().detach() + y[1].sum()
+    plain, = torch.autograd.grad(total, x, retain_graph=True)
+    dx, = torch.autograd.grad(total, x, create_graph=True)
+    assert torch.equal(dx, plain) and dx.requires_grad
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        (total + dx.square().sum()).backward()

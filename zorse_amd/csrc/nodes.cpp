@@ -376,8 +376,9 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     if (gk.defined()) D.dyk_sb = gk.stride(0), D.dyk_ss = gk.stride(1), D.dyk_sh = gk.stride(2);
     variable_list out = qk_bwd(A, D, gq, gk, Tensor(), Tensor());
     out.resize(8);
-    if (!at::GradMode::is_enabled() || !(gq.requires_grad() || (gk.defined() && gk.requires_grad())))
-      return out;
+    // dx and dw depend on the saved inputs as well as on dy, one of which
+    // requires a gradient
+    if (!at::GradMode::is_enabled()) return out;
     // create_graph: what is differentiated once more says so
     for (Tensor& t : out)
       if (t.defined()) t.requires_grad_(true);
