@@ -80,6 +80,18 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// Forward-mode derivatives: a dual tensor carries its tangent beside its values.
+bool is_dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
+// f(t) for a linear f and a dual t, a dual tensor too.
+template <typename F>
+Tensor linear_of_dual(const Tensor& t, const F& f) {
+  const auto [values, tangent] = at::_unpack_dual(t, /*level=*/0);
+  // torch's own zeros may have no memory
+  const Tensor held = tangent._is_zerotensor() ? at::zeros(tangent.sizes(), values.options()) : tangent;
+  return at::_make_dual(f(values), f(held), /*level=*/0);
+}
+
 // -------------------------------------------------------- token embedding ---
 void check_ids(const Tensor& ids) {
   if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong)
@@ -155,11 +167,21 @@ Tensor embedding_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, double 
   return dw;
 }
 
+// Both nodes know no tangents: apply() is for tensors without one, and
+// embedding_of and table_gradient for all.
 struct Embedding : torch::autograd::Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale,
                         int64_t pad, int64_t y_code);
   static variable_list backward(AutogradContext* ctx, variable_list dy);
 };
+
+Tensor embedding_of(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, int64_t y_code) {
+  if (is_dual(weight))
+    return linear_of_dual(weight, [&](const Tensor& w) {
+      return embedding_of(ids, w.contiguous(), scale, pad, y_code);
+    });
+  return Embedding::apply(ids, weight, scale, pad, y_code);
+}
 
 // The table's gradient as a function of dy (a second differentiation): linear
 // in it, and its gradient is the lookup, without the tokens that have none.
@@ -179,10 +201,23 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor none = ids.lt(0).logical_or_(ids.ge(cfg[0]));
     if (cfg[1] >= 0) none.logical_or_(ids.eq(cfg[1]));
-    const Tensor ddy = Embedding::apply(ids, ddw[0].contiguous(), scale, cfg[1], cfg[2]);
+    const Tensor ddy = embedding_of(ids, ddw[0].contiguous(), scale, cfg[1], cfg[2]);
     return {Tensor(), ddy.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
+
+Tensor table_gradient(const Tensor& ids, const Tensor& dy, int64_t vocab, double scale, int64_t pad,
+                      int64_t w_code) {
+  if (is_dual(dy))
+    return linear_of_dual(dy, [&](const Tensor& g) {
+      return table_gradient(ids, g.contiguous(), vocab, scale, pad, w_code);
+    });
+  if (at::GradMode::is_enabled() && dy.requires_grad())  // create_graph
+    return EmbeddingGrad::apply(ids, dy, vocab, scale, pad, w_code);
+  const Tensor dw = at::empty({vocab, dy.size(-1)}, dy.options().dtype(type_of(w_code)));
+  embedding_grad(ids, dy, dw, scale, pad, false);
+  return dw;
+}
 
 Tensor Embedding::forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale,
                           int64_t pad, int64_t y_code) {
@@ -197,14 +232,7 @@ variable_list Embedding::backward(AutogradContext* ctx, variable_list dy) {
   const auto cfg = ctx->saved_data["cfg"].toIntVector();
   const double scale = ctx->saved_data["scale"].toDouble();
   const Tensor g = dy[0].contiguous();
-  Tensor dw;
-  if (at::GradMode::is_enabled() && g.requires_grad()) {  // create_graph
-    dw = EmbeddingGrad::apply(ids, g, cfg[0], scale, cfg[1], cfg[2]);
-  } else {
-    dw = at::empty({cfg[0], g.size(-1)}, g.options().dtype(type_of(cfg[2])));
-    embedding_grad(ids, g, dw, scale, cfg[1], false);
-  }
-  return {Tensor(), dw, Tensor(), Tensor(), Tensor()};
+  return {Tensor(), table_gradient(ids, g, cfg[0], scale, cfg[1], cfg[2]), Tensor(), Tensor(), Tensor()};
 }
 
 // functional.embedding
@@ -218,9 +246,9 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, std::opt
     pad = *padding < 0 ? *padding + rows : *padding;
   }
   const Tensor i = ids.contiguous(), w = weight.contiguous();
-  if (!at::GradMode::is_enabled() || !w.requires_grad())
+  if (!is_dual(w) && (!at::GradMode::is_enabled() || !w.requires_grad()))
     return embedding_fwd(i, w, scale, dtype, MaybeTensor());
-  return Embedding::apply(i, w, scale, pad, float_code("output", dtype.value_or(w.scalar_type())));
+  return embedding_of(i, w, scale, pad, float_code("output", dtype.value_or(w.scalar_type())));
 }
 
 // ---------------------------------------- norm of q and k heads, rotation ---
