@@ -52,3 +52,28 @@ def test_penalty_of_gradients_is_refused(dev, which):
     assert torch.equal(dx, plain) and dx.requires_grad
     with pytest.raises(RuntimeError, match="differentiated once"):
         (total + dx.square().sum()).backward()
+
+
+@pytest.mark.parametrize("which", range(6))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(dev, which, grad):
+    """A tangent of any input, instead of being dropped."""
+    import torch.autograd.forward_ad as fwad
+    from zorse_amd import functional
+    args = [t.requires_grad_(grad and i < 4) for i, t in enumerate(_inputs(dev, 4, 2))]
+    with fwad.dual_level():
+        args[which] = fwad.make_dual(args[which].detach(), torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward"):
+            functional.qk_norm_rope(*args)
+
+
+def test_forward_over_reverse_is_refused(dev):
+    import torch.autograd.forward_ad as fwad
+    from zorse_amd import functional
+    q, k, wq, wk, cos, sin = _inputs(dev, 4, 2)
+    q.requires_grad_()
+    y = functional.qk_norm_rope(q, k, wq, wk, cos, sin)
+    with fwad.dual_level():
+        dy = fwad.make_dual(torch.ones_like(y[0]), torch.ones_like(y[0]))
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(y[0], q, dy)

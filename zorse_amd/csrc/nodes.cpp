@@ -278,6 +278,12 @@ Strides strides_over(const char* name, const Tensor& x, const Tensor& t, bool ou
   return Strides{x.stride(0), x.stride(1), x.stride(2)};
 }
 
+// Neither direction has a forward-mode derivative.
+void no_tangents(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (is_dual(*t)) throw std::runtime_error("qk_norm_rope has no forward-mode derivative");
+}
+
 // The checks of both directions.  qo, ko: y or dx (undefined: new contiguous
 // tensors); gq, gk: dy, of the backward.
 zk_qk_desc qk_checked(const Qk& A, double eps, bool interleaved, const Tensor& qo, const Tensor& ko,
@@ -400,6 +406,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     zk_qk_desc D;
     std::memcpy(&D, ctx->saved_data["desc"].toStringRef().data(), sizeof(D));
     const Tensor gq = rows_of(dy[0]), gk = A.k.defined() ? rows_of(dy[1]) : Tensor();
+    no_tangents({&gq, &gk});
     D.dyq_sb = gq.stride(0), D.dyq_ss = gq.stride(1), D.dyq_sh = gq.stride(2);
     if (gk.defined()) D.dyk_sb = gk.stride(0), D.dyk_ss = gk.stride(1), D.dyk_sh = gk.stride(2);
     variable_list out = qk_bwd(A, D, gq, gk, Tensor(), Tensor());
@@ -423,6 +430,7 @@ QkPair qk_norm_rope(const Tensor& q, const MaybeTensor& k, const Tensor& wq, con
                     bool interleaved) {
   const Qk A{rows_of(q), rows_of(given(k)), wq, given(wk), cos, sin, given(positions)};
   const zk_qk_desc D = qk_checked(A, eps, interleaved, Tensor(), Tensor(), Tensor(), Tensor());
+  no_tangents({&A.q, &A.k, &A.wq, &A.wk, &A.cos, &A.sin});
   bool grad = false;
   for (const Tensor* t : {&A.q, &A.k, &A.wq, &A.wk}) grad = grad || (t->defined() && t->requires_grad());
   if (!grad || !at::GradMode::is_enabled()) {
