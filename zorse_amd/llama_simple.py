@@ -119,13 +119,23 @@ class TokenEmbedding(nn.Embedding):
     """nn.Embedding whose lookup and gradient run on the embedding kernels
     (functional.embedding).  A table on the CPU, of another type than the
     kernels' three, or with options that they do not have (max_norm,
-    scale_grad_by_freq, sparse) is nn.Embedding's."""
+    scale_grad_by_freq, sparse) is nn.Embedding's, and so are calls that no
+    kernel can serve: of tensors without memory of their own (fake and
+    distributed ones, those of torch.func's transforms) and while torch records
+    the operations (torch.compile, torch.export, torch.jit.trace)."""
 
     def forward(self, input):
-        if not self.weight.is_cuda or self.max_norm is not None or self.scale_grad_by_freq \
-                or self.sparse or self.weight.dtype not in K.FLOAT_DTYPES:
+        w = self.weight
+        if not w.is_cuda or self.max_norm is not None or self.scale_grad_by_freq or self.sparse \
+                or w.dtype not in K.FLOAT_DTYPES or not (_has_memory(w) and _has_memory(input)) \
+                or torch.compiler.is_compiling() or torch.jit.is_tracing():
             return super().forward(input)
-        return Fn.embedding(input, self.weight, padding_idx=self.padding_idx)
+        return Fn.embedding(input, w, padding_idx=self.padding_idx)
+
+
+def _has_memory(t):
+    return type(t) in (torch.Tensor, nn.Parameter) \
+        and not torch._C._functorch.is_functorch_wrapped_tensor(t)
 
 
 class LlamaAttention(nn.Module):
