@@ -1,0 +1,75 @@
+"""Loading optimizer states as torch.optim.Optimizer does: hooks (CPU)."""
+import copy
+
+import pytest
+import torch
+
+from zorse_amd import optim
+
+
+def _saved(bits=32, dt=torch.float32):
+    """(parameter, state dict) after a step: moments 0.5 and 2."""
+    p = torch.nn.Parameter(torch.ones(6, dtype=dt))
+    opt = optim.FusedAdamW([p], state_bits=bits)
+    st = opt._init_state(p)
+    st["step"] = 3
+    st["exp_avg"].fill_(0.5 if bits == 32 else 5)
+    st["exp_avg_sq"].fill_(2)
+    return p, opt.state_dict()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_pre_hooks_decide_what_is_loaded(in_place):
+    p, saved = _saved()
+
+    def tenfold(opt, sd):
+        state = {k: {**v, "exp_avg": v["exp_avg"] * 10} for k, v in sd["state"].items()}
+        if in_place:  # the dictionary is torch's own copy
+            sd["state"] = state
+            return None
+        return {**sd, "state": state}
+
+    opt = optim.FusedAdamW([p])
+    opt.register_load_state_dict_pre_hook(tenfold)
+    opt.load_state_dict(saved)
+    assert bool((opt.state[p]["exp_avg"] == 5.0).all()) and opt.state[p]["step"] == 3
+    assert bool((saved["state"][0]["exp_avg"] == 0.5).all())
+    opt.load_state_dict(saved)  # again: no hook of the load itself stays behind
+    assert bool((opt.state[p]["exp_avg"] == 5.0).all())
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == 1
+    assert len(opt._optimizer_load_state_dict_post_hooks) == 0
+
+
+def test_pre_hooks_may_convert_other_moments():
+    """A checkpoint of another width that a hook makes fit is not refused; one
+    that a hook makes unfit is, and leaves the optimizer alone."""
+    p, narrow = _saved(8)
+    _, wide = _saved(32)
+    opt = optim.FusedAdamW([p])
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.load_state_dict(narrow)
+    assert not opt.state and not opt._optimizer_load_state_dict_pre_hooks
+    hook = opt.register_load_state_dict_pre_hook(lambda o, sd: copy.deepcopy(wide))
+    opt.load_state_dict(narrow)
+    assert bool((opt.state[p]["exp_avg"] == 0.5).all())
+    hook.remove()
+    opt.register_load_state_dict_pre_hook(lambda o, sd: copy.deepcopy(narrow))
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.load_state_dict(wide)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_post_hooks_find_and_change_the_state(dt):
+    p, saved = _saved(dt=dt)
+    seen = []
+
+    def halve(opt):
+        seen.append(opt.state[p]["exp_avg"].dtype)
+        opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"] / 2
+
+    opt = optim.FusedAdamW([p])
+    opt.register_load_state_dict_post_hook(halve)
+    opt.load_state_dict(saved)
+    assert seen == [torch.float32]
+    assert bool((opt.state[p]["exp_avg"] == 0.25).all())
+    assert opt.state[p]["exp_avg"].dtype == torch.float32

@@ -175,17 +175,32 @@ class FusedAdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer's, but every state tensor keeps its own
         type (fp32 masters and moments of 16-bit parameters, 8-bit codes)."""
-        saved = state_dict["state"]
+        # between the caller's hooks: what those before the load leave is loaded,
+        # and those after it find the state as it stays
+        saved = {}
+        before = self.register_load_state_dict_pre_hook(
+            lambda _, sd: self._check_loaded(sd, saved))
+        after = self.register_load_state_dict_post_hook(
+            lambda _: self._keep_types(saved), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
+
+    def _check_loaded(self, state_dict, saved: dict) -> None:
         want = torch.uint8 if self.state_bits == 8 else torch.float32
-        for st in saved.values():
+        for st in state_dict["state"].values():
             if "exp_avg" in st and st["exp_avg"].dtype != want:
                 raise ValueError(f"the saved moments are {st['exp_avg'].dtype}, those of "
                                  f"state_bits={self.state_bits} are {want}")
-        super().load_state_dict(state_dict)
-        keys = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        saved.update(state_dict)
+
+    def _keep_types(self, saved: dict) -> None:
+        keys = itertools.chain.from_iterable(g["params"] for g in saved["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for key, p in zip(keys, params):
-            for name, t in saved.get(key, {}).items():
+            for name, t in saved["state"].get(key, {}).items():
                 if torch.is_tensor(t) and name != "step":
                     self.state[p][name] = t.detach().to(device=p.device, copy=True)
 
