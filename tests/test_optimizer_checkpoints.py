@@ -1,4 +1,4 @@
-"""Loading optimizer states as torch.optim.Optimizer does: hooks (CPU)."""
+"""Loading optimizer states as torch.optim.Optimizer does: hooks, types (CPU)."""
 import copy
 
 import pytest
@@ -73,3 +73,24 @@ def test_post_hooks_find_and_change_the_state(dt):
     assert seen == [torch.float32]
     assert bool((opt.state[p]["exp_avg"] == 0.25).all())
     assert opt.state[p]["exp_avg"].dtype == torch.float32
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("param", [torch.float32, torch.bfloat16])
+def test_moments_saved_in_another_float_type(dt, param):
+    """As torch casts them for fp32 parameters; fp32 for 16-bit ones too."""
+    p, saved = _saved(dt=param)
+    st = saved["state"][0] = dict(saved["state"][0])
+    for k in ("exp_avg", "exp_avg_sq", "master"):
+        if k in st:
+            st[k] = torch.linspace(0.1, 1, 6).to(dt)
+    opt = optim.FusedAdamW([p])
+    opt.load_state_dict(saved)
+    for k in ("exp_avg", "exp_avg_sq", "master"):
+        if k in st:
+            got = opt.state[p][k]
+            assert got.dtype == torch.float32 and torch.equal(got, st[k].float())
+    if param == torch.float32:
+        theirs = torch.optim.Adam([p])
+        theirs.load_state_dict(saved)
+        assert torch.equal(theirs.state[p]["exp_avg"], opt.state[p]["exp_avg"])

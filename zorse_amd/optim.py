@@ -173,8 +173,9 @@ class FusedAdamW(torch.optim.Optimizer):
             self._stepped(p)
 
     def load_state_dict(self, state_dict) -> None:
-        """As torch.optim.Optimizer's, but every state tensor keeps its own
-        type (fp32 masters and moments of 16-bit parameters, 8-bit codes)."""
+        """As torch.optim.Optimizer's, but a state tensor's type does not follow
+        the parameter's: masters and 32-bit moments are fp32 whatever type they
+        were saved in, 8-bit codes and others keep their own."""
         # between the caller's hooks: what those before the load leave is loaded,
         # and those after it find the state as it stays
         saved = {}
@@ -189,11 +190,13 @@ class FusedAdamW(torch.optim.Optimizer):
             after.remove()
 
     def _check_loaded(self, state_dict, saved: dict) -> None:
-        want = torch.uint8 if self.state_bits == 8 else torch.float32
         for st in state_dict["state"].values():
-            if "exp_avg" in st and st["exp_avg"].dtype != want:
-                raise ValueError(f"the saved moments are {st['exp_avg'].dtype}, those of "
-                                 f"state_bits={self.state_bits} are {want}")
+            if "exp_avg" not in st:
+                continue
+            dt = st["exp_avg"].dtype
+            if not (dt == torch.uint8 if self.state_bits == 8 else dt.is_floating_point):
+                raise ValueError(f"the saved moments are {dt}, not those of "
+                                 f"state_bits={self.state_bits}")
         saved.update(state_dict)
 
     def _keep_types(self, saved: dict) -> None:
@@ -202,7 +205,9 @@ class FusedAdamW(torch.optim.Optimizer):
         for key, p in zip(keys, params):
             for name, t in saved["state"].get(key, {}).items():
                 if torch.is_tensor(t) and name != "step":
-                    self.state[p][name] = t.detach().to(device=p.device, copy=True)
+                    held = name in ("exp_avg", "exp_avg_sq", "master") and t.is_floating_point()
+                    self.state[p][name] = t.detach().to(
+                        device=p.device, dtype=torch.float32 if held else t.dtype, copy=True)
 
     def master_param(self, p: torch.Tensor) -> torch.Tensor:
         """fp32 master of ``p`` (``p`` itself when it is fp32)."""
