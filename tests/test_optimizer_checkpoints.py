@@ -94,3 +94,14 @@ def test_moments_saved_in_another_float_type(dt, param):
         theirs = torch.optim.Adam([p])
         theirs.load_state_dict(saved)
         assert torch.equal(theirs.state[p]["exp_avg"], opt.state[p]["exp_avg"])
+
+
+def test_seeds_of_counts_that_are_tensors():
+    """torch's own optimizers save the step count as a tensor."""
+    p, _ = _saved(8)
+    opt = optim.FusedAdamW([p, torch.nn.Parameter(torch.ones(2))], state_bits=8)
+    params = opt.param_groups[0]["params"]
+    want = opt._seeds(params, [3, 70000])
+    for dt in (torch.float32, torch.int64):
+        counts = [torch.tensor(n, dtype=dt) for n in (3, 70000)]
+        assert opt._seeds(params, counts) == want

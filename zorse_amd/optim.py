@@ -127,7 +127,7 @@ class FusedAdamW(torch.optim.Optimizer):
         repeats them."""
         place = {id(p): i for i, p in enumerate(itertools.chain.from_iterable(
             g["params"] for g in self.param_groups))}
-        return [(t * 0xC2B2AE3D + place[id(p)] * 0x27D4EB2F) & 0xFFFFFFFF
+        return [(int(t) * 0xC2B2AE3D + place[id(p)] * 0x27D4EB2F) & 0xFFFFFFFF
                 for p, t in zip(params, steps)]
 
     def _step_one(self, group: dict, p: torch.Tensor) -> None:
