@@ -105,3 +105,51 @@ def test_seeds_of_counts_that_are_tensors():
     for dt in (torch.float32, torch.int64):
         counts = [torch.tensor(n, dtype=dt) for n in (3, 70000)]
         assert opt._seeds(params, counts) == want
+
+
+def test_layers_round_with_bits_of_their_own():
+    """The one parameter of each layer's optimizer has the same place in it; the
+    seed is saved, and checkpoints without one repeat what they began with."""
+    from zorse_amd.stage import StageRunner
+    layers = [torch.nn.Linear(3, 3, bias=False) for _ in range(3)]
+    stage = StageRunner(layers, state_bits=8)
+    later = StageRunner(layers, state_bits=8, seed=3)
+
+    def seeds(opt, step=5):
+        return opt._seeds(opt.param_groups[0]["params"], [step])[0]
+
+    opts = stage.optimizers + later.optimizers
+    drawn = {seeds(o, t) for o in opts for t in range(1, 50)}
+    assert len(drawn) == 6 * 49
+    first, other = stage.optimizers[:2]
+    alone = optim.FusedAdamW(list(layers[0].parameters()), state_bits=8)
+    assert seeds(first) == seeds(alone) == (5 * 0xC2B2AE3D) & 0xFFFFFFFF
+    alone.load_state_dict(other.state_dict())
+    assert seeds(alone) == seeds(other) != seeds(first)
+    old = other.state_dict()
+    del old["param_groups"][0]["seed"]
+    other.load_state_dict(old)
+    assert seeds(other) == seeds(first)
+    wide = optim.FusedAdam(list(layers[0].parameters()))
+    assert "seed" not in wide.param_groups[0]
+    assert optim.FusedAdam(layers[0].parameters(), state_bits=8, seed=7).param_groups[0]["seed"] == 7
+
+
+@pytest.mark.gpu
+def test_seeds_change_the_second_moment_alone(dev):
+    """Equal layers with equal gradients: other roundings, with another seed."""
+    g = torch.linspace(1e-3, 1, 5000, device=dev)
+    state = []
+    for seed in (0, 0, 1):
+        p = torch.nn.Parameter(torch.ones_like(g))
+        opt = optim.FusedAdamW([p], state_bits=8, seed=seed)
+        p.grad = g.clone()
+        opt.step()
+        state.append((p.detach(), *opt.moments(p)))
+    for a, b in zip(state[0], state[1]):
+        assert torch.equal(a, b)
+    assert torch.equal(state[0][0], state[2][0]) and torch.equal(state[0][1], state[2][1])
+    # rounded apart where a draw lies between the fraction's two sides: a third
+    # of the elements on average
+    apart = int((state[0][2] != state[2][2]).sum())
+    assert 1000 < apart < 2500

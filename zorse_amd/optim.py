@@ -14,7 +14,9 @@ pass.  With an fp32 parameter the update is in place.
 ``step()`` steps all of a group's parameters on a GPU in one launch (for every
 56), ``step_param`` one of them.  ``state_bits=8`` holds both moments in 8 bits
 a value (kernels.adamw8_multi): 2 bytes an element of state beside the master
-where 32 bits take 8.
+where 32 bits take 8.  ``seed`` sets the random bits of their rounding apart
+from those of other optimizers (a model with one for each layer); it is one of
+the groups' options and saved with them.
 
 ``weight_decay`` is decoupled (AdamW); ``FusedAdam`` is the same optimizer
 with weight decay fixed at 0, which is exactly ``torch.optim.Adam`` with its
@@ -31,7 +33,7 @@ from . import kernels as K
 
 class FusedAdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-                 state_bits=32):
+                 state_bits=32, seed=0):
         if lr < 0 or eps < 0 or weight_decay < 0:
             raise ValueError("lr, eps and weight_decay must be non-negative")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
@@ -39,8 +41,9 @@ class FusedAdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32 (got {state_bits})")
         self.state_bits = state_bits
+        random = {"seed": seed} if state_bits == 8 else {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
-                                      weight_decay=weight_decay))
+                                      weight_decay=weight_decay, **random))
         self._step_hooks = {}   # param -> [callable(param)]
 
     def add_step_hook(self, p: torch.Tensor, fn) -> None:
@@ -122,13 +125,14 @@ class FusedAdamW(torch.optim.Optimizer):
                     weight_decay=group["weight_decay"])
 
     def _seeds(self, params: list, steps: list) -> list:
-        """Of the random bits of each second moment at its step: from the
-        parameter's place in the optimizer and the step, so that a resumed run
-        repeats them."""
-        place = {id(p): i for i, p in enumerate(itertools.chain.from_iterable(
-            g["params"] for g in self.param_groups))}
-        return [(int(t) * 0xC2B2AE3D + place[id(p)] * 0x27D4EB2F) & 0xFFFFFFFF
-                for p, t in zip(params, steps)]
+        """Of the random bits of each second moment at its step: from its group's
+        seed (0 in checkpoints without one), the parameter's place in the
+        optimizer and the step, so that a resumed run repeats them."""
+        own, place = {}, itertools.count()
+        for group in self.param_groups:
+            for p in group["params"]:
+                own[id(p)] = next(place) * 0x27D4EB2F + group.get("seed", 0) * 0x165667B1
+        return [(int(t) * 0xC2B2AE3D + own[id(p)]) & 0xFFFFFFFF for p, t in zip(params, steps)]
 
     def _step_one(self, group: dict, p: torch.Tensor) -> None:
         if self.state_bits == 8:
@@ -229,9 +233,9 @@ class FusedAdam(FusedAdamW):
     no weight decay) -- the optimizer the reference builds per flat shard."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
-                 state_bits=32):
+                 state_bits=32, seed=0):
         if weight_decay != 0:
             raise ValueError("FusedAdam applies no weight decay; use FusedAdamW for "
                              "decoupled weight decay")
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=0.0,
-                         state_bits=state_bits)
+                         state_bits=state_bits, seed=seed)
