@@ -415,7 +415,8 @@ int zk_adamw_step_t(float* param, const void* grad, int grad_dtype,
  * allows (56 tensors each, 44 with 8-bit moments; large ones alone); the same
  * bits as a call for each.  Hyper-parameters are shared, the step counts are
  * not.  lowp NULL: no compute copy.  The table is host memory, read before the
- * call returns. */
+ * call returns.  What a row writes may not overlap what another row reads or
+ * writes: rows are stepped in no order. */
 typedef struct zk_adamw_tensor {
   float* param;
   const void* grad;

@@ -498,14 +498,45 @@ int64_t integer(PyObject* o) {
   return integer(i.ptr());
 }
 
+// Memory of a list's tensor `owner`.
+struct Span {
+  int64_t begin, end;
+  Py_ssize_t owner;
+  bool written;
+  bool operator<(const Span& o) const { return begin < o.begin; }
+};
+
+// Whether, of spans in order, one that is written meets another: workgroups
+// would write it from two places, or read it before or after at random.  A
+// tensor's own columns may be one (a copy that is the parameter): the same
+// thread has the same element of both.
+bool spans_clash(const std::vector<Span>& spans) {
+  struct {
+    Span last{0, 0, -1, false};  // owner -1: several
+    bool is(const Span& s) const {
+      return s.owner == last.owner && s.begin == last.begin && s.end == last.end;
+    }
+    bool meets(const Span& s) const { return s.begin < last.end && !is(s); }
+    void add(const Span& s) {
+      if (s.begin >= last.end) last = s;
+      else if (!is(s)) last = {last.begin, std::max(last.end, s.end), -1, s.written};
+    }
+  } read, written;
+  for (const Span& s : spans) {
+    if (written.meets(s) || (s.written && read.meets(s))) return true;
+    (s.written ? written : read).add(s);
+  }
+  return false;
+}
+
 // (device index, rows of 64-bit fields) of a list of tensors: for each the
 // addresses of the columns, the elements of the first column's, the integers,
 // and the type codes of the columns in `codes`.  A column is (name, tensors,
-// mask of type bits, kind): contiguous tensors on one GPU, as large as the first
-// column's (kind 0; 1: None is allowed too) or two for each block of them (2).
-// `apart`: refuse a first column whose tensors share memory.
+// mask of type bits, kind, written): contiguous tensors on one GPU, as large as
+// the first column's (kind 0; 1: None is allowed too) or two for each block of
+// them (2).  Those that are written share no memory with others.
 py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple& integers,
-               const py::tuple& codes, bool apart) {
+               const py::tuple& codes) {
   const size_t nc = columns.size(), ni = integers.size(), fields = nc + 1 + ni + codes.size();
   std::vector<Sequence> lists;
   for (const auto& c : columns) lists.emplace_back(py::tuple(c.cast<py::tuple>())[1]);
@@ -519,10 +550,13 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
   int64_t* out = reinterpret_cast<int64_t*>(PyBytes_AS_STRING(table.ptr()));
   int64_t index = -1;
   std::vector<int64_t> numel(n), code(n * nc);
-  std::vector<std::pair<int64_t, int64_t>> spans;
+  std::vector<Span> spans;
+  spans.reserve(n * nc);
   for (size_t c = 0; c < nc; ++c) {
     const py::tuple column = columns[c].cast<py::tuple>();
     const int64_t mask = column[2].cast<int64_t>(), kind = column[3].cast<int64_t>();
+    const bool written = column[4].cast<bool>();
+    const size_t before = spans.size();
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = lists[c].items[i];
       int64_t& field = out[i * fields + c];
@@ -550,14 +584,17 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
       }
       field = reinterpret_cast<int64_t>(t.data_ptr());
       code[c * n + i] = bit;
-      if (c == 0 && apart && want > 0)
-        spans.emplace_back(field, field + want * static_cast<int64_t>(t.element_size()));
+      if (want > 0)
+        spans.push_back({field, field + want * static_cast<int64_t>(t.element_size()), i, written});
     }
+    // in order, as the tensors of a column mostly are
+    const auto mid = spans.begin() + before;
+    if (!std::is_sorted(mid, spans.end())) std::sort(mid, spans.end());
+    if (before > 0 && mid != spans.end() && *mid < mid[-1])
+      std::inplace_merge(spans.begin(), mid, spans.end());
   }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    if (spans[i].first < spans[i - 1].second)
-      throw py::value_error(who + ": a parameter is in the list twice, or parameters overlap");
+  if (spans_clash(spans))
+    throw py::value_error(who + ": a tensor that is written is in the lists twice, or overlaps another");
   for (Py_ssize_t i = 0; i < n; ++i) {
     int64_t* row = out + i * fields + nc;
     *row++ = numel[i];

@@ -848,11 +848,13 @@ def spans_meet(at, sizes, itemsize: int) -> bool:
     return False
 
 
-# Types that a column of a list may have, as bits (csrc/nodes.cpp), and what
-# its tensors are beside the first column's: as large, or None, or a base.
+# Types that a column of a list may have, as bits (csrc/nodes.cpp), what its
+# tensors are beside the first column's (as large, or None, or a base), and
+# whether they are written.
 _F32, _U8, _I16 = 1 << _abi.ZK_F32, 1 << 3, 1 << 4
 _FLOATS = sum(1 << dtype_code(dt) for dt in FLOAT_DTYPES)
 _SAME, _OR_NONE, _BASE = 0, 1, 2
+_READ, _WRITTEN = False, True
 
 
 def _step_table(who, states, params, grads, steps, lowp_outs, *seeds):
@@ -860,9 +862,9 @@ def _step_table(who, states, params, grads, steps, lowp_outs, *seeds):
     checks of a step; ``states``: its columns between gradients and copies."""
     if lowp_outs is None:
         lowp_outs = [None] * len(params)
-    columns = (("param", params, _F32, _SAME), ("grad", grads, _FLOATS, _SAME), *states,
-               ("lowp_out", lowp_outs, _FLOATS, _OR_NONE))
-    return _abi.nodes().rows(who, columns, (steps, *seeds), (1, len(columns) - 1), True)
+    columns = (("param", params, _F32, _SAME, _WRITTEN), ("grad", grads, _FLOATS, _SAME, _READ),
+               *states, ("lowp_out", lowp_outs, _FLOATS, _OR_NONE, _WRITTEN))
+    return _abi.nodes().rows(who, columns, (steps, *seeds), (1, len(columns) - 1))
 
 
 def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1: float,
@@ -870,9 +872,10 @@ def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr: float, beta1
     """adamw_step over lists of tensors (any shapes, all contiguous and on one
     device) in one launch for every 56, with the same bits: fp32 ``params``
     and moments, ``grads`` in any of the three types, ``steps`` the step count
-    of each, ``lowp_outs`` a 16- or 32-bit copy of each parameter or None."""
-    index, table = _step_table("adamw_multi", (("exp_avg", exp_avgs, _F32, _SAME),
-                                               ("exp_avg_sq", exp_avg_sqs, _F32, _SAME)),
+    of each, ``lowp_outs`` a 16- or 32-bit copy of each parameter or None.  What
+    is written shares no memory with another parameter's tensors."""
+    index, table = _step_table("adamw_multi", (("exp_avg", exp_avgs, _F32, _SAME, _WRITTEN),
+                                               ("exp_avg_sq", exp_avg_sqs, _F32, _SAME, _WRITTEN)),
                                params, grads, steps, lowp_outs)
     if not table:
         return
@@ -895,9 +898,9 @@ def adamw8_multi(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, seeds, l
     first to nearest, the second up or down at random with the right mean.
     ``seeds``: an integer for each tensor (mod 2^32) that the random bits come
     from, another for each step."""
-    index, table = _step_table("adamw8_multi", (("exp_avg", exp_avgs, _U8, _SAME),
-                                                ("exp_avg_sq", exp_avg_sqs, _U8, _SAME),
-                                                ("base", bases, _I16, _BASE)),
+    index, table = _step_table("adamw8_multi", (("exp_avg", exp_avgs, _U8, _SAME, _WRITTEN),
+                                                ("exp_avg_sq", exp_avg_sqs, _U8, _SAME, _WRITTEN),
+                                                ("base", bases, _I16, _BASE, _WRITTEN)),
                                params, grads, steps, lowp_outs, [s & 0xFFFFFFFF for s in seeds])
     if not table:
         return
@@ -919,9 +922,9 @@ def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.fl
         raise ValueError(f"adamw8_values: values are fp32 or bf16 (got {dtype})")
     values = 1 << dtype_code(dtype)
     index, table = _abi.nodes().rows("adamw8_values", (
-        ("exp_avg", exp_avgs, _U8, _SAME), ("exp_avg_sq", exp_avg_sqs, _U8, _SAME),
-        ("base", bases, _I16, _BASE), ("first moment", outs[0], values, _SAME),
-        ("second moment", outs[1], values, _SAME)), (), (), False)
+        ("exp_avg", exp_avgs, _U8, _SAME, _READ), ("exp_avg_sq", exp_avg_sqs, _U8, _SAME, _READ),
+        ("base", bases, _I16, _BASE, _READ), ("first moment", outs[0], values, _SAME, _WRITTEN),
+        ("second moment", outs[1], values, _SAME, _WRITTEN)), (), ())
     if table:
         with _on(index):
             check(lib().zk_adamw8_values(table, len(exp_avgs), dtype_code(dtype), _stream(index)),
