@@ -558,7 +558,8 @@ int zk_qk_norm_rope_bwd(const zk_qk_desc* desc, const void* q, const void* k,
  * with it only rows that tokens name are touched.  Tokens whose id is
  * padding_idx (-1: none) or outside [0, vocab) have no gradient.  The sums are
  * fp32, in an order that the ids alone decide: equal calls give equal bits.
- * Sizes: tokens < 2^29, vocab < 2^28, hidden < 2^23 (ZK_EINVAL). */
+ * Sizes: tokens < 2^29, vocab < 2^28, hidden < 2^23, tokens x hidden < 2^40
+ * (ZK_EINVAL). */
 int zk_embedding_fwd(const void* ids, int ids_64, int64_t tokens, const void* w,
                      int64_t vocab, int64_t hidden, void* y, float scale,
                      int w_dtype, int y_dtype, zk_stream_t stream);

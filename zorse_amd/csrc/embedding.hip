@@ -611,21 +611,27 @@ static int64_t embed_ws_bytes(int64_t T, int64_t V, int64_t h) {
          pad_to(V * 4, 16) + 16;
 }
 
+// Every launch stays below 2^32 threads, 2^24 workgroups of the gradient: its
+// blocks of 64 tokens are less than 2^23, the waves of its sums less than 2^25.3
+// (a slice is 488 columns or more), 2^23.3 workgroups of four, and those that
+// fill 2^22 and one.
+static constexpr int64_t kMaxFills = int64_t(1) << 22;
 static bool embed_sizes_ok(int64_t T, int64_t V, int64_t h) {
-  // every launch stays below 2^32 threads
   return T >= 0 && T < (int64_t(1) << 29) && V > 0 && V < (int64_t(1) << 28) && h > 0 &&
-         h < (int64_t(1) << 23);
+         h < (int64_t(1) << 23) && T * h < (int64_t(1) << 40);
 }
 
 // Rows that a filling workgroup looks at, up to a wave's lanes: 8 KB of rows
 // above 4 KB, 16 KB of shorter ones, less while there would be less than 1024
-// workgroups.  us of the whole gradient at 8 / 16 / 64 KB: 4096 tokens, 49152 rows
+// workgroups, more while there would be more than kMaxFills (64 rows always do:
+// vocab < 2^28).  us of the whole gradient at 8 / 16 / 64 KB: 4096 tokens, 49152 rows
 // of 8 KB 83 / 91 / 98, 16312 tokens, 32000 rows of 4 KB 60.5 / 58.3 / 60.7, 8192
 // tokens, 32000 rows of 2 KB 32.1 / 30.7 / 30.9.
 static Fill rows_to_fill(int64_t V, int64_t row_bytes) {
   const int64_t most = row_bytes > 4096 ? 8192 : 16384;
   Fill f{64, 0};
   while (f.rows > 1 && (f.rows * row_bytes > most || V / f.rows < 1024)) f.rows >>= 1;
+  while (V / f.rows > kMaxFills) f.rows <<= 1;
   while (f.log_tpr < 8 && (int64_t(16) << f.log_tpr) < row_bytes) ++f.log_tpr;
   return f;
 }
