@@ -501,16 +501,29 @@ int64_t integer(PyObject* o) {
 // Memory of a list's tensor `owner`.
 struct Span {
   int64_t begin, end;
-  Py_ssize_t owner;
+  int owner;
   bool written;
   bool operator<(const Span& o) const { return begin < o.begin; }
 };
 
-// Whether, of spans in order, one that is written meets another: workgroups
-// would write it from two places, or read it before or after at random.  A
-// tensor's own columns may be one (a copy that is the parameter): the same
-// thread has the same element of both.
-bool spans_clash(const std::vector<Span>& spans) {
+// Sorts what mostly is a few ascending runs.
+void sort_runs(std::vector<Span>& spans) {
+  const auto begin = spans.begin();
+  auto mid = std::is_sorted_until(begin, spans.end());
+  for (int run = 1; mid != spans.end(); ++run) {
+    if (run == 8) return std::sort(begin, spans.end());
+    const auto end = std::is_sorted_until(mid, spans.end());
+    std::inplace_merge(begin, mid, end);
+    mid = end;
+  }
+}
+
+// Whether one that is written meets another: workgroups would write it from two
+// places, or read it before or after at random.  A tensor's own columns may be
+// one (a copy that is the parameter): the same thread has the same element of
+// both.
+bool spans_clash(std::vector<Span>& spans) {
+  sort_runs(spans);
   struct {
     Span last{0, 0, -1, false};  // owner -1: several
     bool is(const Span& s) const {
@@ -527,6 +540,32 @@ bool spans_clash(const std::vector<Span>& spans) {
     (s.written ? written : read).add(s);
   }
   return false;
+}
+
+// The memory of a column's tensors, one after another unless `mixed`.
+struct Reach {
+  int64_t begin = INT64_MAX, end = 0;
+  bool written = false, mixed = false;
+  void add(int64_t from, int64_t to) {
+    mixed = mixed || from < end;
+    begin = std::min(begin, from);
+    end = std::max(end, to);
+  }
+  // nothing of the two can clash
+  bool apart(const Reach& o) const {
+    return (!written && !o.written) || begin >= o.end || o.begin >= end;
+  }
+};
+
+// The columns that the reaches alone do not clear.
+std::vector<size_t> unclear(const std::vector<Reach>& columns) {
+  std::vector<size_t> out;
+  for (size_t c = 0; c < columns.size(); ++c) {
+    bool clear = !(columns[c].written && columns[c].mixed);
+    for (size_t d = 0; d < columns.size(); ++d) clear = clear && (d == c || columns[c].apart(columns[d]));
+    if (!clear) out.push_back(c);
+  }
+  return out;
 }
 
 // (device index, rows of 64-bit fields) of a list of tensors: for each the
@@ -550,13 +589,12 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
   int64_t* out = reinterpret_cast<int64_t*>(PyBytes_AS_STRING(table.ptr()));
   int64_t index = -1;
   std::vector<int64_t> numel(n), code(n * nc);
-  std::vector<Span> spans;
-  spans.reserve(n * nc);
+  std::vector<int64_t> ends(n * nc, 0);  // 0: no memory
+  std::vector<Reach> reaches(nc);
   for (size_t c = 0; c < nc; ++c) {
     const py::tuple column = columns[c].cast<py::tuple>();
     const int64_t mask = column[2].cast<int64_t>(), kind = column[3].cast<int64_t>();
-    const bool written = column[4].cast<bool>();
-    const size_t before = spans.size();
+    reaches[c].written = column[4].cast<bool>();
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = lists[c].items[i];
       int64_t& field = out[i * fields + c];
@@ -584,14 +622,20 @@ py::tuple rows(const std::string& who, const py::tuple& columns, const py::tuple
       }
       field = reinterpret_cast<int64_t>(t.data_ptr());
       code[c * n + i] = bit;
-      if (want > 0)
-        spans.push_back({field, field + want * static_cast<int64_t>(t.element_size()), i, written});
+      if (want > 0) {
+        const int64_t end = field + want * static_cast<int64_t>(t.element_size());
+        ends[i * nc + c] = end;
+        reaches[c].add(field, end);
+      }
     }
-    // in order, as the tensors of a column mostly are
-    const auto mid = spans.begin() + before;
-    if (!std::is_sorted(mid, spans.end())) std::sort(mid, spans.end());
-    if (before > 0 && mid != spans.end() && *mid < mid[-1])
-      std::inplace_merge(spans.begin(), mid, spans.end());
+  }
+  std::vector<Span> spans;
+  if (const std::vector<size_t> left = unclear(reaches); !left.empty()) {
+    spans.reserve(n * left.size());
+    for (Py_ssize_t i = 0; i < n; ++i)  // a tensor's columns in turn, as states are allocated
+      for (const size_t c : left)
+        if (ends[i * nc + c] != 0)
+          spans.push_back({out[i * fields + c], ends[i * nc + c], static_cast<int>(i), reaches[c].written});
   }
   if (spans_clash(spans))
     throw py::value_error(who + ": a tensor that is written is in the lists twice, or overlaps another");
