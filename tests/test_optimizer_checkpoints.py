@@ -100,11 +100,11 @@ def test_seeds_of_counts_that_are_tensors():
     """torch's own optimizers save the step count as a tensor."""
     p, _ = _saved(8)
     opt = optim.FusedAdamW([p, torch.nn.Parameter(torch.ones(2))], state_bits=8)
-    params = opt.param_groups[0]["params"]
-    want = opt._seeds(params, [3, 70000])
+    group = opt.param_groups[0]
+    want = opt._seeds(group, group["params"], [3, 70000])
     for dt in (torch.float32, torch.int64):
         counts = [torch.tensor(n, dtype=dt) for n in (3, 70000)]
-        assert opt._seeds(params, counts) == want
+        assert opt._seeds(group, group["params"], counts) == want
 
 
 def test_layers_round_with_bits_of_their_own():
@@ -116,7 +116,8 @@ def test_layers_round_with_bits_of_their_own():
     later = StageRunner(layers, state_bits=8, seed=3)
 
     def seeds(opt, step=5):
-        return opt._seeds(opt.param_groups[0]["params"], [step])[0]
+        group = opt.param_groups[0]
+        return opt._seeds(group, group["params"], [step])[0]
 
     opts = stage.optimizers + later.optimizers
     drawn = {seeds(o, t) for o in opts for t in range(1, 50)}

@@ -124,15 +124,16 @@ class FusedAdamW(torch.optim.Optimizer):
         return dict(lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"],
                     weight_decay=group["weight_decay"])
 
-    def _seeds(self, params: list, steps: list) -> list:
-        """Of the random bits of each second moment at its step: from its group's
+    def _seeds(self, group: dict, params: list, steps: list) -> list:
+        """Of the random bits of each second moment at its step: from the group's
         seed (0 in checkpoints without one), the parameter's place in the
         optimizer and the step, so that a resumed run repeats them."""
-        own, place = {}, itertools.count()
-        for group in self.param_groups:
-            for p in group["params"]:
-                own[id(p)] = next(place) * 0x27D4EB2F + group.get("seed", 0) * 0x165667B1
-        return [(int(t) * 0xC2B2AE3D + own[id(p)]) & 0xFFFFFFFF for p, t in zip(params, steps)]
+        place = {id(p): i for i, p in enumerate(itertools.chain.from_iterable(
+            g["params"] for g in self.param_groups))}
+        own = group.get("seed", 0) * 0x165667B1
+        counts = {t: int(t) * 0xC2B2AE3D + own for t in set(steps)}
+        return [(counts[t] + place[id(p)] * 0x27D4EB2F) & 0xFFFFFFFF
+                for p, t in zip(params, steps)]
 
     def _step_one(self, group: dict, p: torch.Tensor) -> None:
         if self.state_bits == 8:
@@ -150,7 +151,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step_list(self, group: dict, params: list) -> None:
         # one parameter, or parameters that share memory: one by one
         shared = len(params) > 1 and K.spans_meet(
-            [p.data_ptr() for p in params], [p.numel() * p.element_size() for p in params], 1)
+            [p.data_ptr() for p in params], [p.nbytes for p in params], 1)
         if (len(params) == 1 or shared) and self.state_bits == 32:
             for p in params:
                 self._step_one(group, p)
@@ -168,7 +169,7 @@ class FusedAdamW(torch.optim.Optimizer):
         lows = [None if m is None else p for p, m in zip(params, masters)]
         if self.state_bits == 8:
             K.adamw8_multi(*args, [st["exp_base"] for st in states], steps, lowp_outs=lows,
-                           seeds=self._seeds(params, steps), **self._hyper(group))
+                           seeds=self._seeds(group, params, steps), **self._hyper(group))
         else:
             K.adamw_multi(*args, steps, lowp_outs=lows, **self._hyper(group))
         for st, t in zip(states, steps):  # a refused list has not been stepped
