@@ -6,8 +6,8 @@
 // A row's ragged end: where lanes of one wave take different paths in load(),
 // the element path writes registers that the other lanes' wide load still has
 // to fill, and the wave waits for it -- one load in flight instead of many.  So
-// n should be the same for all lanes: kernels let the last chunk of a row
-// overlap the one before it instead (ragged rows of 8 and more).
+// n should be the same for all lanes: kernels that keep many rows in flight let
+// the last chunk of a row overlap the one before it instead (rows of 8 and more).
 #pragma once
 #include "zk_common.h"
 

@@ -109,7 +109,8 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     ``dtype`` (default the table's).  ids int32 / int64; an id outside
     [0, vocab) gives a row of NaN and no gradient (nothing is read back to the
     host to check it).  ``padding_idx`` (negative: from the end, as nn.Embedding
-    takes it): the row whose tokens have no gradient."""
+    takes it): the row whose tokens have no gradient.  Linear in the table: it can
+    be differentiated twice, and forward-mode tangents go through it."""
     return nodes().embedding(ids, weight, scale, padding_idx, dtype)
 
 
@@ -122,7 +123,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, eps=1e-6
     the rotation, in one pass with one rounding.  cos / sin: fp32 [n_pos, d/2]
     tables (rope_tables(..., torch.float32, ...)); ``positions`` int64 [S] or
     [B, S], default 0 .. S-1; a position outside the tables gives NaN.  Any even
-    d up to 1024; q and k may be views of one q|k|v buffer."""
+    d up to 1024; q and k may be views of one q|k|v buffer.  It can be
+    differentiated once, backward."""
     return nodes().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
