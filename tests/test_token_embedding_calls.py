@@ -76,3 +76,17 @@ def test_recorded_calls(both):
     traced = torch.jit.trace(ours, (ids,))
     other = ids.flip(1).contiguous()
     assert torch.equal(traced(other), theirs(other))
+
+
+@pytest.mark.gpu
+def test_compiled_call_has_one_graph(both):
+    """As nn.Embedding's: nothing that would cut the recorded graph."""
+    ours, theirs, ids = both
+    torch._dynamo.reset()
+    compiled = torch.compile(ours, backend="eager", fullgraph=True)
+    for i in (ids, ids.flip(0)):
+        y = compiled(i)
+        assert torch.equal(y, theirs(i))
+    grad, = torch.autograd.grad(y.sum(), ours.weight)
+    want, = torch.autograd.grad(theirs(ids).sum(), theirs.weight)
+    assert torch.equal(grad, want)  # sums of ones

@@ -127,8 +127,8 @@ class TokenEmbedding(nn.Embedding):
     def forward(self, input):
         w = self.weight
         if not w.is_cuda or self.max_norm is not None or self.scale_grad_by_freq or self.sparse \
-                or w.dtype not in K.FLOAT_DTYPES or not (_has_memory(w) and _has_memory(input)) \
-                or torch.compiler.is_compiling() or torch.jit.is_tracing():
+                or w.dtype not in K.FLOAT_DTYPES or torch.compiler.is_compiling() \
+                or torch.jit.is_tracing() or not (_has_memory(w) and _has_memory(input)):
             return super().forward(input)
         return Fn.embedding(input, w, padding_idx=self.padding_idx)
 
