@@ -131,6 +131,8 @@ def test_layers_round_with_bits_of_their_own():
     del old["param_groups"][0]["seed"]
     other.load_state_dict(old)
     assert seeds(other) == seeds(first)
+    with pytest.raises(TypeError):
+        optim.FusedAdamW(layers[0].parameters(), state_bits=8, seed=1.5)
     wide = optim.FusedAdam(list(layers[0].parameters()))
     assert "seed" not in wide.param_groups[0]
     assert optim.FusedAdam(layers[0].parameters(), state_bits=8, seed=7).param_groups[0]["seed"] == 7

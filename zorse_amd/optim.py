@@ -25,6 +25,7 @@ defaults -- the reference's optimizer.
 from __future__ import annotations
 
 import itertools
+import operator
 
 import torch
 
@@ -41,7 +42,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32 (got {state_bits})")
         self.state_bits = state_bits
-        random = {"seed": seed} if state_bits == 8 else {}
+        random = {"seed": operator.index(seed)} if state_bits == 8 else {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, **random))
         self._step_hooks = {}   # param -> [callable(param)]
