@@ -572,6 +572,75 @@ int zk_embedding_bwd(const void* ids, int ids_64, int64_t tokens, const void* dy
                      int accumulate, void* workspace, int64_t workspace_bytes,
                      zk_stream_t stream);
 
+/* --------------------------------------------------------- Packed attention --
+ * Attention within each of the sequences that lie one after another in a run of
+ * T tokens (the reference's attention core, models/llama_simple.py:320-342, for
+ * micro-batches filled with documents): with [lo, hi) token i's sequence, it sees
+ * the tokens of [lo, hi), causal only those up to i, with a window W > 0 only the
+ * last W of these;
+ *     o = softmax(scale q k^T) v,   lse = log sum exp(scale q k^T)
+ * q, o: [T, Hq, d]; k, v: [T, Hkv, d] (strides of tokens _s and of heads _h; unit
+ * stride along d), Hq a multiple of Hkv; lse fp32 [Hq, T] contiguous.  d up to
+ * 128, even for 2-byte types, whose heads start at multiples of 4 bytes (16, and
+ * d 64 or 128, for the kernels without masks).  Tokens behind the last sequence
+ * see nothing: their rows of the outputs are zeros (lse -inf), or with keep_tail
+ * left as they are.  What lies in tokens that a row does not see, infinities and
+ * NaN among it, does not reach the row.
+ *
+ * The plan of a batch's sequences is made on the device once and serves every
+ * layer, both directions: zk_packed_plan_bytes(T) bytes, 16-byte aligned.
+ * offsets: n_seq + 1 ascending token counts from 0 on (int32, or int64 with
+ * offsets_64), the last one at most T; it is read by the kernel, and whatever it
+ * holds, the plan refers to tokens of 0 .. T - 1 only.  positions, when given:
+ * int64 [T], each token's index in its sequence (behind the last one 0). */
+int64_t zk_packed_plan_bytes(int64_t T);
+int zk_packed_plan(const void* offsets, int offsets_64, int64_t n_seq, int64_t T,
+                   void* plan, int64_t plan_bytes, int64_t* positions,
+                   zk_stream_t stream);
+
+typedef struct zk_packed_desc {
+  int64_t T, Hq, Hkv, d;
+  int64_t q_s, q_h, k_s, k_h, v_s, v_h, o_s, o_h;
+  int64_t do_s, do_h, dq_s, dq_h, dk_s, dk_h, dv_s, dv_h; /* backward */
+  int64_t window;
+  float scale;
+  int causal, keep_tail, dtype;
+} zk_packed_desc;
+int zk_attn_packed_fwd(const zk_packed_desc* desc, const void* q, const void* k,
+                       const void* v, const void* plan, void* o, float* lse,
+                       zk_stream_t stream);
+/* Its gradients, from the forward's o and lse.  Sums in one order: equal calls
+ * give equal bits.  The workspace holds two fp32 values a token and query head. */
+int64_t zk_attn_packed_bwd_workspace(const zk_packed_desc* desc);
+int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, const void* k,
+                       const void* v, const void* plan, const void* o,
+                       const void* dout, const float* lse, void* dq, void* dk,
+                       void* dv, void* workspace, int64_t workspace_bytes,
+                       zk_stream_t stream);
+
+/* ------------------------------------------------ Rotation by several axes --
+ * The rotation of apply_rotary_pos_emb (models/llama_simple.py:34-58) with a
+ * position for each of several axes (time, height, width of images and video):
+ * pair i of a head of token t is turned by the angle of row
+ * positions[pair_axes[i]][t] of the tables, in fp32 with one rounding; inverse:
+ * by the opposite angle (the transpose, which takes gradients back).
+ * q: [B, S, Hq, d], k: [B, S, Hkv, d] (Hkv 0: none) with the strides _sb, _ss,
+ * _sh and unit stride along d, outputs with their own (oq_, ok_), which may be
+ * the inputs; d even, up to 512.  cos, sin: fp32 [n_pos, d/2]; positions: int64
+ * [n_axes, B, S]; pair_axes: d/2 bytes on the host, read before the call returns.
+ * A position outside the tables gives NaN in its axis' pairs. */
+typedef struct zk_axes_desc {
+  int64_t B, S, Hq, Hkv, d;
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh;
+  int64_t oq_sb, oq_ss, oq_sh, ok_sb, ok_ss, ok_sh;
+  int64_t n_pos, n_axes;
+  int pairing, inverse, dtype;
+} zk_axes_desc;
+int zk_rope_axes(const zk_axes_desc* desc, const void* q, const void* k, void* q_out,
+                 void* k_out, const float* cos, const float* sin,
+                 const int64_t* positions, const unsigned char* pair_axes,
+                 zk_stream_t stream);
+
 /* ------------------------------------------------------------- Utilities --
  * Dtype conversion of a contiguous buffer (the autocast weight cast and the
  * grad cast of utils/patch.py:115-119 when done outside the AdamW kernel).

@@ -78,6 +78,34 @@ class QkDesc(ctypes.Structure):
     ] + [("eps", _f32), ("pairing", _int), ("dtype", _int), ("w_dtype", _int)]
 
 
+class PackedDesc(ctypes.Structure):
+    """Mirror of ``zk_packed_desc``."""
+
+    _fields_ = [
+        (name, _i64)
+        for name in (
+            "T", "Hq", "Hkv", "d",
+            "q_s", "q_h", "k_s", "k_h", "v_s", "v_h", "o_s", "o_h",
+            "do_s", "do_h", "dq_s", "dq_h", "dk_s", "dk_h", "dv_s", "dv_h",
+            "window",
+        )
+    ] + [("scale", _f32), ("causal", _int), ("keep_tail", _int), ("dtype", _int)]
+
+
+class AxesDesc(ctypes.Structure):
+    """Mirror of ``zk_axes_desc``."""
+
+    _fields_ = [
+        (name, _i64)
+        for name in (
+            "B", "S", "Hq", "Hkv", "d",
+            "q_sb", "q_ss", "q_sh", "k_sb", "k_ss", "k_sh",
+            "oq_sb", "oq_ss", "oq_sh", "ok_sb", "ok_ss", "ok_sh",
+            "n_pos", "n_axes",
+        )
+    ] + [("pairing", _int), ("inverse", _int), ("dtype", _int)]
+
+
 class AdamwRegion(ctypes.Structure):
     """Mirror of ``zk_adamw_region``."""
 
@@ -168,6 +196,15 @@ SIGNATURES = {
     "zk_qk_norm_rope_bwd_workspace": (_i64, [_i64]),
     "zk_qk_norm_rope_bwd": (_int, [ctypes.POINTER(QkDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
                                    _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "zk_packed_plan_bytes": (_i64, [_i64]),
+    "zk_packed_plan": (_int, [_ptr, _int, _i64, _i64, _ptr, _i64, _ptr, _ptr]),
+    "zk_attn_packed_fwd": (_int, [ctypes.POINTER(PackedDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                  _ptr]),
+    "zk_attn_packed_bwd_workspace": (_i64, [ctypes.POINTER(PackedDesc)]),
+    "zk_attn_packed_bwd": (_int, [ctypes.POINTER(PackedDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                  _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "zk_rope_axes": (_int, [ctypes.POINTER(AxesDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                            ctypes.c_char_p, _ptr]),
     "zk_transpose": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "zk_copy_to_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),
     "zk_copy_from_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),
@@ -202,7 +239,7 @@ _nodes = None
 
 
 def nodes():
-    """Load (once) and return the module of csrc/nodes.cpp: autograd nodes and
+    """Load (once) and return the module of csrc/nodes*.cpp: autograd nodes and
     tables for torch's C++ side, over the same library."""
     global _nodes
     if _nodes is None:

@@ -6,7 +6,7 @@ the HIP runtime; when it is loaded after ``import torch`` the dynamic loader
 binds it to the HIP runtime torch already mapped (same SONAME), so torch's
 streams and allocations are shared with the kernels.
 
-``csrc/nodes.cpp`` is host code against torch's headers and becomes
+``csrc/nodes*.cpp`` are host code against torch's headers and become
 ``zorse_amd/_nodes.so``, which is linked to the library beside it.
 
 Usage: ``python -m zorse_amd.build`` or ``zorse_amd.build.build()``.
@@ -39,7 +39,7 @@ HIPCC_FLAGS = [
 ]
 
 
-# Per-source extra flags.  rope.hip: with packed fp32 disabled, the SLP
+# Per-source extra flags.  rope.hip, rope_axes.hip: with packed fp32 disabled, the SLP
 # vectoriser forms two-wide fp32 negations that this compiler cannot select
 # (a backend "Cannot select: v2f32 bitcast" crash in the position-major
 # kernel); the kernels there are memory-bound, so scalar code costs nothing.
@@ -51,7 +51,7 @@ HIPCC_FLAGS = [
 # through the loop (with the default order the both-K-major form moved ~80
 # of them between AGPRs per pass; the NT forms do better with the default).
 _KMAJOR = ["-Wno-inline-asm", "-mllvm", "-greedy-reverse-local-assignment=1"]
-FILE_FLAGS = {"rope.hip": ["-fno-slp-vectorize"], "gemm.hip": ["-Wno-inline-asm"],
+FILE_FLAGS = {"rope.hip": ["-fno-slp-vectorize"], "rope_axes.hip": ["-fno-slp-vectorize"], "gemm.hip": ["-Wno-inline-asm"],
               "gemm_ring.hip": ["-Wno-inline-asm"], "gemm_split.hip": ["-Wno-inline-asm"],
               "gemm_f32.hip": ["-Wno-inline-asm"], "gemm_kmajor.hip": _KMAJOR,
               "gemm_ring_kmajor.hip": _KMAJOR}
@@ -81,15 +81,17 @@ def sources() -> list[str]:
     )
 
 
-def _nodes_commands(obj: str, out: str) -> tuple[list[str], list[str]]:
-    """Compiling csrc/nodes.cpp, and linking it to torch and the library."""
+def _nodes_commands(out: str) -> tuple[list[list[str]], list[str]]:
+    """Compiling each csrc/nodes*.cpp, and linking them to torch and the library."""
     from torch.utils import cpp_extension as ext
     cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
     includes = [*ext.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include"]
-    compile_ = [cxx, "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-                *(f for p in includes for f in ("-isystem", p)), "-c",
-                os.path.join(CSRC, "nodes.cpp"), "-o", obj]
-    link = [cxx, "-shared", "-o", out, obj, *(f"-L{p}" for p in ext.library_paths()), "-lc10",
+    srcs = sorted(f for f in os.listdir(CSRC) if f.startswith("nodes") and f.endswith(".cpp"))
+    objs = [os.path.join(OBJ_DIR, f[:-4] + ".o") for f in srcs]
+    compile_ = [[cxx, "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                 *(f for p in includes for f in ("-isystem", p)), "-c", os.path.join(CSRC, src), "-o", obj]
+                for src, obj in zip(srcs, objs)]
+    link = [cxx, "-shared", "-o", out, *objs, *(f"-L{p}" for p in ext.library_paths()), "-lc10",
             "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{PKG_DIR}",
             f"-l:{os.path.basename(LIB_PATH)}", "-Wl,-rpath,$ORIGIN"]
     return compile_, link
@@ -113,12 +115,12 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         _run(cmd)
         return obj
 
-    nodes_obj = os.path.join(OBJ_DIR, "nodes.o")
-    nodes_compile, nodes_link = _nodes_commands(nodes_obj, NODES_PATH + ".tmp")
+    nodes_compile, nodes_link = _nodes_commands(NODES_PATH + ".tmp")
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        nodes = ex.submit(_run, nodes_compile)
+        nodes = [ex.submit(_run, cmd) for cmd in nodes_compile]
         list(ex.map(compile_one, zip(srcs, objs)))
-        nodes.result()
+        for n in nodes:
+            n.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     if verbose:

@@ -1,0 +1,500 @@
+// Attention over packed sequences, backward (bf16 / fp16 storage), without
+// atomics: two kernels on the caller's stream.
+#include <type_traits>
+
+#include "attn_packed.h"
+
+namespace zk {
+
+int check_packed(const zk_packed_desc* D, const char* who, bool bwd, bool* ragged,
+                 std::initializer_list<const void*> tensors);
+void packed_args(PackedArgs& a, const zk_packed_desc* D, const void* plan);
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Transposed operand of tile X for its 16-row step kk, from the lane's byte offset.
+template <typename T, int D>
+__device__ __forceinline__ typename Mfma<T>::vec8 tr_operand(const T* X, int off, int kk) {
+  const char* base = reinterpret_cast<const char*>(X) + kk * 16 * D * 2;
+  const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + off));
+  const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + 8 * D * 2 + (off ^ 32)));
+  const s16x8 w = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+  return __builtin_bit_cast(typename Mfma<T>::vec8, w);
+}
+
+// --------------------------------------------------------------------- dQ --
+// 4 waves of 32 queries, whose Q and dO rows stay in registers; 64-key tiles of
+// K and V.  Also delta = rowsum(dO o O) and the log2-domain LSE for the other kernel.
+template <typename T, int D, int KR>
+__global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
+  typedef Mfma<T> M;
+  typedef typename M::vec8 V8;
+  constexpr int BM = 128, BN = 64, NT = 256, PF = 2;  // PF: operand reads in flight
+  constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
+  const int hd = KR ? a.d : D;
+  __shared__ __attribute__((aligned(16))) T K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const PackedPlan plan(a);
+  int block, hq;
+  packed_block(a, block, hq);
+  const int q0 = plan.first_row<BM, false>(a, block);
+  const int rows = static_cast<int>(a.T);
+  if (q0 >= rows) return;
+  const int hk = hq / (a.Hq / a.Hkv);
+  const int qw0 = q0 + 32 * wave;
+  const int my_q = qw0 + l32;
+  const bool in = my_q < rows;
+  const float c2 = a.scale_log2;
+
+  const int last = rows - 1;
+  auto clip = [&](int r) __attribute__((always_inline)) { return r < last ? r : last; };
+  auto below = [&](int j) __attribute__((always_inline)) { return j < plan.n ? j : plan.n - 1; };
+  const int b_last = clip(q0 + BM - 1);
+  const int w_first = clip(qw0), w_last = clip(qw0 + 31);
+  const int kv_lo = plan.key_lo(a, q0), kv_hi = below(plan.key_hi(a, b_last)) + 1;
+  const int w_lo = plan.key_lo(a, w_first), w_hi = below(plan.key_hi(a, w_last));
+  const int f_lo = plan.key_lo(a, w_last), f_hi = plan.key_hi(a, w_first);
+  const bool idle = qw0 >= rows;
+  int vis_lo = 0x40000000, vis_span = 0;
+  if (in) {
+    const int lo = plan.key_lo(a, my_q), hi = plan.key_hi(a, my_q);
+    if (hi >= lo) {
+      vis_lo = lo;
+      vis_span = hi - lo;
+    }
+  }
+
+  const T* Qp = static_cast<const T*>(a.q) + hq * a.q_h;
+  const T* Dp = static_cast<const T*>(a.dout) + hq * a.do_h;
+  const T* Kp = static_cast<const T*>(a.k) + hk * a.k_h;
+  const T* Vp = static_cast<const T*>(a.v) + hk * a.v_h;
+  V8 qreg[KS], dreg[KS];
+  load_operand<T, KS, KR>(qreg, in ? Qp + my_q * a.q_s : nullptr, g, hd);
+  load_operand<T, KS, KR>(dreg, in ? Dp + my_q * a.do_s : nullptr, g, hd);
+  float lse2 = INFINITY, del = 0.f;
+  {
+    const T* Op = static_cast<const T*>(a.o) + hq * a.o_h;
+    V8 oreg[KS];
+    load_operand<T, KS, KR>(oreg, in ? Op + my_q * a.o_s : nullptr, g, hd);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) del = fmaf(to_f32(oreg[ks][e]), to_f32(dreg[ks][e]), del);
+    del += other_half(del);
+    if (in) {
+      const int64_t i = static_cast<int64_t>(hq) * a.T + my_q;
+      const float l = my_q < plan.n ? a.lse[i] : -INFINITY;
+      lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
+      if (g == 0) {
+        a.delta[i] = del;
+        a.lse2[i] = lse2;
+      }
+    }
+  }
+
+  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + BN - 1) / BN : 0;
+  PackedLoader<T, D, BN, NT> kload, vload;
+  kload.init(a.k_s, hd);
+  vload.init(a.v_s, hd);
+  auto issue = [&](int t, int st) {
+    const int k0 = kv_lo + t * BN;
+    kload.issue(st ? K1 : K0, Kp, a.k_s, k0, plan.n);
+    vload.issue(st ? V1 : V0, Vp, a.v_s, k0, plan.n);
+  };
+  const int rbase = 2 * tile_off<D>(l32, 8 * g);
+  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+
+  f32x16 dq[NB];
+#pragma unroll
+  for (int nt = 0; nt < NB; ++nt) dq[nt] = f32x16{};
+
+  auto step = [&](auto stage_tag, int t) {
+    constexpr int st = decltype(stage_tag)::value;
+    const int k0 = kv_lo + t * BN;
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (t + 1 < n_t) issue(t + 1, st ^ 1);
+    if (idle || k0 > w_hi || k0 + BN <= w_lo) return;
+    const bool need_mask = k0 < f_lo || k0 + BN - 1 > f_hi;
+    const T* Kt = st ? K1 : K0;
+    const T* Vt = st ? V1 : V0;
+    int rb = rbase, tb = tbase;
+    asm volatile("" : "+v"(rb), "+v"(tb));
+#pragma unroll
+    for (int tt = 0; tt < BN / 32; ++tt) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+      // operands read PF steps ahead; the fences keep the reads where they are
+      auto rowread = [&](const T* X, int ks) __attribute__((always_inline)) {
+        const int ro = (rb ^ (ks << 5)) + tt * 32 * D * 2;
+        return *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(X) + ro);
+      };
+      V8 kq[PF], vq[PF];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        kq[i] = rowread(Kt, i);
+        vq[i] = rowread(Vt, i);
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        __builtin_amdgcn_sched_barrier(0);
+        V8 kA = kq[ks % PF], vA = vq[ks % PF];
+        if (ragged_step<KR>(ks)) {
+          kA = mask_cols<T>(kA, 16 * ks + 8 * g, hd);
+          vA = mask_cols<T>(vA, 16 * ks + 8 * g, hd);
+        }
+        if (ks + PF < KS) {
+          kq[ks % PF] = rowread(Kt, ks + PF);
+          vq[ks % PF] = rowread(Vt, ks + PF);
+        }
+        s = M::mma(kA, qreg[ks], s);
+        dp = M::mma(vA, dreg[ks], dp);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      V8 sb[2];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -lse2));
+        float w = p * (dp[j] - del);
+        if (need_mask) {
+          const int rel = k0 - vis_lo + 32 * tt + 8 * (j >> 2) + 4 * g + (j & 3);
+          if (static_cast<unsigned>(rel) > static_cast<unsigned>(vis_span)) w = 0.f;
+        }
+        sb[j >> 3][j & 7] = static_cast<T>(w);
+      }
+      constexpr int NM = 2 * NB;
+      auto trread = [&](int m) __attribute__((always_inline)) {
+        return tr_operand<T, D>(Kt, tb ^ ((m % NB) << 6), 2 * tt + m / NB);
+      };
+      V8 tq[PF];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) tq[i] = trread(i);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        __builtin_amdgcn_sched_barrier(0);
+        const V8 w = tq[m % PF];
+        if (m + PF < NM) tq[m % PF] = trread(m + PF);
+        dq[m % NB] = M::mma(w, sb[m / NB], dq[m % NB]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (n_t > 0) issue(0, 0);
+  for (int t = 0; t < n_t; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  const bool put = in && (my_q < plan.n || !a.keep_tail);
+  T* out = static_cast<T*>(a.dq) + hq * a.dq_h + my_q * a.dq_s;
+  const bool bad = row_has_nan<NB>(dq, g, hd);
+  if (put) store_accumulators<T, NB, KR>(out, dq, a.scale, g, hd);
+  if (__any(bad)) {  // see row_has_nan
+    const T* Qr = Qp + clip(my_q) * a.q_s;
+    const T* Dr = Dp + clip(my_q) * a.do_s;
+#pragma unroll 1
+    for (int n = 0; n < KS; ++n) {  // both halves alike: they exchange sums
+      const int c = 16 * n + 8 * g;
+      float acc[8] = {};
+#pragma unroll 1
+      for (int j = w_lo; j <= w_hi; ++j) {
+        const float dp = dot_two_rows<T>(Dr, Vp + j * a.v_s, g, hd);
+        const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd);
+        if (static_cast<unsigned>(j - vis_lo) > static_cast<unsigned>(vis_span)) continue;
+        const float w = __builtin_amdgcn_exp2f(fmaf(s, c2, -lse2)) * (dp - del);
+        for (int e = 0; e < 8; ++e)
+          if (c + e < hd) acc[e] = fmaf(w, to_f32(Kp[j * a.k_s + c + e]), acc[e]);
+      }
+      for (int e = 0; e < 8; ++e)
+        if (bad && put && c + e < hd) out[c + e] = static_cast<T>(acc[e] * a.scale);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ dK / dV --
+// 4 waves of 32 keys (K rows in registers, V rows in LDS); 32-query blocks of
+// every query head of the group, whose sums stay in the accumulators.
+template <typename T, int D, int KR>
+__global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
+  typedef Mfma<T> M;
+  typedef typename M::vec8 V8;
+  constexpr int BK = 128, MQ = 32;
+  constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
+  const int hd = KR ? a.d : D;
+  __shared__ __attribute__((aligned(16))) T Q0[MQ * D], Q1[MQ * D], dO0[MQ * D], dO1[MQ * D];
+  __shared__ __attribute__((aligned(16))) float lse2s[2][4][64];  // 64 lanes load, MQ used
+  __shared__ __attribute__((aligned(16))) float dels[2][4][64];
+  __shared__ __attribute__((aligned(16))) T Vw[4][32 * D];
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const PackedPlan plan(a);
+  const int block = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, n_rep = a.Hq / a.Hkv;
+  const int k0 = plan.first_row<BK, true>(a, block);
+  const int rows = static_cast<int>(a.T);
+  if (k0 >= rows) return;
+  const int kw0 = k0 + 32 * wave;
+  const int my_key = kw0 + l32;
+  const bool in = my_key < rows;
+  const float c2 = a.scale_log2;
+
+  const int last = rows - 1;
+  auto clip = [&](int r) __attribute__((always_inline)) { return r < last ? r : last; };
+  auto below = [&](int j) __attribute__((always_inline)) { return j < plan.n ? j : plan.n - 1; };
+  const int b_last = clip(k0 + BK - 1);
+  const int w_first = clip(kw0), w_last = clip(kw0 + 31);
+  const int q_lo = plan.query_lo(a, k0), q_hi = below(plan.query_hi(a, b_last)) + 1;
+  const int w_lo = plan.query_lo(a, w_first), w_hi = below(plan.query_hi(a, w_last));
+  const int f_lo = plan.query_lo(a, w_last), f_hi = plan.query_hi(a, w_first);
+  const bool idle = kw0 >= rows;
+  int vis_lo = 0x40000000, vis_span = 0;
+  if (in) {
+    const int lo = plan.query_lo(a, my_key), hi = plan.query_hi(a, my_key);
+    if (hi >= lo) {
+      vis_lo = lo;
+      vis_span = hi - lo;
+    }
+  }
+
+  const T* Kp = static_cast<const T*>(a.k) + hk * a.k_h;
+  const T* Vp = static_cast<const T*>(a.v) + hk * a.v_h;
+  V8 kreg[KS];
+  T* Vme = Vw[wave];
+  {
+    V8 vv[KS];
+    load_operand<T, KS, KR>(kreg, in ? Kp + my_key * a.k_s : nullptr, g, hd);
+    load_operand<T, KS, KR>(vv, in ? Vp + my_key * a.v_s : nullptr, g, hd);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      *reinterpret_cast<V8*>(&Vme[tile_off<D>(l32, 16 * ks + 8 * g)]) = vv[ks];
+  }
+
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int nt = 0; nt < NB; ++nt) {
+    dk[nt] = f32x16{};
+    dv[nt] = f32x16{};
+  }
+  const int rbase = 2 * tile_off<D>(l32, 8 * g);
+  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+
+  const int n_qb = q_hi > q_lo ? (q_hi - q_lo + MQ - 1) / MQ : 0;
+  const int n_it = n_qb * n_rep;
+  PackedLoader<T, D, MQ, 256> qload, dload;
+  qload.init(a.q_s, hd);
+  dload.init(a.do_s, hd);
+  auto issue = [&](int qb, int hr, int st) {
+    const int hq = hk * n_rep + hr;
+    const int qb0 = q_lo + qb * MQ;
+    qload.issue(st ? Q1 : Q0, static_cast<const T*>(a.q) + hq * a.q_h, a.q_s, qb0, plan.n);
+    dload.issue(st ? dO1 : dO0, static_cast<const T*>(a.dout) + hq * a.do_h, a.do_s, qb0, plan.n);
+    int qi = qb0 + lane;
+    if (qi > plan.n - 1) qi = plan.n - 1;
+    const int64_t r0 = static_cast<int64_t>(hq) * a.T + qb0;
+    const uint32_t off = static_cast<uint32_t>((qi - qb0) * 4);
+    dma_lds<4>(raw_rsrc(a.lse2 + r0), off, 0, &lse2s[st][wave][0]);
+    dma_lds<4>(raw_rsrc(a.delta + r0), off, 0, &dels[st][wave][0]);
+  };
+
+  auto step = [&](auto stage_tag, int qb, int nxt_qb, int nxt_hr, bool has_next) {
+    constexpr int st = decltype(stage_tag)::value;
+    const int qb0 = q_lo + qb * MQ;
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (has_next) issue(nxt_qb, nxt_hr, st ^ 1);
+    if (idle || qb0 > w_hi || qb0 + MQ <= w_lo) return;
+    const bool need_mask = qb0 < f_lo || qb0 + MQ - 1 > f_hi;
+    const T* Qt = st ? Q1 : Q0;
+    const T* dOt = st ? dO1 : dO0;
+    const float* l2v = lse2s[st][wave];
+    const float* dlv = dels[st][wave];
+    {
+      int rb = rbase, tb = tbase;  // opaque: addresses derived in the step
+      asm volatile("" : "+v"(rb), "+v"(tb));
+      f32x16 s = f32x16{}, dp = f32x16{};
+      // each step's Q operand is read one step ahead
+      V8 qa = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Qt) + rb);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int ro = rb ^ (ks << 5);
+        V8 da = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(dOt) + ro);
+        const V8 vb = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Vme) + ro);
+        V8 qn = qa;
+        if (ks + 1 < KS)
+          qn = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Qt) + (rb ^ ((ks + 1) << 5)));
+        if (ragged_step<KR>(ks)) {
+          qa = mask_cols<T>(qa, 16 * ks + 8 * g, hd);
+          da = mask_cols<T>(da, 16 * ks + 8 * g, hd);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        s = M::mma(qa, kreg[ks], s);
+        dp = M::mma(da, vb, dp);
+        qa = qn;
+      }
+      // one body with the mask in a branch of its own: two bodies, as in the
+      // forward, take more registers than there are here
+      if (need_mask) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int rel = qb0 - vis_lo + 8 * (j >> 2) + 4 * g + (j & 3);
+          s[j] = static_cast<unsigned>(rel) <= static_cast<unsigned>(vis_span) ? s[j] : -INFINITY;
+        }
+      }
+      V8 pb[2], sb[2];
+#pragma unroll
+      for (int a4 = 0; a4 < 4; ++a4) {
+        const int r0 = 8 * a4 + 4 * g;
+        const float4 l4 = *reinterpret_cast<const float4*>(&l2v[r0]);
+        const float4 d4 = *reinterpret_cast<const float4*>(&dlv[r0]);
+        const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * a4 + e;
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -lv[e]));
+          pb[j >> 3][j & 7] = static_cast<T>(p);
+          sb[j >> 3][j & 7] = static_cast<T>(p * (dp[j] - dl[e]));
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NB; ++nt) {
+          dv[nt] = M::mma(tr_operand<T, D>(dOt, tb ^ (nt << 6), kk), pb[kk], dv[nt]);
+          dk[nt] = M::mma(tr_operand<T, D>(Qt, tb ^ (nt << 6), kk), sb[kk], dk[nt]);
+        }
+    }
+  };
+
+  int qb = 0, hr = 0;
+  auto advance = [&](int& q, int& h) {
+    if (++q == n_qb) {
+      q = 0;
+      ++h;
+    }
+  };
+  if (n_it > 0) issue(0, 0, 0);
+  for (int it = 0; it < n_it; it += 2) {
+    int nq = qb, nh = hr;
+    advance(nq, nh);
+    step(std::integral_constant<int, 0>{}, qb, nq, nh, it + 1 < n_it);
+    qb = nq;
+    hr = nh;
+    if (it + 1 < n_it) {
+      advance(nq, nh);
+      step(std::integral_constant<int, 1>{}, qb, nq, nh, it + 2 < n_it);
+      qb = nq;
+      hr = nh;
+    }
+  }
+
+  const bool put = in && (my_key < plan.n || !a.keep_tail);
+  T* dkp = static_cast<T*>(a.dk) + hk * a.dk_h + my_key * a.dk_s;
+  T* dvp = static_cast<T*>(a.dv) + hk * a.dv_h + my_key * a.dv_s;
+  const bool bad_k = row_has_nan<NB>(dk, g, hd), bad_v = row_has_nan<NB>(dv, g, hd);
+  if (put) {
+    store_accumulators<T, NB, KR>(dkp, dk, a.scale, g, hd);
+    store_accumulators<T, NB, KR>(dvp, dv, 1.f, g, hd);
+  }
+  if (__any(bad_k | bad_v)) {  // see row_has_nan; dK, then dV
+    const T* Kr = Kp + clip(my_key) * a.k_s;
+    const T* Vr = Vp + clip(my_key) * a.v_s;
+#pragma unroll 1
+    for (int n = 0; n < 2 * KS; ++n) {
+      const bool second = n >= KS;
+      const int c0 = 16 * (second ? n - KS : n) + 8 * g;
+      float acc[8] = {};
+#pragma unroll 1
+      for (int h = hk * n_rep; h < (hk + 1) * n_rep; ++h) {
+        const T* Qp = static_cast<const T*>(a.q) + h * a.q_h;
+        const T* Dp = static_cast<const T*>(a.dout) + h * a.do_h;
+        const int64_t at = static_cast<int64_t>(h) * a.T;
+        const T* rows_of = second ? Dp : Qp;
+        const int64_t ld = second ? a.do_s : a.q_s;
+#pragma unroll 1
+        for (int i = w_lo; i <= w_hi; ++i) {
+          const float s = dot_two_rows<T>(Kr, Qp + i * a.q_s, g, hd);
+          const float dp = dot_two_rows<T>(Vr, Dp + i * a.do_s, g, hd);
+          if (static_cast<unsigned>(i - vis_lo) > static_cast<unsigned>(vis_span)) continue;
+          const float p = __builtin_amdgcn_exp2f(fmaf(s, c2, -a.lse2[at + i]));
+          const float w = second ? p : p * (dp - a.delta[at + i]) * a.scale;
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e < hd) acc[e] = fmaf(w, to_f32(rows_of[i * ld + c0 + e]), acc[e]);
+        }
+      }
+      T* row = second ? dvp : dkp;
+      for (int e = 0; e < 8; ++e)
+        if ((second ? bad_v : bad_k) && put && c0 + e < hd) row[c0 + e] = static_cast<T>(acc[e]);
+    }
+  }
+}
+
+template <typename T, int D, int KR>
+static void launch_packed_bwd(const PackedArgs& a, hipStream_t s) {
+  const int64_t blocks = packed_blocks(a.T, 128);
+  hipLaunchKernelGGL((packed_dq_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hq)),
+                     dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hkv)),
+                     dim3(256), 0, s, a);
+}
+template <typename T>
+static void launch_packed_bwd_t(const PackedArgs& a, bool ragged, hipStream_t s) {
+  if (!ragged) {
+    if (a.d == 128) launch_packed_bwd<T, 128, 0>(a, s);
+    else launch_packed_bwd<T, 64, 0>(a, s);
+    return;
+  }
+  switch ((a.d + 15) / 16) {
+    case 1:
+    case 2: launch_packed_bwd<T, 64, 2>(a, s); break;
+    case 3: launch_packed_bwd<T, 64, 3>(a, s); break;
+    case 4: launch_packed_bwd<T, 64, 4>(a, s); break;
+    case 5: launch_packed_bwd<T, 128, 5>(a, s); break;
+    case 6: launch_packed_bwd<T, 128, 6>(a, s); break;
+    case 7: launch_packed_bwd<T, 128, 7>(a, s); break;
+    default: launch_packed_bwd<T, 128, 8>(a, s); break;
+  }
+}
+
+}  // namespace zk
+
+using namespace zk;
+
+extern "C" int64_t zk_attn_packed_bwd_workspace(const zk_packed_desc* desc) {
+  if (desc == nullptr || desc->T < 0 || desc->Hq < 0) return 0;
+  return 2 * ((desc->Hq * desc->T + 63) / 64 * 64) * 4 + 256;
+}
+
+extern "C" int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, const void* k,
+                                  const void* v, const void* plan, const void* o,
+                                  const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                                  void* workspace, int64_t workspace_bytes, zk_stream_t stream) {
+  const char* who = "zk_attn_packed_bwd";
+  bool ragged;
+  const int rc = check_packed(desc, who, true, &ragged, {q, k, v, o, dout, dq, dk, dv});
+  if (rc != ZK_OK) return rc;
+  if (desc->T == 0) return ZK_OK;
+  ZK_REQUIRE(plan && lse, ZK_EINVAL, "%s: null pointer", who);
+  ZK_REQUIRE(aligned(plan, 4) && aligned(lse, 4), ZK_EALIGN, "%s: plan and lse must be 4-byte aligned", who);
+  const int64_t need = zk_attn_packed_bwd_workspace(desc);
+  ZK_REQUIRE(workspace != nullptr && workspace_bytes >= need, ZK_EWORKSPACE,
+             "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes, (long long)need);
+  PackedArgs a = {};
+  packed_args(a, desc, plan);
+  a.q = q; a.k = k; a.v = v; a.o = o; a.dout = dout; a.lse = lse;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.delta = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  a.lse2 = a.delta + (desc->Hq * desc->T + 63) / 64 * 64;
+  hipStream_t s = as_stream(stream);
+  if (desc->dtype == ZK_F32)
+    launch_packed_bwd_f32(a, s);
+  else if (desc->dtype == ZK_BF16)
+    launch_packed_bwd_t<bf16>(a, ragged, s);
+  else
+    launch_packed_bwd_t<f16>(a, ragged, s);
+  return launch_status(who);
+}

@@ -1,0 +1,422 @@
+// Attention over packed sequences, forward (bf16 / fp16 storage): the plan, the
+// kernel and the entry.
+#include <type_traits>
+
+#include "attn_packed.h"
+
+namespace zk {
+
+// ------------------------------------------------------------------- plan --
+// Each token's sequence by a search among the offsets.  What the offsets hold
+// is not trusted: whatever they are, start <= token < end <= n <= T.
+template <typename I>
+__global__ __launch_bounds__(256) void packed_rows_kernel(const I* __restrict__ offsets, int64_t n_seq,
+                                                          int64_t T, int32_t* __restrict__ plan,
+                                                          int64_t* __restrict__ positions) {
+  const int64_t last = n_seq > 0 ? static_cast<int64_t>(offsets[n_seq]) : 0;
+  const int n = static_cast<int>(last < 0 ? 0 : last > T ? T : last);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i == 0) plan[0] = n;
+  if (i >= T) return;
+  int lo = static_cast<int>(i), hi = lo;
+  if (i < n) {
+    int64_t a = 0, b = n_seq;  // offsets[a] <= i < offsets[b], as if offsets[0] were 0
+    while (b - a > 1) {
+      const int64_t m = (a + b) / 2;
+      if (static_cast<int64_t>(offsets[m]) <= i) a = m; else b = m;
+    }
+    const int64_t s = static_cast<int64_t>(offsets[a]), e = static_cast<int64_t>(offsets[b]);
+    lo = static_cast<int>(s < 0 || s > i ? 0 : s);
+    hi = static_cast<int>(e <= i ? i + 1 : e > n ? n : e);
+  }
+  plan[kPlanHeader + i] = lo;
+  plan[kPlanHeader + T + i] = hi;
+  if (positions != nullptr) positions[i] = i - lo;
+}
+
+// Blocks by their work, most first: a counting sort on the tokens that the
+// block's last query (first key) sees under the causal mask, one workgroup.  The
+// largest blocks start first, so that the launch's end is short whatever the
+// lengths are.
+__global__ __launch_bounds__(1024) void packed_order_kernel(int64_t T, int32_t* __restrict__ plan) {
+  const int32_t* start = plan + kPlanHeader;
+  const int32_t* end = start + T;
+  __shared__ int hist[1024];
+  int shift = 5;
+  while ((T >> shift) >= 1024) ++shift;
+  for (int which = 0; which < 3; ++which) {
+    const int rows = which == 0 ? 256 : 128, nb = static_cast<int>((T + rows - 1) / rows);
+    int32_t* order = plan + plan_order_at(T, which);
+    auto key = [&](int b) {
+      const int64_t first = static_cast<int64_t>(b) * rows;
+      const int64_t past = first + rows < T ? first + rows : T;
+      const int64_t work = which < 2 ? past - start[first] : end[past - 1] - first;
+      const int bin = static_cast<int>((work < 0 ? 0 : work) >> shift);
+      return 1023 - (bin < 1024 ? bin : 1023);  // the largest in bin 0
+    };
+    hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += 1024) atomicAdd(&hist[key(b)], 1);
+    __syncthreads();
+    for (int step = 1; step < 1024; step *= 2) {  // inclusive sums
+      const int add = static_cast<int>(threadIdx.x) >= step ? hist[threadIdx.x - step] : 0;
+      __syncthreads();
+      hist[threadIdx.x] += add;
+      __syncthreads();
+    }
+    // a bin's blocks from its end down; their order within it changes no result
+    for (int b = threadIdx.x; b < nb; b += 1024) order[atomicSub(&hist[key(b)], 1) - 1] = b;
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- forward --
+static constexpr float kGrowth = 8.0f;  // log2 growth of the maximum before a rescale
+
+// NW waves of 32 queries.  KR: 0 for a head dim of D and 16-byte aligned heads,
+// else ceil(d / 16), at least 2.
+template <typename T, int D, int NW, int KR>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+void packed_fwd_kernel(PackedArgs a) {
+  typedef Mfma<T> M;
+  typedef typename M::vec8 V8;
+  constexpr int BM = 32 * NW, BN = 64, NT = 64 * NW;
+  constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
+  const int hd = KR ? a.d : D;
+  __shared__ __attribute__((aligned(16))) T K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const PackedPlan plan(a);
+  int block, hq;
+  packed_block(a, block, hq);
+  const int q0 = plan.first_row<BM, false>(a, block);
+  const int rows = static_cast<int>(a.T);
+  if (q0 >= rows) return;
+  const int hk = hq / (a.Hq / a.Hkv);
+  const int qw0 = q0 + 32 * wave;
+  const int my_q = qw0 + l32;
+  const bool in = my_q < rows;
+
+  // the wave's and the block's ranges of keys (scalar: their rows are uniform)
+  const int last = rows - 1;
+  auto clip = [&](int r) __attribute__((always_inline)) { return r < last ? r : last; };
+  const int b_last = clip(q0 + BM - 1);
+  const int w_first = clip(qw0), w_last = clip(qw0 + 31);
+  auto below = [&](int j) __attribute__((always_inline)) { return j < plan.n ? j : plan.n - 1; };
+  const int kv_lo = plan.key_lo(a, q0), kv_hi = below(plan.key_hi(a, b_last)) + 1;
+  const int w_lo = plan.key_lo(a, w_first), w_hi = below(plan.key_hi(a, w_last));  // seen by any
+  const int f_lo = plan.key_lo(a, w_last), f_hi = plan.key_hi(a, w_first);         // seen by all
+  const bool idle = qw0 >= rows;
+  int vis_lo = 0x40000000, vis_span = 0;
+  bool any_key = false;
+  if (in) {
+    const int lo = plan.key_lo(a, my_q), hi = plan.key_hi(a, my_q);
+    if (hi >= lo) {
+      vis_lo = lo;
+      vis_span = hi - lo;
+      any_key = true;
+    }
+  }
+
+  const T* Qp = static_cast<const T*>(a.q) + hq * a.q_h;
+  const T* Kp = static_cast<const T*>(a.k) + hk * a.k_h;
+  const T* Vp = static_cast<const T*>(a.v) + hk * a.v_h;
+  V8 qreg[KS];
+  load_operand<T, KS, KR>(qreg, in ? Qp + my_q * a.q_s : nullptr, g, hd);
+
+  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + BN - 1) / BN : 0;
+  PackedLoader<T, D, BN, NT> kload, vload;
+  kload.init(a.k_s, hd);
+  vload.init(a.v_s, hd);
+  auto issue = [&](int t, int st) {
+    const int k0 = kv_lo + t * BN;
+    kload.issue(st ? K1 : K0, Kp, a.k_s, k0, plan.n);
+    vload.issue(st ? V1 : V0, Vp, a.v_s, k0, plan.n);
+  };
+  // LDS byte offsets from two per-lane bases (the swizzle XORs chunk indices)
+  const int rbase = 2 * tile_off<D>(l32, 8 * g);
+  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+
+  f32x16 o[NB];
+#pragma unroll
+  for (int nt = 0; nt < NB; ++nt) o[nt] = f32x16{};
+  float m_ref = -INFINITY, l_i = 0.f;
+  const float c2 = a.scale_log2;
+
+  auto step = [&](auto stage_tag, int t) {
+    constexpr int st = decltype(stage_tag)::value;
+    const int k0 = kv_lo + t * BN;
+    wait_vmcnt<0>();  // this wave's loads of tile t have landed
+    __syncthreads();  // ... and every other wave's; all are done with the other stage
+    if (t + 1 < n_t) issue(t + 1, st ^ 1);
+    if (idle || k0 > w_hi || k0 + BN <= w_lo) return;
+    const bool need_mask = k0 < f_lo || k0 + BN - 1 > f_hi;
+    const T* Kt = st ? K1 : K0;
+    const T* Vt = st ? V1 : V0;
+    auto tile = [&](auto mask_tag) {
+      constexpr bool kMask = decltype(mask_tag)::value;
+      // opaque, so that addresses are derived in the step, and in each body: what
+      // both share is not moved before the branch, where it would be held (and
+      // spilled) over it
+      int rb = rbase, tb = tbase;
+      asm volatile("" : "+v"(rb), "+v"(tb));
+      f32x16 s[BN / 32];
+#pragma unroll
+      for (int tt = 0; tt < BN / 32; ++tt) {
+        s[tt] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          V8 kv = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Kt) +
+                                               (rb ^ (ks << 5)) + tt * 32 * D * 2);
+          if (ragged_step<KR>(ks)) kv = mask_cols<T>(kv, 16 * ks + 8 * g, hd);
+          s[tt] = M::mma(kv, qreg[ks], s[tt]);
+        }
+      }
+      if (kMask) {
+        const int kb = k0 + 4 * g - vis_lo;
+#pragma unroll
+        for (int tt = 0; tt < BN / 32; ++tt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int rel = kb + 32 * tt + 8 * (j >> 2) + (j & 3);
+            s[tt][j] = static_cast<unsigned>(rel) <= static_cast<unsigned>(vis_span) ? s[tt][j]
+                                                                                    : -INFINITY;
+          }
+      }
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int tt = 0; tt < BN / 32; ++tt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, s[tt][j]);
+      mloc = fmaxf(mloc, other_half(mloc));
+      const bool grow = (mloc - m_ref) * c2 > kGrowth;
+      if (__any(grow)) {
+        const float m_new = fmaxf(m_ref, mloc);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_ref - m_new) * c2);
+        m_ref = m_new;
+        l_i *= alpha;
+#pragma unroll
+        for (int nt = 0; nt < NB; ++nt) o[nt] *= alpha;
+      }
+      const float mc = m_ref == -INFINITY ? 0.f : m_ref * c2;
+      V8 pb[BN / 16];
+      float lsum = 0.f;
+#pragma unroll
+      for (int tt = 0; tt < BN / 32; ++tt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[tt][j], c2, -mc));
+          lsum += p;
+          pb[2 * tt + (j >> 3)][j & 7] = static_cast<T>(p);
+        }
+      l_i += lsum;
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk) {
+#pragma unroll
+        for (int nt = 0; nt < NB; ++nt) {
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          typedef short s16x8 __attribute__((ext_vector_type(8)));
+          typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+          const char* vb = reinterpret_cast<const char*>(Vt) + kk * 16 * D * 2;
+          const int off = tb ^ (nt << 6);
+          const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + off));
+          const s16x4 x1 =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + 8 * D * 2 + (off ^ 32)));
+          const s16x8 w = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+          o[nt] = M::mma(__builtin_bit_cast(V8, w), pb[kk], o[nt]);
+        }
+      }
+    };
+    if (need_mask)
+      tile(std::true_type{});
+    else
+      tile(std::false_type{});
+  };
+
+  if (n_t > 0) issue(0, 0);
+  for (int t = 0; t < n_t; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  const float l_tot = l_i + other_half(l_i);
+  // no weight although keys are visible: every score is -inf or NaN, and so is O
+  const float inv = l_tot > 0.f ? 1.0f / l_tot : any_key ? NAN : 0.f;
+  const bool put = in && (my_q < plan.n || !a.keep_tail);
+  T* Op = static_cast<T*>(a.out) + hq * a.o_h + my_q * a.o_s;
+  float* lp = a.lse_out + static_cast<int64_t>(hq) * a.T + my_q;
+  const bool bad = row_has_nan<NB>(o, g, hd);
+  if (put) {
+    store_accumulators<T, NB, KR>(Op, o, inv, g, hd);
+    if (g == 0) *lp = l_tot > 0.f ? m_ref * a.scale + logf(l_tot) : any_key ? NAN : -INFINITY;
+  }
+  if (__any(bad)) {  // see row_has_nan
+    const T* Qr = Qp + clip(my_q) * a.q_s;
+    auto seen = [&](int j) __attribute__((always_inline)) {
+      return static_cast<unsigned>(j - vis_lo) <= static_cast<unsigned>(vis_span);
+    };
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int j = w_lo; j <= w_hi; ++j) {
+      const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd) * c2;
+      if (!seen(j)) continue;
+      const float m_new = fmaxf(m, s), ref = m_new == -INFINITY ? 0.f : m_new;
+      l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(s - ref);
+      m = m_new;
+    }
+    const float ref = m == -INFINITY ? 0.f : m, w = l > 0.f ? 1.0f / l : any_key ? NAN : 0.f;
+    if (bad && put && g == 0) *lp = l > 0.f ? m / kLog2e + logf(l) : any_key ? NAN : -INFINITY;
+#pragma unroll 1
+    for (int n = 0; n < KS; ++n) {  // both halves alike: they exchange sums
+      const int c = 16 * n + 8 * g;
+      float acc[8] = {};
+#pragma unroll 1
+      for (int j = w_lo; j <= w_hi; ++j) {
+        const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd) * c2;
+        if (!seen(j)) continue;
+        const float p = __builtin_amdgcn_exp2f(s - ref);
+        for (int e = 0; e < 8; ++e)
+          if (c + e < hd) acc[e] = fmaf(p, to_f32(Vp[j * a.v_s + c + e]), acc[e]);
+      }
+      for (int e = 0; e < 8; ++e)
+        if (bad && put && c + e < hd) Op[c + e] = static_cast<T>(acc[e] * w);
+    }
+  }
+}
+
+int check_packed(const zk_packed_desc* D, const char* who, bool bwd, bool* ragged,
+                 std::initializer_list<const void*> tensors) {
+  ZK_REQUIRE(D != nullptr, ZK_EINVAL, "%s: null descriptor", who);
+  ZK_REQUIRE(valid_dtype(D->dtype), ZK_EDTYPE, "%s: bad dtype %d", who, D->dtype);
+  ZK_REQUIRE(D->T >= 0 && D->T < (int64_t(1) << 30), ZK_EINVAL, "%s: T=%lld tokens, 0 .. 2^30 - 1",
+             who, (long long)D->T);
+  ZK_REQUIRE(D->Hq > 0 && D->Hkv > 0 && D->Hq < 65536 && D->Hq % D->Hkv == 0, ZK_EINVAL,
+             "%s: Hq=%lld not a multiple of Hkv=%lld", who, (long long)D->Hq, (long long)D->Hkv);
+  ZK_REQUIRE(D->window >= 0 && (D->causal || D->window == 0), ZK_EINVAL,
+             "%s: a window (%lld) needs causal attention", who, (long long)D->window);
+  ZK_REQUIRE(D->scale > 0.f && D->scale < INFINITY, ZK_EINVAL, "%s: scale must be positive", who);
+  ZK_REQUIRE(D->d > 0 && D->d <= 128 && (D->dtype == ZK_F32 || D->d % 2 == 0), ZK_EUNSUPPORTED,
+             "%s: head dims up to 128, even ones for 2-byte types (got %lld)", who, (long long)D->d);
+  const int64_t strides[] = {D->q_s, D->q_h, D->k_s, D->k_h, D->v_s, D->v_h, D->o_s, D->o_h,
+                             D->do_s, D->do_h, D->dq_s, D->dq_h, D->dk_s, D->dk_h, D->dv_s, D->dv_h};
+  bool vec16 = D->d == 64 || D->d == 128, vec4 = true;
+  for (int i = 0; i < (bwd ? 16 : 8); ++i) {
+    vec16 = vec16 && strides[i] % 8 == 0;
+    vec4 = vec4 && strides[i] % 2 == 0;
+    // the tile loaders keep a tile's rows in a 32-bit byte offset
+    ZK_REQUIRE(i % 2 != 0 || (strides[i] >= 0 && strides[i] < (int64_t(1) << 23)), ZK_EUNSUPPORTED,
+               "%s: row stride %lld out of range", who, (long long)strides[i]);
+  }
+  for (const void* p : tensors) {
+    ZK_REQUIRE(p != nullptr || D->T == 0, ZK_EINVAL, "%s: null pointer", who);
+    vec16 = vec16 && aligned(p, 16);
+    vec4 = vec4 && aligned(p, 4);
+  }
+  bool at4 = true;
+  for (const void* p : tensors) at4 = at4 && aligned(p, 4);
+  ZK_REQUIRE(D->dtype == ZK_F32 ? at4 : vec4, ZK_EALIGN, "%s: heads start at multiples of 4 bytes",
+             who);
+  ZK_REQUIRE(D->Hq * ((D->T + 127) / 128) * 4 < 0x7fffffffLL, ZK_EINVAL, "%s: grid too large", who);
+  *ragged = !vec16;
+  return ZK_OK;
+}
+
+void packed_args(PackedArgs& a, const zk_packed_desc* D, const void* plan) {
+  a.plan = static_cast<const int32_t*>(plan);
+  a.T = D->T; a.Hq = static_cast<int>(D->Hq); a.Hkv = static_cast<int>(D->Hkv); a.d = static_cast<int>(D->d);
+  a.q_s = D->q_s; a.q_h = D->q_h; a.k_s = D->k_s; a.k_h = D->k_h; a.v_s = D->v_s; a.v_h = D->v_h;
+  a.o_s = D->o_s; a.o_h = D->o_h; a.do_s = D->do_s; a.do_h = D->do_h;
+  a.dq_s = D->dq_s; a.dq_h = D->dq_h; a.dk_s = D->dk_s; a.dk_h = D->dk_h; a.dv_s = D->dv_s; a.dv_h = D->dv_h;
+  a.scale = D->scale;
+  a.scale_log2 = D->scale * kLog2e;
+  a.causal = D->causal != 0;
+  // a window of all tokens is none
+  a.window = D->window >= D->T ? 0 : static_cast<int>(D->window);
+  a.keep_tail = D->keep_tail != 0;
+}
+
+}  // namespace zk
+
+using namespace zk;
+
+extern "C" int64_t zk_packed_plan_bytes(int64_t T) {
+  if (T < 0 || T >= (int64_t(1) << 30)) {
+    set_error("zk_packed_plan_bytes: T=%lld tokens, 0 .. 2^30 - 1", (long long)T);
+    return ZK_EINVAL;
+  }
+  return 4 * plan_order_at(T, 3);
+}
+
+extern "C" int zk_packed_plan(const void* offsets, int offsets_64, int64_t n_seq, int64_t T, void* plan,
+                              int64_t plan_bytes, int64_t* positions, zk_stream_t stream) {
+  const char* who = "zk_packed_plan";
+  ZK_REQUIRE(T >= 0 && T < (int64_t(1) << 30) && n_seq >= 0 && n_seq < (int64_t(1) << 31), ZK_EINVAL,
+             "%s: T=%lld tokens (0 .. 2^30 - 1), %lld sequences", who, (long long)T, (long long)n_seq);
+  ZK_REQUIRE(offsets != nullptr && plan != nullptr, ZK_EINVAL, "%s: null pointer", who);
+  ZK_REQUIRE(aligned(plan, 16) && aligned(offsets, offsets_64 ? 8 : 4) && aligned(positions, 8), ZK_EALIGN,
+             "%s: the plan must be 16-byte aligned, offsets and positions as their types", who);
+  ZK_REQUIRE(plan_bytes >= zk_packed_plan_bytes(T), ZK_EWORKSPACE, "%s: plan %lld < %lld bytes", who,
+             (long long)plan_bytes, (long long)zk_packed_plan_bytes(T));
+  hipStream_t s = as_stream(stream);
+  int32_t* p = static_cast<int32_t*>(plan);
+  const dim3 grid(static_cast<unsigned>(T > 0 ? (T + 255) / 256 : 1));
+  if (offsets_64)
+    hipLaunchKernelGGL(packed_rows_kernel<int64_t>, grid, dim3(256), 0, s,
+                       static_cast<const int64_t*>(offsets), n_seq, T, p, positions);
+  else
+    hipLaunchKernelGGL(packed_rows_kernel<int32_t>, grid, dim3(256), 0, s,
+                       static_cast<const int32_t*>(offsets), n_seq, T, p, positions);
+  if (T > 0) hipLaunchKernelGGL(packed_order_kernel, dim3(1), dim3(1024), 0, s, T, p);
+  return launch_status(who);
+}
+
+namespace zk {
+template <typename T, int D, int NW, int KR>
+static void launch_packed_fwd(const PackedArgs& a, hipStream_t s) {
+  const int64_t blocks = packed_blocks(a.T, 32 * NW);
+  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, KR>), dim3(static_cast<unsigned>(blocks * a.Hq)),
+                     dim3(64 * NW), 0, s, a);
+}
+template <typename T>
+static void launch_packed_fwd_t(const PackedArgs& a, bool ragged, hipStream_t s) {
+  if (!ragged) {
+    if (a.d == 128) launch_packed_fwd<T, 128, 8, 0>(a, s);
+    else launch_packed_fwd<T, 64, 4, 0>(a, s);
+    return;
+  }
+  switch ((a.d + 15) / 16) {
+    case 1:
+    case 2: launch_packed_fwd<T, 64, 4, 2>(a, s); break;
+    case 3: launch_packed_fwd<T, 64, 4, 3>(a, s); break;
+    case 4: launch_packed_fwd<T, 64, 4, 4>(a, s); break;
+    case 5: launch_packed_fwd<T, 128, 8, 5>(a, s); break;
+    case 6: launch_packed_fwd<T, 128, 8, 6>(a, s); break;
+    case 7: launch_packed_fwd<T, 128, 8, 7>(a, s); break;
+    default: launch_packed_fwd<T, 128, 8, 8>(a, s); break;
+  }
+}
+}  // namespace zk
+
+extern "C" int zk_attn_packed_fwd(const zk_packed_desc* desc, const void* q, const void* k,
+                                  const void* v, const void* plan, void* o, float* lse,
+                                  zk_stream_t stream) {
+  const char* who = "zk_attn_packed_fwd";
+  bool ragged;
+  const int rc = check_packed(desc, who, false, &ragged, {q, k, v, o});
+  if (rc != ZK_OK) return rc;
+  if (desc->T == 0) return ZK_OK;
+  ZK_REQUIRE(plan && lse, ZK_EINVAL, "%s: null pointer", who);
+  ZK_REQUIRE(aligned(plan, 4) && aligned(lse, 4), ZK_EALIGN, "%s: plan and lse must be 4-byte aligned", who);
+  PackedArgs a = {};
+  packed_args(a, desc, plan);
+  a.q = q; a.k = k; a.v = v; a.out = o; a.lse_out = lse;
+  hipStream_t s = as_stream(stream);
+  if (desc->dtype == ZK_F32)
+    launch_packed_fwd_f32(a, s);
+  else if (desc->dtype == ZK_BF16)
+    launch_packed_fwd_t<bf16>(a, ragged, s);
+  else
+    launch_packed_fwd_t<f16>(a, ragged, s);
+  return launch_status(who);
+}

@@ -8,80 +8,9 @@
 // own lookup takes 54, of which the kernels are 10.  A node in C++ touches no
 // Python object.  The tables of 150 tensors are 750 checks and 1500 numbers,
 // 350 us of Python and 20 us here.
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <pybind11/stl.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include <algorithm>
-#include <cstring>
-#include <optional>
-#include <string>
-#include <utility>
-#include <vector>
-
-#include "../../include/zorse_amd.h"
-
-namespace py = pybind11;
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-typedef std::optional<Tensor> MaybeTensor;
+#include "nodes.h"
 
 namespace {
-
-[[noreturn]] void bad(const std::string& what) { throw py::value_error(what); }
-
-void check(int status, const char* who) {
-  if (status == 0) return;
-  static const char* const names[] = {"ZK_EINVAL", "ZK_EDTYPE", "ZK_EALIGN", "ZK_EUNSUPPORTED",
-                                      "ZK_EWORKSPACE"};
-  throw std::runtime_error(std::string(who) + " failed with " +
-                           (status < 0 && status >= -5 ? names[-1 - status]
-                                                       : "hipError " + std::to_string(status)) +
-                           ": " + zk_last_error());
-}
-
-zk_stream_t stream_of(const Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.get_device()).stream();
-}
-
-at::ScalarType type_of(int64_t code) {
-  return code == ZK_F32 ? at::kFloat : code == ZK_F16 ? at::kHalf : at::kBFloat16;
-}
-int code_of(at::ScalarType t) {
-  return t == at::kFloat ? ZK_F32 : t == at::kHalf ? ZK_F16 : t == at::kBFloat16 ? ZK_BF16 : -1;
-}
-int float_code(const char* name, at::ScalarType t) {
-  const int code = code_of(t);
-  if (code < 0) bad(c10::str("unsupported ", name, " dtype ", t));
-  return code;
-}
-
-constexpr const char* kNeedGpu = "zorse_amd kernels need GPU tensors (got a CPU tensor)";
-
-void one_gpu(std::initializer_list<const Tensor*> tensors) {
-  const Tensor& first = **tensors.begin();
-  for (const Tensor* t : tensors) {
-    if (!t->defined()) continue;
-    if (!t->is_cuda()) bad(kNeedGpu);
-    if (t->get_device() != first.get_device()) bad("tensors are on different devices");
-  }
-}
-
-void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
-
-Tensor workspace(int64_t bytes, const Tensor& like) {
-  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
-}
-
-// Forward-mode derivatives: a dual tensor carries its tangent beside its values.
-bool is_dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 
 // f(t) for a linear f and a dual t, a dual tensor too.
 template <typename F>
@@ -256,11 +185,6 @@ struct Qk {  // operands; k, wk and positions may be undefined
   Tensor q, k, wq, wk, cos, sin, positions;
 };
 
-// Unit stride along d (expanded heads and gradients have none).
-Tensor rows_of(const Tensor& t) {
-  return !t.defined() || t.dim() == 0 || t.stride(-1) == 1 ? t : t.contiguous();
-}
-
 struct Strides {
   int64_t b = 0, s = 0, h = 0;
 };
@@ -422,7 +346,6 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
 };
 
 typedef std::pair<Tensor, MaybeTensor> QkPair;
-MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 // functional.qk_norm_rope
 QkPair qk_norm_rope(const Tensor& q, const MaybeTensor& k, const Tensor& wq, const MaybeTensor& wk,
@@ -659,4 +582,5 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, free_gil);
   m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, free_gil);
   m.def("rows", &rows);
+  bind_packed(m);
 }

@@ -1,6 +1,7 @@
 """Autograd functions over the HIP kernels (RMSNorm, RoPE + flash attention,
-SwiGLU, token embedding, the norm of query and key heads), usable on their own;
-the fused decoder layer lives in ``layer.py``.
+attention over packed sequences, the rotation by several axes, SwiGLU, token
+embedding, the norm of query and key heads), usable on their own; the fused
+decoder layer lives in ``layer.py``.
 
 RoPE tables are built once per (S, d, theta, pairing, dtype, device) with the
 reference's formula (models/llama_simple.py:75-81, 115-137: inv_freq and the
@@ -172,3 +173,97 @@ def flash_attention(q, k, v, *, causal=True, window=0, scale=None, rope_theta=No
         scale = 1.0 / math.sqrt(q.shape[-1])
     return FlashAttentionFunction.apply(q, k, v, bool(causal), int(window or 0),
                                         float(scale), rope_theta, bool(interleaved))
+
+
+# ------------------------------------------- Packed sequences, their attention --
+
+class PackedSequences:
+    """Sequences that lie one after another in one run of ``tokens`` tokens:
+    sequence s is the tokens offsets[s] .. offsets[s + 1] - 1.  It is made once
+    a batch and serves every layer, forward and backward.
+
+    ``offsets``: sequences + 1 ascending token counts from 0 on, int32 / int64.
+    On the GPU they are not read back to the host to check them, and ``tokens``
+    is needed; a list or a CPU tensor is checked, moved to ``device`` (default
+    the current GPU) and gives ``tokens`` (default the last offset).  Tokens
+    behind the last sequence are padding.
+
+    ``plan`` holds the kernels' tables, ``positions`` (int64 [tokens]) every
+    token's place in its sequence, for the rotations."""
+
+    def __init__(self, offsets, tokens=None, *, device=None):
+        offsets = self._offsets(offsets, tokens, device)
+        if tokens is None:
+            if self._last is None:
+                raise ValueError("PackedSequences: tokens is needed for offsets on the GPU")
+            tokens = self._last
+        self.tokens = int(tokens)
+        self.plan = torch.empty(K.packed_plan_words(self.tokens), device=offsets.device,
+                                dtype=torch.int32)
+        self.positions = torch.empty(self.tokens, device=offsets.device, dtype=torch.int64)
+        self._make(offsets)
+
+    def update(self, offsets) -> "PackedSequences":
+        """Other sequences of the same run of tokens, in the same tables: what a
+        captured graph that uses them replays with."""
+        self._make(self._offsets(offsets, self.tokens, self.plan.device))
+        torch.autograd.graph.increment_version((self.plan, self.positions))
+        return self
+
+    def _offsets(self, offsets, tokens, device):
+        self._last = None
+        if torch.is_tensor(offsets) and offsets.is_cuda:
+            return offsets.contiguous()
+        offsets = torch.as_tensor(offsets)
+        if offsets.dim() != 1 or offsets.numel() == 0 or offsets.is_floating_point():
+            raise ValueError("PackedSequences: offsets are [sequences + 1] integers")
+        steps = offsets.tolist()
+        if steps[0] != 0 or any(b < a for a, b in zip(steps, steps[1:])):
+            raise ValueError("PackedSequences: offsets start at 0 and ascend")
+        if tokens is not None and steps[-1] > tokens:
+            raise ValueError(f"PackedSequences: the sequences have {steps[-1]} tokens, "
+                             f"more than {tokens}")
+        self._last = steps[-1]
+        return offsets.to(device="cuda" if device is None else device, dtype=torch.int64)
+
+    def _make(self, offsets) -> None:
+        K.packed_plan(offsets, self.tokens, self.plan, self.positions)
+
+
+def packed_attention(q, k, v, sequences, *, causal=True, window=0, scale=None):
+    """Attention within each of the ``sequences`` (PackedSequences): q
+    [tokens, Hq, d], k / v [tokens, Hkv, d], Hq a multiple of Hkv, d up to 128
+    (even in bf16 / fp16) -> [tokens, Hq, d].  ``causal``: a token sees those up
+    to itself, with ``window`` > 0 the last ``window`` of them; otherwise its
+    whole sequence.  Padding rows of the result and of the gradients are zeros,
+    and nothing of a token that a row does not see reaches it, be it infinite or
+    NaN.  It can be differentiated once, backward; rotate q and k before
+    (``sequences.positions``)."""
+    return nodes().packed_attention(q, k, v, sequences.plan, causal, window or 0, scale)
+
+
+# ------------------------------------------------ Rotation by several axes --
+
+def rope_axes(q, k, cos, sin, positions, pair_axes, *, interleaved=False):
+    """(q', k'): the rotation of q [tokens, Hq, d] and k [tokens, Hkv, d] (or
+    [B, S, H, d]; k may be None) by positions of several axes.  ``positions``
+    int64 [axes, tokens] (or [axes, B, S]); ``pair_axes``: the axis of each of
+    the d/2 pairs (pair_axes_of); cos / sin: fp32 [n_pos, d/2] tables
+    (rope_tables(..., torch.float32, ...)), pair i of a token turned by their row
+    positions[pair_axes[i], token].  fp32 with one rounding; a position outside
+    the tables gives NaN in its axis' pairs.  Any even d up to 512; q and k may
+    be views of one q|k|v buffer.  Linear in q and k: it can be differentiated
+    any number of times, backward."""
+    return nodes().rope_axes(q, k, cos, sin, positions, bytes(pair_axes), interleaved)
+
+
+def pair_axes_of(sections, *, turns=False):
+    """The axis of each pair, for ``sections[a]`` pairs of axis a: one axis' pairs
+    after another's, or, with ``turns``, the axes in turn as long as each has
+    pairs left."""
+    sections = [int(n) for n in sections]
+    if not sections or min(sections) < 0 or len(sections) > 256:
+        raise ValueError(f"pair_axes_of: numbers of pairs are needed (got {sections})")
+    if not turns:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    return bytes(a for i in range(max(sections)) for a, n in enumerate(sections) if i < n)

@@ -932,6 +932,51 @@ def adamw8_values(exp_avgs, exp_avg_sqs, bases, *, dtype: torch.dtype = torch.fl
     return outs
 
 
+# -------------------------------------------- Packed sequences, rotations ---
+
+def packed_plan_words(tokens: int) -> int:
+    """int32 elements of the plan of a run of ``tokens`` tokens."""
+    n = lib().zk_packed_plan_bytes(tokens)
+    if n < 0:
+        raise ValueError(_abi.last_error())
+    return n // 4
+
+
+def packed_plan(offsets, tokens: int, plan=None, positions=None):
+    """(plan, positions): the tables of attn_packed_fwd / bwd for the sequences
+    that ``offsets`` (int32 / int64 [sequences + 1] on the GPU) cut from a run of
+    ``tokens`` tokens, and every token's place in its sequence (int64).  The
+    offsets are read by the kernel, and whatever they hold the plan refers to
+    tokens of the run only."""
+    if plan is None:
+        plan = torch.empty(packed_plan_words(tokens), device=offsets.device, dtype=torch.int32)
+    _abi.nodes().packed_plan(offsets, tokens, plan, positions)
+    return plan, positions
+
+
+def attn_packed_fwd(q, k, v, plan, *, causal: bool = True, window: int = 0, scale=None, out=None):
+    """(o, lse) of attention within packed sequences (functional.packed_attention);
+    q [tokens, Hq, d], k / v [tokens, Hkv, d], lse fp32 [Hq, tokens].  Rows behind
+    the last sequence are zeros in a new o and left as they are in ``out``."""
+    return _abi.nodes().attn_packed_fwd(q, k, v, plan, causal, window, scale, out)
+
+
+def attn_packed_bwd(q, k, v, o, dout, lse, plan, *, causal: bool = True, window: int = 0,
+                    scale=None, dq=None, dk=None, dv=None):
+    """(dq, dk, dv) from the forward's o and lse; rows behind the last sequence as
+    in attn_packed_fwd."""
+    return tuple(_abi.nodes().attn_packed_bwd(q, k, v, o, dout, lse, plan, causal, window, scale,
+                                              dq, dk, dv))
+
+
+def rope_axes(q, k, cos, sin, positions, pair_axes, *, interleaved: bool = False,
+              inverse: bool = False, q_out=None, k_out=None):
+    """functional.rope_axes without gradients, in either direction (``inverse``: by
+    the opposite angles); the outputs may be q and k themselves."""
+    return _abi.nodes().rope_axes_to(q, k, cos, sin, positions, bytes(pair_axes), interleaved,
+                                     inverse, q_out, k_out)
+
+
 def cast_(src: torch.Tensor, dst: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
     """dst = round(src) (or dst = round(dst + src)); contiguous, same numel."""
     dev = _require_gpu(src, dst)
