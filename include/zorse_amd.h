@@ -641,6 +641,44 @@ int zk_rope_axes(const zk_axes_desc* desc, const void* q, const void* k, void* q
                  const int64_t* positions, const unsigned char* pair_axes,
                  zk_stream_t stream);
 
+/* -------------------------------------------------- Orthogonal updates -----
+ * The orthogonal factors of a list of matrices by Newton-Schulz products, and the
+ * optimizer step that takes them (no counterpart in the reference; beside the
+ * AdamW steps).  X = u / (|u| + eps) with the Frobenius norm, then `steps` times
+ *     X <- a X + (b X X^T + c (X X^T)^2) X     (X^T X on the right for tall ones)
+ * in fp16 products with fp32 sums, X in 22 bits; matrices whose shorter side is at
+ * most 128, and those with fp32 results, in 22 bits throughout.
+ *   zk_orthogonalize:  out = X of u = grad
+ *   zk_muon_multi:     m = momentum m + (1 - momentum) grad
+ *                      u = (1 - momentum) grad + momentum m   (nesterov), or m
+ *                      param = param (1 - lr weight_decay) - lr f X
+ *                      out = round(param), unless NULL
+ * with f = sqrt(max(1, rows / cols)) (ZK_MUON_ORIGINAL) or 0.2 sqrt(max(rows,
+ * cols)) (ZK_MUON_MATCH_RMS, the size of an AdamW step).  Rows of cols elements
+ * ld_ apart; param and momentum fp32 (NULL for zk_orthogonalize), grad and out any
+ * of the three types; sides below 2^20.  The polynomial's iterates on [0, 1] may
+ * not exceed 16 (ZK_EINVAL).  The list is read before the call returns.  Equal
+ * calls give equal bits; a matrix' result does not depend on its neighbours but
+ * for the sizes of the products' tiles. */
+enum zk_muon_adjust { ZK_MUON_ORIGINAL = 0, ZK_MUON_MATCH_RMS = 1 };
+typedef struct zk_muon_matrix {
+  const void* grad;
+  void* out;
+  float* param;
+  float* momentum;
+  int64_t rows, cols, ld_grad, ld_out, ld_param, ld_momentum;
+  int64_t grad_dtype, out_dtype;
+} zk_muon_matrix;
+/* Bytes of workspace for a list. */
+int64_t zk_muon_workspace(const zk_muon_matrix* list, int64_t n);
+int zk_orthogonalize(const zk_muon_matrix* list, int64_t n, int steps, double a,
+                     double b, double c, double eps, void* workspace,
+                     int64_t workspace_bytes, zk_stream_t stream);
+int zk_muon_multi(const zk_muon_matrix* list, int64_t n, int steps, double a,
+                  double b, double c, double eps, double lr, double momentum,
+                  double weight_decay, int nesterov, int adjust, void* workspace,
+                  int64_t workspace_bytes, zk_stream_t stream);
+
 /* ------------------------------------------------------------- Utilities --
  * Dtype conversion of a contiguous buffer (the autocast weight cast and the
  * grad cast of utils/patch.py:115-119 when done outside the AdamW kernel).

@@ -21,6 +21,7 @@ NODES_PATH = os.path.join(os.path.dirname(LIB_PATH), "_nodes.so")
 
 ZK_F32, ZK_F16, ZK_BF16 = 0, 1, 2
 ZK_ROPE_HALF, ZK_ROPE_INTERLEAVED = 0, 1
+ZK_MUON_ORIGINAL, ZK_MUON_MATCH_RMS = 0, 1
 
 STATUS_NAMES = {
     -1: "ZK_EINVAL",
@@ -104,6 +105,14 @@ class AxesDesc(ctypes.Structure):
             "n_pos", "n_axes",
         )
     ] + [("pairing", _int), ("inverse", _int), ("dtype", _int)]
+
+
+class MuonMatrix(ctypes.Structure):
+    """Mirror of ``zk_muon_matrix``."""
+
+    _fields_ = [(name, _ptr) for name in ("grad", "out", "param", "momentum")] + [
+        (name, _i64) for name in ("rows", "cols", "ld_grad", "ld_out", "ld_param", "ld_momentum",
+                                  "grad_dtype", "out_dtype")]
 
 
 class AdamwRegion(ctypes.Structure):
@@ -205,6 +214,11 @@ SIGNATURES = {
                                   _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "zk_rope_axes": (_int, [ctypes.POINTER(AxesDesc), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
                             ctypes.c_char_p, _ptr]),
+    "zk_muon_workspace": (_i64, [ctypes.POINTER(MuonMatrix), _i64]),
+    "zk_orthogonalize": (_int, [ctypes.POINTER(MuonMatrix), _i64, _int, _f64, _f64, _f64, _f64,
+                                _ptr, _i64, _ptr]),
+    "zk_muon_multi": (_int, [ctypes.POINTER(MuonMatrix), _i64, _int, _f64, _f64, _f64, _f64, _f64,
+                             _f64, _f64, _int, _int, _ptr, _i64, _ptr]),
     "zk_transpose": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _int, _ptr]),
     "zk_copy_to_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),
     "zk_copy_from_host": (_int, [_ptr, _ptr, _i64, _int, _ptr]),

@@ -54,7 +54,8 @@ _KMAJOR = ["-Wno-inline-asm", "-mllvm", "-greedy-reverse-local-assignment=1"]
 FILE_FLAGS = {"rope.hip": ["-fno-slp-vectorize"], "rope_axes.hip": ["-fno-slp-vectorize"], "gemm.hip": ["-Wno-inline-asm"],
               "gemm_ring.hip": ["-Wno-inline-asm"], "gemm_split.hip": ["-Wno-inline-asm"],
               "gemm_f32.hip": ["-Wno-inline-asm"], "gemm_kmajor.hip": _KMAJOR,
-              "gemm_ring_kmajor.hip": _KMAJOR}
+              "gemm_ring_kmajor.hip": _KMAJOR, "muon_gemm.hip": ["-Wno-inline-asm"],
+              "muon_gemm_kmajor.hip": _KMAJOR}
 
 
 def _hipcc() -> str:

@@ -56,6 +56,8 @@
 // -greedy-reverse-local-assignment none are, while the NT forms do better
 // with the default.
 #pragma once
+#include <type_traits>
+
 #include "attn_common.h"
 #include "rope_math.h"
 #include "vec.h"
@@ -146,7 +148,71 @@ struct GemmArgs {
   int64_t rnpos, rS, rcols;
   int rhalf, rpair;
   int64_t split_k;  // EPI 3: the reduction range of one workgroup
+  // EPI 4, with c2, r and z above: see PolyGroup
+  const void* a2;
+  float alpha, beta;
+  int tri, thrice;
 };
+
+// EPI 4: a product of each of up to kPolyMost matrices in one launch,
+//   c = alpha op(a) op(b)^T + beta (r + z),   c2 = what c's rounding left
+// (r, z, c2 may be NULL; row strides ldc for all of them).  tri: the product is
+// symmetric (M = N), and only its tiles on and below the diagonal are computed,
+// each stored transposed too.  thrice (gemm_ring.h): the operands are a + a2 and
+// b + b2, and a b^T + a b2^T + a2 b^T is summed, one after another along the
+// reduction.
+constexpr int kPolyMost = 8;
+struct PolyGroup {
+  GemmArgs p[kPolyMost];
+  int first[kPolyMost + 1];  // tiles before each matrix' own
+  int n;
+};
+
+// The arguments that a workgroup works with: its launch's, or (EPI 4) those of
+// its matrix, and its tile's number among that one's.
+__device__ __forceinline__ const GemmArgs& problem_of(const GemmArgs& launch, int64_t&) {
+  return launch;
+}
+__device__ __forceinline__ const GemmArgs& problem_of(const PolyGroup& launch, int64_t& pid) {
+  int i = 0;
+  while (i + 1 < launch.n && pid >= launch.first[i + 1]) ++i;
+  pid -= launch.first[i];
+  return launch.p[i];
+}
+
+// Row and column of tile `pid` of a lower triangle, row by row.
+__device__ __forceinline__ void triangle_tile(int64_t pid, int64_t& m, int64_t& n) {
+  int i = static_cast<int>((__builtin_sqrtf(8.f * static_cast<float>(pid) + 1.f) - 1.f) * 0.5f);
+  while (static_cast<int64_t>(i) * (i + 1) / 2 > pid) --i;
+  while (static_cast<int64_t>(i + 1) * (i + 2) / 2 <= pid) ++i;
+  m = i;
+  n = pid - static_cast<int64_t>(i) * (i + 1) / 2;
+}
+
+// EPI 4: v = alpha v + beta (r + z) of 8 elements at `at`, and their stores.
+template <typename T>
+__device__ __forceinline__ void poly_chunk(const GemmArgs& args, int64_t at, float (&v)[8]) {
+  float t[8] = {};
+  if (args.r != nullptr) Vec8<T>::load(static_cast<const T*>(args.r) + at, t);
+  if (args.z != nullptr) {
+    float u[8];
+    Vec8<T>::load(static_cast<const T*>(args.z) + at, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] += u[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = fmaf(args.alpha, v[e], args.beta * t[e]);
+}
+template <typename T>
+__device__ __forceinline__ void poly_store(const GemmArgs& args, int64_t at, const float (&v)[8]) {
+  Vec8<T>::store(static_cast<T*>(args.c) + at, v);
+  if (args.c2 != nullptr) {
+    float left[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) left[e] = v[e] - round_to<T>(v[e]);
+    Vec8<T>::store(static_cast<T*>(args.c2) + at, left);
+  }
+}
 
 // NT tile swizzle: the 16-byte chunk c of row r sits at chunk position
 // c ^ nt_sw(r).  An operand read (ds_read_b128) gives lane l row r0 + l % 16,
@@ -311,9 +377,12 @@ constexpr int read_order(int MB, int i) { return i == 0 ? 0 : i <= 8 ? MB + i - 
 // 128 tiles).
 template <typename T, int EPI, bool AKM, bool BKM, bool RAG = false, int MB = 8>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void gemm_tiled_kernel(GemmArgs args) {
-  static_assert(EPI == 0 || (!AKM && !BKM) || (EPI == 3 && !AKM && RAG),
+void gemm_tiled_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) {
+  static_assert(EPI == 0 || (!AKM && !BKM) || (EPI == 3 && !AKM && RAG) || (EPI == 4 && !AKM && !RAG),
                 "the SwiGLU and RoPE epilogues take NT operands, partial sums A along K");
+  int64_t pid = blockIdx.x;
+  if constexpr (EPI == 4) pid = xcd_order(pid, launch.first[launch.n]);
+  const GemmArgs& args = problem_of(launch, pid);
   static_assert(MB == 8 || (MB == 4 && EPI != 1 && !AKM && !RAG), "128-row tiles");
   constexpr int TBM = 32 * MB;  // tile rows
   constexpr int WR = 16 * MB;   // rows per wave
@@ -338,17 +407,23 @@ void gemm_tiled_kernel(GemmArgs args) {
   const int wm = wave >> 1, wn = wave & 1;
   const int64_t n_m = RAG ? (M + TBM - 1) / TBM : M / TBM;
   const int64_t n_n = RAG ? (N + BN - 1) / BN : N / BN, nwg = n_m * n_n;
-  int64_t pid = blockIdx.x;
   if constexpr (RAG)
     pid = xcd_order(pid, nwg);
-  else if ((nwg & 7) == 0)
+  else if (EPI != 4 && (nwg & 7) == 0)
     pid = (pid & 7) * (nwg >> 3) + (pid >> 3);
   const int64_t per_group = static_cast<int64_t>(GROUP_M) * n_n;
   const int64_t grp = pid / per_group;
   const int64_t mf = grp * GROUP_M;
   const int64_t gm = n_m - mf < GROUP_M ? n_m - mf : GROUP_M;
   const int64_t in_grp = pid - grp * per_group;
-  const int64_t m0 = (mf + in_grp % gm) * TBM, n0 = (in_grp / gm) * BN;
+  int64_t m0 = (mf + in_grp % gm) * TBM, n0 = (in_grp / gm) * BN;
+  if constexpr (EPI == 4) {
+    if (args.tri) {
+      triangle_tile(pid, m0, n0);
+      m0 *= TBM;
+      n0 *= BN;
+    }
+  }
   // first element of the tile and the step between K steps, per layout
   const T* Ab = AKM ? A + m0 : A + m0 * lda;
   const T* Bb = BKM ? B + n0 : B + n0 * ldb;
@@ -694,6 +769,13 @@ void gemm_tiled_kernel(GemmArgs args) {
           *reinterpret_cast<float4*>(W + 4) = hi;
           continue;
         }
+        if constexpr (EPI == 4) {
+          const int64_t at = grow * args.ldc + gcol;
+          poly_chunk<T>(args, at, v);
+          poly_store<T>(args, at, v);
+          if (args.tri && m0 != n0) Vec8<float>::store(&ws[rr * 132 + 8 * ch], v);
+          continue;
+        }
         if (R != nullptr) {
           const T8 rv = *reinterpret_cast<const T8*>(R + grow * args.ldr + gcol);
 #pragma unroll
@@ -703,6 +785,19 @@ void gemm_tiled_kernel(GemmArgs args) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[e]);
         *reinterpret_cast<T8*>(C + grow * args.ldc + gcol) = o;
+      }
+      if constexpr (EPI == 4) {
+        // the block transposed: 128 rows of 16, two runs of 8 each
+        if (args.tri && m0 != n0) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = (q >> 1) * 64 + el, r8 = 8 * (q & 1);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ws[(r8 + e) * 132 + c];
+            Vec8<T>::store(C + (n0 + wn * 128 + c) * args.ldc + row0 + r8, v);
+          }
+        }
       }
     } else {
       // g, u rounded as the GEMM would store them; z = round(round(silu(g)) u)

@@ -154,9 +154,13 @@ __device__ __forceinline__ typename RingOp<T>::vec kmaj_operand_n(const T* tile,
 // (whole heads of 2 rhalf columns, which divide the tile's width).
 template <typename T, int EPI, bool AKM, bool BKM, int MB, int NB, int RB, int WPE, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
-void gemm_ring_kernel(GemmArgs args) {
-  static_assert(EPI == 0 || (EPI == 3 && !AKM) || (!AKM && !BKM),
+void gemm_ring_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) {
+  static_assert(EPI == 0 || (EPI == 3 && !AKM) || (!AKM && !BKM) ||
+                    (EPI == 4 && !AKM && KS == 1 && MB == NB),
                 "the SwiGLU and RoPE epilogues take NT operands");
+  int64_t pid = blockIdx.x;
+  if constexpr (EPI == 4) pid = xcd_order(pid, launch.first[launch.n]);
+  const GemmArgs& args = problem_of(launch, pid);
   constexpr int TBM = 32 * MB, TBN = 32 * NB, WR = 16 * MB, WC = 16 * NB;
   typedef RingOp<T> Mm;
   typedef typename Mm::vec V8;
@@ -182,13 +186,20 @@ void gemm_ring_kernel(GemmArgs args) {
   const int wm = (wave >> 1) & 1, wn = wave & 1;
   // tiles in groups of GROUP_M along M, consecutive tiles on one XCD
   const int64_t n_m = (M + TBM - 1) / TBM, n_n = (N + TBN - 1) / TBN;
-  const int64_t pid = xcd_order(blockIdx.x, n_m * n_n);
+  if constexpr (EPI != 4) pid = xcd_order(blockIdx.x, n_m * n_n);
   const int64_t per_group = static_cast<int64_t>(GROUP_M) * n_n;
   const int64_t grp = pid / per_group;
   const int64_t mf = grp * GROUP_M;
   const int64_t gm = n_m - mf < GROUP_M ? n_m - mf : GROUP_M;
   const int64_t in_grp = pid - grp * per_group;
-  const int64_t m0 = (mf + in_grp % gm) * TBM, n0 = (in_grp / gm) * TBN;
+  int64_t m0 = (mf + in_grp % gm) * TBM, n0 = (in_grp / gm) * TBN;
+  if constexpr (EPI == 4) {
+    if (args.tri) {
+      triangle_tile(pid, m0, n0);
+      m0 *= TBM;
+      n0 *= TBN;
+    }
+  }
   const int64_t f0 = n0 / 2;  // EPI 1: the tile's first feature
 
   // first element of each operand's tile, bytes left from there to the
@@ -263,14 +274,35 @@ void gemm_ring_kernel(GemmArgs args) {
     v4i r, r2;
     uint32_t voff;
   };
+  // EPI 4, thrice: three reductions of seg steps, with a2 in the last one and b2 in
+  // the one before (K is a multiple of BK then)
+  const int64_t seg = EPI == 4 && args.thrice ? K / BK : 0;
   auto a_src = [&](int64_t k) __attribute__((always_inline)) {
     Src s;
+    if constexpr (EPI == 4) {
+      if (seg > 0 && k >= seg) {
+        const int64_t in = k < 2 * seg ? k - seg : k - 2 * seg;
+        const char* base = k < 2 * seg ? Ab : static_cast<const char*>(args.a2) + ES * m0 * lda;
+        s.r = rsrc_left(base + in * a_step, in < seg ? a_left - in * a_step : 0);
+        s.voff = ta.lane_off;
+        return s;
+      }
+    }
     s.r = rsrc_left(Ab + k * a_step, a_left - k * a_step);
     s.voff = AKM || k * BK + ta.kcol < K ? ta.lane_off : 0x80000000u;
     return s;
   };
   auto b_src = [&](int64_t k) __attribute__((always_inline)) {
     Src s;
+    if constexpr (EPI == 4) {
+      if (seg > 0 && k >= seg) {
+        const int64_t in = k < 2 * seg ? k - seg : k - 2 * seg;
+        const char* base = k >= 2 * seg ? Bb : static_cast<const char*>(args.b2) + ES * (BKM ? n0 : n0 * ldb);
+        s.r = rsrc_left(base + in * b_step, in < seg ? b_left - in * b_step : 0);
+        s.voff = tb.lane_off;
+        return s;
+      }
+    }
     s.r = rsrc_left(Bb + k * b_step, b_left - k * b_step);
     if constexpr (EPI == 1) s.r2 = rsrc_left(B2b + k * b_step, b_left - k * b_step);
     s.voff = BKM || k * BK + tb.kcol < K ? tb.lane_off : 0x80000000u;
@@ -317,7 +349,7 @@ void gemm_ring_kernel(GemmArgs args) {
     }
   };
 
-  const int64_t n_k = (K + BK - 1) / BK;
+  const int64_t n_k = (K + BK - 1) / BK * (EPI == 4 && args.thrice ? 3 : 1);
 #pragma unroll
   for (int p = 0; p < RB; ++p) {
     const Src sa = a_src(p), sb = b_src(p);
@@ -495,6 +527,12 @@ void gemm_ring_kernel(GemmArgs args) {
         Vec8<float>::store(static_cast<float*>(args.c) + (blockIdx.y * M + gr) * N + gc, v);
         continue;
       }
+      if constexpr (EPI == 4) {
+        poly_chunk<T>(args, gr * args.ldc + gc, v);
+        poly_store<T>(args, gr * args.ldc + gc, v);
+        if (args.tri && m0 != n0) Vec8<float>::store(&ws[row * EP + 8 * ch], v);
+        continue;
+      }
       if constexpr (EPI == 2) if (gc < args.rcols) {
         // this chunk rotated: its pair is the chunk rhalf columns away in the
         // same head (half-split) or inside the chunk (interleaved); the
@@ -545,6 +583,21 @@ void gemm_ring_kernel(GemmArgs args) {
         for (int e = 0; e < 8; ++e) v[e] += rv[e];
       }
       Vec8<T>::store(C + gr * args.ldc + gc, v);
+    }
+    if constexpr (EPI == 4) {
+      if (args.tri && m0 != n0) {  // the tile transposed
+        __syncthreads();
+#pragma unroll
+        for (int it = 0; it < TBM * CPR / NT; ++it) {
+          const int id = it * NT + tid, col = id / CPR, ch = id % CPR;
+          const int64_t gr = n0 + col, gc = m0 + 8 * ch;
+          if (gr >= N || gc >= M) continue;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = ws[(8 * ch + e) * EP + col];
+          poly_store<T>(args, gr * args.ldc + gc, v);
+        }
+      }
     }
   }
 }

@@ -1,0 +1,427 @@
+// Orthogonal factors of matrices by Newton-Schulz products, and the step that
+// takes them (momentum, factor, weights), over lists of matrices.
+//
+// With s <= t the sides of a matrix U, X0 = U / (|U| + eps) as [s, t] (tall ones
+// transposed), each of the steps makes
+//   G = X X^T,   P = b G + c G G,   X <- a X + P X,
+// a polynomial a z + b z^3 + c z^5 of every singular value.  G and P are
+// symmetric: their tiles on and below the diagonal are computed, and stored
+// twice.  s^2 t + s^3 + 2 s^2 t multiply-adds' operations a step, on the fp16
+// matrix cores.
+//
+// Numbers.  The products' operands are fp16, with sums in fp32: singular values
+// lie below 1.3, so scaled by powers of two that the host takes from the
+// polynomial's bounds (X by S, G with it by S^2, P by R) they use fp16's whole
+// range, and its step is an eighth of bf16's at the same rate.  X itself is held
+// in two fp16 numbers (22 bits), and a X is added in fp32: small singular values
+// grow by a = 3.4 a step, and a rounding of X relative to the largest ones would
+// grow with them (a matrix of 8 strong directions over noise a hundredth as
+// large: 3.6e-2 off with X in one fp16 number, 0.3 in bf16, 3e-4 like this; other
+// spectra 0.3 - 1.7e-3).  Matrices with s <= kExactSide, whose products cost no
+// time, and results in fp32 have G and P in two numbers as well, and products of
+// three terms.
+#include <cmath>
+
+#include "muon.h"
+
+namespace zk {
+
+namespace {
+
+constexpr int kPartials = 256;       // partial sums of squares of a matrix
+constexpr int64_t kExactSide = 128;  // matrices up to here are computed with 22 bits throughout
+constexpr int kTile = 64;
+
+// One matrix of a launch of the element-wise kernels.
+struct Matrix {
+  const void* grad;
+  float* momentum;   // step: else NULL
+  float* param;
+  void* out;         // factors, or the step's rounded copy
+  f16* hi;           // X, [sp, tp]
+  f16* lo;
+  double* partial;   // [kPartials]
+  int64_t rows, cols, ld_grad, ld_momentum, ld_param, ld_out;
+  int64_t sp, tp;    // padded sides
+  float lr_scale;
+  int grad_dtype, out_dtype, tall;
+};
+struct MatrixGroup {
+  Matrix p[gemm::kPolyMost];
+  int first[gemm::kPolyMost + 1];
+  int n;
+  float mu, decay, lr, scale, eps;
+  int nesterov;
+};
+
+__device__ __forceinline__ const Matrix& matrix_of(const MatrixGroup& g, int64_t& at) {
+  int i = 0;
+  while (i + 1 < g.n && at >= g.first[i + 1]) ++i;
+  at -= g.first[i];
+  return g.p[i];
+}
+
+// What is orthogonalised, from the gradient and the momentum after this step's.
+__device__ __forceinline__ float update_of(const MatrixGroup& g, float grad, float m) {
+  return g.nesterov ? fmaf(g.mu, m, (1.f - g.mu) * grad) : m;
+}
+
+// The momentum's step, and kPartials sums of squares (64 bits: squares of small
+// gradients leave fp32's range): runs of 1024 columns of a row, workgroup w of
+// the matrix taking runs w, w + kPartials, ..
+__global__ __launch_bounds__(256) void muon_begin_kernel(MatrixGroup g) {
+  int64_t w = blockIdx.x;
+  const Matrix& x = matrix_of(g, w);
+  const int64_t per_row = (x.cols + 1023) / 1024, runs = x.rows * per_row;
+  double sum = 0;
+  for (int64_t u = w; u < runs; u += kPartials) {
+    const int64_t row = u / per_row, c0 = (u - row * per_row) * 1024;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t c = c0 + k * 256 + threadIdx.x;
+      if (c < x.cols) {
+        float v = load_dt(x.grad, row * x.ld_grad + c, x.grad_dtype);
+        if (x.momentum != nullptr) {
+          float* m = x.momentum + row * x.ld_momentum + c;
+          const float next = fmaf(g.mu, *m, (1.f - g.mu) * v);
+          *m = next;
+          v = update_of(g, v, next);
+        }
+        sum += static_cast<double>(v) * v;
+      }
+    }
+  }
+  __shared__ double part[256];
+  part[threadIdx.x] = sum;
+  __syncthreads();
+  for (int n = 128; n > 0; n /= 2) {
+    if (static_cast<int>(threadIdx.x) < n) part[threadIdx.x] += part[threadIdx.x + n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) x.partial[w] = part[0];
+}
+
+// X0, padded with zeros: 64 x 64 tiles of X, through LDS where U is tall.
+__global__ __launch_bounds__(256) void muon_scale_kernel(MatrixGroup g) {
+  int64_t at = blockIdx.x;
+  const Matrix& x = matrix_of(g, at);
+  __shared__ double total;
+  __shared__ float tile[kTile][kTile + 1];
+  if (threadIdx.x < 64) {
+    double v = 0;
+    for (int i = threadIdx.x; i < kPartials; i += 64) v += x.partial[i];
+    for (int n = 32; n > 0; n /= 2) v += __shfl_xor(v, n, 64);
+    if (threadIdx.x == 0) total = v;
+  }
+  const int64_t per_row = x.tp / kTile;
+  const int64_t s0 = at / per_row * kTile, t0 = at % per_row * kTile;
+  // U's rows and columns of this tile
+  const int64_t r0 = x.tall ? t0 : s0, c0 = x.tall ? s0 : t0;
+  const int col = threadIdx.x % kTile, row0 = threadIdx.x / kTile;
+#pragma unroll
+  for (int k = 0; k < kTile / 4; ++k) {
+    const int64_t r = r0 + row0 + 4 * k, c = c0 + col;
+    float v = 0.f;
+    if (r < x.rows && c < x.cols) {
+      v = load_dt(x.grad, r * x.ld_grad + c, x.grad_dtype);
+      if (x.momentum != nullptr) v = update_of(g, v, x.momentum[r * x.ld_momentum + c]);
+    }
+    tile[row0 + 4 * k][col] = v;
+  }
+  __syncthreads();
+  const float f = static_cast<float>(g.scale / (sqrt(total) + static_cast<double>(g.eps)));
+#pragma unroll
+  for (int k = 0; k < kTile / 4; ++k) {
+    const int r = row0 + 4 * k;
+    const float v = (x.tall ? tile[col][r] : tile[r][col]) * f;
+    const f16 hi = static_cast<f16>(v);
+    const int64_t i = (s0 + r) * x.tp + t0 + col;
+    x.hi[i] = hi;
+    x.lo[i] = static_cast<f16>(v - static_cast<float>(hi));
+  }
+}
+
+// The factor to its place, or the weights' step with it: 64 x 64 tiles of U.
+__global__ __launch_bounds__(256) void muon_finish_kernel(MatrixGroup g) {
+  int64_t at = blockIdx.x;
+  const Matrix& x = matrix_of(g, at);
+  __shared__ float tile[kTile][kTile + 1];
+  const int64_t per_row = x.tp / kTile;
+  const int64_t s0 = at / per_row * kTile, t0 = at % per_row * kTile;
+  const int col = threadIdx.x % kTile, row0 = threadIdx.x / kTile;
+#pragma unroll
+  for (int k = 0; k < kTile / 4; ++k) {
+    const int r = row0 + 4 * k;
+    const int64_t i = (s0 + r) * x.tp + t0 + col;
+    tile[r][col] = (static_cast<float>(x.hi[i]) + static_cast<float>(x.lo[i])) / g.scale;
+  }
+  __syncthreads();
+  const int64_t r0 = x.tall ? t0 : s0, c0 = x.tall ? s0 : t0;
+#pragma unroll
+  for (int k = 0; k < kTile / 4; ++k) {
+    const int64_t r = r0 + row0 + 4 * k, c = c0 + col;
+    if (r >= x.rows || c >= x.cols) continue;
+    float v = x.tall ? tile[col][row0 + 4 * k] : tile[row0 + 4 * k][col];
+    if (x.param != nullptr) {
+      float* p = x.param + r * x.ld_param + c;
+      v = fmaf(-g.lr * x.lr_scale, v, *p * (1.f - g.decay));
+      *p = v;
+    }
+    if (x.out != nullptr) store_dt(x.out, r * x.ld_out + c, x.out_dtype, v);
+  }
+}
+
+// ---------------------------------------------------------------------- host --
+struct Sides {
+  int64_t s, t, sp, tp;
+  bool exact;
+};
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// Tiles of a run of matrices: the 256 x 256 pipeline where its tiles fill most of
+// the CUs, else 128 x 128, else 64 x 64.
+gemm::Tile tile_of(const Sides* x, int n) {
+  if (x[0].exact) return gemm::k64;
+  int64_t n256 = 0, n128 = 0;
+  for (int i = 0; i < n; ++i) {
+    n256 += gemm::tile_count(gemm::k256, x[i].s, x[i].t);
+    n128 += gemm::tile_count(gemm::k128, x[i].s, x[i].t);
+  }
+  if (n256 >= 160) return gemm::k256;
+  return n128 >= 200 ? gemm::k128 : gemm::k64;
+}
+
+Sides sides_of(const zk_muon_matrix& x) {
+  Sides d;
+  d.s = x.rows < x.cols ? x.rows : x.cols;
+  d.t = x.rows < x.cols ? x.cols : x.rows;
+  d.exact = d.s <= kExactSide || (x.param == nullptr && x.out_dtype == ZK_F32);
+  d.sp = d.tp = 0;
+  return d;
+}
+
+// A run of matrices that share launches: of one precision, at most kPolyMost.
+int run_length(const zk_muon_matrix* list, int64_t n) {
+  int len = 0;
+  while (len < n && len < gemm::kPolyMost && sides_of(list[len]).exact == sides_of(list[0]).exact) ++len;
+  return len;
+}
+
+int64_t bytes_of(const Sides& d) {
+  const int64_t square = d.sp * d.sp * 2, x = d.sp * d.tp * 2;
+  return up(4 * x + (d.exact ? 4 : 2) * square + kPartials * 8, 256);
+}
+
+gemm::Tile plan_run(const zk_muon_matrix* list, int n, Sides* d) {
+  for (int i = 0; i < n; ++i) d[i] = sides_of(list[i]);
+  const gemm::Tile t = tile_of(d, n);
+  const int64_t to = t == gemm::k256 ? 256 : 64;
+  for (int i = 0; i < n; ++i) {
+    d[i].sp = up(d[i].s, to);
+    d[i].tp = up(d[i].t, to);
+  }
+  return t;
+}
+
+// Bounds of the polynomial's iterates on [0, 1]: the powers of two that S^2 G and
+// R P stay in fp16's range with.  False: the iterates leave it.
+bool scales_of(int steps, double a, double b, double c, float* S, float* R) {
+  if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c))) return false;
+  double most = 1.0, most_p = 0, most_l = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    double next = 0;
+    for (int i = 0; i <= 4096; ++i) {
+      const double z = most * i / 4096, l = z * z, p = b * l + c * l * l;
+      next = fmax(next, fabs(z * (a + p)));
+      most_p = fmax(most_p, fabs(p));
+    }
+    if (!(next < 16.0)) return false;
+    most = next * 1.02;  // between the samples, and roundings
+    most_l = fmax(most_l, most * most);
+  }
+  // S = 2^i, S^2 most_l < 2^15.5; R = 2^j
+  *S = static_cast<float>(exp2(floor(0.5 * log2(46000.0 / most_l))));
+  *R = most_p > 0 ? static_cast<float>(exp2(fmin(13.0, floor(log2(46000.0 / most_p))))) : 1.f;
+  return true;
+}
+
+int check_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step) {
+  ZK_REQUIRE(n >= 0 && (n == 0 || list != nullptr), ZK_EINVAL, "%s: no list", who);
+  for (int64_t i = 0; i < n; ++i) {
+    const zk_muon_matrix& x = list[i];
+    ZK_REQUIRE(x.rows > 0 && x.cols > 0 && x.rows < (int64_t(1) << 20) && x.cols < (int64_t(1) << 20),
+               ZK_EINVAL, "%s: matrix %lld is %lld x %lld (1 .. 2^20 - 1)", who, (long long)i,
+               (long long)x.rows, (long long)x.cols);
+    ZK_REQUIRE(x.rows * x.cols <= int64_t(1) << 32, ZK_EINVAL, "%s: matrix %lld has more than 2^32 elements",
+               who, (long long)i);
+    ZK_REQUIRE(valid_dtype(static_cast<int>(x.grad_dtype)) && (x.out == nullptr || valid_dtype(static_cast<int>(x.out_dtype))), ZK_EDTYPE,
+               "%s: matrix %lld has a bad dtype", who, (long long)i);
+    ZK_REQUIRE(x.grad != nullptr && (step ? x.param != nullptr && x.momentum != nullptr
+                                          : x.out != nullptr && x.param == nullptr && x.momentum == nullptr),
+               ZK_EINVAL, "%s: matrix %lld lacks a pointer, or has one too many", who, (long long)i);
+    ZK_REQUIRE(x.ld_grad >= x.cols && (!step || (x.ld_param >= x.cols && x.ld_momentum >= x.cols)) &&
+                   (x.out == nullptr || x.ld_out >= x.cols),
+               ZK_EINVAL, "%s: rows of matrix %lld overlap", who, (long long)i);
+    ZK_REQUIRE(aligned(x.grad, dtype_bytes(static_cast<int>(x.grad_dtype))) && aligned(x.param, 4) && aligned(x.momentum, 4) &&
+                   (x.out == nullptr || aligned(x.out, dtype_bytes(static_cast<int>(x.out_dtype)))),
+               ZK_EALIGN, "%s: matrix %lld is not aligned to its elements", who, (long long)i);
+  }
+  return ZK_OK;
+}
+
+struct Hyper {
+  int steps;
+  double a, b, c, eps, lr, mu, decay;
+  int nesterov, adjust;
+};
+
+int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, const Hyper& h,
+             void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  const int rc = check_list(who, list, n, step);
+  if (rc != ZK_OK) return rc;
+  ZK_REQUIRE(h.steps >= 1 && h.steps <= 100, ZK_EINVAL, "%s: %d steps (1 .. 100)", who, h.steps);
+  ZK_REQUIRE(h.eps >= 0, ZK_EINVAL, "%s: eps must not be negative", who);
+  float S, R;
+  ZK_REQUIRE(scales_of(h.steps, h.a, h.b, h.c, &S, &R), ZK_EINVAL,
+             "%s: the polynomial (%g, %g, %g) grows beyond 16 within %d steps", who, h.a, h.b, h.c, h.steps);
+  if (n == 0) return ZK_OK;
+  const int64_t need = zk_muon_workspace(list, n);
+  ZK_REQUIRE((workspace != nullptr && workspace_bytes >= need), ZK_EWORKSPACE,
+             "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes, (long long)need);
+  for (int64_t at = 0; at < n;) {
+    Sides d[gemm::kPolyMost];
+    const int len = run_length(list + at, n - at);
+    const gemm::Tile tile = plan_run(list + at, len, d);
+    char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+    MatrixGroup m = {};
+    f16 *hi[2][gemm::kPolyMost], *lo[2][gemm::kPolyMost], *G[2][gemm::kPolyMost], *P[2][gemm::kPolyMost];
+    m.n = len;
+    m.mu = static_cast<float>(h.mu); m.decay = static_cast<float>(h.lr * h.decay);
+    m.lr = static_cast<float>(h.lr); m.scale = S; m.eps = static_cast<float>(h.eps);
+    m.nesterov = h.nesterov;
+    for (int i = 0; i < len; ++i) {
+      const zk_muon_matrix& x = list[at + i];
+      const int64_t big = d[i].sp * d[i].tp, square = d[i].sp * d[i].sp;
+      f16* p = reinterpret_cast<f16*>(ws);
+      for (int k = 0; k < 2; ++k) {
+        hi[k][i] = p; p += big;
+        lo[k][i] = p; p += big;
+      }
+      for (int k = 0; k < (d[i].exact ? 2 : 1); ++k) {
+        G[k][i] = p; p += square;
+        P[k][i] = p; p += square;
+      }
+      if (!d[i].exact) G[1][i] = P[1][i] = nullptr;
+      Matrix& y = m.p[i];
+      y.partial = reinterpret_cast<double*>(p);
+      ws += bytes_of(d[i]);
+      y.grad = x.grad; y.momentum = x.momentum; y.param = x.param; y.out = x.out;
+      y.hi = hi[0][i]; y.lo = lo[0][i];
+      y.rows = x.rows; y.cols = x.cols;
+      y.ld_grad = x.ld_grad; y.ld_momentum = x.ld_momentum; y.ld_param = x.ld_param; y.ld_out = x.ld_out;
+      y.sp = d[i].sp; y.tp = d[i].tp;
+      y.grad_dtype = static_cast<int>(x.grad_dtype); y.out_dtype = static_cast<int>(x.out_dtype);
+      y.tall = x.rows > x.cols;
+      y.lr_scale = static_cast<float>(
+          h.adjust == ZK_MUON_MATCH_RMS ? 0.2 * sqrt(static_cast<double>(d[i].t))
+                                        : sqrt(fmax(1.0, static_cast<double>(x.rows) / x.cols)));
+    }
+    auto spread = [&](auto&& count) {
+      for (int i = 0; i < len; ++i) m.first[i + 1] = m.first[i] + static_cast<int>(count(i));
+      return dim3(static_cast<unsigned>(m.first[len]));
+    };
+    const dim3 begin = spread([](int) { return kPartials; });
+    hipLaunchKernelGGL(muon_begin_kernel, begin, dim3(256), 0, s, m);
+    const dim3 tiles = spread([&](int i) { return d[i].sp / kTile * (d[i].tp / kTile); });
+    hipLaunchKernelGGL(muon_scale_kernel, tiles, dim3(256), 0, s, m);
+
+    // product `which` of step k: 0 G, 1 P, 2 X
+    auto product = [&](int k, int which) {
+      gemm::PolyGroup g = {};
+      g.n = len;
+      for (int i = 0; i < len; ++i) {
+        gemm::GemmArgs& q = g.p[i];
+        const Sides& e = d[i];
+        f16 *const xh = hi[k & 1][i], *const xl = lo[k & 1][i];
+        q.thrice = e.exact;
+        q.M = e.sp;
+        if (which == 0) {
+          q.a = q.b = xh; q.a2 = q.b2 = xl;
+          q.lda = q.ldb = e.tp; q.K = e.tp; q.N = e.sp;
+          q.c = G[0][i]; q.c2 = G[1][i]; q.ldc = e.sp;
+          q.alpha = 1.f; q.tri = 1;
+        } else if (which == 1) {
+          q.a = q.b = q.r = G[0][i]; q.a2 = q.b2 = q.z = G[1][i];
+          q.lda = q.ldb = e.sp; q.K = e.sp; q.N = e.sp;
+          q.c = P[0][i]; q.c2 = P[1][i]; q.ldc = e.sp;
+          q.alpha = static_cast<float>(h.c * R / (static_cast<double>(S) * S * S * S));
+          q.beta = static_cast<float>(h.b * R / (static_cast<double>(S) * S));
+          q.tri = 1;
+        } else {
+          q.a = P[0][i]; q.a2 = P[1][i]; q.lda = e.sp;
+          q.b = xh; q.b2 = xl; q.ldb = e.tp;
+          q.K = e.sp; q.N = e.tp;
+          q.r = xh; q.z = xl;
+          q.c = hi[1 - (k & 1)][i]; q.c2 = lo[1 - (k & 1)][i]; q.ldc = e.tp;
+          q.alpha = 1.f / R; q.beta = static_cast<float>(h.a);
+        }
+        const int64_t rows = (q.M + gemm::tile_rows(tile) - 1) / gemm::tile_rows(tile);
+        g.first[i + 1] = g.first[i] + static_cast<int>(q.tri ? rows * (rows + 1) / 2
+                                                             : gemm::tile_count(tile, q.M, q.N));
+      }
+      if (which == 2)
+        gemm::launch_poly_kmajor(tile, g, s);
+      else
+        gemm::launch_poly(tile, g, s);
+    };
+    for (int k = 0; k < h.steps; ++k)
+      for (int which = 0; which < 3; ++which) product(k, which);
+    for (int i = 0; i < len; ++i) {
+      m.p[i].hi = hi[h.steps & 1][i];
+      m.p[i].lo = lo[h.steps & 1][i];
+    }
+    hipLaunchKernelGGL(muon_finish_kernel, tiles, dim3(256), 0, s, m);
+    at += len;
+  }
+  return launch_status(who);
+}
+
+}  // namespace
+
+}  // namespace zk
+
+using namespace zk;
+
+extern "C" int64_t zk_muon_workspace(const zk_muon_matrix* list, int64_t n) {
+  if (list == nullptr || n <= 0) return 0;
+  int64_t most = 0;
+  for (int64_t at = 0; at < n;) {
+    Sides d[gemm::kPolyMost];
+    const int len = run_length(list + at, n - at);
+    plan_run(list + at, len, d);
+    int64_t sum = 256;
+    for (int i = 0; i < len; ++i) sum += bytes_of(d[i]);
+    most = sum > most ? sum : most;
+    at += len;
+  }
+  return most;
+}
+
+extern "C" int zk_orthogonalize(const zk_muon_matrix* list, int64_t n, int steps, double a, double b,
+                                double c, double eps, void* workspace, int64_t workspace_bytes,
+                                zk_stream_t stream) {
+  const Hyper h = {steps, a, b, c, eps, 0, 0, 0, 0, 0};
+  return run_list("zk_orthogonalize", list, n, false, h, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int zk_muon_multi(const zk_muon_matrix* list, int64_t n, int steps, double a, double b, double c,
+                             double eps, double lr, double momentum, double weight_decay, int nesterov,
+                             int adjust, void* workspace, int64_t workspace_bytes, zk_stream_t stream) {
+  const char* who = "zk_muon_multi";
+  ZK_REQUIRE(lr >= 0 && weight_decay >= 0 && momentum >= 0 && momentum < 1, ZK_EINVAL,
+             "%s: lr %g, momentum %g, weight decay %g", who, lr, momentum, weight_decay);
+  ZK_REQUIRE(adjust == ZK_MUON_ORIGINAL || adjust == ZK_MUON_MATCH_RMS, ZK_EINVAL, "%s: bad adjustment %d",
+             who, adjust);
+  const Hyper h = {steps, a, b, c, eps, lr, momentum, weight_decay, nesterov, adjust};
+  return run_list(who, list, n, true, h, workspace, workspace_bytes, as_stream(stream));
+}

@@ -583,4 +583,5 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, free_gil);
   m.def("rows", &rows);
   bind_packed(m);
+  bind_muon(m);
 }

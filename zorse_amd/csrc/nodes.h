@@ -24,14 +24,15 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 typedef std::optional<Tensor> MaybeTensor;
 
-// Adds nodes_packed.cpp's functions to the module.
+// Add the functions of nodes_packed.cpp and nodes_muon.cpp to the module.
 void bind_packed(py::module_& m);
+void bind_muon(py::module_& m);
 
 namespace {
 
-[[noreturn]] void bad(const std::string& what) { throw py::value_error(what); }
+[[noreturn]] inline void bad(const std::string& what) { throw py::value_error(what); }
 
-void check(int status, const char* who) {
+inline void check(int status, const char* who) {
   if (status == 0) return;
   static const char* const names[] = {"ZK_EINVAL", "ZK_EDTYPE", "ZK_EALIGN", "ZK_EUNSUPPORTED",
                                       "ZK_EWORKSPACE"};
@@ -41,17 +42,17 @@ void check(int status, const char* who) {
                            ": " + zk_last_error());
 }
 
-zk_stream_t stream_of(const Tensor& t) {
+inline zk_stream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.get_device()).stream();
 }
 
-[[maybe_unused]] at::ScalarType type_of(int64_t code) {
+inline at::ScalarType type_of(int64_t code) {
   return code == ZK_F32 ? at::kFloat : code == ZK_F16 ? at::kHalf : at::kBFloat16;
 }
-int code_of(at::ScalarType t) {
+inline int code_of(at::ScalarType t) {
   return t == at::kFloat ? ZK_F32 : t == at::kHalf ? ZK_F16 : t == at::kBFloat16 ? ZK_BF16 : -1;
 }
-int float_code(const char* name, at::ScalarType t) {
+inline int float_code(const char* name, at::ScalarType t) {
   const int code = code_of(t);
   if (code < 0) bad(c10::str("unsupported ", name, " dtype ", t));
   return code;
@@ -59,7 +60,7 @@ int float_code(const char* name, at::ScalarType t) {
 
 constexpr const char* kNeedGpu = "zorse_amd kernels need GPU tensors (got a CPU tensor)";
 
-void one_gpu(std::initializer_list<const Tensor*> tensors) {
+inline void one_gpu(std::initializer_list<const Tensor*> tensors) {
   const Tensor& first = **tensors.begin();
   for (const Tensor* t : tensors) {
     if (!t->defined()) continue;
@@ -68,22 +69,22 @@ void one_gpu(std::initializer_list<const Tensor*> tensors) {
   }
 }
 
-void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+inline void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+inline Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 
-Tensor workspace(int64_t bytes, const Tensor& like) {
+inline Tensor workspace(int64_t bytes, const Tensor& like) {
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
 // Forward-mode derivatives: a dual tensor carries its tangent beside its values.
-bool is_dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+inline bool is_dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 
 // Unit stride along d (expanded heads and gradients have none).
-Tensor rows_of(const Tensor& t) {
+inline Tensor rows_of(const Tensor& t) {
   return !t.defined() || t.dim() == 0 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
-MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+inline MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 }  // namespace

@@ -1,0 +1,173 @@
+// The lists of the orthogonal updates on torch's C++ side: checks, tables and the
+// launches through the C ABI.
+#include "nodes.h"
+
+namespace {
+
+std::vector<MaybeTensor> list_of(const std::string& who, const py::object& o) {
+  std::vector<MaybeTensor> out;
+  for (const py::handle h : o) {
+    if (h.is_none()) {
+      out.emplace_back();
+      continue;
+    }
+    if (!THPVariable_Check(h.ptr())) throw py::type_error(who + ": lists of tensors are needed");
+    out.emplace_back(THPVariable_Unpack(h.ptr()));
+  }
+  return out;
+}
+
+struct Span {
+  uintptr_t begin, end;
+  bool written;
+};
+
+// A matrix of a list: its row stride, after the checks.
+int64_t matrix(const std::string& who, const char* name, size_t i, const Tensor& t, const Tensor& like,
+               int types, bool written, std::vector<Span>& spans) {
+  if (!t.is_cuda()) bad(kNeedGpu);
+  const std::string at = who + ": " + name + " " + std::to_string(i);
+  if (t.dim() != 2) bad(at + " must be a matrix");
+  if (t.sizes() != like.sizes() || t.get_device() != like.get_device())
+    bad(at + " must have its matrix' shape and device");
+  const int code = code_of(t.scalar_type());
+  if (code < 0 || !(types >> code & 1)) bad(at + (types == 1 << ZK_F32 ? " must be fp32" : " must be fp32, fp16 or bf16"));
+  const int64_t rows = t.size(0), cols = t.size(1);
+  const int64_t ld = rows > 1 ? t.stride(0) : cols;
+  if ((cols > 1 && t.stride(1) != 1) || ld < cols)
+    bad(at + " needs unit column stride and rows that do not overlap");
+  if (rows > 0 && cols > 0) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    spans.push_back({p, p + ((rows - 1) * ld + cols) * t.element_size(), written});
+  }
+  return ld;
+}
+
+void no_overlaps(const std::string& who, std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t read = 0, written = 0;  // the ends so far
+  for (const Span& s : spans) {
+    if (s.begin < written || (s.written && s.begin < read))
+      bad(who + ": a tensor that is written is in the lists twice, or overlaps another");
+    (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+  }
+}
+
+void one_device(const std::string& who, const Tensor& t, const Tensor& first) {
+  if (!t.is_cuda()) bad(kNeedGpu);
+  if (t.get_device() != first.get_device()) bad(who + ": tensors are on different devices");
+}
+
+constexpr int kAnyFloat = 1 << ZK_F32 | 1 << ZK_F16 | 1 << ZK_BF16;
+
+// kernels.orthogonalize
+std::vector<Tensor> orthogonalize(const py::object& matrices, const py::object& given_outs,
+                                  std::optional<at::ScalarType> dtype, int steps, double a, double b,
+                                  double c, double eps) {
+  const std::string who = "orthogonalize";
+  const std::vector<MaybeTensor> xs = list_of(who, matrices);
+  std::vector<MaybeTensor> outs;
+  if (!given_outs.is_none()) {
+    outs = list_of(who, given_outs);
+    if (outs.size() != xs.size()) bad(who + ": the lists differ in length");
+  }
+  std::vector<Tensor> result;
+  std::vector<zk_muon_matrix> table;
+  std::vector<Span> spans;
+  for (size_t i = 0; i < xs.size(); ++i) {
+    if (!xs[i]) bad(who + ": matrix " + std::to_string(i) + " is None");
+    const Tensor& x = *xs[i];
+    zk_muon_matrix m{};
+    m.ld_grad = matrix(who, "matrix", i, x, x, kAnyFloat, false, spans);
+    one_device(who, x, *xs[0]);
+    m.grad = x.data_ptr();
+    m.rows = x.size(0), m.cols = x.size(1);
+    m.grad_dtype = code_of(x.scalar_type());
+    Tensor out;
+    if (!outs.empty()) {
+      if (!outs[i]) bad(who + ": out " + std::to_string(i) + " is None");
+      out = *outs[i];
+      if (dtype && out.scalar_type() != *dtype) bad(who + ": outs are not of dtype");
+    } else {
+      const at::ScalarType type = dtype.value_or(x.scalar_type());
+      float_code("output", type);
+      const c10::DeviceGuard on(x.device());
+      out = at::empty(x.sizes(), x.options().dtype(type));
+    }
+    m.ld_out = matrix(who, "out", i, out, x, kAnyFloat, true, spans);
+    m.out = out.data_ptr();
+    m.out_dtype = code_of(out.scalar_type());
+    result.push_back(out);
+    if (x.numel() > 0) table.push_back(m);
+  }
+  no_overlaps(who, spans);
+  const int64_t n = static_cast<int64_t>(table.size()), bytes = zk_muon_workspace(table.data(), n);
+  const py::gil_scoped_release free_gil;
+  std::optional<c10::DeviceGuard> on;
+  Tensor ws;
+  zk_stream_t stream = nullptr;
+  if (n > 0) {
+    on.emplace(result[0].device());
+    ws = workspace(bytes, result[0]);
+    stream = stream_of(result[0]);
+  }
+  check(zk_orthogonalize(table.data(), n, steps, a, b, c, eps, address(ws), bytes, stream), "zk_orthogonalize");
+  return result;
+}
+
+// kernels.muon_multi
+void muon_multi(const py::object& params_, const py::object& grads_, const py::object& momenta_,
+                const py::object& lows_, int steps, double a, double b, double c, double eps, double lr,
+                double momentum, double weight_decay, bool nesterov, bool match_rms) {
+  const std::string who = "muon_multi";
+  const std::vector<MaybeTensor> params = list_of(who, params_), grads = list_of(who, grads_),
+                                 momenta = list_of(who, momenta_);
+  std::vector<MaybeTensor> lows(params.size());
+  if (!lows_.is_none()) lows = list_of(who, lows_);
+  if (grads.size() != params.size() || momenta.size() != params.size() || lows.size() != params.size())
+    bad(who + ": the lists differ in length");
+  std::vector<zk_muon_matrix> table;
+  std::vector<Span> spans;
+  for (size_t i = 0; i < params.size(); ++i) {
+    if (!params[i] || !grads[i] || !momenta[i])
+      bad(who + ": tensor " + std::to_string(i) + " is None");
+    const Tensor& p = *params[i];
+    zk_muon_matrix m{};
+    m.ld_param = matrix(who, "param", i, p, p, 1 << ZK_F32, true, spans);
+    one_device(who, p, *params[0]);
+    m.ld_grad = matrix(who, "grad", i, *grads[i], p, kAnyFloat, false, spans);
+    m.ld_momentum = matrix(who, "momentum", i, *momenta[i], p, 1 << ZK_F32, true, spans);
+    m.param = static_cast<float*>(p.data_ptr());
+    m.grad = grads[i]->data_ptr();
+    m.momentum = static_cast<float*>(momenta[i]->data_ptr());
+    m.rows = p.size(0), m.cols = p.size(1);
+    m.grad_dtype = code_of(grads[i]->scalar_type());
+    if (lows[i]) {
+      m.ld_out = matrix(who, "lowp_out", i, *lows[i], p, kAnyFloat, true, spans);
+      m.out = lows[i]->data_ptr();
+      m.out_dtype = code_of(lows[i]->scalar_type());
+    }
+    if (p.numel() > 0) table.push_back(m);
+  }
+  no_overlaps(who, spans);
+  const int64_t n = static_cast<int64_t>(table.size()), bytes = zk_muon_workspace(table.data(), n);
+  const py::gil_scoped_release free_gil;
+  std::optional<c10::DeviceGuard> on;
+  Tensor ws;
+  zk_stream_t stream = nullptr;
+  if (n > 0) {
+    on.emplace(params[0]->device());
+    ws = workspace(bytes, *params[0]);
+    stream = stream_of(*params[0]);
+  }
+  check(zk_muon_multi(table.data(), n, steps, a, b, c, eps, lr, momentum, weight_decay, nesterov,
+                      match_rms ? ZK_MUON_MATCH_RMS : ZK_MUON_ORIGINAL, address(ws), bytes, stream),
+        "zk_muon_multi");
+}
+
+}  // namespace
+
+void bind_muon(py::module_& m) {
+  m.def("orthogonalize", &orthogonalize);
+  m.def("muon_multi", &muon_multi);
+}

@@ -977,6 +977,42 @@ def rope_axes(q, k, cos, sin, positions, pair_axes, *, interleaved: bool = False
                                      inverse, q_out, k_out)
 
 
+# ------------------------------------------------------ Orthogonal updates ---
+
+MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # singular values to 0.7 - 1.2 in five steps
+
+
+def orthogonalize(matrices, *, steps: int = 5, coefficients=MUON_COEFFICIENTS, eps: float = 1e-7,
+                  dtype: torch.dtype | None = None, outs=None) -> list:
+    """The orthogonal factors of a list of matrices by Newton-Schulz products
+    (zk_orthogonalize): X = u / (|u| + eps), then ``steps`` times
+    X <- a X + (b X X^T + c (X X^T)^2) X with ``coefficients`` (a, b, c).
+    ``matrices``: 2-D tensors with unit column stride in any of the three types;
+    results in ``dtype`` (default each matrix' own) or in ``outs``.  Products are
+    fp16 with fp32 sums, off by 0.3 - 1.7e-3 of the factor; with fp32 results, or
+    a side of at most 128, by 1e-5."""
+    return _abi.nodes().orthogonalize(matrices, outs, dtype, steps, *coefficients, eps)
+
+
+def muon_multi(params, grads, momenta, *, lr: float, momentum: float, weight_decay: float,
+               nesterov: bool = True, adjust: str = "original", steps: int = 5,
+               coefficients=MUON_COEFFICIENTS, eps: float = 1e-7, lowp_outs=None) -> None:
+    """One step of a list of matrices by the orthogonal factors of their momenta
+    (zk_muon_multi), in place:
+        m = momentum m + (1 - momentum) g
+        u = (1 - momentum) g + momentum m if nesterov else m
+        p = p (1 - lr weight_decay) - lr f orthogonalize(u)
+    ``params`` and ``momenta`` fp32, ``grads`` any of the three types,
+    ``lowp_outs`` (None, or a tensor or None for each) take the rounded
+    parameters; 2-D tensors with unit column stride.  f: "original",
+    sqrt(max(1, rows / cols)), or "match_rms_adamw", 0.2 sqrt(max(rows, cols)).
+    What is written may not overlap anything else in the lists."""
+    if adjust not in ("original", "match_rms_adamw"):
+        raise ValueError(f"muon_multi: adjust is 'original' or 'match_rms_adamw' (got {adjust!r})")
+    _abi.nodes().muon_multi(params, grads, momenta, lowp_outs, steps, *coefficients, eps, lr, momentum,
+                            weight_decay, nesterov, adjust == "match_rms_adamw")
+
+
 def cast_(src: torch.Tensor, dst: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
     """dst = round(src) (or dst = round(dst + src)); contiguous, same numel."""
     dev = _require_gpu(src, dst)

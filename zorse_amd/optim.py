@@ -1,4 +1,4 @@
-"""Fused AdamW on flat parameter shards and on lists of tensors.
+"""Fused AdamW on flat parameter shards and on lists of tensors, and Muon.
 
 Replaces ``torch.optim.Adam(fused=True)`` as the reference builds it for each
 FSDP module's flat shard (zorse_utils/pipeline.py:150-181) and steps it from
@@ -205,13 +205,15 @@ class FusedAdamW(torch.optim.Optimizer):
                                  f"state_bits={self.state_bits}")
         saved.update(state_dict)
 
+    _HELD = ("exp_avg", "exp_avg_sq", "master")  # in fp32, whatever they were saved in
+
     def _keep_types(self, saved: dict) -> None:
         keys = itertools.chain.from_iterable(g["params"] for g in saved["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for key, p in zip(keys, params):
             for name, t in saved["state"].get(key, {}).items():
                 if torch.is_tensor(t) and name != "step":
-                    held = name in ("exp_avg", "exp_avg_sq", "master") and t.is_floating_point()
+                    held = name in self._HELD and t.is_floating_point()
                     self.state[p][name] = t.detach().to(
                         device=p.device, dtype=torch.float32 if held else t.dtype, copy=True)
 
@@ -241,3 +243,171 @@ class FusedAdam(FusedAdamW):
                              "decoupled weight decay")
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=0.0,
                          state_bits=state_bits, seed=seed)
+
+
+def flat_matrices(module) -> list:
+    """The matrices of a decoder layer's (or a Block's) flat parameter, as Muon's
+    ``matrices``: (offset, rows, cols) of its projections (the norms' weights are
+    none)."""
+    specs = [m.spec for m in module.modules() if hasattr(m, "flat_param")]
+    if len(specs) != 1:
+        raise ValueError(f"flat_matrices: a module with one flat parameter is needed (got {len(specs)})")
+    shapes = specs[0].shapes()
+    return [(a, *shapes[k]) for k, (a, _) in specs[0].offsets().items() if len(shapes[k]) == 2]
+
+
+class Muon(FusedAdamW):
+    """Matrices stepped by the orthogonal factor of their momentum
+    (kernels.muon_multi), all of a group's in the same launches; everything else
+    by AdamW.
+
+    A group's ``matrices``: None, every 2-D parameter is a matrix; or a list of
+    (offset, rows, cols) that each of its parameters holds in its elements
+    (flat_matrices(layer) for a decoder layer's flat parameter; [] for none, as
+    for embeddings and heads).  What lies in none of them (norm weights, biases)
+    takes AdamW's step with ``adam_lr`` (default lr), ``adam_betas`` and
+    ``adam_eps``, with the same weight decay.
+
+    ``adjust``: "original" multiplies a factor by sqrt(max(1, rows / cols)),
+    "match_rms_adamw" by 0.2 sqrt(max(rows, cols)), so that one learning rate
+    suits both steps.  bf16 / fp16 parameters keep an fp32 master."""
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, weight_decay=0.1, nesterov=True, ns_steps=5,
+                 ns_coefficients=K.MUON_COEFFICIENTS, eps=1e-7, adjust="original", matrices=None,
+                 adam_lr=None, adam_betas=(0.9, 0.999), adam_eps=1e-8):
+        if lr < 0 or eps < 0 or weight_decay < 0 or adam_eps < 0 or (adam_lr or 0) < 0:
+            raise ValueError("lr, eps and weight_decay must be non-negative")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"invalid momentum {momentum}")
+        if not (0.0 <= adam_betas[0] < 1.0 and 0.0 <= adam_betas[1] < 1.0):
+            raise ValueError(f"invalid betas {adam_betas}")
+        if adjust not in ("original", "match_rms_adamw"):
+            raise ValueError(f"adjust is 'original' or 'match_rms_adamw' (got {adjust!r})")
+        self.state_bits = 32
+        torch.optim.Optimizer.__init__(self, params, dict(
+            lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov,
+            ns_steps=operator.index(ns_steps), ns_coefficients=tuple(ns_coefficients), eps=eps,
+            adjust=adjust, matrices=matrices, adam_lr=adam_lr, adam_betas=tuple(adam_betas),
+            adam_eps=adam_eps))
+        self._step_hooks = {}
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            for p in group["params"]:
+                self._layout(group, p)
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _layout(group: dict, p: torch.Tensor):
+        """(matrices, rest) of p: (offset, rows, cols) and (offset, elements)."""
+        n = p.numel()
+        if group["matrices"] is None:
+            mats = [(0, *p.shape)] if p.dim() == 2 else []
+        else:
+            mats = sorted((int(a), int(r), int(c)) for a, r, c in group["matrices"])
+        mats = [m for m in mats if m[1] * m[2] != 0]
+        rest, at = [], 0
+        for a, r, c in mats:
+            if a < at or min(r, c) < 0 or a + r * c > n:
+                raise ValueError(f"matrices of a parameter of {n} elements overlap or leave it: "
+                                 f"{r} x {c} at {a}")
+            if a > at:
+                rest.append((at, a - at))
+            at = a + r * c
+        if at < n:
+            rest.append((at, n - at))
+        return mats, rest
+
+    def _init_state(self, p: torch.Tensor) -> dict:
+        st = self.state[p]
+        if not st:
+            group = next(g for g in self.param_groups if any(q is p for q in g["params"]))
+            mats, rest = self._layout(group, p)
+            kw = {"dtype": torch.float32, "device": p.device}
+            st["step"] = 0
+            st["momentum_buffer"] = torch.zeros(sum(r * c for _, r, c in mats), **kw)
+            if rest:
+                n = sum(k for _, k in rest)
+                st["exp_avg"], st["exp_avg_sq"] = torch.zeros(n, **kw), torch.zeros(n, **kw)
+            if p.dtype != torch.float32:
+                st["master"] = p.detach().reshape(-1).to(torch.float32)
+        return st
+
+    def _checked(self, p: torch.Tensor) -> dict:
+        if p.grad.is_sparse:
+            raise RuntimeError("Muon does not support sparse gradients")
+        if not p.is_contiguous() or not p.grad.is_contiguous():
+            raise ValueError("Muon needs contiguous parameters and gradients")
+        st = self._init_state(p)
+        if st["momentum_buffer"].device != p.device:
+            for k, t in st.items():
+                if torch.is_tensor(t) and k != "step":
+                    st[k] = t.to(p.device)
+        return st
+
+    def _step_one(self, group: dict, p: torch.Tensor) -> None:
+        self._step_list(group, [p])
+
+    def _step_list(self, group: dict, params: list) -> None:
+        if len(params) > 1 and K.spans_meet([p.data_ptr() for p in params],
+                                            [p.nbytes for p in params], 1):
+            for p in params:
+                self._step_list(group, [p])
+            return
+        states = [self._checked(p) for p in params]
+        mats = ([], [], [], [])   # params, grads, momenta, rounded copies
+        rest = ([], [], [], [], [])  # params, grads, moments, rounded copies
+        steps = []
+        for p, st in zip(params, states):
+            master, grad, low = st.get("master"), p.grad.view(-1), None
+            flat = p.detach().view(-1)
+            if master is not None:
+                flat, low = master, flat
+            where, others = self._layout(group, p)
+            at = 0
+            for a, r, c in where:
+                cut = slice(a, a + r * c)
+                mats[0].append(flat[cut].view(r, c))
+                mats[1].append(grad[cut].view(r, c))
+                mats[2].append(st["momentum_buffer"][at:at + r * c].view(r, c))
+                mats[3].append(None if low is None else low[cut].view(r, c))
+                at += r * c
+            at = 0
+            for a, n in others:
+                rest[0].append(flat[a:a + n])
+                rest[1].append(grad[a:a + n])
+                rest[2].append(st["exp_avg"][at:at + n])
+                rest[3].append(st["exp_avg_sq"][at:at + n])
+                rest[4].append(None if low is None else low[a:a + n])
+                steps.append(st["step"] + 1)
+                at += n
+        if mats[0]:
+            K.muon_multi(*mats[:3], lowp_outs=mats[3], lr=group["lr"], momentum=group["momentum"],
+                         weight_decay=group["weight_decay"], nesterov=group["nesterov"],
+                         adjust=group["adjust"], steps=group["ns_steps"],
+                         coefficients=group["ns_coefficients"], eps=group["eps"])
+        if rest[0]:
+            lr = group["lr"] if group["adam_lr"] is None else group["adam_lr"]
+            b1, b2 = group["adam_betas"]
+            K.adamw_multi(*rest[:4], steps, lowp_outs=rest[4], lr=lr, beta1=b1, beta2=b2,
+                          eps=group["adam_eps"], weight_decay=group["weight_decay"])
+        for st in states:
+            st["step"] = st["step"] + 1
+        for p in params:
+            self._stepped(p)
+
+    def _check_loaded(self, state_dict, saved: dict) -> None:
+        for st in state_dict["state"].values():
+            if "momentum_buffer" not in st:
+                raise ValueError("the saved state is not Muon's")
+        saved.update(state_dict)
+
+    _HELD = ("momentum_buffer", "exp_avg", "exp_avg_sq", "master")
+
+    def moments(self, p: torch.Tensor):
+        """The momentum of p's matrices, fp32, one matrix after another."""
+        return self._init_state(p)["momentum_buffer"]

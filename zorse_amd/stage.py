@@ -46,7 +46,7 @@ class StageRunner:
     def __init__(self, layers: Sequence[nn.Module], lr=1e-4, betas=(0.9, 0.95), eps=1e-8,
                  weight_decay=0.1, optimizer_in_backwards=True, recompute=False,
                  cache_attention=True, optimizer_overlap="attention", offload_inputs=False,
-                 state_bits=32, seed=0):
+                 state_bits=32, seed=0, optimizer=None):
         if optimizer_overlap not in ("attention", "immediate"):
             raise ValueError(f"optimizer_overlap {optimizer_overlap!r}: 'attention' or 'immediate'")
         if offload_inputs and not recompute:
@@ -92,8 +92,11 @@ class StageRunner:
         # of the first one; stages of one model pass the layers before them)
         for i, layer in enumerate(self.layers):
             params = [p for p in layer.parameters() if p.requires_grad]
-            opt = FusedAdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                             state_bits=state_bits, seed=seed + i)
+            # ``optimizer(layer, params)``: another one for each layer (optim.Muon),
+            # instead of AdamW with the arguments above
+            opt = optimizer(layer, params) if optimizer is not None else \
+                FusedAdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                           state_bits=state_bits, seed=seed + i)
             self.optimizers.append(opt)
             if optimizer_in_backwards:
                 for p in params:
