@@ -189,22 +189,41 @@ __device__ __forceinline__ void triangle_tile(int64_t pid, int64_t& m, int64_t& 
   n = pid - static_cast<int64_t>(i) * (i + 1) / 2;
 }
 
+// Workgroup n of a grouped launch: runs of 32 tiles to one XCD, so that neighbours
+// share its L2, the runs round the eight of them: matrices whose tiles take longer
+// (another reduction) then lie on all.
+__device__ __forceinline__ int64_t group_order(int64_t bid, int64_t n) {
+  const int64_t whole = n >> 8 << 8;
+  if (bid >= whole) return whole + xcd_order(bid - whole, n - whole);
+  const int64_t x = bid & 7, slot = bid >> 3;
+  return (slot >> 5 << 8) + (x << 5) + (slot & 31);
+}
+
 // EPI 4: v = alpha v + beta (r + z) of 8 elements at `at`, and their stores.
 template <typename T>
-__device__ __forceinline__ void poly_chunk(const GemmArgs& args, int64_t at, float (&v)[8]) {
-  float t[8] = {};
-  if (args.r != nullptr) Vec8<T>::load(static_cast<const T*>(args.r) + at, t);
-  if (args.z != nullptr) {
-    float u[8];
-    Vec8<T>::load(static_cast<const T*>(args.z) + at, u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] += u[e];
+struct PolyIn {  // r and z of 8 elements, loaded ahead of their use
+  Raw8<T> r, z;
+  __device__ __forceinline__ void load(const GemmArgs& args, int64_t at) {
+    if (args.r != nullptr) r.load(static_cast<const T*>(args.r) + at);
+    if (args.z != nullptr) z.load(static_cast<const T*>(args.z) + at);
   }
+  __device__ __forceinline__ void apply(const GemmArgs& args, float (&v)[8]) const {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = fmaf(args.alpha, v[e], args.beta * t[e]);
-}
+    for (int e = 0; e < 8; ++e) {
+      float t = 0.f;
+      if (args.r != nullptr) t = r[e];
+      if (args.z != nullptr) t += z[e];
+      v[e] = fmaf(args.alpha, v[e], args.beta * t);
+    }
+  }
+};
 template <typename T>
-__device__ __forceinline__ void poly_store(const GemmArgs& args, int64_t at, const float (&v)[8]) {
+__device__ __forceinline__ void poly_store(const GemmArgs& args, int64_t at, float (&v)[8]) {
+  // the fp32 values themselves: a conversion that the compiler joins to the
+  // operation before it (v_fma_mix) rounds once, one that it does not twice, and
+  // c and what its rounding left would not belong together
+#pragma unroll
+  for (int e = 0; e < 8; ++e) asm("" : "+v"(v[e]));
   Vec8<T>::store(static_cast<T*>(args.c) + at, v);
   if (args.c2 != nullptr) {
     float left[8];
@@ -381,7 +400,7 @@ void gemm_tiled_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch)
   static_assert(EPI == 0 || (!AKM && !BKM) || (EPI == 3 && !AKM && RAG) || (EPI == 4 && !AKM && !RAG),
                 "the SwiGLU and RoPE epilogues take NT operands, partial sums A along K");
   int64_t pid = blockIdx.x;
-  if constexpr (EPI == 4) pid = xcd_order(pid, launch.first[launch.n]);
+  if constexpr (EPI == 4) pid = group_order(pid, launch.first[launch.n]);
   const GemmArgs& args = problem_of(launch, pid);
   static_assert(MB == 8 || (MB == 4 && EPI != 1 && !AKM && !RAG), "128-row tiles");
   constexpr int TBM = 32 * MB;  // tile rows
@@ -669,8 +688,21 @@ void gemm_tiled_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch)
   // half-split pairing: 8-column chunks per half head, 2^hcl (8 for head dim
   // 128, 4 for 64)
   const int hcl = args.rhalf == 64 ? 3 : 2, hcm = (1 << hcl) - 1;
+  // EPI 4: r and z of a block are loaded while the one before it is stored
+  PolyIn<T> pin[2][4];
+  auto poly_load = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = q * 64 + el;
+      pin[i & 1][q].load(args, (m0 + wm * WR + 16 * i + (c >> 4)) * args.ldc + n0 + wn * 128 + 8 * (c & 15));
+    }
+  };
+  if constexpr (EPI == 4) poly_load(0);
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
+    if constexpr (EPI == 4) {
+      if (i + 1 < MB) poly_load(i + 1);
+    }
     // EPI 2, half-split pairing: this block's cos / sin, loaded before the
     // staging stores below so that their latency overlaps them
     float4 rc0[2], rc1[2], rsn0[2], rsn1[2];
@@ -771,7 +803,7 @@ void gemm_tiled_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch)
         }
         if constexpr (EPI == 4) {
           const int64_t at = grow * args.ldc + gcol;
-          poly_chunk<T>(args, at, v);
+          pin[i & 1][q].apply(args, v);
           poly_store<T>(args, at, v);
           if (args.tri && m0 != n0) Vec8<float>::store(&ws[rr * 132 + 8 * ch], v);
           continue;

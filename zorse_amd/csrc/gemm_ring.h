@@ -159,7 +159,7 @@ void gemm_ring_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) 
                     (EPI == 4 && !AKM && KS == 1 && MB == NB),
                 "the SwiGLU and RoPE epilogues take NT operands");
   int64_t pid = blockIdx.x;
-  if constexpr (EPI == 4) pid = xcd_order(pid, launch.first[launch.n]);
+  if constexpr (EPI == 4) pid = group_order(pid, launch.first[launch.n]);
   const GemmArgs& args = problem_of(launch, pid);
   constexpr int TBM = 32 * MB, TBN = 32 * NB, WR = 16 * MB, WC = 16 * NB;
   typedef RingOp<T> Mm;
@@ -528,7 +528,9 @@ void gemm_ring_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) 
         continue;
       }
       if constexpr (EPI == 4) {
-        poly_chunk<T>(args, gr * args.ldc + gc, v);
+        PolyIn<T> in;
+        in.load(args, gr * args.ldc + gc);
+        in.apply(args, v);
         poly_store<T>(args, gr * args.ldc + gc, v);
         if (args.tri && m0 != n0) Vec8<float>::store(&ws[row * EP + 8 * ch], v);
         continue;

@@ -20,6 +20,7 @@
 // spectra 0.3 - 1.7e-3).  Matrices with s <= kExactSide, whose products cost no
 // time, and results in fp32 have G and P in two numbers as well, and products of
 // three terms.
+#include <algorithm>
 #include <cmath>
 
 #include "muon.h"
@@ -45,12 +46,13 @@ struct Matrix {
   int64_t sp, tp;    // padded sides
   float lr_scale;
   int grad_dtype, out_dtype, tall;
+  int vec;           // columns, rows and addresses are multiples of four elements
 };
 struct MatrixGroup {
   Matrix p[gemm::kPolyMost];
   int first[gemm::kPolyMost + 1];
   int n;
-  float mu, decay, lr, scale, eps;
+  float mu, nu, keep, lr, scale, eps;  // nu = 1 - mu, keep = 1 - lr weight_decay
   int nesterov;
 };
 
@@ -63,32 +65,84 @@ __device__ __forceinline__ const Matrix& matrix_of(const MatrixGroup& g, int64_t
 
 // What is orthogonalised, from the gradient and the momentum after this step's.
 __device__ __forceinline__ float update_of(const MatrixGroup& g, float grad, float m) {
-  return g.nesterov ? fmaf(g.mu, m, (1.f - g.mu) * grad) : m;
+  return g.nesterov ? fmaf(g.mu, m, g.nu * grad) : m;
+}
+
+// Four elements of a row from column c on (those below `cols`, else zeros); vec:
+// rows and columns are multiples of four elements and aligned.
+__device__ __forceinline__ float4 load4(const void* p, int64_t at, int dt, bool vec, int64_t left) {
+  if (vec) {
+    if (dt == ZK_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + at);
+    if (dt == ZK_BF16) {
+      const bf16x4 v = __builtin_bit_cast(bf16x4, w);
+      return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    const f16x4 v = __builtin_bit_cast(f16x4, w);
+    return make_float4(v[0], v[1], v[2], v[3]);
+  }
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < left ? load_dt(p, at + e, dt) : 0.f;
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(void* p, int64_t at, int dt, bool vec, int64_t left, float4 x) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  if (vec) {
+    if (dt == ZK_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p) + at) = x;
+    } else if (dt == ZK_BF16) {
+      *reinterpret_cast<bf16x4*>(static_cast<bf16*>(p) + at) =
+          bf16x4{static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
+    } else {
+      *reinterpret_cast<f16x4*>(static_cast<f16*>(p) + at) =
+          f16x4{static_cast<f16>(v[0]), static_cast<f16>(v[1]), static_cast<f16>(v[2]), static_cast<f16>(v[3])};
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) store_dt(p, at + e, dt, v[e]);
+}
+__device__ __forceinline__ float4 update4(const MatrixGroup& g, const float4& v, const float4& m) {
+  return make_float4(update_of(g, v.x, m.x), update_of(g, v.y, m.y), update_of(g, v.z, m.z),
+                     update_of(g, v.w, m.w));
 }
 
 // The momentum's step, and kPartials sums of squares (64 bits: squares of small
-// gradients leave fp32's range): runs of 1024 columns of a row, workgroup w of
-// the matrix taking runs w, w + kPartials, ..
+// gradients leave fp32's range): runs of 4096 columns of a row, workgroup w of
+// the matrix taking runs w, w + kPartials, ..; a run's loads are issued together.
 __global__ __launch_bounds__(256) void muon_begin_kernel(MatrixGroup g) {
   int64_t w = blockIdx.x;
   const Matrix& x = matrix_of(g, w);
-  const int64_t per_row = (x.cols + 1023) / 1024, runs = x.rows * per_row;
+  const int64_t per_row = (x.cols + 4095) / 4096, runs = x.rows * per_row;
+  const bool step = x.momentum != nullptr;
   double sum = 0;
   for (int64_t u = w; u < runs; u += kPartials) {
-    const int64_t row = u / per_row, c0 = (u - row * per_row) * 1024;
+    const int64_t row = u / per_row, c0 = (u - row * per_row) * 4096 + 4 * threadIdx.x;
+    float4 v[4], m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t c = c0 + k * 256 + threadIdx.x;
-      if (c < x.cols) {
-        float v = load_dt(x.grad, row * x.ld_grad + c, x.grad_dtype);
-        if (x.momentum != nullptr) {
-          float* m = x.momentum + row * x.ld_momentum + c;
-          const float next = fmaf(g.mu, *m, (1.f - g.mu) * v);
-          *m = next;
-          v = update_of(g, v, next);
-        }
-        sum += static_cast<double>(v) * v;
+      const int64_t c = c0 + k * 1024;
+      v[k] = m[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c >= x.cols) continue;
+      v[k] = load4(x.grad, row * x.ld_grad + c, x.grad_dtype, x.vec, x.cols - c);
+      if (step) m[k] = load4(x.momentum, row * x.ld_momentum + c, ZK_F32, x.vec, x.cols - c);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t c = c0 + k * 1024;
+      if (c >= x.cols) continue;
+      float4 t = v[k];
+      if (step) {
+        const float h = g.nu;
+        const float4 n = make_float4(fmaf(g.mu, m[k].x, h * t.x), fmaf(g.mu, m[k].y, h * t.y),
+                                     fmaf(g.mu, m[k].z, h * t.z), fmaf(g.mu, m[k].w, h * t.w));
+        store4(x.momentum, row * x.ld_momentum + c, ZK_F32, x.vec, x.cols - c, n);
+        t = update4(g, t, n);
       }
+      sum += static_cast<double>(t.x) * t.x + static_cast<double>(t.y) * t.y +
+             (static_cast<double>(t.z) * t.z + static_cast<double>(t.w) * t.w);
     }
   }
   __shared__ double part[256];
@@ -117,27 +171,44 @@ __global__ __launch_bounds__(256) void muon_scale_kernel(MatrixGroup g) {
   const int64_t s0 = at / per_row * kTile, t0 = at % per_row * kTile;
   // U's rows and columns of this tile
   const int64_t r0 = x.tall ? t0 : s0, c0 = x.tall ? s0 : t0;
-  const int col = threadIdx.x % kTile, row0 = threadIdx.x / kTile;
+  const int col = threadIdx.x % 16 * 4, row0 = threadIdx.x / 16;
+  float4 v[4], m[4];
 #pragma unroll
-  for (int k = 0; k < kTile / 4; ++k) {
-    const int64_t r = r0 + row0 + 4 * k, c = c0 + col;
-    float v = 0.f;
-    if (r < x.rows && c < x.cols) {
-      v = load_dt(x.grad, r * x.ld_grad + c, x.grad_dtype);
-      if (x.momentum != nullptr) v = update_of(g, v, x.momentum[r * x.ld_momentum + c]);
+  for (int k = 0; k < 4; ++k) {
+    const int64_t r = r0 + row0 + 16 * k, c = c0 + col;
+    v[k] = m[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r >= x.rows || c >= x.cols) continue;
+    v[k] = load4(x.grad, r * x.ld_grad + c, x.grad_dtype, x.vec, x.cols - c);
+    if (x.momentum != nullptr) m[k] = load4(x.momentum, r * x.ld_momentum + c, ZK_F32, x.vec, x.cols - c);
+  }
+  if (x.momentum != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = update4(g, v[k], m[k]);
+  }
+  if (x.tall) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float* row = &tile[row0 + 16 * k][col];
+      row[0] = v[k].x; row[1] = v[k].y; row[2] = v[k].z; row[3] = v[k].w;
     }
-    tile[row0 + 4 * k][col] = v;
   }
   __syncthreads();
   const float f = static_cast<float>(g.scale / (sqrt(total) + static_cast<double>(g.eps)));
 #pragma unroll
-  for (int k = 0; k < kTile / 4; ++k) {
-    const int r = row0 + 4 * k;
-    const float v = (x.tall ? tile[col][r] : tile[r][col]) * f;
-    const f16 hi = static_cast<f16>(v);
+  for (int k = 0; k < 4; ++k) {
+    const int r = row0 + 16 * k;
+    if (x.tall) v[k] = make_float4(tile[col][r], tile[col + 1][r], tile[col + 2][r], tile[col + 3][r]);
+    float y[4] = {v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f};
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      asm("" : "+v"(y[e]));  // see poly_store
+      hi[e] = static_cast<f16>(y[e]);
+      lo[e] = static_cast<f16>(y[e] - static_cast<float>(hi[e]));
+    }
     const int64_t i = (s0 + r) * x.tp + t0 + col;
-    x.hi[i] = hi;
-    x.lo[i] = static_cast<f16>(v - static_cast<float>(hi));
+    *reinterpret_cast<f16x4*>(x.hi + i) = hi;
+    *reinterpret_cast<f16x4*>(x.lo + i) = lo;
   }
 }
 
@@ -148,26 +219,47 @@ __global__ __launch_bounds__(256) void muon_finish_kernel(MatrixGroup g) {
   __shared__ float tile[kTile][kTile + 1];
   const int64_t per_row = x.tp / kTile;
   const int64_t s0 = at / per_row * kTile, t0 = at % per_row * kTile;
-  const int col = threadIdx.x % kTile, row0 = threadIdx.x / kTile;
+  const int64_t r0 = x.tall ? t0 : s0, c0 = x.tall ? s0 : t0;
+  const int col = threadIdx.x % 16 * 4, row0 = threadIdx.x / 16;
+  f16x4 hi[4], lo[4];
+  float4 p[4];
 #pragma unroll
-  for (int k = 0; k < kTile / 4; ++k) {
-    const int r = row0 + 4 * k;
-    const int64_t i = (s0 + r) * x.tp + t0 + col;
-    tile[r][col] = (static_cast<float>(x.hi[i]) + static_cast<float>(x.lo[i])) / g.scale;
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = (s0 + row0 + 16 * k) * x.tp + t0 + col;
+    hi[k] = *reinterpret_cast<const f16x4*>(x.hi + i);
+    lo[k] = *reinterpret_cast<const f16x4*>(x.lo + i);
+    const int64_t r = r0 + row0 + 16 * k, c = c0 + col;
+    p[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (x.param != nullptr && r < x.rows && c < x.cols)
+      p[k] = load4(x.param, r * x.ld_param + c, ZK_F32, x.vec, x.cols - c);
+  }
+  float4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      y[e] = (static_cast<float>(hi[k][e]) + static_cast<float>(lo[k][e])) / g.scale;
+    v[k] = make_float4(y[0], y[1], y[2], y[3]);
+    if (x.tall) {
+      float* row = &tile[row0 + 16 * k][col];
+      row[0] = y[0]; row[1] = y[1]; row[2] = y[2]; row[3] = y[3];
+    }
   }
   __syncthreads();
-  const int64_t r0 = x.tall ? t0 : s0, c0 = x.tall ? s0 : t0;
+  const float f = -g.lr * x.lr_scale, keep = g.keep;
 #pragma unroll
-  for (int k = 0; k < kTile / 4; ++k) {
-    const int64_t r = r0 + row0 + 4 * k, c = c0 + col;
+  for (int k = 0; k < 4; ++k) {
+    const int rr = row0 + 16 * k;
+    const int64_t r = r0 + rr, c = c0 + col;
     if (r >= x.rows || c >= x.cols) continue;
-    float v = x.tall ? tile[col][row0 + 4 * k] : tile[row0 + 4 * k][col];
+    if (x.tall) v[k] = make_float4(tile[col][rr], tile[col + 1][rr], tile[col + 2][rr], tile[col + 3][rr]);
     if (x.param != nullptr) {
-      float* p = x.param + r * x.ld_param + c;
-      v = fmaf(-g.lr * x.lr_scale, v, *p * (1.f - g.decay));
-      *p = v;
+      v[k] = make_float4(fmaf(f, v[k].x, p[k].x * keep), fmaf(f, v[k].y, p[k].y * keep),
+                         fmaf(f, v[k].z, p[k].z * keep), fmaf(f, v[k].w, p[k].w * keep));
+      store4(x.param, r * x.ld_param + c, ZK_F32, x.vec, x.cols - c, v[k]);
     }
-    if (x.out != nullptr) store_dt(x.out, r * x.ld_out + c, x.out_dtype, v);
+    if (x.out != nullptr) store4(x.out, r * x.ld_out + c, x.out_dtype, x.vec, x.cols - c, v[k]);
   }
 }
 
@@ -296,7 +388,8 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
     MatrixGroup m = {};
     f16 *hi[2][gemm::kPolyMost], *lo[2][gemm::kPolyMost], *G[2][gemm::kPolyMost], *P[2][gemm::kPolyMost];
     m.n = len;
-    m.mu = static_cast<float>(h.mu); m.decay = static_cast<float>(h.lr * h.decay);
+    m.mu = static_cast<float>(h.mu); m.nu = static_cast<float>(1 - h.mu);
+    m.keep = static_cast<float>(1 - h.lr * h.decay);
     m.lr = static_cast<float>(h.lr); m.scale = S; m.eps = static_cast<float>(h.eps);
     m.nesterov = h.nesterov;
     for (int i = 0; i < len; ++i) {
@@ -322,6 +415,10 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
       y.sp = d[i].sp; y.tp = d[i].tp;
       y.grad_dtype = static_cast<int>(x.grad_dtype); y.out_dtype = static_cast<int>(x.out_dtype);
       y.tall = x.rows > x.cols;
+      y.vec = x.cols % 4 == 0 && x.ld_grad % 4 == 0 && aligned(x.grad, 4 * dtype_bytes(y.grad_dtype)) &&
+              (!step || (x.ld_momentum % 4 == 0 && x.ld_param % 4 == 0 && aligned(x.momentum, 16) &&
+                         aligned(x.param, 16))) &&
+              (x.out == nullptr || (x.ld_out % 4 == 0 && aligned(x.out, 4 * dtype_bytes(y.out_dtype))));
       y.lr_scale = static_cast<float>(
           h.adjust == ZK_MUON_MATCH_RMS ? 0.2 * sqrt(static_cast<double>(d[i].t))
                                         : sqrt(fmax(1.0, static_cast<double>(x.rows) / x.cols)));
@@ -335,12 +432,17 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
     const dim3 tiles = spread([&](int i) { return d[i].sp / kTile * (d[i].tp / kTile); });
     hipLaunchKernelGGL(muon_scale_kernel, tiles, dim3(256), 0, s, m);
 
+    // tiles with the longest reduction start first
+    int by_length[gemm::kPolyMost];
+    for (int i = 0; i < len; ++i) by_length[i] = i;
+    std::stable_sort(by_length, by_length + len, [&](int a, int b) { return d[a].tp > d[b].tp; });
     // product `which` of step k: 0 G, 1 P, 2 X
     auto product = [&](int k, int which) {
       gemm::PolyGroup g = {};
       g.n = len;
-      for (int i = 0; i < len; ++i) {
-        gemm::GemmArgs& q = g.p[i];
+      for (int n = 0; n < len; ++n) {
+        const int i = which == 0 ? by_length[n] : n;
+        gemm::GemmArgs& q = g.p[n];
         const Sides& e = d[i];
         f16 *const xh = hi[k & 1][i], *const xl = lo[k & 1][i];
         q.thrice = e.exact;
@@ -366,7 +468,7 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
           q.alpha = 1.f / R; q.beta = static_cast<float>(h.a);
         }
         const int64_t rows = (q.M + gemm::tile_rows(tile) - 1) / gemm::tile_rows(tile);
-        g.first[i + 1] = g.first[i] + static_cast<int>(q.tri ? rows * (rows + 1) / 2
+        g.first[n + 1] = g.first[n] + static_cast<int>(q.tri ? rows * (rows + 1) / 2
                                                              : gemm::tile_count(tile, q.M, q.N));
       }
       if (which == 2)
