@@ -516,6 +516,16 @@ void gemm_ring_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) 
   } else {
     constexpr int CPR = TBN / 8;
     const T* const R = static_cast<const T*>(args.r);
+    // EPI 4: every r and z of the tile is loaded before a result is stored
+    constexpr int NIN = EPI == 4 ? TBM * CPR / NT : 1;
+    PolyIn<T> in[NIN];
+    if constexpr (EPI == 4) {
+#pragma unroll
+      for (int it = 0; it < NIN; ++it) {
+        const int id = it * NT + tid, row = id / CPR, ch = id % CPR;
+        if (m0 + row < M && n0 + 8 * ch < N) in[it].load(args, (m0 + row) * args.ldc + n0 + 8 * ch);
+      }
+    }
 #pragma unroll
     for (int it = 0; it < TBM * CPR / NT; ++it) {
       const int id = it * NT + tid, row = id / CPR, ch = id % CPR;
@@ -528,9 +538,7 @@ void gemm_ring_kernel(std::conditional_t<EPI == 4, PolyGroup, GemmArgs> launch) 
         continue;
       }
       if constexpr (EPI == 4) {
-        PolyIn<T> in;
-        in.load(args, gr * args.ldc + gc);
-        in.apply(args, v);
+        in[it].apply(args, v);
         poly_store<T>(args, gr * args.ldc + gc, v);
         if (args.tri && m0 != n0) Vec8<float>::store(&ws[row * EP + 8 * ch], v);
         continue;
