@@ -71,16 +71,38 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int64_t T, int32_t* 
 }
 
 // ---------------------------------------------------------------- forward --
-static constexpr float kGrowth = 8.0f;  // log2 growth of the maximum before a rescale
+// NW waves of 32 queries, whose Q rows stay in registers; 64-key tiles of K and V
+// in LDS, row-major with swizzled 16-byte chunks.  Scores are computed transposed
+// (S^T = K Q^T): a lane holds one query's scores of 32 keys, so the softmax is per
+// lane with one exchange between the wave's halves, and the probabilities are the
+// next product's operand as they are (O^T += V^T P^T, V^T by transposed reads).
+// The reference maximum moves when a score exceeds it by 2^8 only.
+static constexpr float kGrowth = 8.0f;  // in the exp2 domain
 
-// NW waves of 32 queries.  KR: 0 for a head dim of D and 16-byte aligned heads,
-// else ceil(d / 16), at least 2.
-template <typename T, int D, int NW, int KR>
+// Orders the compiler's memory accesses and waits for the other waves, but not for
+// this wave's loads in flight.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// kPhases (8 waves): the softmax of a 64-key tile takes a wave about as long on the
+// vector units as its two products take on the matrix units, but waves that run in
+// step do the same thing at the same time.  Waves 0-3 (one on each SIMD) and 4-7
+// therefore alternate: while one group multiplies (the scores of tile t and P V of
+// tile t - 1), the other one is at the softmax of a tile, with a barrier between
+// the phases.  Tile t + 1 of K and t of V are loaded over two phases.
+// KR: 0 for a head dim of D and 16-byte aligned heads, else ceil(d / 16), at least 2.
+template <typename T, int D, int NW, int KR, bool kPhases>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
 void packed_fwd_kernel(PackedArgs a) {
   typedef Mfma<T> M;
   typedef typename M::vec8 V8;
   constexpr int BM = 32 * NW, BN = 64, NT = 64 * NW;
+  constexpr int PF = 4;  // operand reads in flight
   constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
   const int hd = KR ? a.d : D;
   __shared__ __attribute__((aligned(16))) T K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
@@ -129,115 +151,227 @@ void packed_fwd_kernel(PackedArgs a) {
   PackedLoader<T, D, BN, NT> kload, vload;
   kload.init(a.k_s, hd);
   vload.init(a.v_s, hd);
-  auto issue = [&](int t, int st) {
-    const int k0 = kv_lo + t * BN;
-    kload.issue(st ? K1 : K0, Kp, a.k_s, k0, plan.n);
-    vload.issue(st ? V1 : V0, Vp, a.v_s, k0, plan.n);
+  auto issue_k = [&](int t, int st) {
+    kload.issue(st ? K1 : K0, Kp, a.k_s, kv_lo + t * BN, plan.n);
+  };
+  auto issue_v = [&](int t, int st) {
+    vload.issue(st ? V1 : V0, Vp, a.v_s, kv_lo + t * BN, plan.n);
   };
   // LDS byte offsets from two per-lane bases (the swizzle XORs chunk indices)
   const int rbase = 2 * tile_off<D>(l32, 8 * g);
   const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
 
-  f32x16 o[NB];
+  f32x16 o[NB], s[BN / 32];
+  V8 pb[BN / 16];
 #pragma unroll
   for (int nt = 0; nt < NB; ++nt) o[nt] = f32x16{};
   float m_ref = -INFINITY, l_i = 0.f;
   const float c2 = a.scale_log2;
 
-  auto step = [&](auto stage_tag, int t) {
-    constexpr int st = decltype(stage_tag)::value;
+  auto skipped = [&](int t) __attribute__((always_inline)) {
     const int k0 = kv_lo + t * BN;
-    wait_vmcnt<0>();  // this wave's loads of tile t have landed
-    __syncthreads();  // ... and every other wave's; all are done with the other stage
-    if (t + 1 < n_t) issue(t + 1, st ^ 1);
-    if (idle || k0 > w_hi || k0 + BN <= w_lo) return;
+    return idle || t < 0 || t >= n_t || k0 > w_hi || k0 + BN <= w_lo;
+  };
+  // S^T = K Q^T of tile t, which starts from -inf where a key is not seen
+  auto scores = [&](const T* Kt, int t) __attribute__((always_inline)) {
+    int rb = rbase;  // opaque: addresses derived here
+    asm volatile("" : "+v"(rb));
+    const int k0 = kv_lo + t * BN;
     const bool need_mask = k0 < f_lo || k0 + BN - 1 > f_hi;
-    const T* Kt = st ? K1 : K0;
-    const T* Vt = st ? V1 : V0;
-    auto tile = [&](auto mask_tag) {
-      constexpr bool kMask = decltype(mask_tag)::value;
-      // opaque, so that addresses are derived in the step, and in each body: what
-      // both share is not moved before the branch, where it would be held (and
-      // spilled) over it
-      int rb = rbase, tb = tbase;
-      asm volatile("" : "+v"(rb), "+v"(tb));
-      f32x16 s[BN / 32];
+    // operands are read PF products ahead; the fences keep the reads there (left
+    // alone, the compiler reads all of them first and has no registers left)
+    auto rowread = [&](int i) __attribute__((always_inline)) {
+      const int ks = i / (BN / 32), tt = i % (BN / 32);
+      return *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Kt) + (rb ^ (ks << 5)) +
+                                          tt * 32 * D * 2);
+    };
+    constexpr int NM = KS * (BN / 32);
+    V8 kq[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i) kq[i] = rowread(i);
+#pragma unroll
+    for (int tt = 0; tt < BN / 32; ++tt) {
+      if (ragged_step<KR>(0)) kq[tt] = mask_cols<T>(kq[tt], 8 * g, hd);
+    }
+    // each branch with its own first products: what they leave needs no copies
+    if (need_mask) {
+      const int kb = k0 + 4 * g - vis_lo;
 #pragma unroll
       for (int tt = 0; tt < BN / 32; ++tt) {
-        s[tt] = f32x16{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          V8 kv = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Kt) +
-                                               (rb ^ (ks << 5)) + tt * 32 * D * 2);
-          if (ragged_step<KR>(ks)) kv = mask_cols<T>(kv, 16 * ks + 8 * g, hd);
-          s[tt] = M::mma(kv, qreg[ks], s[tt]);
-        }
-      }
-      if (kMask) {
-        const int kb = k0 + 4 * g - vis_lo;
-#pragma unroll
-        for (int tt = 0; tt < BN / 32; ++tt)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int rel = kb + 32 * tt + 8 * (j >> 2) + (j & 3);
-            s[tt][j] = static_cast<unsigned>(rel) <= static_cast<unsigned>(vis_span) ? s[tt][j]
-                                                                                    : -INFINITY;
-          }
-      }
-      float mloc = -INFINITY;
-#pragma unroll
-      for (int tt = 0; tt < BN / 32; ++tt)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, s[tt][j]);
-      mloc = fmaxf(mloc, other_half(mloc));
-      const bool grow = (mloc - m_ref) * c2 > kGrowth;
-      if (__any(grow)) {
-        const float m_new = fmaxf(m_ref, mloc);
-        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_ref - m_new) * c2);
-        m_ref = m_new;
-        l_i *= alpha;
-#pragma unroll
-        for (int nt = 0; nt < NB; ++nt) o[nt] *= alpha;
-      }
-      const float mc = m_ref == -INFINITY ? 0.f : m_ref * c2;
-      V8 pb[BN / 16];
-      float lsum = 0.f;
-#pragma unroll
-      for (int tt = 0; tt < BN / 32; ++tt)
+        f32x16 c;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[tt][j], c2, -mc));
-          lsum += p;
-          pb[2 * tt + (j >> 3)][j & 7] = static_cast<T>(p);
+          const int rel = kb + 32 * tt + 8 * (j >> 2) + (j & 3);
+          c[j] = static_cast<unsigned>(rel) <= static_cast<unsigned>(vis_span) ? 0.f : -INFINITY;
         }
-      l_i += lsum;
-#pragma unroll
-      for (int kk = 0; kk < BN / 16; ++kk) {
-#pragma unroll
-        for (int nt = 0; nt < NB; ++nt) {
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
-          typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-          const char* vb = reinterpret_cast<const char*>(Vt) + kk * 16 * D * 2;
-          const int off = tb ^ (nt << 6);
-          const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + off));
-          const s16x4 x1 =
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + 8 * D * 2 + (off ^ 32)));
-          const s16x8 w = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-          o[nt] = M::mma(__builtin_bit_cast(V8, w), pb[kk], o[nt]);
-        }
+        s[tt] = M::mma(kq[tt], qreg[0], c);
       }
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < BN / 32; ++tt) s[tt] = M::mma(kq[tt], qreg[0], f32x16{});
+    }
+#pragma unroll
+    for (int i = 0; i < BN / 32; ++i)
+      if (i + PF < NM) kq[i % PF] = rowread(i + PF);
+#pragma unroll
+    for (int i = BN / 32; i < NM; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int ks = i / (BN / 32), tt = i % (BN / 32);
+      V8 kv = kq[i % PF];
+      if (ragged_step<KR>(ks)) kv = mask_cols<T>(kv, 16 * ks + 8 * g, hd);
+      if (i + PF < NM) kq[i % PF] = rowread(i + PF);
+      s[tt] = M::mma(kv, qreg[ks], s[tt]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // P^T from S^T, and the running maximum and sum
+  auto softmax = [&]() __attribute__((always_inline)) {
+    // opaque here and at the end: the vector work stays between the barriers
+#pragma unroll
+    for (int tt = 0; tt < BN / 32; ++tt) asm volatile("" : "+v"(s[tt]));
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int tt = 0; tt < BN / 32; ++tt)
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) mloc = fmaxf(fmaxf(mloc, s[tt][j]), s[tt][j + 1]);
+    mloc = fmaxf(mloc, other_half(mloc));
+    const bool grow = (mloc - m_ref) * c2 > kGrowth;
+    if (__any(grow)) {
+      const float m_new = fmaxf(m_ref, mloc);
+      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_ref - m_new) * c2);
+      m_ref = m_new;
+      l_i *= alpha;
+#pragma unroll
+      for (int nt = 0; nt < NB; ++nt) o[nt] *= alpha;
+    }
+    const float mc = m_ref == -INFINITY ? 0.f : m_ref * c2;
+    float lsum[4] = {};
+#pragma unroll
+    for (int tt = 0; tt < BN / 32; ++tt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[tt][j], c2, -mc));
+        lsum[j & 3] += p;
+        pb[2 * tt + (j >> 3)][j & 7] = static_cast<T>(p);
+      }
+    l_i += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+#pragma unroll
+    for (int kk = 0; kk < BN / 16; ++kk) asm volatile("" : "+v"(pb[kk]));
+    asm volatile("" : "+v"(l_i));
+  };
+  // O^T += V^T P^T (V^T read transposed from the row-major tile)
+  auto weighted = [&](const T* Vt) __attribute__((always_inline)) {
+    int tb = tbase;
+    asm volatile("" : "+v"(tb));
+    auto trread = [&](int i) __attribute__((always_inline)) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const char* vb = reinterpret_cast<const char*>(Vt) + i / NB * 16 * D * 2;
+      const int off = tb ^ ((i % NB) << 6);
+      const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + off));
+      const s16x4 x1 =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + 8 * D * 2 + (off ^ 32)));
+      const s16x8 w = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+      return __builtin_bit_cast(V8, w);
     };
-    if (need_mask)
-      tile(std::true_type{});
-    else
-      tile(std::false_type{});
+    constexpr int NM = BN / 16 * NB;
+    V8 tq[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i) tq[i] = trread(i);
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      const V8 w = tq[i % PF];
+      if (i + PF < NM) tq[i % PF] = trread(i + PF);
+      o[i % NB] = M::mma(w, pb[i / NB], o[i % NB]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  if (n_t > 0) issue(0, 0);
-  for (int t = 0; t < n_t; t += 2) {
-    step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
+  if constexpr (kPhases) {
+    // Tiles outside a wave's range are not left out here: it would wait for the
+    // others at the next barrier all the same, and branches around what lives from
+    // one phase to the next cost registers.  par: t % 2.
+    auto begin = [&](auto par, int t) __attribute__((always_inline)) {
+      constexpr int p = decltype(par)::value;
+      wait_vmcnt<0>();  // K of tile t and V of tile t - 1
+      phase_barrier();  // ... and every wave's; all are done with what they replaced
+      if (t < n_t) issue_v(t, p);
+      if (t + 1 < n_t) issue_k(t + 1, p ^ 1);
+    };
+    auto step = [&](auto par, auto second, int t) __attribute__((always_inline)) {
+      constexpr int p = decltype(par)::value;
+      begin(par, t);
+      if constexpr (decltype(second)::value) {
+        softmax();
+      } else {
+        weighted(p ? V0 : V1);
+        scores(p ? K1 : K0, t);
+      }
+      phase_barrier();
+      if constexpr (decltype(second)::value) {
+        weighted(p ? V0 : V1);
+        scores(p ? K1 : K0, t);
+      } else {
+        softmax();
+      }
+    };
+    auto end = [&](auto par, auto second) __attribute__((always_inline)) {
+      constexpr int p = decltype(par)::value;
+      begin(par, n_t);
+      if constexpr (decltype(second)::value) softmax(); else weighted(p ? V0 : V1);
+      phase_barrier();
+      if constexpr (decltype(second)::value) weighted(p ? V0 : V1);
+    };
+    auto run = [&](auto second) __attribute__((always_inline)) {
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
+      begin(even, 0);
+      if constexpr (!decltype(second)::value) scores(K0, 0);
+      phase_barrier();
+      if constexpr (decltype(second)::value) scores(K0, 0); else softmax();
+      int t = 1;
+      for (; t + 1 < n_t; t += 2) {
+        step(odd, second, t);
+        step(even, second, t + 1);
+      }
+      if (t < n_t) {
+        step(odd, second, t);
+        end(even, second);
+      } else {
+        end(odd, second);
+      }
+    };
+    if (n_t > 0) {
+      issue_k(0, 0);
+      if (wave < NW / 2)
+        run(std::false_type{});
+      else
+        run(std::true_type{});
+    }
+  } else {
+    auto step = [&](auto par, int t) __attribute__((always_inline)) {
+      constexpr int p = decltype(par)::value;
+      wait_vmcnt<0>();  // this wave's loads of tile t have landed
+      __syncthreads();  // ... and every other wave's; all are done with the other stage
+      if (t + 1 < n_t) {
+        issue_k(t + 1, p ^ 1);
+        issue_v(t + 1, p ^ 1);
+      }
+      if (skipped(t)) return;
+      scores(p ? K1 : K0, t);
+      softmax();
+      weighted(p ? V1 : V0);
+    };
+    if (n_t > 0) {
+      issue_k(0, 0);
+      issue_v(0, 0);
+    }
+    for (int t = 0; t < n_t; t += 2) {
+      step(std::integral_constant<int, 0>{}, t);
+      if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
+    }
   }
 
   const float l_tot = l_i + other_half(l_i);
@@ -375,7 +509,7 @@ namespace zk {
 template <typename T, int D, int NW, int KR>
 static void launch_packed_fwd(const PackedArgs& a, hipStream_t s) {
   const int64_t blocks = packed_blocks(a.T, 32 * NW);
-  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, KR>), dim3(static_cast<unsigned>(blocks * a.Hq)),
+  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, KR, NW == 8>), dim3(static_cast<unsigned>(blocks * a.Hq)),
                      dim3(64 * NW), 0, s, a);
 }
 template <typename T>
