@@ -44,6 +44,11 @@ struct PackedArgs {
   void* dv;
   float* delta;  // backward workspace, fp32 [Hq, T] each
   float* lse2;
+  // dK / dV of the query heads of a key head in `parts` sums: parts > 1 are stored
+  // in fp32, [parts, T, Hkv, d] each, and added by a launch of their own
+  float* dk_part;
+  float* dv_part;
+  int parts;
   const int32_t* plan;
   int64_t T;
   int Hq, Hkv, d;

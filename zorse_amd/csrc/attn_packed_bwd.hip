@@ -14,6 +14,19 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// Stores this lane's accumulators in fp32 (rows of an even number of elements).
+template <int NB, int KR>
+__device__ __forceinline__ void store_partial(float* row, const f32x16 (&x)[NB], float scale, int g, int d) {
+#pragma unroll
+  for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+    for (int a2 = 0; a2 < 8; ++a2) {
+      const int d0 = 32 * nt + 8 * (a2 >> 1) + 4 * g + 2 * (a2 & 1);
+      if (KR == 0 || d0 < d)
+        *reinterpret_cast<float2*>(row + d0) = make_float2(x[nt][2 * a2] * scale, x[nt][2 * a2 + 1] * scale);
+    }
+}
+
 // Transposed operand of tile X for its 16-row step kk, from the lane's byte offset.
 template <typename T, int D>
 __device__ __forceinline__ typename Mfma<T>::vec8 tr_operand(const T* X, int off, int kk) {
@@ -233,7 +246,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const PackedPlan plan(a);
-  const int block = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, n_rep = a.Hq / a.Hkv;
+  const int block = blockIdx.x / (a.Hkv * a.parts), in_block = blockIdx.x % (a.Hkv * a.parts);
+  const int hk = in_block % a.Hkv, part = in_block / a.Hkv;
+  // this part's query heads
+  const int n_rep = a.Hq / a.Hkv / a.parts, h_first = (hk * a.parts + part) * n_rep;
   const int k0 = plan.first_row<BK, true>(a, block);
   const int rows = static_cast<int>(a.T);
   if (k0 >= rows) return;
@@ -288,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
   qload.init(a.q_s, hd);
   dload.init(a.do_s, hd);
   auto issue = [&](int qb, int hr, int st) {
-    const int hq = hk * n_rep + hr;
+    const int hq = h_first + hr;
     const int qb0 = q_lo + qb * MQ;
     qload.issue(st ? Q1 : Q0, static_cast<const T*>(a.q) + hq * a.q_h, a.q_s, qb0, plan.n);
     dload.issue(st ? dO1 : dO0, static_cast<const T*>(a.dout) + hq * a.do_h, a.do_s, qb0, plan.n);
@@ -392,13 +408,18 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
     }
   }
 
-  const bool put = in && (my_key < plan.n || !a.keep_tail);
+  const bool whole = a.parts == 1;
+  const bool put = in && (my_key < plan.n || (whole && !a.keep_tail));
   T* dkp = static_cast<T*>(a.dk) + hk * a.dk_h + my_key * a.dk_s;
   T* dvp = static_cast<T*>(a.dv) + hk * a.dv_h + my_key * a.dv_s;
+  const int64_t at_part = ((static_cast<int64_t>(part) * a.T + my_key) * a.Hkv + hk) * hd;
   const bool bad_k = row_has_nan<NB>(dk, g, hd), bad_v = row_has_nan<NB>(dv, g, hd);
-  if (put) {
+  if (put && whole) {
     store_accumulators<T, NB, KR>(dkp, dk, a.scale, g, hd);
     store_accumulators<T, NB, KR>(dvp, dv, 1.f, g, hd);
+  } else if (put) {
+    store_partial<NB, KR>(a.dk_part + at_part, dk, a.scale, g, hd);
+    store_partial<NB, KR>(a.dv_part + at_part, dv, 1.f, g, hd);
   }
   if (__any(bad_k | bad_v)) {  // see row_has_nan; dK, then dV
     const T* Kr = Kp + clip(my_key) * a.k_s;
@@ -409,7 +430,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
       const int c0 = 16 * (second ? n - KS : n) + 8 * g;
       float acc[8] = {};
 #pragma unroll 1
-      for (int h = hk * n_rep; h < (hk + 1) * n_rep; ++h) {
+      for (int h = h_first; h < h_first + n_rep; ++h) {
         const T* Qp = static_cast<const T*>(a.q) + h * a.q_h;
         const T* Dp = static_cast<const T*>(a.dout) + h * a.do_h;
         const int64_t at = static_cast<int64_t>(h) * a.T;
@@ -427,10 +448,59 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
         }
       }
       T* row = second ? dvp : dkp;
+      float* part_row = (second ? a.dv_part : a.dk_part) + at_part;
       for (int e = 0; e < 8; ++e)
-        if ((second ? bad_v : bad_k) && put && c0 + e < hd) row[c0 + e] = static_cast<T>(acc[e]);
+        if ((second ? bad_v : bad_k) && put && c0 + e < hd) {
+          if (whole)
+            row[c0 + e] = static_cast<T>(acc[e]);
+          else
+            part_row[c0 + e] = acc[e];
+        }
     }
   }
+}
+
+// The parts' sum, first to last, in the storage type; zeros behind the last
+// sequence.  Two elements a thread (heads of even dims).
+template <typename T>
+__global__ __launch_bounds__(256) void packed_sum_kernel(PackedArgs a) {
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  const int64_t n = a.T * a.Hkv * a.d, i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 2;
+  if (i >= n) return;
+  const int e = static_cast<int>(i % a.d);
+  const int64_t r = i / a.d;
+  const int h = static_cast<int>(r % a.Hkv);
+  const int64_t t = r / a.Hkv;
+  const bool tail = t >= a.plan[0];
+  if (tail && a.keep_tail) return;
+  float2 k = make_float2(0.f, 0.f), v = k;
+  if (!tail)
+    for (int p = 0; p < a.parts; ++p) {
+      const float2 x = *reinterpret_cast<const float2*>(a.dk_part + p * n + i);
+      const float2 y = *reinterpret_cast<const float2*>(a.dv_part + p * n + i);
+      k.x += x.x;
+      k.y += x.y;
+      v.x += y.x;
+      v.y += y.y;
+    }
+  *reinterpret_cast<T2*>(static_cast<T*>(a.dk) + t * a.dk_s + h * a.dk_h + e) =
+      T2{static_cast<T>(k.x), static_cast<T>(k.y)};
+  *reinterpret_cast<T2*>(static_cast<T*>(a.dv) + t * a.dv_s + h * a.dv_h + e) =
+      T2{static_cast<T>(v.x), static_cast<T>(v.y)};
+}
+
+// Sums of a key head's query heads: one where its key blocks are enough to fill the
+// chip and to even out their different work (a causal block's is from nothing to the
+// whole sequence), else as many as make them so.  8192 causal tokens, 32 query heads
+// of 8 key heads: one sum 1640 us, two 1160 us with their addition.  A window far
+// below T evens blocks out itself.
+static int packed_parts(int64_t T, int64_t Hq, int64_t Hkv, int64_t window, int dtype) {
+  if (dtype == ZK_F32) return 1;
+  const bool even = window > 0 && window < T / 4;
+  const int64_t rep = Hq / Hkv, n = packed_blocks(T, 128) * Hkv, want = device_cus() * (even ? 3 : 7) / 2;
+  for (int64_t p = 1; p < rep; ++p)
+    if (rep % p == 0 && n * p >= want) return static_cast<int>(p);
+  return static_cast<int>(rep);
 }
 
 template <typename T, int D, int KR>
@@ -438,8 +508,13 @@ static void launch_packed_bwd(const PackedArgs& a, hipStream_t s) {
   const int64_t blocks = packed_blocks(a.T, 128);
   hipLaunchKernelGGL((packed_dq_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hq)),
                      dim3(256), 0, s, a);
-  hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hkv)),
+  hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hkv * a.parts)),
                      dim3(256), 0, s, a);
+  if (a.parts > 1) {
+    const int64_t pairs = a.T * a.Hkv * a.d / 2;
+    hipLaunchKernelGGL(packed_sum_kernel<T>, dim3(static_cast<unsigned>((pairs + 255) / 256)), dim3(256), 0,
+                       s, a);
+  }
 }
 template <typename T>
 static void launch_packed_bwd_t(const PackedArgs& a, bool ragged, hipStream_t s) {
@@ -465,8 +540,11 @@ static void launch_packed_bwd_t(const PackedArgs& a, bool ragged, hipStream_t s)
 using namespace zk;
 
 extern "C" int64_t zk_attn_packed_bwd_workspace(const zk_packed_desc* desc) {
-  if (desc == nullptr || desc->T < 0 || desc->Hq < 0) return 0;
-  return 2 * ((desc->Hq * desc->T + 63) / 64 * 64) * 4 + 256;
+  if (desc == nullptr || desc->T < 0 || desc->Hq <= 0 || desc->Hkv <= 0 || desc->Hq % desc->Hkv != 0)
+    return 0;
+  const int parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window, desc->dtype);
+  const int64_t sums = parts > 1 ? 2 * parts * desc->T * desc->Hkv * desc->d : 0;
+  return (2 * ((desc->Hq * desc->T + 63) / 64 * 64) + sums) * 4 + 256;
 }
 
 extern "C" int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, const void* k,
@@ -489,6 +567,9 @@ extern "C" int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, con
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.delta = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   a.lse2 = a.delta + (desc->Hq * desc->T + 63) / 64 * 64;
+  a.parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window, desc->dtype);
+  a.dk_part = a.lse2 + (desc->Hq * desc->T + 63) / 64 * 64;
+  a.dv_part = a.dk_part + a.parts * desc->T * desc->Hkv * desc->d;
   hipStream_t s = as_stream(stream);
   if (desc->dtype == ZK_F32)
     launch_packed_bwd_f32(a, s);

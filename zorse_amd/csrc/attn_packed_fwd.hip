@@ -71,12 +71,18 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int64_t T, int32_t* 
 }
 
 // ---------------------------------------------------------------- forward --
-// NW waves of 32 queries, whose Q rows stay in registers; 64-key tiles of K and V
-// in LDS, row-major with swizzled 16-byte chunks.  Scores are computed transposed
-// (S^T = K Q^T): a lane holds one query's scores of 32 keys, so the softmax is per
-// lane with one exchange between the wave's halves, and the probabilities are the
-// next product's operand as they are (O^T += V^T P^T, V^T by transposed reads).
+// 128 queries of one head, 32 a wave, whose Q rows stay in registers; 64-key tiles of
+// K and V in LDS, row-major with swizzled 16-byte chunks.  Scores are computed
+// transposed (S^T = K Q^T): a lane holds one query's scores of 32 keys, so the softmax
+// is per lane with one exchange between the wave's halves, and the probabilities are
+// the next product's operand as they are (O^T += V^T P^T, V^T by transposed reads).
 // The reference maximum moves when a score exceeds it by 2^8 only.
+//
+// Four waves, so that two workgroups share a CU (four at d 64): the one's loads of Q,
+// first tiles and stores lie beside the other's products.  Eight waves and 256 queries
+// are 3 % faster for one sequence of 8192 tokens (505 us against 520, 32 heads of
+// 128: 1060 TFLOP/s) and 37 % slower for documents of 128 tokens (41 us for 4096
+// tokens against 30, where the tensors' own bytes take 27).
 static constexpr float kGrowth = 8.0f;  // in the exp2 domain
 
 // Orders the compiler's memory accesses and waits for the other waves, but not for
@@ -89,23 +95,27 @@ __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// kPhases (8 waves): the softmax of a 64-key tile takes a wave about as long on the
-// vector units as its two products take on the matrix units, but waves that run in
-// step do the same thing at the same time.  Waves 0-3 (one on each SIMD) and 4-7
-// therefore alternate: while one group multiplies (the scores of tile t and P V of
-// tile t - 1), the other one is at the softmax of a tile, with a barrier between
-// the phases.  Tile t + 1 of K and t of V are loaded over two phases.
+// kSplit: two groups of four waves take every other tile of the same queries and join
+// their sums at the end, for launches of so few blocks that they wait for the one with
+// the most tiles (8 heads of 4096 causal tokens 60 us against 80).
+// The groups alternate: the softmax of a tile takes a wave about as long on the vector
+// units as its two products take on the matrix units, and waves that run in step do the
+// same thing at the same time; so while one group multiplies (P V of its last tile and
+// the scores of the next one) the other one is at its softmax, with a barrier between
+// the phases.
 // KR: 0 for a head dim of D and 16-byte aligned heads, else ceil(d / 16), at least 2.
-template <typename T, int D, int NW, int KR, bool kPhases>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+template <typename T, int D, int KR, bool kSplit>
+__global__ __launch_bounds__(kSplit ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2)))
 void packed_fwd_kernel(PackedArgs a) {
   typedef Mfma<T> M;
   typedef typename M::vec8 V8;
-  constexpr int BM = 32 * NW, BN = 64, NT = 64 * NW;
-  constexpr int PF = 4;  // operand reads in flight
+  constexpr int QW = 4, NW = kSplit ? 2 * QW : QW;
+  constexpr int BM = 32 * QW, BN = 64, NT = 64 * NW;
+  constexpr int TN = kSplit ? 2 * BN : BN;  // keys of a step
+  constexpr int PF = 4;                     // operand reads in flight
   constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
   const int hd = KR ? a.d : D;
-  __shared__ __attribute__((aligned(16))) T K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+  __shared__ __attribute__((aligned(16))) T K0[TN * D], K1[TN * D], V0[TN * D], V1[TN * D];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -116,7 +126,8 @@ void packed_fwd_kernel(PackedArgs a) {
   const int rows = static_cast<int>(a.T);
   if (q0 >= rows) return;
   const int hk = hq / (a.Hq / a.Hkv);
-  const int qw0 = q0 + 32 * wave;
+  const int qw0 = q0 + 32 * (wave % QW);
+  const int k_off = kSplit ? wave / QW * BN : 0;  // this wave's keys in a step
   const int my_q = qw0 + l32;
   const bool in = my_q < rows;
 
@@ -147,19 +158,19 @@ void packed_fwd_kernel(PackedArgs a) {
   V8 qreg[KS];
   load_operand<T, KS, KR>(qreg, in ? Qp + my_q * a.q_s : nullptr, g, hd);
 
-  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + BN - 1) / BN : 0;
-  PackedLoader<T, D, BN, NT> kload, vload;
+  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + TN - 1) / TN : 0;
+  PackedLoader<T, D, TN, NT> kload, vload;
   kload.init(a.k_s, hd);
   vload.init(a.v_s, hd);
   auto issue_k = [&](int t, int st) {
-    kload.issue(st ? K1 : K0, Kp, a.k_s, kv_lo + t * BN, plan.n);
+    kload.issue(st ? K1 : K0, Kp, a.k_s, kv_lo + t * TN, plan.n);
   };
   auto issue_v = [&](int t, int st) {
-    vload.issue(st ? V1 : V0, Vp, a.v_s, kv_lo + t * BN, plan.n);
+    vload.issue(st ? V1 : V0, Vp, a.v_s, kv_lo + t * TN, plan.n);
   };
   // LDS byte offsets from two per-lane bases (the swizzle XORs chunk indices)
-  const int rbase = 2 * tile_off<D>(l32, 8 * g);
-  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+  const int rbase = 2 * (tile_off<D>(l32, 8 * g) + k_off * D);
+  const int tbase = 2 * (tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) + k_off * D);
 
   f32x16 o[NB], s[BN / 32];
   V8 pb[BN / 16];
@@ -169,14 +180,14 @@ void packed_fwd_kernel(PackedArgs a) {
   const float c2 = a.scale_log2;
 
   auto skipped = [&](int t) __attribute__((always_inline)) {
-    const int k0 = kv_lo + t * BN;
+    const int k0 = kv_lo + t * TN + k_off;
     return idle || t < 0 || t >= n_t || k0 > w_hi || k0 + BN <= w_lo;
   };
   // S^T = K Q^T of tile t, which starts from -inf where a key is not seen
   auto scores = [&](const T* Kt, int t) __attribute__((always_inline)) {
     int rb = rbase;  // opaque: addresses derived here
     asm volatile("" : "+v"(rb));
-    const int k0 = kv_lo + t * BN;
+    const int k0 = kv_lo + t * TN + k_off;
     const bool need_mask = k0 < f_lo || k0 + BN - 1 > f_hi;
     // operands are read PF products ahead; the fences keep the reads there (left
     // alone, the compiler reads all of them first and has no registers left)
@@ -289,7 +300,7 @@ void packed_fwd_kernel(PackedArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  if constexpr (kPhases) {
+  if constexpr (kSplit) {
     // Tiles outside a wave's range are not left out here: it would wait for the
     // others at the next barrier all the same, and branches around what lives from
     // one phase to the next cost registers.  par: t % 2.
@@ -345,7 +356,7 @@ void packed_fwd_kernel(PackedArgs a) {
     };
     if (n_t > 0) {
       issue_k(0, 0);
-      if (wave < NW / 2)
+      if (wave < QW)
         run(std::false_type{});
       else
         run(std::true_type{});
@@ -374,6 +385,34 @@ void packed_fwd_kernel(PackedArgs a) {
     }
   }
 
+  if constexpr (kSplit) {
+    // the second group's maximum, sum and O to the first, through the tiles' memory
+    const int slot = threadIdx.x & (64 * QW - 1);
+    float* ml = reinterpret_cast<float*>(V0);
+    auto at = [&](int nt, int j) __attribute__((always_inline)) {
+      return reinterpret_cast<float*>(nt < 2 ? K0 : K1) + ((nt & 1) * 16 + j) * (64 * QW) + slot;
+    };
+    __syncthreads();  // every wave is past its last product
+    if (wave >= QW) {
+      ml[slot] = m_ref;
+      ml[64 * QW + slot] = l_i;
+#pragma unroll
+      for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) *at(nt, j) = o[nt][j];
+    }
+    __syncthreads();
+    if (wave >= QW) return;
+    const float m2 = ml[slot], m_new = fmaxf(m_ref, m2);
+    const float f1 = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_ref - m_new) * c2);
+    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - m_new) * c2);
+    m_ref = m_new;
+    l_i = l_i * f1 + ml[64 * QW + slot] * f2;
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[nt][j] = o[nt][j] * f1 + *at(nt, j) * f2;
+  }
   const float l_tot = l_i + other_half(l_i);
   // no weight although keys are visible: every score is -inf or NaN, and so is O
   const float inv = l_tot > 0.f ? 1.0f / l_tot : any_key ? NAN : 0.f;
@@ -506,28 +545,30 @@ extern "C" int zk_packed_plan(const void* offsets, int offsets_64, int64_t n_seq
 }
 
 namespace zk {
-template <typename T, int D, int NW, int KR>
+template <typename T, int D, int KR>
 static void launch_packed_fwd(const PackedArgs& a, hipStream_t s) {
-  const int64_t blocks = packed_blocks(a.T, 32 * NW);
-  hipLaunchKernelGGL((packed_fwd_kernel<T, D, NW, KR, NW == 8>), dim3(static_cast<unsigned>(blocks * a.Hq)),
-                     dim3(64 * NW), 0, s, a);
+  const int64_t n = packed_blocks(a.T, 128) * a.Hq;
+  if (n <= device_cus())
+    hipLaunchKernelGGL((packed_fwd_kernel<T, D, KR, true>), dim3(static_cast<unsigned>(n)), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((packed_fwd_kernel<T, D, KR, false>), dim3(static_cast<unsigned>(n)), dim3(256), 0, s, a);
 }
 template <typename T>
 static void launch_packed_fwd_t(const PackedArgs& a, bool ragged, hipStream_t s) {
   if (!ragged) {
-    if (a.d == 128) launch_packed_fwd<T, 128, 8, 0>(a, s);
-    else launch_packed_fwd<T, 64, 4, 0>(a, s);
+    if (a.d == 128) launch_packed_fwd<T, 128, 0>(a, s);
+    else launch_packed_fwd<T, 64, 0>(a, s);
     return;
   }
   switch ((a.d + 15) / 16) {
     case 1:
-    case 2: launch_packed_fwd<T, 64, 4, 2>(a, s); break;
-    case 3: launch_packed_fwd<T, 64, 4, 3>(a, s); break;
-    case 4: launch_packed_fwd<T, 64, 4, 4>(a, s); break;
-    case 5: launch_packed_fwd<T, 128, 8, 5>(a, s); break;
-    case 6: launch_packed_fwd<T, 128, 8, 6>(a, s); break;
-    case 7: launch_packed_fwd<T, 128, 8, 7>(a, s); break;
-    default: launch_packed_fwd<T, 128, 8, 8>(a, s); break;
+    case 2: launch_packed_fwd<T, 64, 2>(a, s); break;
+    case 3: launch_packed_fwd<T, 64, 3>(a, s); break;
+    case 4: launch_packed_fwd<T, 64, 4>(a, s); break;
+    case 5: launch_packed_fwd<T, 128, 5>(a, s); break;
+    case 6: launch_packed_fwd<T, 128, 6>(a, s); break;
+    case 7: launch_packed_fwd<T, 128, 7>(a, s); break;
+    default: launch_packed_fwd<T, 128, 8>(a, s); break;
   }
 }
 }  // namespace zk
