@@ -270,17 +270,36 @@ struct Sides {
 };
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// Tiles of a run of matrices: the 256 x 256 pipeline where its tiles fill most of
-// the CUs, else 128 x 128, else 64 x 64.
-gemm::Tile tile_of(const Sides* x, int n) {
+// Tiles of one product of a run of matrices (`square`: of its two symmetric ones,
+// whose tiles above the diagonal alone are computed).
+//  * 256 x 256 where the 128 x 128 tiles would not fit on the CUs at once, two to
+//    each: 2048 x 5632 772 us a matrix against 818, but two of 2048 x 2048 684
+//    against 639, whose X has 512 of the smaller tiles.  Not where sides far from
+//    multiples of 256 make padding of a twentieth of it (five odd matrices of 546 to
+//    2748 485 us against 416).
+//  * else 128 x 128 where that ends sooner than 64 x 64.  Steps along K: a tile of
+//    128 rows takes one step's time alone on its CU, one of 64 half a step's when
+//    several share a CU.  So few tiles, or some with a far longer K than the others',
+//    are cut small: 1024 x 4096 293 us against 427, two 414 against 496; but one of
+//    2048 x 2048 459 against 496, four of 512 x 2048 217 against 232 (X).
+gemm::Tile tile_of(const Sides* x, int n, bool square) {
   if (x[0].exact) return gemm::k64;
-  int64_t n256 = 0, n128 = 0;
+  int64_t tiles256 = 0, tiles128 = 0, steps128 = 0, steps64 = 0, longest = 0;
   for (int i = 0; i < n; ++i) {
-    n256 += gemm::tile_count(gemm::k256, x[i].s, x[i].t);
-    n128 += gemm::tile_count(gemm::k128, x[i].s, x[i].t);
+    const auto count = [&](gemm::Tile t) {
+      const int64_t rows = (x[i].s + gemm::tile_rows(t) - 1) / gemm::tile_rows(t);
+      return square ? rows * (rows + 1) / 2 : gemm::tile_count(t, x[i].s, x[i].t);
+    };
+    const int64_t k = square ? x[i].t : x[i].s;
+    tiles256 += count(gemm::k256);
+    tiles128 += count(gemm::k128);
+    steps128 += count(gemm::k128) * k;
+    steps64 += count(gemm::k64) * k;
+    longest = std::max(longest, k);
   }
-  if (n256 >= 160) return gemm::k256;
-  return n128 >= 200 ? gemm::k128 : gemm::k64;
+  const int64_t cus = device_cus();
+  if (tiles128 > 2 * cus && 80 * tiles256 <= 21 * tiles128) return gemm::k256;
+  return std::max(longest * cus, steps128) < steps64 / 2 ? gemm::k128 : gemm::k64;
 }
 
 Sides sides_of(const zk_muon_matrix& x) {
@@ -304,15 +323,13 @@ int64_t bytes_of(const Sides& d) {
   return up(4 * x + (d.exact ? 4 : 2) * square + kPartials * 8, 256);
 }
 
-gemm::Tile plan_run(const zk_muon_matrix* list, int n, Sides* d) {
+void plan_run(const zk_muon_matrix* list, int n, Sides* d) {
   for (int i = 0; i < n; ++i) d[i] = sides_of(list[i]);
-  const gemm::Tile t = tile_of(d, n);
-  const int64_t to = t == gemm::k256 ? 256 : 64;
+  const bool wide = tile_of(d, n, true) == gemm::k256 || tile_of(d, n, false) == gemm::k256;
   for (int i = 0; i < n; ++i) {
-    d[i].sp = up(d[i].s, to);
-    d[i].tp = up(d[i].t, to);
+    d[i].sp = up(d[i].s, wide ? 256 : 64);
+    d[i].tp = up(d[i].t, wide ? 256 : 64);
   }
-  return t;
 }
 
 // Bounds of the polynomial's iterates on [0, 1]: the powers of two that S^2 G and
@@ -383,7 +400,8 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
   for (int64_t at = 0; at < n;) {
     Sides d[gemm::kPolyMost];
     const int len = run_length(list + at, n - at);
-    const gemm::Tile tile = plan_run(list + at, len, d);
+    plan_run(list + at, len, d);
+    const gemm::Tile tile_square = tile_of(d, len, true), tile_x = tile_of(d, len, false);
     char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
     MatrixGroup m = {};
     f16 *hi[2][gemm::kPolyMost], *lo[2][gemm::kPolyMost], *G[2][gemm::kPolyMost], *P[2][gemm::kPolyMost];
@@ -438,6 +456,7 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
     std::stable_sort(by_length, by_length + len, [&](int a, int b) { return d[a].tp > d[b].tp; });
     // product `which` of step k: 0 G, 1 P, 2 X
     auto product = [&](int k, int which) {
+      const gemm::Tile tile = which == 2 ? tile_x : tile_square;
       gemm::PolyGroup g = {};
       g.n = len;
       for (int n = 0; n < len; ++n) {
