@@ -12,16 +12,16 @@ namespace {
 
 constexpr int kTile = 32;  // rows per LDS tile
 
-// Rows r0 .. r0 + 31 (of `rows`) of a [.., d] tensor, D / 8 floats per
-// thread: load() issues the global loads, store() writes the LDS tile.
-template <int D, bool kVec>
+// Rows r0 .. r0 + ROWS - 1 (of `rows`) of a [.., d] tensor, spread over THREADS:
+// load() issues the global loads, store() writes the LDS tile.
+template <int D, bool kVec, int ROWS = kTile, int THREADS = 256>
 struct TileReg {
-  static constexpr int NC = kTile * D / 4 / 256;  // 4-float chunks per thread
+  static constexpr int NC = ROWS * D / 4 / THREADS;  // 4-float chunks per thread
   float4 v[NC];
   __device__ __forceinline__ void load(const float* base, int64_t ld, int64_t r0, int64_t rows, int d) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int id = i * 256 + static_cast<int>(threadIdx.x);
+      const int id = i * THREADS + static_cast<int>(threadIdx.x);
       const int r = id / (D / 4), c = 4 * (id % (D / 4));
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r0 + r < rows && c < d) {
@@ -43,7 +43,7 @@ struct TileReg {
     float z = 0.f;  // stays 0 for finite values, else NaN
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int id = i * 256 + static_cast<int>(threadIdx.x);
+      const int id = i * THREADS + static_cast<int>(threadIdx.x);
       *reinterpret_cast<float4*>(&tile[(id / (D / 4)) * (D + 4) + 4 * (id % (D / 4))]) = v[i];
       z += 0.f * v[i].x + 0.f * v[i].y + 0.f * v[i].z + 0.f * v[i].w;
     }
@@ -135,14 +135,15 @@ __device__ __forceinline__ float group_max(float x) {
   return fmaxf(x, __shfl_xor(x, 32, 64));
 }
 
-// This lane's accumulators (elements 16 nt + 4 q4 + e of its row), scaled, to
-// the row at dst.
-template <int D, bool kVec>
-__device__ __forceinline__ void store_row(float* dst, const f32x4 (&x)[D / 16], float scale, int d) {
+// This lane's accumulators (elements 16 (nt0 + nt) + 4 q4 + e of its row), scaled,
+// to the row at dst.
+template <int D, bool kVec, int N = D / 16>
+__device__ __forceinline__ void store_row(float* dst, const f32x4 (&x)[N], float scale, int d,
+                                          int nt0 = 0) {
   const int q4 = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int nt = 0; nt < D / 16; ++nt) {
-    const int e0 = 16 * nt + 4 * q4;
+  for (int nt = 0; nt < N; ++nt) {
+    const int e0 = 16 * (nt0 + nt) + 4 * q4;
     if (kVec) {
       if (e0 < d)
         *reinterpret_cast<float4*>(dst + e0) = make_float4(x[nt][0] * scale, x[nt][1] * scale,

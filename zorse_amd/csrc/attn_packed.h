@@ -13,9 +13,8 @@
 //   [16 ..]        start[T], end[T]: a token's sequence; tokens from n on have
 //                  start = end = their own index, so they see and are seen by
 //                  nothing
-//   then           orders of blocks, most work first: blocks of 256 and of 128
-//                  rows for kernels that own queries, of 128 for those that own
-//                  keys
+//   then           two orders of the blocks of 128 rows, most work first: for
+//                  kernels that own queries, and for those that own keys
 #pragma once
 #include "attn_common.h"
 
@@ -23,11 +22,11 @@ namespace zk {
 
 constexpr int kPlanHeader = 16;
 
-// Words before order `which` (0: 256 queries, 1: 128 queries, 2: 128 keys; 3: of
-// the whole plan).
+constexpr int kPlanRows = 128;  // rows of a listed block
+
+// Words before order `which` (0: of queries, 1: of keys; 2: of the whole plan).
 __host__ __device__ inline int64_t plan_order_at(int64_t T, int which) {
-  const int64_t n256 = (T + 255) / 256, n128 = (T + 127) / 128;
-  return kPlanHeader + 2 * T + (which > 0 ? n256 : 0) + (which > 1 ? n128 : 0) + (which > 2 ? n128 : 0);
+  return kPlanHeader + 2 * T + which * ((T + kPlanRows - 1) / kPlanRows);
 }
 
 struct PackedArgs {
@@ -68,13 +67,13 @@ struct PackedPlan {
     start = a.plan + kPlanHeader;
     end = start + a.T;
   }
-  // first row of the block of ROWS (up to 256) in the order of launch
+  // first row of a block of ROWS, a divisor of the listed blocks' rows, in the order
+  // of launch
   template <int ROWS, bool kKeys>
   __device__ __forceinline__ int first_row(const PackedArgs& a, int block) const {
-    static_assert(ROWS <= 128 || (ROWS == 256 && !kKeys), "block size");
-    constexpr int LISTED = ROWS > 128 ? 256 : 128, PER = LISTED / ROWS;
-    const int32_t* order = a.plan + plan_order_at(a.T, kKeys ? 2 : ROWS > 128 ? 0 : 1);
-    return order[block / PER] * LISTED + (block % PER) * ROWS;
+    constexpr int PER = kPlanRows / ROWS;
+    const int32_t* order = a.plan + plan_order_at(a.T, kKeys);
+    return order[block / PER] * kPlanRows + (block % PER) * ROWS;
   }
   // keys that query i sees: [key_lo, key_hi]
   __device__ __forceinline__ int key_lo(const PackedArgs& a, int i) const {
@@ -102,8 +101,7 @@ void launch_packed_bwd_f32(const PackedArgs& a, hipStream_t s);
 
 // Workgroups for blocks of `rows` rows of T: whole listed blocks.
 __host__ __device__ inline int64_t packed_blocks(int64_t T, int rows) {
-  const int listed = rows > 128 ? 256 : 128;
-  return (T + listed - 1) / listed * (listed / rows);
+  return (T + kPlanRows - 1) / kPlanRows * (kPlanRows / rows);
 }
 
 // Head of a block in the order of launch: the workgroups of one XCD (dispatch

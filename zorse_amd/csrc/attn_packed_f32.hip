@@ -1,7 +1,19 @@
-// Attention over packed sequences for fp32 layers, on the fp32 matrix cores; the
-// arrangement is that of attn_f32.hip with the ranges of attn_packed.h.  4 waves of
-// 16 rows, 32-row tiles of the other side.  Products and sums are fp32; a tile that
-// holds an infinity or a NaN is added row by row, masked rows left out.
+// Attention over packed sequences for fp32 layers, on the fp32 matrix cores (the
+// operands' lanes are those of attn_f32.hip), with the ranges of attn_packed.h.  A wave
+// owns 16 rows and meets the other side in LDS tiles.  Two shapes:
+//  * Whole: 64 rows a workgroup, 4 waves, each meets whole tiles of 32 rows.
+//  * Split: 32 rows, 8 waves; the four waves of 16 rows take 16 rows each of tiles of
+//    64, and their partial sums are joined through LDS at the end.
+//   Bound by the matrix instructions (a 16 x 16 x 4 product takes its SIMD 32 cycles),
+// and where a launch has few workgroups by those of the one with the most tiles, of
+// which Split does a quarter at a time.  So Split up to two of Whole's workgroups a CU
+// (head dim 64, causal, forward and backward in us, Whole against Split: 1024 tokens,
+// 8 heads 78 + 357 against 42 + 153; 2048, 16 heads 180 + 526 against 135 + 414, but in
+// sequences of 200 31 + 86 against 31 + 104), Whole past it (4096 tokens, 16 heads of
+// 128: 811 + 2570, 67 - 85 TFLOP/s of the 157 that the matrix cores have in fp32;
+// Split 991 + 2970).
+//   Products and sums are fp32; a tile that holds an infinity or a NaN is added row by
+// row, masked rows left out.
 #include "attn_f32.h"
 #include "attn_packed.h"
 
@@ -9,37 +21,74 @@ namespace zk {
 
 namespace {
 
-constexpr int kRows = 64;  // rows per workgroup
+// SETS sets of 16 rows, SLICES waves to each, PIECES times 16 rows of a tile a wave.
+template <int SETS, int SLICES, int PIECES>
+struct Shape {
+  static constexpr int sets = SETS, slices = SLICES, pieces = PIECES;
+  static constexpr int rows = 16 * SETS, tile = 16 * SLICES * PIECES, threads = 64 * SETS * SLICES;
+};
+typedef Shape<4, 1, 2> Whole;
+typedef Shape<2, 4, 1> Split;
+
+// Sums acc over the waves of a row set; a wave is left with its share of the columns,
+// N times 16 from N times its slice on.
+// `lds`: two tiles of rows of D + 4 floats that no wave reads any more.
+template <typename G, int D, int N = D / 16 / G::slices>
+__device__ __forceinline__ void join(f32x4 (&sum)[N], const f32x4 (&acc)[D / 16], float* lds, int set,
+                                     int slice) {
+  constexpr int SLICE = G::sets * (D / 16) * 64;
+  static_assert(G::slices == 1 || G::threads * (D / 4) <= 2 * G::tile * (D + 4),
+                "the sums do not fit in the tiles");
+  if constexpr (G::slices == 1) {
+#pragma unroll
+    for (int nt = 0; nt < N; ++nt) sum[nt] = acc[nt];
+  } else {
+    f32x4* const all = reinterpret_cast<f32x4*>(lds) + set * (D / 16) * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int nt = 0; nt < D / 16; ++nt) all[slice * SLICE + nt * 64] = acc[nt];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      f32x4 x = all[(slice * N + j) * 64];
+#pragma unroll
+      for (int i = 1; i < G::slices; ++i) x += all[i * SLICE + (slice * N + j) * 64];
+      sum[j] = x;
+    }
+  }
+}
 
 // The workgroup's block and head; whether there is such a block.
-template <bool kKeys>
+template <typename G, bool kKeys>
 __device__ __forceinline__ bool block_of(const PackedArgs& a, const PackedPlan& plan, int& r0, int& h) {
   const int64_t bid = group_id();
   const int H = kKeys ? a.Hkv : a.Hq;
-  if (bid >= packed_blocks(a.T, kRows) * H) return false;
+  if (bid >= packed_blocks(a.T, G::rows) * H) return false;
   h = static_cast<int>(bid % H);
-  r0 = plan.first_row<kRows, kKeys>(a, static_cast<int>(bid / H));
+  r0 = plan.first_row<G::rows, kKeys>(a, static_cast<int>(bid / H));
   return r0 < a.T;
 }
 
-// Tokens [lo, hi) that rows r0 .. r0 + kRows - 1 meet.
-template <bool kKeys>
+// Tokens [lo, hi) that rows r0 .. r0 + G::rows - 1 meet.
+template <typename G, bool kKeys>
 __device__ __forceinline__ void tokens_of(const PackedArgs& a, const PackedPlan& plan, int r0, int& lo,
                                           int& hi) {
-  const int past = r0 + kRows < a.T ? r0 + kRows : static_cast<int>(a.T);
+  const int past = r0 + G::rows < a.T ? r0 + G::rows : static_cast<int>(a.T);
   lo = kKeys ? plan.query_lo(a, r0) : plan.key_lo(a, r0);
   hi = (kKeys ? plan.query_hi(a, past - 1) : plan.key_hi(a, past - 1)) + 1;
   if (hi > plan.n) hi = plan.n;
 }
 
-template <int D, bool kVec>
-__global__ __launch_bounds__(256) void packed_fwd_f32(PackedArgs a) {
-  __shared__ __attribute__((aligned(16))) float Ks[kTile * (D + 4)], Vs[kTile * (D + 4)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
+template <typename G, int D, bool kVec>
+__global__ __launch_bounds__(G::threads, D > 64 ? 2 : G::slices > 1 ? 4 : 3) void packed_fwd_f32(PackedArgs a) {
+  __shared__ __attribute__((aligned(16))) float tiles[2 * G::tile * (D + 4)];
+  float *const Ks = tiles, *const Vs = tiles + G::tile * (D + 4);
+  __shared__ float ms[G::slices][G::rows], ls[G::slices][G::rows];
+  const int lane = threadIdx.x & 63, set = (threadIdx.x >> 6) % G::sets, l16 = lane & 15, q4 = lane >> 4;
+  const int slice = threadIdx.x / (64 * G::sets), at = 16 * G::pieces * slice;
   const PackedPlan plan(a);
   int q0, hq;
-  if (!block_of<false>(a, plan, q0, hq)) return;
-  const int hk = hq / (a.Hq / a.Hkv), my_q = q0 + 16 * wave + l16, d = a.d;
+  if (!block_of<G, false>(a, plan, q0, hq)) return;
+  const int hk = hq / (a.Hq / a.Hkv), my_q = q0 + 16 * set + l16, d = a.d;
   const bool in = my_q < a.T;
   const float* K = static_cast<const float*>(a.k) + hk * a.k_h;
   const float* V = static_cast<const float*>(a.v) + hk * a.v_h;
@@ -51,31 +100,32 @@ __global__ __launch_bounds__(256) void packed_fwd_f32(PackedArgs a) {
   for (int nt = 0; nt < D / 16; ++nt) o[nt] = f32x4{};
   float m = -INFINITY, l = 0.f;
   int lo, hi;
-  tokens_of<false>(a, plan, q0, lo, hi);
-  TileReg<D, kVec> kr, vr;
+  tokens_of<G, false>(a, plan, q0, lo, hi);
+  TileReg<D, kVec, G::tile, G::threads> kr, vr;
   if (lo < hi) {
     kr.load(K, a.k_s, lo, plan.n, d);
     vr.load(V, a.v_s, lo, plan.n, d);
   }
-  for (int k0 = lo; k0 < hi; k0 += kTile) {
+  for (int k0 = lo; k0 < hi; k0 += G::tile) {
     __syncthreads();  // the previous tile's reads are done
     kr.store(Ks);
     const bool odd = __syncthreads_or(vr.store(Vs));
     auto visible = [&](int r) __attribute__((always_inline)) {
       return k0 + r >= my_lo && k0 + r <= my_hi;
     };
-    if (k0 + kTile < hi) {
-      kr.load(K, a.k_s, k0 + kTile, plan.n, d);
-      vr.load(V, a.v_s, k0 + kTile, plan.n, d);
+    if (k0 + G::tile < hi) {
+      kr.load(K, a.k_s, k0 + G::tile, plan.n, d);
+      vr.load(V, a.v_s, k0 + G::tile, plan.n, d);
     }
-    f32x4 s[2];
+    if (!__any(my_lo < k0 + at + 16 * G::pieces && my_hi >= k0 + at)) continue;
+    f32x4 s[G::pieces];
     float mloc = -INFINITY;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] = dot_rows<D>(Ks, 16 * h, q);
+    for (int h = 0; h < G::pieces; ++h) {
+      s[h] = dot_rows<D>(Ks, at + 16 * h, q);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[h][e] = visible(16 * h + 4 * q4 + e) ? s[h][e] * a.scale : -INFINITY;
+        s[h][e] = visible(at + 16 * h + 4 * q4 + e) ? s[h][e] * a.scale : -INFINITY;
         mloc = fmaxf(mloc, s[h][e]);
       }
     }
@@ -87,37 +137,57 @@ __global__ __launch_bounds__(256) void packed_fwd_f32(PackedArgs a) {
 #pragma unroll
     for (int nt = 0; nt < D / 16; ++nt) o[nt] *= alpha;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < G::pieces; ++h) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[h][e] = expf(s[h][e] - ref);
         l += s[h][e];
       }
       if (odd)
-        add_rows_visible<D>(o, Vs, 16 * h, s[h], visible);
+        add_rows_visible<D>(o, Vs, at + 16 * h, s[h], visible);
       else
-        add_rows<D>(o, Vs, 16 * h, s[h]);
+        add_rows<D>(o, Vs, at + 16 * h, s[h]);
     }
   }
   l = group_sum(l);
+  if constexpr (G::slices > 1) {  // the row's maximum and sum over the slices
+    if (q4 == 0) {
+      ms[slice][16 * set + l16] = m;
+      ls[slice][16 * set + l16] = l;
+    }
+    __syncthreads();
+    const float mine = m;
+#pragma unroll
+    for (int i = 0; i < G::slices; ++i) m = fmaxf(m, ms[i][16 * set + l16]);
+    const float ref = m == -INFINITY ? 0.f : m, alpha = expf(mine - ref);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < G::slices; ++i) l += ls[i][16 * set + l16] * expf(ms[i][16 * set + l16] - ref);
+#pragma unroll
+    for (int nt = 0; nt < D / 16; ++nt) o[nt] *= alpha;
+  }
+  f32x4 out[D / 16 / G::slices];
+  join<G, D>(out, o, tiles, set, slice);
   if (!in || (my_q >= plan.n && a.keep_tail)) return;
   const bool any_key = my_hi >= my_lo;
   // no weight although keys are visible: every score is -inf or NaN, and so is O
-  store_row<D, kVec>(static_cast<float*>(a.out) + hq * a.o_h + my_q * a.o_s, o,
-                     l > 0.f ? 1.0f / l : any_key ? NAN : 0.f, d);
-  if (q4 == 0)
+  store_row<D, kVec>(static_cast<float*>(a.out) + hq * a.o_h + my_q * a.o_s, out,
+                     l > 0.f ? 1.0f / l : any_key ? NAN : 0.f, d, slice * (D / 16 / G::slices));
+  if (slice == 0 && q4 == 0)
     a.lse_out[static_cast<int64_t>(hq) * a.T + my_q] = l > 0.f ? m + logf(l) : any_key ? NAN : -INFINITY;
 }
 
 // dQ, and delta = rowsum(dO o O) and the LSE for the dK / dV kernel that follows.
-template <int D, bool kVec>
-__global__ __launch_bounds__(256) void packed_dq_f32(PackedArgs a) {
-  __shared__ __attribute__((aligned(16))) float Ks[kTile * (D + 4)], Vs[kTile * (D + 4)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
+template <typename G, int D, bool kVec>
+__global__ __launch_bounds__(G::threads, D > 64 || G::slices > 1 ? 2 : 3) void packed_dq_f32(PackedArgs a) {
+  __shared__ __attribute__((aligned(16))) float tiles[2 * G::tile * (D + 4)];
+  float *const Ks = tiles, *const Vs = tiles + G::tile * (D + 4);
+  const int lane = threadIdx.x & 63, set = (threadIdx.x >> 6) % G::sets, l16 = lane & 15, q4 = lane >> 4;
+  const int slice = threadIdx.x / (64 * G::sets), at = 16 * G::pieces * slice;
   const PackedPlan plan(a);
   int q0, hq;
-  if (!block_of<false>(a, plan, q0, hq)) return;
-  const int hk = hq / (a.Hq / a.Hkv), my_q = q0 + 16 * wave + l16, d = a.d;
+  if (!block_of<G, false>(a, plan, q0, hq)) return;
+  const int hk = hq / (a.Hq / a.Hkv), my_q = q0 + 16 * set + l16, d = a.d;
   const bool in = my_q < a.T;
   const float* K = static_cast<const float*>(a.k) + hk * a.k_h;
   const float* V = static_cast<const float*>(a.v) + hk * a.v_h;
@@ -140,7 +210,7 @@ __global__ __launch_bounds__(256) void packed_dq_f32(PackedArgs a) {
     if (in) {
       const int64_t i = static_cast<int64_t>(hq) * a.T + my_q;
       lse = my_q < plan.n ? a.lse[i] : -INFINITY;
-      if (q4 == 0) {
+      if (slice == 0 && q4 == 0) {
         a.delta[i] = del;
         a.lse2[i] = lse;
       }
@@ -150,50 +220,57 @@ __global__ __launch_bounds__(256) void packed_dq_f32(PackedArgs a) {
 #pragma unroll
   for (int nt = 0; nt < D / 16; ++nt) dq[nt] = f32x4{};
   int lo, hi;
-  tokens_of<false>(a, plan, q0, lo, hi);
-  TileReg<D, kVec> kr, vr;
+  tokens_of<G, false>(a, plan, q0, lo, hi);
+  TileReg<D, kVec, G::tile, G::threads> kr, vr;
   if (lo < hi) {
     kr.load(K, a.k_s, lo, plan.n, d);
     vr.load(V, a.v_s, lo, plan.n, d);
   }
-  for (int k0 = lo; k0 < hi; k0 += kTile) {
+  for (int k0 = lo; k0 < hi; k0 += G::tile) {
     __syncthreads();
     vr.store(Vs);
     const bool odd = __syncthreads_or(kr.store(Ks));
     auto visible = [&](int r) __attribute__((always_inline)) {
       return k0 + r >= my_lo && k0 + r <= my_hi;
     };
-    if (k0 + kTile < hi) {
-      kr.load(K, a.k_s, k0 + kTile, plan.n, d);
-      vr.load(V, a.v_s, k0 + kTile, plan.n, d);
+    if (k0 + G::tile < hi) {
+      kr.load(K, a.k_s, k0 + G::tile, plan.n, d);
+      vr.load(V, a.v_s, k0 + G::tile, plan.n, d);
     }
+    if (!__any(my_lo < k0 + at + 16 * G::pieces && my_hi >= k0 + at)) continue;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 s = dot_rows<D>(Ks, 16 * h, q);
-      const f32x4 dp = dot_rows<D>(Vs, 16 * h, g);
+    for (int r = at; r < at + 16 * G::pieces; r += 16) {
+      f32x4 s = dot_rows<D>(Ks, r, q);
+      const f32x4 dp = dot_rows<D>(Vs, r, g);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        s[e] = visible(16 * h + 4 * q4 + e) ? expf(s[e] * a.scale - lse) * (dp[e] - del) : 0.f;
+        s[e] = visible(r + 4 * q4 + e) ? expf(s[e] * a.scale - lse) * (dp[e] - del) : 0.f;
       if (odd)
-        add_rows_visible<D>(dq, Ks, 16 * h, s, visible);
+        add_rows_visible<D>(dq, Ks, r, s, visible);
       else
-        add_rows<D>(dq, Ks, 16 * h, s);
+        add_rows<D>(dq, Ks, r, s);
     }
   }
+  f32x4 out[D / 16 / G::slices];
+  if (G::slices > 1) __syncthreads();
+  join<G, D>(out, dq, tiles, set, slice);
   if (in && (my_q < plan.n || !a.keep_tail))
-    store_row<D, kVec>(static_cast<float*>(a.dq) + hq * a.dq_h + my_q * a.dq_s, dq, a.scale, d);
+    store_row<D, kVec>(static_cast<float*>(a.dq) + hq * a.dq_h + my_q * a.dq_s, out, a.scale, d,
+                       slice * (D / 16 / G::slices));
 }
 
-// dK and dV of 64 keys, summed over the query heads of the group.
-template <int D, bool kVec>
-__global__ __launch_bounds__(256) void packed_dkdv_f32(PackedArgs a) {
-  __shared__ __attribute__((aligned(16))) float Qs[kTile * (D + 4)], Gs[kTile * (D + 4)];
-  __shared__ __attribute__((aligned(16))) float ls[kTile], ds[kTile];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
+// dK and dV of a block of keys, summed over the query heads of the group.
+template <typename G, int D, bool kVec>
+__global__ __launch_bounds__(G::threads, D > 64 || G::slices > 1 ? 2 : 3) void packed_dkdv_f32(PackedArgs a) {
+  __shared__ __attribute__((aligned(16))) float tiles[2 * G::tile * (D + 4)];
+  float *const Qs = tiles, *const Gs = tiles + G::tile * (D + 4);
+  __shared__ __attribute__((aligned(16))) float ls[G::tile], ds[G::tile];
+  const int lane = threadIdx.x & 63, set = (threadIdx.x >> 6) % G::sets, l16 = lane & 15, q4 = lane >> 4;
+  const int slice = threadIdx.x / (64 * G::sets), at = 16 * G::pieces * slice;
   const PackedPlan plan(a);
   int k0, hk;
-  if (!block_of<true>(a, plan, k0, hk)) return;
-  const int n_rep = a.Hq / a.Hkv, my_k = k0 + 16 * wave + l16, d = a.d;
+  if (!block_of<G, true>(a, plan, k0, hk)) return;
+  const int n_rep = a.Hq / a.Hkv, my_k = k0 + 16 * set + l16, d = a.d;
   const bool in = my_k < a.T;
   const int my_lo = in ? plan.query_lo(a, my_k) : 1, my_hi = in ? plan.query_hi(a, my_k) : 0;
   float4 k[D / 16], v[D / 16];
@@ -206,15 +283,15 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32(PackedArgs a) {
     dv[nt] = f32x4{};
   }
   int lo, hi;
-  tokens_of<true>(a, plan, k0, lo, hi);
-  const int nt = hi > lo ? (hi - lo + kTile - 1) / kTile : 0, n_it = nt * n_rep;
-  TileReg<D, kVec> qr, gr;
+  tokens_of<G, true>(a, plan, k0, lo, hi);
+  const int nt = hi > lo ? (hi - lo + G::tile - 1) / G::tile : 0, n_it = nt * n_rep;
+  TileReg<D, kVec, G::tile, G::threads> qr, gr;
   float lr = 0.f, dr = 0.f;
   auto load = [&](int it) __attribute__((always_inline)) {
-    const int hq = hk * n_rep + it / nt, r0 = lo + it % nt * kTile;
+    const int hq = hk * n_rep + it / nt, r0 = lo + it % nt * G::tile;
     qr.load(static_cast<const float*>(a.q) + hq * a.q_h, a.q_s, r0, plan.n, d);
     gr.load(static_cast<const float*>(a.dout) + hq * a.do_h, a.do_s, r0, plan.n, d);
-    if (threadIdx.x < kTile) {
+    if (threadIdx.x < G::tile) {
       const int qi = r0 + static_cast<int>(threadIdx.x);
       const int64_t i = static_cast<int64_t>(hq) * a.T + qi;
       lr = qi < plan.n ? a.lse2[i] : INFINITY;
@@ -225,52 +302,68 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32(PackedArgs a) {
   for (int it = 0; it < n_it; ++it) {
     __syncthreads();
     const int odd_q = qr.store(Qs), odd_g = gr.store(Gs);
-    if (threadIdx.x < kTile) {
+    if (threadIdx.x < G::tile) {
       ls[threadIdx.x] = lr;
       ds[threadIdx.x] = dr;
     }
     const bool odd = __syncthreads_or(odd_q | odd_g);
     if (it + 1 < n_it) load(it + 1);
-    const int r0 = lo + it % nt * kTile;
+    const int r0 = lo + it % nt * G::tile;
     auto visible = [&](int r) __attribute__((always_inline)) {
       return r0 + r >= my_lo && r0 + r <= my_hi;
     };
+    if (!__any(my_lo < r0 + at + 16 * G::pieces && my_hi >= r0 + at)) continue;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 s = dot_rows<D>(Qs, 16 * h, k);
-      const f32x4 dp = dot_rows<D>(Gs, 16 * h, v);
+    for (int row = at; row < at + 16 * G::pieces; row += 16) {
+      const f32x4 s = dot_rows<D>(Qs, row, k);
+      const f32x4 dp = dot_rows<D>(Gs, row, v);
       f32x4 p, w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = 16 * h + 4 * q4 + e;
+        const int r = row + 4 * q4 + e;
         const bool vis = visible(r);
         p[e] = vis ? expf(s[e] * a.scale - ls[r]) : 0.f;
         w[e] = vis ? p[e] * (dp[e] - ds[r]) : 0.f;
       }
       if (odd) {
-        add_rows_visible<D>(dv, Gs, 16 * h, p, visible);
-        add_rows_visible<D>(dk, Qs, 16 * h, w, visible);
+        add_rows_visible<D>(dv, Gs, row, p, visible);
+        add_rows_visible<D>(dk, Qs, row, w, visible);
       } else {
-        add_rows<D>(dv, Gs, 16 * h, p);
-        add_rows<D>(dk, Qs, 16 * h, w);
+        add_rows<D>(dv, Gs, row, p);
+        add_rows<D>(dk, Qs, row, w);
       }
     }
   }
+  f32x4 dk_sum[D / 16 / G::slices], dv_sum[D / 16 / G::slices];
+  if (G::slices > 1) __syncthreads();
+  join<G, D>(dk_sum, dk, tiles, set, slice);
+  if (G::slices > 1) __syncthreads();
+  join<G, D>(dv_sum, dv, tiles, set, slice);
   if (!in || (my_k >= plan.n && a.keep_tail)) return;
-  store_row<D, kVec>(static_cast<float*>(a.dk) + hk * a.dk_h + my_k * a.dk_s, dk, a.scale, d);
-  store_row<D, kVec>(static_cast<float*>(a.dv) + hk * a.dv_h + my_k * a.dv_s, dv, 1.f, d);
+  store_row<D, kVec>(static_cast<float*>(a.dk) + hk * a.dk_h + my_k * a.dk_s, dk_sum, a.scale, d,
+                     slice * (D / 16 / G::slices));
+  store_row<D, kVec>(static_cast<float*>(a.dv) + hk * a.dv_h + my_k * a.dv_s, dv_sum, 1.f, d,
+                     slice * (D / 16 / G::slices));
 }
 
-#define ZK_PACKED_F32(KERNEL, GRID)                                              \
-  do {                                                                           \
-    if (a.d <= 64 && vec)                                                        \
-      hipLaunchKernelGGL((KERNEL<64, true>), GRID, dim3(256), 0, s, a);          \
-    else if (a.d <= 64)                                                          \
-      hipLaunchKernelGGL((KERNEL<64, false>), GRID, dim3(256), 0, s, a);         \
-    else if (vec)                                                                \
-      hipLaunchKernelGGL((KERNEL<128, true>), GRID, dim3(256), 0, s, a);         \
-    else                                                                         \
-      hipLaunchKernelGGL((KERNEL<128, false>), GRID, dim3(256), 0, s, a);        \
+#define ZK_PACKED_F32_OF(KERNEL, G, HEADS)                                                \
+  do {                                                                                    \
+    const dim3 grid = group_grid(packed_blocks(a.T, G::rows) * (HEADS)), block(G::threads); \
+    if (a.d <= 64 && vec)                                                                 \
+      hipLaunchKernelGGL((KERNEL<G, 64, true>), grid, block, 0, s, a);                    \
+    else if (a.d <= 64)                                                                   \
+      hipLaunchKernelGGL((KERNEL<G, 64, false>), grid, block, 0, s, a);                   \
+    else if (vec)                                                                         \
+      hipLaunchKernelGGL((KERNEL<G, 128, true>), grid, block, 0, s, a);                   \
+    else                                                                                  \
+      hipLaunchKernelGGL((KERNEL<G, 128, false>), grid, block, 0, s, a);                  \
+  } while (0)
+#define ZK_PACKED_F32(KERNEL, HEADS)                                                      \
+  do {                                                                                    \
+    if (packed_blocks(a.T, Whole::rows) * (HEADS) <= 2 * device_cus())                    \
+      ZK_PACKED_F32_OF(KERNEL, Split, HEADS);                                             \
+    else                                                                                  \
+      ZK_PACKED_F32_OF(KERNEL, Whole, HEADS);                                             \
   } while (0)
 
 }  // namespace
@@ -278,18 +371,15 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32(PackedArgs a) {
 void launch_packed_fwd_f32(const PackedArgs& a, hipStream_t s) {
   const bool vec = vec4_ok(a.d, {a.q_s, a.q_h, a.k_s, a.k_h, a.v_s, a.v_h, a.o_s, a.o_h},
                            {a.q, a.k, a.v, a.out});
-  const dim3 grid = group_grid(packed_blocks(a.T, kRows) * a.Hq);
-  ZK_PACKED_F32(packed_fwd_f32, grid);
+  ZK_PACKED_F32(packed_fwd_f32, a.Hq);
 }
 
 void launch_packed_bwd_f32(const PackedArgs& a, hipStream_t s) {
   const bool vec = vec4_ok(a.d, {a.q_s, a.q_h, a.k_s, a.k_h, a.v_s, a.v_h, a.o_s, a.o_h, a.do_s, a.do_h,
                                  a.dq_s, a.dq_h, a.dk_s, a.dk_h, a.dv_s, a.dv_h},
                            {a.q, a.k, a.v, a.o, a.dout, a.dq, a.dk, a.dv});
-  const dim3 qgrid = group_grid(packed_blocks(a.T, kRows) * a.Hq);
-  const dim3 kgrid = group_grid(packed_blocks(a.T, kRows) * a.Hkv);
-  ZK_PACKED_F32(packed_dq_f32, qgrid);
-  ZK_PACKED_F32(packed_dkdv_f32, kgrid);
+  ZK_PACKED_F32(packed_dq_f32, a.Hq);
+  ZK_PACKED_F32(packed_dkdv_f32, a.Hkv);
 }
 
 }  // namespace zk

@@ -44,13 +44,13 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int64_t T, int32_t* 
   __shared__ int hist[1024];
   int shift = 5;
   while ((T >> shift) >= 1024) ++shift;
-  for (int which = 0; which < 3; ++which) {
-    const int rows = which == 0 ? 256 : 128, nb = static_cast<int>((T + rows - 1) / rows);
+  for (int which = 0; which < 2; ++which) {
+    const int rows = kPlanRows, nb = static_cast<int>((T + rows - 1) / rows);
     int32_t* order = plan + plan_order_at(T, which);
     auto key = [&](int b) {
       const int64_t first = static_cast<int64_t>(b) * rows;
       const int64_t past = first + rows < T ? first + rows : T;
-      const int64_t work = which < 2 ? past - start[first] : end[past - 1] - first;
+      const int64_t work = which == 0 ? past - start[first] : end[past - 1] - first;
       const int bin = static_cast<int>((work < 0 ? 0 : work) >> shift);
       return 1023 - (bin < 1024 ? bin : 1023);  // the largest in bin 0
     };
@@ -518,7 +518,7 @@ extern "C" int64_t zk_packed_plan_bytes(int64_t T) {
     set_error("zk_packed_plan_bytes: T=%lld tokens, 0 .. 2^30 - 1", (long long)T);
     return ZK_EINVAL;
   }
-  return 4 * plan_order_at(T, 3);
+  return 4 * plan_order_at(T, 2);
 }
 
 extern "C" int zk_packed_plan(const void* offsets, int offsets_64, int64_t n_seq, int64_t T, void* plan,
