@@ -104,6 +104,13 @@ __host__ __device__ inline int64_t packed_blocks(int64_t T, int rows) {
   return (T + kPlanRows - 1) / kPlanRows * (kPlanRows / rows);
 }
 
+// Whether the 2-byte kernels take a block in two groups of waves (their kSplit) in a
+// launch of n workgroups: one a CU at most, and rows that may meet more than 256
+// tokens.  64 tokens in two groups: forward 8 us, backward 20, else 6 and 17.
+inline bool packed_split(const PackedArgs& a, int64_t n) {
+  return n <= device_cus() && a.T > 256 && (a.window == 0 || a.window > 128);
+}
+
 // Head of a block in the order of launch: the workgroups of one XCD (dispatch
 // goes round the eight of them) take the query heads of as few key heads as
 // possible, so that a key head's tiles are fetched into one L2.

@@ -37,17 +37,52 @@ __device__ __forceinline__ typename Mfma<T>::vec8 tr_operand(const T* X, int off
   return __builtin_bit_cast(typename Mfma<T>::vec8, w);
 }
 
+// Adds the second group's accumulators (waves 4 .. 7) to the first's, through four
+// tiles of BYTES that no wave reads any more; whether this wave is of the first.
+// (Tiles of their own, not parts of one array: for parts the compiler makes every read
+// wait for all loads in flight, 10 % of the forward's time.)
+template <int BYTES, int NB>
+__device__ __forceinline__ bool join_groups(f32x16 (&x)[NB], void* t0, void* t1, void* t2, void* t3) {
+  constexpr int EACH = BYTES / (4 * 8 * 256);  // pieces of 8 accumulators in a tile
+  static_assert(4 * EACH >= 2 * NB, "the sums do not fit in the tiles");
+  void* const tile[4] = {t0, t1, t2, t3};
+  auto at = [&](int nt, int j) __attribute__((always_inline)) {
+    const int n = 2 * nt + j / 8;
+    return static_cast<float*>(tile[n / EACH]) + (n % EACH * 8 + j % 8) * 256 + (threadIdx.x & 255);
+  };
+  const bool first = threadIdx.x < 256;
+  if (!first) {
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) *at(nt, j) = x[nt][j];
+  }
+  __syncthreads();
+  if (first) {
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[nt][j] += *at(nt, j);
+  }
+  return first;
+}
+
 // --------------------------------------------------------------------- dQ --
 // 4 waves of 32 queries, whose Q and dO rows stay in registers; 64-key tiles of
 // K and V.  Also delta = rowsum(dO o O) and the log2-domain LSE for the other kernel.
-template <typename T, int D, int KR>
-__global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
+// kSplit, here and below: two groups of four waves take every other tile of the same
+// rows and join their sums at the end, for launches of so few blocks that they wait for
+// the one with the most tiles (head dim 128, causal, both kernels: 8 heads of 4096 tokens
+// 300 us, split 216; 2 of 8192 573 and 390; but 2048 tokens in sequences of 200 46 and 48).
+template <typename T, int D, int KR, bool kSplit>
+__global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(PackedArgs a) {
   typedef Mfma<T> M;
   typedef typename M::vec8 V8;
-  constexpr int BM = 128, BN = 64, NT = 256, PF = 2;  // PF: operand reads in flight
+  constexpr int BM = 128, BN = 64, PF = 2;  // PF: operand reads in flight
+  constexpr int NT = kSplit ? 512 : 256, TN = kSplit ? 2 * BN : BN;  // TN: keys of a step
   constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
   const int hd = KR ? a.d : D;
-  __shared__ __attribute__((aligned(16))) T K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+  __shared__ __attribute__((aligned(16))) T K0[TN * D], K1[TN * D], V0[TN * D], V1[TN * D];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -58,7 +93,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   const int rows = static_cast<int>(a.T);
   if (q0 >= rows) return;
   const int hk = hq / (a.Hq / a.Hkv);
-  const int qw0 = q0 + 32 * wave;
+  const int qw0 = q0 + 32 * (wave & 3);
+  const int k_off = kSplit ? wave / 4 * BN : 0;  // this wave's keys in a step
   const int my_q = qw0 + l32;
   const bool in = my_q < rows;
   const float c2 = a.scale_log2;
@@ -102,24 +138,25 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
       const int64_t i = static_cast<int64_t>(hq) * a.T + my_q;
       const float l = my_q < plan.n ? a.lse[i] : -INFINITY;
       lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
-      if (g == 0) {
+      if (g == 0 && k_off == 0) {
         a.delta[i] = del;
         a.lse2[i] = lse2;
       }
     }
   }
 
-  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + BN - 1) / BN : 0;
-  PackedLoader<T, D, BN, NT> kload, vload;
+  const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + TN - 1) / TN : 0;
+  PackedLoader<T, D, TN, NT> kload, vload;
   kload.init(a.k_s, hd);
   vload.init(a.v_s, hd);
   auto issue = [&](int t, int st) {
-    const int k0 = kv_lo + t * BN;
+    const int k0 = kv_lo + t * TN;
     kload.issue(st ? K1 : K0, Kp, a.k_s, k0, plan.n);
     vload.issue(st ? V1 : V0, Vp, a.v_s, k0, plan.n);
   };
-  const int rbase = 2 * tile_off<D>(l32, 8 * g);
-  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+  const int rbase = 2 * (tile_off<D>(l32, 8 * g) + k_off * D);
+  const int tbase =
+      2 * (tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) + k_off * D);
 
   f32x16 dq[NB];
 #pragma unroll
@@ -127,7 +164,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 
   auto step = [&](auto stage_tag, int t) {
     constexpr int st = decltype(stage_tag)::value;
-    const int k0 = kv_lo + t * BN;
+    const int k0 = kv_lo + t * TN + k_off;
     wait_vmcnt<0>();
     __syncthreads();
     if (t + 1 < n_t) issue(t + 1, st ^ 1);
@@ -202,6 +239,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
   }
 
+  if constexpr (kSplit) {
+    __syncthreads();  // every wave is past its last product
+    if (!join_groups<TN * D * 2>(dq, K0, K1, V0, V1)) return;
+  }
   const bool put = in && (my_q < plan.n || !a.keep_tail);
   T* out = static_cast<T*>(a.dq) + hq * a.dq_h + my_q * a.dq_s;
   const bool bad = row_has_nan<NB>(dq, g, hd);
@@ -231,16 +272,17 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 // ------------------------------------------------------------------ dK / dV --
 // 4 waves of 32 keys (K rows in registers, V rows in LDS); 32-query blocks of
 // every query head of the group, whose sums stay in the accumulators.
-template <typename T, int D, int KR>
-__global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
+template <typename T, int D, int KR, bool kSplit>
+__global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(PackedArgs a) {
   typedef Mfma<T> M;
   typedef typename M::vec8 V8;
   constexpr int BK = 128, MQ = 32;
+  constexpr int NT = kSplit ? 512 : 256, TQ = kSplit ? 2 * MQ : MQ;  // TQ: queries of a step
   constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
   const int hd = KR ? a.d : D;
-  __shared__ __attribute__((aligned(16))) T Q0[MQ * D], Q1[MQ * D], dO0[MQ * D], dO1[MQ * D];
-  __shared__ __attribute__((aligned(16))) float lse2s[2][4][64];  // 64 lanes load, MQ used
-  __shared__ __attribute__((aligned(16))) float dels[2][4][64];
+  __shared__ __attribute__((aligned(16))) T Q0[TQ * D], Q1[TQ * D], dO0[TQ * D], dO1[TQ * D];
+  __shared__ __attribute__((aligned(16))) float lse2s[2][NT / 64][64];  // 64 lanes load, MQ used
+  __shared__ __attribute__((aligned(16))) float dels[2][NT / 64][64];
   __shared__ __attribute__((aligned(16))) T Vw[4][32 * D];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
@@ -253,7 +295,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
   const int k0 = plan.first_row<BK, true>(a, block);
   const int rows = static_cast<int>(a.T);
   if (k0 >= rows) return;
-  const int kw0 = k0 + 32 * wave;
+  const int kw0 = k0 + 32 * (wave & 3);
+  const int q_off = kSplit ? wave / 4 * MQ : 0;  // this wave's queries in a step
   const int my_key = kw0 + l32;
   const bool in = my_key < rows;
   const float c2 = a.scale_log2;
@@ -279,10 +322,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
   const T* Kp = static_cast<const T*>(a.k) + hk * a.k_h;
   const T* Vp = static_cast<const T*>(a.v) + hk * a.v_h;
   V8 kreg[KS];
-  T* Vme = Vw[wave];
-  {
+  T* Vme = Vw[wave & 3];
+  load_operand<T, KS, KR>(kreg, in ? Kp + my_key * a.k_s : nullptr, g, hd);
+  if (wave < 4) {  // a barrier stands before the first read
     V8 vv[KS];
-    load_operand<T, KS, KR>(kreg, in ? Kp + my_key * a.k_s : nullptr, g, hd);
     load_operand<T, KS, KR>(vv, in ? Vp + my_key * a.v_s : nullptr, g, hd);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
@@ -295,30 +338,30 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
     dk[nt] = f32x16{};
     dv[nt] = f32x16{};
   }
-  const int rbase = 2 * tile_off<D>(l32, 8 * g);
-  const int tbase = 2 * tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+  const int rbase = 2 * (tile_off<D>(l32, 8 * g) + q_off * D);
+  const int tbase =
+      2 * (tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) + q_off * D);
 
-  const int n_qb = q_hi > q_lo ? (q_hi - q_lo + MQ - 1) / MQ : 0;
+  const int n_qb = q_hi > q_lo ? (q_hi - q_lo + TQ - 1) / TQ : 0;
   const int n_it = n_qb * n_rep;
-  PackedLoader<T, D, MQ, 256> qload, dload;
+  PackedLoader<T, D, TQ, NT> qload, dload;
   qload.init(a.q_s, hd);
   dload.init(a.do_s, hd);
   auto issue = [&](int qb, int hr, int st) {
     const int hq = h_first + hr;
-    const int qb0 = q_lo + qb * MQ;
+    const int qb0 = q_lo + qb * TQ;
     qload.issue(st ? Q1 : Q0, static_cast<const T*>(a.q) + hq * a.q_h, a.q_s, qb0, plan.n);
     dload.issue(st ? dO1 : dO0, static_cast<const T*>(a.dout) + hq * a.do_h, a.do_s, qb0, plan.n);
-    int qi = qb0 + lane;
-    if (qi > plan.n - 1) qi = plan.n - 1;
-    const int64_t r0 = static_cast<int64_t>(hq) * a.T + qb0;
-    const uint32_t off = static_cast<uint32_t>((qi - qb0) * 4);
+    const int first = below(qb0 + q_off), qi = below(first + lane);
+    const int64_t r0 = static_cast<int64_t>(hq) * a.T + first;
+    const uint32_t off = static_cast<uint32_t>((qi - first) * 4);
     dma_lds<4>(raw_rsrc(a.lse2 + r0), off, 0, &lse2s[st][wave][0]);
     dma_lds<4>(raw_rsrc(a.delta + r0), off, 0, &dels[st][wave][0]);
   };
 
   auto step = [&](auto stage_tag, int qb, int nxt_qb, int nxt_hr, bool has_next) {
     constexpr int st = decltype(stage_tag)::value;
-    const int qb0 = q_lo + qb * MQ;
+    const int qb0 = q_lo + qb * TQ + q_off;
     wait_vmcnt<0>();
     __syncthreads();
     if (has_next) issue(nxt_qb, nxt_hr, st ^ 1);
@@ -331,6 +374,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
     {
       int rb = rbase, tb = tbase;  // opaque: addresses derived in the step
       asm volatile("" : "+v"(rb), "+v"(tb));
+      const int vb0 = kSplit ? rb - 2 * q_off * D : rb;
       f32x16 s = f32x16{}, dp = f32x16{};
       // each step's Q operand is read one step ahead
       V8 qa = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Qt) + rb);
@@ -338,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
       for (int ks = 0; ks < KS; ++ks) {
         const int ro = rb ^ (ks << 5);
         V8 da = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(dOt) + ro);
-        const V8 vb = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Vme) + ro);
+        const V8 vb = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Vme) + (vb0 ^ (ks << 5)));
         V8 qn = qa;
         if (ks + 1 < KS)
           qn = *reinterpret_cast<const V8*>(reinterpret_cast<const char*>(Qt) + (rb ^ ((ks + 1) << 5)));
@@ -408,6 +452,13 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv_kernel(PackedArgs a) {
     }
   }
 
+  if constexpr (kSplit) {
+    __syncthreads();
+    const bool first = join_groups<TQ * D * 2>(dk, Q0, Q1, dO0, dO1);
+    __syncthreads();
+    join_groups<TQ * D * 2>(dv, Q0, Q1, dO0, dO1);
+    if (!first) return;
+  }
   const bool whole = a.parts == 1;
   const bool put = in && (my_key < plan.n || (whole && !a.keep_tail));
   T* dkp = static_cast<T*>(a.dk) + hk * a.dk_h + my_key * a.dk_s;
@@ -505,11 +556,16 @@ static int packed_parts(int64_t T, int64_t Hq, int64_t Hkv, int64_t window, int 
 
 template <typename T, int D, int KR>
 static void launch_packed_bwd(const PackedArgs& a, hipStream_t s) {
-  const int64_t blocks = packed_blocks(a.T, 128);
-  hipLaunchKernelGGL((packed_dq_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hq)),
-                     dim3(256), 0, s, a);
-  hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR>), dim3(static_cast<unsigned>(blocks * a.Hkv * a.parts)),
-                     dim3(256), 0, s, a);
+  const int64_t blocks = packed_blocks(a.T, 128), nq = blocks * a.Hq, nk = blocks * a.Hkv * a.parts;
+  const dim3 gq(static_cast<unsigned>(nq)), gk(static_cast<unsigned>(nk));
+  if (packed_split(a, nq))
+    hipLaunchKernelGGL((packed_dq_kernel<T, D, KR, true>), gq, dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((packed_dq_kernel<T, D, KR, false>), gq, dim3(256), 0, s, a);
+  if (packed_split(a, nk))
+    hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR, true>), gk, dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR, false>), gk, dim3(256), 0, s, a);
   if (a.parts > 1) {
     const int64_t pairs = a.T * a.Hkv * a.d / 2;
     hipLaunchKernelGGL(packed_sum_kernel<T>, dim3(static_cast<unsigned>((pairs + 255) / 256)), dim3(256), 0,

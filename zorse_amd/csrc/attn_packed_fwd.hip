@@ -390,7 +390,9 @@ void packed_fwd_kernel(PackedArgs a) {
     const int slot = threadIdx.x & (64 * QW - 1);
     float* ml = reinterpret_cast<float*>(V0);
     auto at = [&](int nt, int j) __attribute__((always_inline)) {
-      return reinterpret_cast<float*>(nt < 2 ? K0 : K1) + ((nt & 1) * 16 + j) * (64 * QW) + slot;
+      constexpr int EACH = TN * D / 2 / (16 * 64 * QW);  // accumulators that a tile has room for
+      static_assert(2 * EACH >= NB, "the sums do not fit in the tiles");
+      return reinterpret_cast<float*>(nt < EACH ? K0 : K1) + (nt % EACH * 16 + j) * (64 * QW) + slot;
     };
     __syncthreads();  // every wave is past its last product
     if (wave >= QW) {
@@ -548,7 +550,7 @@ namespace zk {
 template <typename T, int D, int KR>
 static void launch_packed_fwd(const PackedArgs& a, hipStream_t s) {
   const int64_t n = packed_blocks(a.T, 128) * a.Hq;
-  if (n <= device_cus())
+  if (packed_split(a, n))
     hipLaunchKernelGGL((packed_fwd_kernel<T, D, KR, true>), dim3(static_cast<unsigned>(n)), dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL((packed_fwd_kernel<T, D, KR, false>), dim3(static_cast<unsigned>(n)), dim3(256), 0, s, a);
