@@ -169,6 +169,22 @@ def test_against_64_bits(dev, lengths, pad, H, Hk, d, causal, window, dt):
         [i for n in lengths for i in range(n)] + [0] * pad))
 
 
+# more blocks than the chip holds at once, where a block is one group of waves
+MANY = [
+    ((600, 1, 370), 40, 32, 32, 64, True, 0, BF),
+    ((600, 1, 370), 40, 32, 8, 128, True, 0, FP),
+    ((700, 300), 3, 32, 8, 64, True, 200, FP),
+    ((333, 600), 3, 32, 32, 100, False, 0, BF),
+    ((555, 401), 3, 34, 34, 64, True, 0, F4),
+    ((555, 401), 3, 36, 36, 99, True, 300, F4),
+]
+
+
+@pytest.mark.parametrize("lengths,pad,H,Hk,d,causal,window,dt", MANY)
+def test_launches_of_many_blocks(dev, lengths, pad, H, Hk, d, causal, window, dt):
+    test_against_64_bits(dev, lengths, pad, H, Hk, d, causal, window, dt)
+
+
 @pytest.mark.parametrize("dt,d", [(BF, 128), (FP, 64), (BF, 72), (F4, 64)])
 @pytest.mark.parametrize("scale", [0.02, 1.5])
 def test_scales_and_large_scores(dev, dt, d, scale):
@@ -208,6 +224,23 @@ def test_odd_values_stay_in_their_rows(dev, dt, d, value):
     do[3] = value
     got = _run(dev, q, k, v, do, offsets, True, 0)
     _near(got, want, "later keys", torch.tensor([*range(4, 200)]))
+
+
+@pytest.mark.parametrize("dt,H,d", [(BF, 4, 128), (FP, 4, 64), (BF, 4, 100), (FP, 32, 64), (F4, 48, 64)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_odd_values_in_long_runs(dev, dt, H, d, value):
+    """The same where blocks are taken in two groups of waves, and where they are many."""
+    offsets, T = [0, 300, 420, 800], 870
+    q, k, v, do = _inputs(T, H, H // 2, d, dt, 14)
+    want, _ = _reference(q, k, v, do, offsets, True, 0, 1 / math.sqrt(d), dt)
+    for t in (q, k, v, do):
+        t[300:420] = value
+        t[800:] = value
+    got = _run(dev, q, k, v, do, offsets, True, 0)
+    _near(got, want, "neighbours", torch.tensor([*range(300), *range(420, 800)]))
+    for x in got:
+        assert not bool(x[800:].any())
+    assert not bool(torch.isfinite(got[0][300:420]).any())
 
 
 def test_no_weight_is_nan(dev):
