@@ -610,7 +610,9 @@ int zk_attn_packed_fwd(const zk_packed_desc* desc, const void* q, const void* k,
                        const void* v, const void* plan, void* o, float* lse,
                        zk_stream_t stream);
 /* Its gradients, from the forward's o and lse.  Sums in one order: equal calls
- * give equal bits.  The workspace holds two fp32 values a token and query head. */
+ * give equal bits.  The workspace holds two fp32 values a token and query head,
+ * and where few key heads have several query heads each, partial sums of dk and dv
+ * in fp32. */
 int64_t zk_attn_packed_bwd_workspace(const zk_packed_desc* desc);
 int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, const void* k,
                        const void* v, const void* plan, const void* o,

@@ -174,6 +174,7 @@ MANY = [
     ((600, 1, 370), 40, 32, 32, 64, True, 0, BF),
     ((600, 1, 370), 40, 32, 8, 128, True, 0, FP),
     ((700, 300), 3, 32, 8, 64, True, 200, FP),
+    ((700, 300), 3, 96, 24, 64, True, 200, BF),  # two query heads a sum
     ((333, 600), 3, 32, 32, 100, False, 0, BF),
     ((555, 401), 3, 34, 34, 64, True, 0, F4),
     ((555, 401), 3, 36, 36, 99, True, 300, F4),

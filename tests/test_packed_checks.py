@@ -40,6 +40,7 @@ def test_attention_entry_points_refuse():
         assert call(d=130) == -4 and call(d=63) == -4 and call(d=0) == -4
         assert call(q_s=-8) == -4 and call(k_s=1 << 23) == -4
         assert call(q_h=63) == -3
+        assert call(T=1 << 24, Hq=64) == -4
         assert call(T=0) == 0
     assert fwd(q=None) == -1 and fwd(o=None) == -1 and fwd(plan=None) == -1 and fwd(lse=None) == -1
     assert fwd(q=ODD) == -3 and fwd(lse=ODD) == -3 and fwd(dtype=0, v=ODD) == -3

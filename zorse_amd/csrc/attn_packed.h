@@ -106,7 +106,9 @@ __host__ __device__ inline int64_t packed_blocks(int64_t T, int rows) {
 
 // Whether the 2-byte kernels take a block in two groups of waves (their kSplit) in a
 // launch of n workgroups: one a CU at most, and rows that may meet more than 256
-// tokens.  64 tokens in two groups: forward 8 us, backward 20, else 6 and 17.
+// tokens.  64 tokens in two groups: forward 8 us, backward 20, else 6 and 17.  At two
+// a CU long sequences gain by it (16 heads of 4096 causal tokens forward 105 and 90 us)
+// what sequences of 500 tokens lose (24 and 33).
 inline bool packed_split(const PackedArgs& a, int64_t n) {
   return n <= device_cus() && a.T > 256 && (a.window == 0 || a.window > 128);
 }

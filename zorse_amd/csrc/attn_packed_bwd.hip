@@ -1,5 +1,13 @@
 // Attention over packed sequences, backward (bf16 / fp16 storage), without
-// atomics: two kernels on the caller's stream.
+// atomics: two kernels on the caller's stream.  With P = exp(S - LSE), dP = dO V^T
+// and dS = P (dP - rowsum(dO O)):  dV = P^T dO, dQ = scale dS K, dK = scale dS^T Q.
+//   Bound by the matrix instructions: seven products where five are needed, because
+// each kernel forms S and dP for itself (one kernel for all three would add dQ in
+// fp32 with atomics, in no fixed order).  32 causal heads of 128, 8 key heads, 8192
+// tokens: dQ 750 us (3 products, 1100 TFLOP/s), dK / dV 1040 (4, 1057), their sums
+// 29; documents of 30 to 2500 of 4096 tokens, 32 heads: 74 and 100, where the blocks
+// of the longest document end last.  P and dS are rounded to the storage type as
+// operands of the products that follow, with fp32 sums.
 #include <type_traits>
 
 #include "attn_packed.h"

@@ -492,7 +492,9 @@ int check_packed(const zk_packed_desc* D, const char* who, bool bwd, bool* ragge
   for (const void* p : tensors) at4 = at4 && aligned(p, 4);
   ZK_REQUIRE(D->dtype == ZK_F32 ? at4 : vec4, ZK_EALIGN, "%s: heads start at multiples of 4 bytes",
              who);
-  ZK_REQUIRE(D->Hq * ((D->T + 127) / 128) * 4 < 0x7fffffffLL, ZK_EINVAL, "%s: grid too large", who);
+  // a launch holds fewer than 2^32 threads
+  ZK_REQUIRE(D->Hq * ((D->T + 127) / 128) < int64_t(1) << 23, ZK_EUNSUPPORTED,
+             "%s: %lld heads of %lld tokens: 2^30 rows or more", who, (long long)D->Hq, (long long)D->T);
   *ragged = !vec16;
   return ZK_OK;
 }

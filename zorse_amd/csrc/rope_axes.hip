@@ -7,7 +7,11 @@
 // Bound by the bytes of q and k, read and written once.  A thread owns V
 // neighbouring pairs (16 bytes of each half where alignment allows) and turns
 // them in up to kHeads heads of one token, all loads of which are issued before
-// any is used; its cosines and sines are read once and serve them all.
+// any is used; its cosines and sines are read once and serve them all.  16384
+// tokens of 40 heads of 128 in bf16: 66 us a direction, 5.1 TB/s, the rate of a
+// large copy; with one, two and eight heads in flight 112, 86 and 67.  Nontemporal
+// loads and stores take such a pass to 61 us but a layer's rotation with the
+// attention that reads it (4096 tokens, 64 heads) from 70 us to 75.
 #include "zk_common.h"
 
 namespace zk {
