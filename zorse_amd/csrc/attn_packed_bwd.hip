@@ -279,17 +279,21 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
 
 // ------------------------------------------------------------------ dK / dV --
 // 4 waves of 32 keys (K rows in registers, V rows in LDS); 32-query blocks of
-// every query head of the group, whose sums stay in the accumulators.
+// every query head of the group, whose sums stay in the accumulators.  At a head dim
+// of 64, whose blocks take half as long, two of them between barriers: the loads of the
+// next ones have that time (8000 tokens, window 1024, 32 heads of 8: both kernels 345 us
+// with one, 314 with two; three waves a SIMD or 128 keys a step in dQ: slower).
 template <typename T, int D, int KR, bool kSplit>
 __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(PackedArgs a) {
   typedef Mfma<T> M;
   typedef typename M::vec8 V8;
   constexpr int BK = 128, MQ = 32;
-  constexpr int NT = kSplit ? 512 : 256, TQ = kSplit ? 2 * MQ : MQ;  // TQ: queries of a step
+  constexpr int NT = kSplit ? 512 : 256;
+  constexpr int SUB = D == 64 ? 2 : 1, TQ = (kSplit ? 2 : 1) * SUB * MQ;  // blocks of a wave in a step; queries
   constexpr int KS = KR ? KR : D / 16, NB = (KS + 1) / 2;
   const int hd = KR ? a.d : D;
   __shared__ __attribute__((aligned(16))) T Q0[TQ * D], Q1[TQ * D], dO0[TQ * D], dO1[TQ * D];
-  __shared__ __attribute__((aligned(16))) float lse2s[2][NT / 64][64];  // 64 lanes load, MQ used
+  __shared__ __attribute__((aligned(16))) float lse2s[2][NT / 64][64];  // 64 lanes load, SUB MQ used
   __shared__ __attribute__((aligned(16))) float dels[2][NT / 64][64];
   __shared__ __attribute__((aligned(16))) T Vw[4][32 * D];
 
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
   const int rows = static_cast<int>(a.T);
   if (k0 >= rows) return;
   const int kw0 = k0 + 32 * (wave & 3);
-  const int q_off = kSplit ? wave / 4 * MQ : 0;  // this wave's queries in a step
+  const int q_off = kSplit ? wave / 4 * (SUB * MQ) : 0;  // this wave's queries in a step
   const int my_key = kw0 + l32;
   const bool in = my_key < rows;
   const float c2 = a.scale_log2;
@@ -369,17 +373,19 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
 
   auto step = [&](auto stage_tag, int qb, int nxt_qb, int nxt_hr, bool has_next) {
     constexpr int st = decltype(stage_tag)::value;
-    const int qb0 = q_lo + qb * TQ + q_off;
+    const int qb_first = q_lo + qb * TQ + q_off;
     wait_vmcnt<0>();
     __syncthreads();
     if (has_next) issue(nxt_qb, nxt_hr, st ^ 1);
-    if (idle || qb0 > w_hi || qb0 + MQ <= w_lo) return;
-    const bool need_mask = qb0 < f_lo || qb0 + MQ - 1 > f_hi;
-    const T* Qt = st ? Q1 : Q0;
-    const T* dOt = st ? dO1 : dO0;
-    const float* l2v = lse2s[st][wave];
-    const float* dlv = dels[st][wave];
-    {
+#pragma unroll
+    for (int sub = 0; sub < SUB; ++sub) {
+      const int qb0 = qb_first + sub * MQ;
+      if (idle || qb0 > w_hi || qb0 + MQ <= w_lo) continue;
+      const bool need_mask = qb0 < f_lo || qb0 + MQ - 1 > f_hi;
+      const T* Qt = (st ? Q1 : Q0) + sub * MQ * D;
+      const T* dOt = (st ? dO1 : dO0) + sub * MQ * D;
+      const float* l2v = lse2s[st][wave] + sub * MQ;
+      const float* dlv = dels[st][wave] + sub * MQ;
       int rb = rbase, tb = tbase;  // opaque: addresses derived in the step
       asm volatile("" : "+v"(rb), "+v"(tb));
       const int vb0 = kSplit ? rb - 2 * q_off * D : rb;
