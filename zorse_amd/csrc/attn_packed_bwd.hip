@@ -526,11 +526,12 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
 }
 
 // The parts' sum, first to last, in the storage type; zeros behind the last
-// sequence.  Two elements a thread (heads of even dims).
-template <typename T>
+// sequence.  V elements a thread (2-byte heads have an even number).
+template <typename T, int V>
 __global__ __launch_bounds__(256) void packed_sum_kernel(PackedArgs a) {
-  typedef T T2 __attribute__((ext_vector_type(2)));
-  const int64_t n = a.T * a.Hkv * a.d, i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 2;
+  typedef T TV __attribute__((ext_vector_type(V)));
+  typedef float FV __attribute__((ext_vector_type(V)));
+  const int64_t n = a.T * a.Hkv * a.d, i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
   if (i >= n) return;
   const int e = static_cast<int>(i % a.d);
   const int64_t r = i / a.d;
@@ -538,20 +539,32 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackedArgs a) {
   const int64_t t = r / a.Hkv;
   const bool tail = t >= a.plan[0];
   if (tail && a.keep_tail) return;
-  float2 k = make_float2(0.f, 0.f), v = k;
+  float k[V] = {}, v[V] = {};
   if (!tail)
     for (int p = 0; p < a.parts; ++p) {
-      const float2 x = *reinterpret_cast<const float2*>(a.dk_part + p * n + i);
-      const float2 y = *reinterpret_cast<const float2*>(a.dv_part + p * n + i);
-      k.x += x.x;
-      k.y += x.y;
-      v.x += y.x;
-      v.y += y.y;
+      const FV x = *reinterpret_cast<const FV*>(a.dk_part + p * n + i);
+      const FV y = *reinterpret_cast<const FV*>(a.dv_part + p * n + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        k[j] += x[j];
+        v[j] += y[j];
+      }
     }
-  *reinterpret_cast<T2*>(static_cast<T*>(a.dk) + t * a.dk_s + h * a.dk_h + e) =
-      T2{static_cast<T>(k.x), static_cast<T>(k.y)};
-  *reinterpret_cast<T2*>(static_cast<T*>(a.dv) + t * a.dv_s + h * a.dv_h + e) =
-      T2{static_cast<T>(v.x), static_cast<T>(v.y)};
+  TV ks, vs;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    ks[j] = static_cast<T>(k[j]);
+    vs[j] = static_cast<T>(v[j]);
+  }
+  *reinterpret_cast<TV*>(static_cast<T*>(a.dk) + t * a.dk_s + h * a.dk_h + e) = ks;
+  *reinterpret_cast<TV*>(static_cast<T*>(a.dv) + t * a.dv_s + h * a.dv_h + e) = vs;
+}
+template <typename T, int V>
+static void launch_packed_sum(const PackedArgs& a, hipStream_t s) {
+  if (a.parts == 1) return;
+  const int64_t threads = a.T * a.Hkv * a.d / V;
+  hipLaunchKernelGGL((packed_sum_kernel<T, V>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
+                     s, a);
 }
 
 // Sums of a key head's query heads: one where its key blocks are enough to fill the
@@ -559,8 +572,7 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackedArgs a) {
 // whole sequence), else as many as make them so.  8192 causal tokens, 32 query heads
 // of 8 key heads: one sum 1640 us, two 1160 us with their addition.  A window far
 // below T evens blocks out itself.
-static int packed_parts(int64_t T, int64_t Hq, int64_t Hkv, int64_t window, int dtype) {
-  if (dtype == ZK_F32) return 1;
+static int packed_parts(int64_t T, int64_t Hq, int64_t Hkv, int64_t window) {
   const bool even = window > 0 && window < T / 4;
   const int64_t rep = Hq / Hkv, n = packed_blocks(T, 128) * Hkv, want = device_cus() * (even ? 3 : 7) / 2;
   for (int64_t p = 1; p < rep; ++p)
@@ -580,11 +592,7 @@ static void launch_packed_bwd(const PackedArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR, true>), gk, dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL((packed_dkdv_kernel<T, D, KR, false>), gk, dim3(256), 0, s, a);
-  if (a.parts > 1) {
-    const int64_t pairs = a.T * a.Hkv * a.d / 2;
-    hipLaunchKernelGGL(packed_sum_kernel<T>, dim3(static_cast<unsigned>((pairs + 255) / 256)), dim3(256), 0,
-                       s, a);
-  }
+  launch_packed_sum<T, 2>(a, s);
 }
 template <typename T>
 static void launch_packed_bwd_t(const PackedArgs& a, bool ragged, hipStream_t s) {
@@ -612,7 +620,7 @@ using namespace zk;
 extern "C" int64_t zk_attn_packed_bwd_workspace(const zk_packed_desc* desc) {
   if (desc == nullptr || desc->T < 0 || desc->Hq <= 0 || desc->Hkv <= 0 || desc->Hq % desc->Hkv != 0)
     return 0;
-  const int parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window, desc->dtype);
+  const int parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window);
   const int64_t sums = parts > 1 ? 2 * parts * desc->T * desc->Hkv * desc->d : 0;
   return (2 * ((desc->Hq * desc->T + 63) / 64 * 64) + sums) * 4 + 256;
 }
@@ -637,15 +645,17 @@ extern "C" int zk_attn_packed_bwd(const zk_packed_desc* desc, const void* q, con
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.delta = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   a.lse2 = a.delta + (desc->Hq * desc->T + 63) / 64 * 64;
-  a.parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window, desc->dtype);
+  a.parts = packed_parts(desc->T, desc->Hq, desc->Hkv, desc->window);
   a.dk_part = a.lse2 + (desc->Hq * desc->T + 63) / 64 * 64;
   a.dv_part = a.dk_part + a.parts * desc->T * desc->Hkv * desc->d;
   hipStream_t s = as_stream(stream);
-  if (desc->dtype == ZK_F32)
+  if (desc->dtype == ZK_F32) {
     launch_packed_bwd_f32(a, s);
-  else if (desc->dtype == ZK_BF16)
+    launch_packed_sum<float, 1>(a, s);
+  } else if (desc->dtype == ZK_BF16) {
     launch_packed_bwd_t<bf16>(a, ragged, s);
-  else
+  } else {
     launch_packed_bwd_t<f16>(a, ragged, s);
+  }
   return launch_status(who);
 }

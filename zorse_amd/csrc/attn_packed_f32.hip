@@ -8,10 +8,11 @@
 // and where a launch has few workgroups by those of the one with the most tiles, of
 // which Split does a quarter at a time.  So Split up to two of Whole's workgroups a CU
 // (head dim 64, causal, forward and backward in us, Whole against Split: 1024 tokens,
-// 8 heads 78 + 357 against 42 + 153; 2048, 16 heads 180 + 526 against 135 + 414, but in
+// 8 heads 78 + 357 against 42 + 153 (one sum a key head); 2048, 16 heads 180 + 526 against 135 + 414, but in
 // sequences of 200 31 + 86 against 31 + 104), Whole past it (4096 tokens, 16 heads of
 // 128: 811 + 2570, 67 - 85 TFLOP/s of the 157 that the matrix cores have in fp32;
-// Split 991 + 2970).
+// Split 991 + 2970).  A key head's query heads go to several workgroups as for the
+// 2-byte types (1024 tokens, 8 heads of 4: 153 us backward, 110 with two sums).
 //   Products and sums are fp32; a tile that holds an infinity or a NaN is added row by
 // row, masked rows left out.
 #include "attn_f32.h"
@@ -61,7 +62,7 @@ __device__ __forceinline__ void join(f32x4 (&sum)[N], const f32x4 (&acc)[D / 16]
 template <typename G, bool kKeys>
 __device__ __forceinline__ bool block_of(const PackedArgs& a, const PackedPlan& plan, int& r0, int& h) {
   const int64_t bid = group_id();
-  const int H = kKeys ? a.Hkv : a.Hq;
+  const int H = kKeys ? a.Hkv * a.parts : a.Hq;  // h of a key block: part Hkv + head
   if (bid >= packed_blocks(a.T, G::rows) * H) return false;
   h = static_cast<int>(bid % H);
   r0 = plan.first_row<G::rows, kKeys>(a, static_cast<int>(bid / H));
@@ -268,9 +269,12 @@ __global__ __launch_bounds__(G::threads, D > 64 || G::slices > 1 ? 2 : 3) void p
   const int lane = threadIdx.x & 63, set = (threadIdx.x >> 6) % G::sets, l16 = lane & 15, q4 = lane >> 4;
   const int slice = threadIdx.x / (64 * G::sets), at = 16 * G::pieces * slice;
   const PackedPlan plan(a);
-  int k0, hk;
-  if (!block_of<G, true>(a, plan, k0, hk)) return;
-  const int n_rep = a.Hq / a.Hkv, my_k = k0 + 16 * set + l16, d = a.d;
+  int k0, in_block;
+  if (!block_of<G, true>(a, plan, k0, in_block)) return;
+  const int hk = in_block % a.Hkv, part = in_block / a.Hkv;
+  // this part's query heads
+  const int n_rep = a.Hq / a.Hkv / a.parts, h_first = (hk * a.parts + part) * n_rep;
+  const int my_k = k0 + 16 * set + l16, d = a.d;
   const bool in = my_k < a.T;
   const int my_lo = in ? plan.query_lo(a, my_k) : 1, my_hi = in ? plan.query_hi(a, my_k) : 0;
   float4 k[D / 16], v[D / 16];
@@ -288,7 +292,7 @@ __global__ __launch_bounds__(G::threads, D > 64 || G::slices > 1 ? 2 : 3) void p
   TileReg<D, kVec, G::tile, G::threads> qr, gr;
   float lr = 0.f, dr = 0.f;
   auto load = [&](int it) __attribute__((always_inline)) {
-    const int hq = hk * n_rep + it / nt, r0 = lo + it % nt * G::tile;
+    const int hq = h_first + it / nt, r0 = lo + it % nt * G::tile;
     qr.load(static_cast<const float*>(a.q) + hq * a.q_h, a.q_s, r0, plan.n, d);
     gr.load(static_cast<const float*>(a.dout) + hq * a.do_h, a.do_s, r0, plan.n, d);
     if (threadIdx.x < G::tile) {
@@ -339,11 +343,13 @@ __global__ __launch_bounds__(G::threads, D > 64 || G::slices > 1 ? 2 : 3) void p
   join<G, D>(dk_sum, dk, tiles, set, slice);
   if (G::slices > 1) __syncthreads();
   join<G, D>(dv_sum, dv, tiles, set, slice);
-  if (!in || (my_k >= plan.n && a.keep_tail)) return;
-  store_row<D, kVec>(static_cast<float*>(a.dk) + hk * a.dk_h + my_k * a.dk_s, dk_sum, a.scale, d,
-                     slice * (D / 16 / G::slices));
-  store_row<D, kVec>(static_cast<float*>(a.dv) + hk * a.dv_h + my_k * a.dv_s, dv_sum, 1.f, d,
-                     slice * (D / 16 / G::slices));
+  const bool whole = a.parts == 1;
+  if (!in || (my_k >= plan.n && (a.keep_tail || !whole))) return;
+  const int64_t at_part = ((static_cast<int64_t>(part) * a.T + my_k) * a.Hkv + hk) * d;
+  float* dkp = whole ? static_cast<float*>(a.dk) + hk * a.dk_h + my_k * a.dk_s : a.dk_part + at_part;
+  float* dvp = whole ? static_cast<float*>(a.dv) + hk * a.dv_h + my_k * a.dv_s : a.dv_part + at_part;
+  store_row<D, kVec>(dkp, dk_sum, a.scale, d, slice * (D / 16 / G::slices));
+  store_row<D, kVec>(dvp, dv_sum, 1.f, d, slice * (D / 16 / G::slices));
 }
 
 #define ZK_PACKED_F32_OF(KERNEL, G, HEADS)                                                \
@@ -379,7 +385,7 @@ void launch_packed_bwd_f32(const PackedArgs& a, hipStream_t s) {
                                  a.dq_s, a.dq_h, a.dk_s, a.dk_h, a.dv_s, a.dv_h},
                            {a.q, a.k, a.v, a.o, a.dout, a.dq, a.dk, a.dv});
   ZK_PACKED_F32(packed_dq_f32, a.Hq);
-  ZK_PACKED_F32(packed_dkdv_f32, a.Hkv);
+  ZK_PACKED_F32(packed_dkdv_f32, a.Hkv * a.parts);
 }
 
 }  // namespace zk
