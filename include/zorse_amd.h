@@ -648,8 +648,9 @@ int zk_rope_axes(const zk_axes_desc* desc, const void* q, const void* k, void* q
  * optimizer step that takes them (no counterpart in the reference; beside the
  * AdamW steps).  X = u / (|u| + eps) with the Frobenius norm, then `steps` times
  *     X <- a X + (b X X^T + c (X X^T)^2) X     (X^T X on the right for tall ones)
- * in fp16 products with fp32 sums, X in 22 bits; matrices whose shorter side is at
- * most 128, and those with fp32 results, in 22 bits throughout.
+ * in fp16 products with fp32 sums, X in 22 bits (elements below 2^-18 keep fewer);
+ * matrices whose shorter side is at most 128, and those with fp32 results, in 22 bits
+ * throughout, so that the fp32 sums weigh most.
  *   zk_orthogonalize:  out = X of u = grad
  *   zk_muon_multi:     m = momentum m + (1 - momentum) grad
  *                      u = (1 - momentum) grad + momentum m   (nesterov), or m

@@ -299,3 +299,89 @@ def test_refusals_on_the_gpu(dev):
         K.orthogonalize([a], coefficients=(9.0, 0.0, 0.0))
     with pytest.raises(ValueError, match="differ in length"):
         K.muon_multi([a], [], [b], **kw)
+
+
+def _in_fp32_sums(p, q, run):
+    """p q^T of operands in two numbers as the kernels add them: hi hi, hi lo and lo
+    hi one after another into fp32 sums, each rounded after every `run` products."""
+    acc = torch.zeros(p[0].shape[0], q[0].shape[0], dtype=torch.float64, device=p[0].device)
+    for i, j in ((0, 0), (0, 1), (1, 0)):
+        for k in range(0, p[0].shape[1], run):
+            acc = (acc + p[i][:, k:k + run] @ q[j][:, k:k + run].T.contiguous()).float().double()
+    return acc
+
+
+def _near_on_gpu(got, u, dt, what):
+    """_near for large sizes, the references on the GPU.  With an fp32 result the fp32
+    sums weigh more than the two numbers (for a few strong directions over noise,
+    whose small values grow 400 times over the steps), so the steps are taken with
+    them: an instruction adds 32 products to a sum; it is allowed to round it after
+    every four, and the norm of the error may be 1.5 times that of such steps.  X is
+    scaled by 2^15, G and P by S and R."""
+    got, u = got.double(), u.double()
+    ref = _exact(u)
+    norm = float(ref.norm())
+    if dt == F4:
+        sx, tall = 2.0 ** 15, u.shape[0] > u.shape[1]
+        x = u * float(torch.tensor(sx / (float(u.norm()) + 1e-7), dtype=F4))
+        hi, lo = _two((x.T if tall else x).contiguous())
+        for _ in range(5):
+            g = _two(_in_fp32_sums((hi, lo), (hi, lo), 4) * (S / sx) ** 2)
+            p = _two(C * R / S ** 4 * _in_fp32_sums(g, g, 4) + B * R / S ** 2 * (g[0] + g[1]))
+            px = _in_fp32_sums(p, (hi.T.contiguous(), lo.T.contiguous()), 4)
+            hi, lo = _two((A * (hi + lo) + px / R).float().double())
+        fmt = (hi + lo) / sx
+        fmt = fmt.T if tall else fmt
+    else:
+        fmt = _rounded(u, False)
+    bound = 1.5 * float((fmt - ref).norm()) + torch.finfo(dt).eps / 2 * norm
+    off = float((got - ref).norm())
+    assert off <= bound, f"{what}: {off / norm:.2e} off, {bound / norm:.2e} allowed"
+    assert float((got - ref).abs().max()) <= 40 * bound / math.sqrt(ref.numel()) + \
+        torch.finfo(dt).eps * float(ref.abs().max())
+
+
+@pytest.mark.parametrize("m,n", [(2048, 2048), (2816, 1024)])
+def test_fp32_results_of_large_matrices(dev, m, n):
+    """Eight strong directions over noise."""
+    from zorse_amd import kernels as K
+    g = torch.Generator().manual_seed(m)
+    mk = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    u = (1e-3 * (mk(m, 8) @ mk(8, n) + 0.01 * mk(m, n))).float().to(dev)
+    _near_on_gpu(K.orthogonalize([u])[0], u, F4, f"{m} x {n}")
+
+
+@pytest.mark.parametrize("m,n", [(200, 230), (90, 60)])
+def test_small_elements_keep_their_bits(dev, m, n):
+    """One element in each row and column, so that no sum is rounded and each goes
+    its own way: z <- a z + P z, P = b z^2 + c z^4.  A step rounds an element in two
+    numbers (2^-23 of itself, where the second is a normal one: scaled by 2^15, from
+    2^-18 on), P twice so (P and z^2: 2^-22 of it at most) and in fp32, the product and
+    the sum (2^-24 of their magnitudes).  Relative to a z + P z that is below 2^-21 while
+    P is small, and where |P| is up to 3.1, in the last two steps, (a + |P|) / (a + P) <
+    6 times as much over two: 3 early steps and the scaling 4 2^-21, two late ones 6 2^-21."""
+    from zorse_amd import kernels as K
+    k = min(m, n)
+    g = torch.Generator().manual_seed(k)
+    z = torch.logspace(0, -4.5, k, dtype=torch.float64) * (1 - 2 * (torch.arange(k) % 2)) * 0.4
+    rows, cols = torch.randperm(m, generator=g)[:k], torch.randperm(n, generator=g)[:k]
+    u = torch.zeros(m, n)
+    u[rows, cols] = z.float()
+    got = K.orthogonalize([u.to(dev)])[0].cpu().double()
+    ref = _exact(u)
+    small = (u[rows, cols].double() / u.double().norm()).abs()
+    small = (small < 0.002) & (small > 2.0 ** -18)
+    assert int(small.sum()) > k // 3
+    x, y = got[rows, cols][small], ref[rows, cols][small]
+    assert float(((x - y) / y).abs().max()) <= 10 * 2.0 ** -21
+    got[rows, cols] = 0
+    assert not bool(got.any())
+
+
+def test_tiny_matrices_without_eps(dev):
+    """The scale of X over the norm leaves fp32's range."""
+    from zorse_amd import kernels as K
+    u = _matrix(200, 300, "noise", 1) * 1e-34
+    got = K.orthogonalize([u.to(dev)], eps=0.0)[0].cpu().double()
+    ref = _exact(u.double(), eps=0.0)
+    assert float((got - ref).norm()) <= 2e-4 * float(ref.norm())

@@ -11,13 +11,17 @@
 //
 // Numbers.  The products' operands are fp16, with sums in fp32: singular values
 // lie below 1.3, so scaled by powers of two that the host takes from the
-// polynomial's bounds (X by S, G with it by S^2, P by R) they use fp16's whole
+// polynomial's bounds (X by Sx, G by S^2, P by R) they use fp16's whole
 // range, and its step is an eighth of bf16's at the same rate.  X itself is held
 // in two fp16 numbers (22 bits), and a X is added in fp32: small singular values
 // grow by a = 3.4 a step, and a rounding of X relative to the largest ones would
 // grow with them (a matrix of 8 strong directions over noise a hundredth as
 // large: 3.6e-2 off with X in one fp16 number, 0.3 in bf16, 3e-4 like this; other
-// spectra 0.3 - 1.7e-3).  Matrices with s <= kExactSide, whose products cost no
+// spectra 0.3 - 1.7e-3).  The second number has its bits only where the first is
+// above 2^-3 (below that it is subnormal): X's elements, about 1 / sqrt(t), need
+// the largest scale there is, 2^15 for singular values up to 1.23 (2048 x 2048 of
+// that spectrum in two numbers throughout: 4.0e-5 off with Sx = 2^7, S's, and
+// 7e-6 with 2^15).  Matrices with s <= kExactSide, whose products cost no
 // time, and results in fp32 have G and P in two numbers as well, and products of
 // three terms.
 //
@@ -58,7 +62,7 @@ struct MatrixGroup {
   Matrix p[gemm::kPolyMost];
   int first[gemm::kPolyMost + 1];
   int n;
-  float mu, nu, keep, lr, scale, eps;  // nu = 1 - mu, keep = 1 - lr weight_decay
+  float mu, nu, keep, lr, scale, eps;  // nu = 1 - mu, keep = 1 - lr weight_decay; scale: Sx
   int nesterov;
 };
 
@@ -199,12 +203,14 @@ __global__ __launch_bounds__(256) void muon_scale_kernel(MatrixGroup g) {
     }
   }
   __syncthreads();
-  const float f = static_cast<float>(g.scale / (sqrt(total) + static_cast<double>(g.eps)));
+  // in 64 bits: Sx / |u| may leave fp32's range where u Sx / |u| does not
+  const double f = g.scale / (sqrt(total) + static_cast<double>(g.eps));
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int r = row0 + 16 * k;
     if (x.tall) v[k] = make_float4(tile[col][r], tile[col + 1][r], tile[col + 2][r], tile[col + 3][r]);
-    float y[4] = {v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f};
+    float y[4] = {static_cast<float>(v[k].x * f), static_cast<float>(v[k].y * f),
+                  static_cast<float>(v[k].z * f), static_cast<float>(v[k].w * f)};
     f16x4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -338,9 +344,9 @@ void plan_run(const zk_muon_matrix* list, int n, Sides* d) {
   }
 }
 
-// Bounds of the polynomial's iterates on [0, 1]: the powers of two that S^2 G and
-// R P stay in fp16's range with.  False: the iterates leave it.
-bool scales_of(int steps, double a, double b, double c, float* S, float* R) {
+// Bounds of the polynomial's iterates on [0, 1]: the powers of two that Sx X, S^2 G
+// and R P stay in fp16's range with.  False: the iterates leave it.
+bool scales_of(int steps, double a, double b, double c, float* Sx, float* S, float* R) {
   if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c))) return false;
   double most = 1.0, most_p = 0, most_l = 1.0;
   for (int k = 0; k < steps; ++k) {
@@ -354,7 +360,8 @@ bool scales_of(int steps, double a, double b, double c, float* S, float* R) {
     most = next * 1.02;  // between the samples, and roundings
     most_l = fmax(most_l, most * most);
   }
-  // S = 2^i, S^2 most_l < 2^15.5; R = 2^j
+  // Sx = 2^h, Sx^2 most_l < 2^31; S = 2^i, S^2 most_l < 2^15.5; R = 2^j
+  *Sx = static_cast<float>(exp2(floor(log2(46000.0 / sqrt(most_l)))));
   *S = static_cast<float>(exp2(floor(0.5 * log2(46000.0 / most_l))));
   *R = most_p > 0 ? static_cast<float>(exp2(fmin(13.0, floor(log2(46000.0 / most_p))))) : 1.f;
   return true;
@@ -396,8 +403,8 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
   if (rc != ZK_OK) return rc;
   ZK_REQUIRE(h.steps >= 1 && h.steps <= 100, ZK_EINVAL, "%s: %d steps (1 .. 100)", who, h.steps);
   ZK_REQUIRE(h.eps >= 0, ZK_EINVAL, "%s: eps must not be negative", who);
-  float S, R;
-  ZK_REQUIRE(scales_of(h.steps, h.a, h.b, h.c, &S, &R), ZK_EINVAL,
+  float Sx, S, R;
+  ZK_REQUIRE(scales_of(h.steps, h.a, h.b, h.c, &Sx, &S, &R), ZK_EINVAL,
              "%s: the polynomial (%g, %g, %g) grows beyond 16 within %d steps", who, h.a, h.b, h.c, h.steps);
   if (n == 0) return ZK_OK;
   const int64_t need = zk_muon_workspace(list, n);
@@ -414,7 +421,7 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
     m.n = len;
     m.mu = static_cast<float>(h.mu); m.nu = static_cast<float>(1 - h.mu);
     m.keep = static_cast<float>(1 - h.lr * h.decay);
-    m.lr = static_cast<float>(h.lr); m.scale = S; m.eps = static_cast<float>(h.eps);
+    m.lr = static_cast<float>(h.lr); m.scale = Sx; m.eps = static_cast<float>(h.eps);
     m.nesterov = h.nesterov;
     for (int i = 0; i < len; ++i) {
       const zk_muon_matrix& x = list[at + i];
@@ -476,7 +483,7 @@ int run_list(const char* who, const zk_muon_matrix* list, int64_t n, bool step, 
           q.a = q.b = xh; q.a2 = q.b2 = xl;
           q.lda = q.ldb = e.tp; q.K = e.tp; q.N = e.sp;
           q.c = G[0][i]; q.c2 = G[1][i]; q.ldc = e.sp;
-          q.alpha = 1.f; q.tri = 1;
+          q.alpha = S * S / (Sx * Sx); q.tri = 1;
         } else if (which == 1) {
           q.a = q.b = q.r = G[0][i]; q.a2 = q.b2 = q.z = G[1][i];
           q.lda = q.ldb = e.sp; q.K = e.sp; q.N = e.sp;

@@ -990,7 +990,9 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=MUON_COEFFICIENTS, e
     ``matrices``: 2-D tensors with unit column stride in any of the three types;
     results in ``dtype`` (default each matrix' own) or in ``outs``.  Products are
     fp16 with fp32 sums, off by 0.3 - 1.7e-3 of the factor; with fp32 results, or
-    a side of at most 128, by 1e-5."""
+    a side of at most 128, in two fp16 numbers each, off by what the fp32 sums leave:
+    1e-6, and where a few strong directions lie over small ones, which grow, more
+    (8 over noise a hundredth as large: 6e-5 at 2048 x 2048)."""
     return _abi.nodes().orthogonalize(matrices, outs, dtype, steps, *coefficients, eps)
 
 
