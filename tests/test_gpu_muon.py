@@ -385,3 +385,13 @@ def test_tiny_matrices_without_eps(dev):
     got = K.orthogonalize([u.to(dev)], eps=0.0)[0].cpu().double()
     ref = _exact(u.double(), eps=0.0)
     assert float((got - ref).norm()) <= 2e-4 * float(ref.norm())
+
+
+def test_symmetric_products_in_large_tiles(dev):
+    """Sides of 2305 and more, in launches of over 512 tiles of 128 x 128 even for G
+    and P: 256 x 256 tiles and their transposed copies, whole and padded."""
+    from zorse_amd import kernels as K
+    for m, n in ((2500, 2600), (2560, 2560)):
+        us = [_matrix(m, n, "noise", 3 * m + i, BF).to(dev) for i in range(3)]
+        for u, o in zip(us, K.orthogonalize(us, dtype=FP)):
+            _near_on_gpu(o, u, FP, f"{m} x {n}")
