@@ -7,7 +7,7 @@
 // tokens: dQ 750 us (3 products, 1100 TFLOP/s), dK / dV 1040 (4, 1057), their sums
 // 29; documents of 30 to 2500 of 4096 tokens, 32 heads: 74 and 100, where the blocks
 // of the longest document end last.  P and dS are rounded to the storage type as
-// operands of the products that follow, with fp32 sums.
+// operands of the products that follow, with fp32 sums; in fp16 scaled first (kScaled).
 #include <type_traits>
 
 #include "attn_packed.h"
@@ -43,6 +43,38 @@ __device__ __forceinline__ typename Mfma<T>::vec8 tr_operand(const T* X, int off
   const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + 8 * D * 2 + (off ^ 32)));
   const s16x8 w = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
   return __builtin_bit_cast(typename Mfma<T>::vec8, w);
+}
+
+// fp16's range.  P (dP - delta) may leave it: dO may be small or large, and P is about
+// 1 / T.  So fp16 operands are scaled by powers of two, which the results take out
+// again (in bf16, with fp32's range, nothing is scaled):
+//  * P by 2^kPShift where dK / dV round it (P is at most 1), with the LSE that dQ
+//    leaves for them;
+//  * dS by 2^e, where e is the row's own and follows the largest of its dS so far, as
+//    the reference maximum of a softmax does: above 2^15 it moves so that this one lies
+//    in [2^7, 2^8).  A dS is then off by half a step of itself, or by 2^-31 of its row's
+//    largest so far.
+// dO of size 1e-4, 1500 tokens: dQ off by 6e-4 of itself, 1.4e-2 without; the forward and
+// both kernels at 8000 tokens, window 1024, 32 heads of 64: 378 us, 367 without.
+template <typename T>
+constexpr bool kScaled = std::is_same<T, f16>::value;
+template <typename T>
+constexpr float kPShift = kScaled<T> ? 15.f : 0.f;
+constexpr float kFirstE = 60.f;  // any row's first dS moves it but for one below 2^-45
+
+// For 16 scaled dS of a lane's row: what e moves by, 0 or less (both halves of a row
+// alike; the common case, no row of the wave moves, is false).
+__device__ __forceinline__ bool moved_e(const f32x16& w, float& by) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) m = fmaxf(fmaxf(m, fabsf(w[j])), fabsf(w[j + 1]));
+  if (!__any(m > 32768.f)) return false;
+  m = 0.f;  // of those that are finite
+#pragma unroll
+  for (int j = 0; j < 16; ++j) m = fmaxf(m, fabsf(w[j]) < INFINITY ? fabsf(w[j]) : 0.f);
+  m = fmaxf(m, other_half(m));
+  by = m > 32768.f ? 134.f - static_cast<float>(__float_as_uint(m) >> 23) : 0.f;
+  return true;
 }
 
 // Adds the second group's accumulators (waves 4 .. 7) to the first's, through four
@@ -148,10 +180,11 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
       lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
       if (g == 0 && k_off == 0) {
         a.delta[i] = del;
-        a.lse2[i] = lse2;
+        a.lse2[i] = lse2 - kPShift<T>;
       }
     }
   }
+  float e_q = kScaled<T> ? kFirstE : 0.f, lse2_e = lse2 - e_q;
 
   const int n_t = kv_hi > kv_lo ? (kv_hi - kv_lo + TN - 1) / TN : 0;
   PackedLoader<T, D, TN, NT> kload, vload;
@@ -215,13 +248,29 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
       V8 sb[2];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -lse2));
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -lse2_e));
         float w = p * (dp[j] - del);
         if (need_mask) {
           const int rel = k0 - vis_lo + 32 * tt + 8 * (j >> 2) + 4 * g + (j & 3);
           if (static_cast<unsigned>(rel) > static_cast<unsigned>(vis_span)) w = 0.f;
         }
-        sb[j >> 3][j & 7] = static_cast<T>(w);
+        if constexpr (kScaled<T>)
+          dp[j] = w;
+        else
+          sb[j >> 3][j & 7] = static_cast<T>(w);
+      }
+      if constexpr (kScaled<T>) {
+        float by;
+        if (moved_e(dp, by)) {
+          const float f = __builtin_amdgcn_exp2f(by);
+          e_q += by;
+          lse2_e = lse2 - e_q;
+          dp *= f;
+#pragma unroll
+          for (int nt = 0; nt < NB; ++nt) dq[nt] *= f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sb[j >> 3][j & 7] = static_cast<T>(dp[j]);
       }
       constexpr int NM = 2 * NB;
       auto trread = [&](int m) __attribute__((always_inline)) {
@@ -247,6 +296,11 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
     if (t + 1 < n_t) step(std::integral_constant<int, 1>{}, t + 1);
   }
 
+  if constexpr (kScaled<T>) {
+    const float f = __builtin_amdgcn_exp2f(-e_q);
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt) dq[nt] *= f;
+  }
   if constexpr (kSplit) {
     __syncthreads();  // every wave is past its last product
     if (!join_groups<TN * D * 2>(dq, K0, K1, V0, V1)) return;
@@ -350,6 +404,7 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
     dk[nt] = f32x16{};
     dv[nt] = f32x16{};
   }
+  float e_k = kFirstE, f_k = __builtin_amdgcn_exp2f(kFirstE - kPShift<T>);  // e and 2^(e - kPShift)
   const int rbase = 2 * (tile_off<D>(l32, 8 * g) + q_off * D);
   const int tbase =
       2 * (tile_off<D>(4 * g + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) + q_off * D);
@@ -431,8 +486,24 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
           const int j = 4 * a4 + e;
           const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -lv[e]));
           pb[j >> 3][j & 7] = static_cast<T>(p);
-          sb[j >> 3][j & 7] = static_cast<T>(p * (dp[j] - dl[e]));
+          if constexpr (kScaled<T>)
+            dp[j] = p * ((dp[j] - dl[e]) * f_k);
+          else
+            sb[j >> 3][j & 7] = static_cast<T>(p * (dp[j] - dl[e]));
         }
+      }
+      if constexpr (kScaled<T>) {
+        float by;
+        if (moved_e(dp, by)) {
+          const float f = __builtin_amdgcn_exp2f(by);
+          e_k += by;
+          f_k *= f;
+          dp *= f;
+#pragma unroll
+          for (int nt = 0; nt < NB; ++nt) dk[nt] *= f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sb[j >> 3][j & 7] = static_cast<T>(dp[j]);
       }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -466,6 +537,14 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
     }
   }
 
+  if constexpr (kScaled<T>) {
+    const float f = __builtin_amdgcn_exp2f(-e_k);
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt) {
+      dk[nt] *= f;
+      dv[nt] *= 1.f / 32768.f;  // 2^-kPShift
+    }
+  }
   if constexpr (kSplit) {
     __syncthreads();
     const bool first = join_groups<TQ * D * 2>(dk, Q0, Q1, dO0, dO1);
@@ -506,7 +585,7 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
           const float s = dot_two_rows<T>(Kr, Qp + i * a.q_s, g, hd);
           const float dp = dot_two_rows<T>(Vr, Dp + i * a.do_s, g, hd);
           if (static_cast<unsigned>(i - vis_lo) > static_cast<unsigned>(vis_span)) continue;
-          const float p = __builtin_amdgcn_exp2f(fmaf(s, c2, -a.lse2[at + i]));
+          const float p = __builtin_amdgcn_exp2f(fmaf(s, c2, -a.lse2[at + i] - kPShift<T>));
           const float w = second ? p : p * (dp - a.delta[at + i]) * a.scale;
           for (int e = 0; e < 8; ++e)
             if (c0 + e < hd) acc[e] = fmaf(w, to_f32(rows_of[i * ld + c0 + e]), acc[e]);
