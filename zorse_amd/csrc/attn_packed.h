@@ -124,6 +124,15 @@ __device__ __forceinline__ void packed_block(const PackedArgs& a, int& block, in
                         : static_cast<int>(r);
 }
 
+// The lane's row and half of the wave once more: loops before that are short of registers
+// then need not keep what is made of them.
+__device__ __forceinline__ void relane(int& l32, int& g) {
+  int n = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(n));
+  l32 = n & 31;
+  g = n >> 5;
+}
+
 // Tile loads (asynchronous, global memory to LDS) of ROWS tokens from token g0
 // on: rows at or past `nrows` and, for a head dim d < D (KR != 0), chunks past
 // the head arrive as zeros, the offsets of a chunk that straddles its end as
@@ -161,27 +170,30 @@ struct PackedLoader {
   }
 };
 
-// This lane's 8 elements 16 ks + 8 g .. of each step of a row of d (null: zeros).
+// Whether step ks of a ragged head (its columns 16 ks .. 16 ks + 15) may hold elements
+// from d on (d above 16 KR - 16, or any for the smallest KR, 2).
+template <int KR>
+__host__ __device__ constexpr bool ragged_step(int ks) {
+  return KR != 0 && (ks >= KR - 1 || KR == 2);
+}
+
+// This lane's 8 elements 16 ks + 8 g .. of a row of d (null: zeros), and those of each
+// step.
+template <typename T, int KR>
+__device__ __forceinline__ typename Mfma<T>::vec8 operand_step(const T* row, int ks, int g, int d) {
+  typedef typename Mfma<T>::vec8 V8;
+  if (row == nullptr) return V8{};
+  typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+  if (ragged_step<KR>(ks)) return load_cols8<T>(row, 16 * ks + 8 * g, d);
+  if constexpr (KR != 0)
+    return __builtin_bit_cast(V8, static_cast<u32x4>(*reinterpret_cast<const u32x4_a4*>(row + 16 * ks + 8 * g)));
+  return *reinterpret_cast<const V8*>(row + 16 * ks + 8 * g);
+}
 template <typename T, int KS, int KR>
 __device__ __forceinline__ void load_operand(typename Mfma<T>::vec8 (&x)[KS], const T* row, int g,
                                              int d) {
-  typedef typename Mfma<T>::vec8 V8;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    if (row == nullptr)
-      x[ks] = V8{};
-    else if constexpr (KR != 0)
-      x[ks] = load_cols8<T>(row, 16 * ks + 8 * g, d);
-    else
-      x[ks] = *reinterpret_cast<const V8*>(row + 16 * ks + 8 * g);
-  }
-}
-
-// Whether step ks of a ragged head may hold elements from d on (d above 16 KR -
-// 16, or any for the smallest KR, 2).
-template <int KR>
-__host__ __device__ constexpr bool ragged_step(int ks) {
-  return KR != 0 && (ks == KR - 1 || KR == 2);
+  for (int ks = 0; ks < KS; ++ks) x[ks] = operand_step<T, KR>(row, ks, g, d);
 }
 
 // Stores this lane's accumulators (elements 32 nt + 8 (j / 4) + 4 g + j % 4 of a
@@ -198,39 +210,162 @@ __device__ __forceinline__ void store_accumulators(T* row, const f32x16 (&x)[NB]
       T4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(x[nt][4 * a4 + e] * scale);
-      if constexpr (KR != 0)
+      typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+      if (ragged_step<KR>(2 * nt + a4 / 2))
         store_cols4(row, d0, d, w);
+      else if constexpr (KR != 0)
+        *reinterpret_cast<u32x2_a4*>(row + d0) = __builtin_bit_cast(u32x2, w);
       else
         *reinterpret_cast<T4*>(row + d0) = w;
     }
 }
 
+// ---- Rows with a NaN ("odd": an infinity or a NaN).
+// A masked probability is an exact zero, and the matrix product adds its product with
+// the masked row as well: NaN where that row holds an odd element.  So a wave that finds
+// a NaN among its rows' results (row_has_nan) asks whether a masked row can be the
+// cause: whether among the tokens that it met and some row does not see any is odd.
+// These are few (the tiles on the diagonal and at sequences' ends), so a pass whose
+// results are NaN by right, as those of a step that overflows under a loss scale are,
+// takes no longer.  Where one is, the wave takes its rows once more, in tiles of 32
+// tokens from global memory: in tiles that some row does not see, the product takes
+// zeros for the odd elements (add_columns), and those that are seen are added one by one
+// (add_odd); but a row that sees all of a tile takes its product, and one that sees
+// nothing of it leaves it out.  It ends early when every element is NaN.
+//   32 heads of 128 over 8 key heads, 8192 causal tokens, forward and backward 2.3 - 2.6
+// ms: with a NaN in the last row of dO 2.5, an infinity in one of its middle 6.0 and a
+// NaN in its first (which all keys of the first tile but one do not see) 9.8, NaN in all
+// of q, k, v or dO 2.3 - 2.7, infinities in all of v 8.4.
+
 // Whether a lane's row (both halves of it) holds a NaN in its first d elements.
-// A masked probability is an exact zero, and the matrix product adds its
-// product with the masked row as well: NaN where that row holds an infinity or
-// a NaN.  Such rows are computed again from what they see alone, 16 columns at a
-// time (few registers, so that the loops before keep theirs; no one waits for it).
-template <int NB>
+template <int NB, int KR>
 __device__ __forceinline__ bool row_has_nan(const f32x16 (&x)[NB], int g, int d) {
   bool bad = false;
 #pragma unroll
   for (int nt = 0; nt < NB; ++nt)
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      bad |= 32 * nt + 8 * (j >> 2) + 4 * g + (j & 3) < d && x[nt][j] != x[nt][j];
+      bad |= (!ragged_step<KR>(2 * nt + j / 8) || 32 * nt + 8 * (j >> 2) + 4 * g + (j & 3) < d) &&
+             x[nt][j] != x[nt][j];
   const uint64_t b = __ballot(bad);
   return ((b >> (threadIdx.x & 31)) | (b >> ((threadIdx.x & 31) + 32))) & 1;
 }
 
-// x . y of two rows of d elements, each half of the wave taking half of them.
+// Whether all of this lane's elements below d are NaN, of the columns from c0 on (not 0
+// for one block of 32 only).
+template <int NB, int KR>
+__device__ __forceinline__ bool all_nan(const f32x16 (&x)[NB], int c0, int g, int d) {
+  bool all = true;
+#pragma unroll
+  for (int nt = 0; nt < NB; ++nt)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const bool may_end = KR != 0 && (NB == 1 || ragged_step<KR>(2 * nt + j / 8));
+      all &= (may_end && c0 + 32 * nt + 8 * (j >> 2) + 4 * g + (j & 3) >= d) || x[nt][j] != x[nt][j];
+    }
+  return all;
+}
+
+// Stores one block of accumulators, the columns from c0 on, scaled.
 template <typename T>
-__device__ __forceinline__ float dot_two_rows(const T* x, const T* y, int g, int d) {
-  float s = 0.f;
+__device__ __forceinline__ void store_block(T* row, const f32x16& x, float scale, int c0, int g, int d) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int c = c0 + 8 * (j >> 2) + 4 * g + (j & 3);
+    if (c < d) row[c] = static_cast<T>(x[j] * scale);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool is_odd(T x) {
+  return !(fabsf(to_f32(x)) < INFINITY);
+}
+template <typename T>
+__device__ __forceinline__ bool any_odd(typename Mfma<T>::vec8 x) {
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) odd |= is_odd<T>(x[e]);
+  return odd;
+}
+
+// Bit r: row r0 + r of X (below past) holds an odd element and lies outside
+// [in_lo, in_hi].
+template <typename T, int KS, int KR>
+__device__ __forceinline__ uint32_t odd_rows(const T* X, int64_t ld, int r0, int past, int in_lo, int in_hi,
+                                             int g, int d) {
+  const int r = r0 + static_cast<int>(threadIdx.x & 31);
+  const T* row = r < past && (r < in_lo || r > in_hi) ? X + r * ld : nullptr;
+  bool odd = false;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) odd |= any_odd<T>(operand_step<T, KR>(row, ks, g, d));
+  const uint64_t b = __ballot(odd);
+  return static_cast<uint32_t>(b | b >> 32);
+}
+
+// A column, which the compiler does not know: nothing made of it is kept outside the
+// loops around.
+__device__ __forceinline__ int column(int c) {
+  asm volatile("" : "+s"(c));
+  return c;
+}
+
+// acc += X^T w of the columns from c0 on of 32 rows of X from r0 on, as tr_operand's
+// products; kept: with odd
+// elements, for the lanes that see all of the rows (the others see none of them), else
+// with zeros in their place.  Rows from past on, which are not kept and whose weights are
+// zero, are read as the last one; columns from d on, which nothing stores, as the last one.
+template <typename T, int NB>
+__device__ __forceinline__ void add_columns(f32x16 (&acc)[NB], const T* X, int64_t ld, int r0, int past,
+                                            int c0, const typename Mfma<T>::vec8 (&w)[2], bool kept,
+                                            bool sees_all, int g, int d) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt) {
+      __builtin_amdgcn_sched_barrier(0);  // one block's loads at a time: few registers
+      const int c = column(c0 + 32 * nt) + static_cast<int>(threadIdx.x & 31), at = c < d ? c : d - 1;
+      typename Mfma<T>::vec8 x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = r0 + 16 * kk + 8 * (e >> 2) + 4 * g + (e & 3);
+        x[e] = X[(r < past ? r : past - 1) * ld + at];
+        if (!kept && is_odd<T>(x[e])) x[e] = static_cast<T>(0.f);
+      }
+      const f32x16 sum = Mfma<T>::mma(x, w[kk], acc[nt]);
+      const bool mine = !kept || sees_all;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[nt][j] = mine ? sum[j] : acc[nt][j];
+    }
+}
+
+// acc += weight X[r] of the odd elements of these columns of the rows r0 + (bits of rows)
+// that the lane's row sees.  weights: of the tile's 32 rows, where the products leave
+// them (row 8 (j / 4) + 4 g + j % 4).
+template <typename T, int NB, typename S>
+__device__ __forceinline__ void add_odd(f32x16 (&acc)[NB], const T* X, int64_t ld, int r0, uint32_t rows,
+                                        int c0, const f32x16& weights, S&& seen, int g, int d) {
 #pragma unroll 1
-  for (int c = 8 * g; c < d; c += 16)
-    for (int e = 0; e < 8; ++e)
-      if (c + e < d) s = fmaf(to_f32(x[c + e]), to_f32(y[c + e]), s);
-  return s + other_half(s);
+  while (rows != 0) {
+    const int at = __builtin_ctz(rows), r = r0 + at;
+    rows &= rows - 1;
+    float w = weights[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) w = (at >> 3) * 4 + (at & 3) == j ? weights[j] : w;
+    const float other = other_half(w);
+    if ((at >> 2 & 1) != g) w = other;
+    const bool mine = seen(r);
+    const T* row = X + r * ld;
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt) {
+      const int c_nt = column(c0 + 32 * nt) + 4 * g;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int c = c_nt + 8 * (j >> 2) + (j & 3);
+        const T x = row[c < d ? c : d - 1];
+        if (mine && is_odd<T>(x)) acc[nt][j] = fmaf(w, to_f32(x), acc[nt][j]);
+      }
+    }
+  }
 }
 
 }  // namespace zk

@@ -30,7 +30,7 @@ __device__ __forceinline__ void store_partial(float* row, const f32x16 (&x)[NB],
 #pragma unroll
     for (int a2 = 0; a2 < 8; ++a2) {
       const int d0 = 32 * nt + 8 * (a2 >> 1) + 4 * g + 2 * (a2 & 1);
-      if (KR == 0 || d0 < d)
+      if (!ragged_step<KR>(2 * nt + a2 / 4) || d0 < d)
         *reinterpret_cast<float2*>(row + d0) = make_float2(x[nt][2 * a2] * scale, x[nt][2 * a2 + 1] * scale);
     }
 }
@@ -124,7 +124,8 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
   const int hd = KR ? a.d : D;
   __shared__ __attribute__((aligned(16))) T K0[TN * D], K1[TN * D], V0[TN * D], V1[TN * D];
 
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63;
+  int l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const PackedPlan plan(a);
   int block, hq;
@@ -135,8 +136,8 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
   const int hk = hq / (a.Hq / a.Hkv);
   const int qw0 = q0 + 32 * (wave & 3);
   const int k_off = kSplit ? wave / 4 * BN : 0;  // this wave's keys in a step
-  const int my_q = qw0 + l32;
-  const bool in = my_q < rows;
+  int my_q = qw0 + l32;
+  bool in = my_q < rows;
   const float c2 = a.scale_log2;
 
   const int last = rows - 1;
@@ -305,29 +306,75 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dq_kernel(Packed
     __syncthreads();  // every wave is past its last product
     if (!join_groups<TN * D * 2>(dq, K0, K1, V0, V1)) return;
   }
+  relane(l32, g);
+  my_q = qw0 + l32;
+  in = my_q < rows;
   const bool put = in && (my_q < plan.n || !a.keep_tail);
   T* out = static_cast<T*>(a.dq) + hq * a.dq_h + my_q * a.dq_s;
-  const bool bad = row_has_nan<NB>(dq, g, hd);
+  const bool bad = put && row_has_nan<NB, KR>(dq, g, hd);
   if (put) store_accumulators<T, NB, KR>(out, dq, a.scale, g, hd);
-  if (__any(bad)) {  // see row_has_nan
-    const T* Qr = Qp + clip(my_q) * a.q_s;
-    const T* Dr = Dp + clip(my_q) * a.do_s;
+  if (__builtin_expect(!__any(bad), 1)) return;
+
+  // see row_has_nan.  A masked dS is zero whatever V and K hold, so only K's own odd
+  // elements are a cause.
+  auto seen = [&](int j) __attribute__((always_inline)) {
+    return static_cast<unsigned>(j - vis_lo) <= static_cast<unsigned>(vis_span);
+  };
+  auto by_all = [&](int k0) __attribute__((always_inline)) { return k0 >= f_lo && k0 + 31 <= f_hi; };
+  auto sees_all = [&](int k0) __attribute__((always_inline)) { return seen(k0) && seen(k0 + 31); };
+  // whether every row sees all of a tile or nothing of it
+  auto whole_rows = [&](int k0) __attribute__((always_inline)) {
+    return !__any(!sees_all(k0) && k0 + 31 >= vis_lo && k0 <= vis_lo + vis_span);
+  };
+  bool found = false;
+  {
+    const int t_lo = w_lo > kv_lo ? kv_lo + ((w_lo - kv_lo) & ~(BN - 1)) : kv_lo;
+    int past = kv_lo + ((w_hi - kv_lo) & ~(BN - 1)) + BN;
+    past = past < plan.n ? past : plan.n;
 #pragma unroll 1
-    for (int n = 0; n < KS; ++n) {  // both halves alike: they exchange sums
-      const int c = 16 * n + 8 * g;
-      float acc[8] = {};
+    for (int k0 = t_lo; k0 < past && !found; k0 += 32)
+      if (!by_all(k0)) found = odd_rows<T, KS, KR>(Kp, a.k_s, k0, past, f_lo, f_hi, g, hd) != 0;
+  }
+  if (__builtin_expect(!found, 1)) return;
 #pragma unroll 1
-      for (int j = w_lo; j <= w_hi; ++j) {
-        const float dp = dot_two_rows<T>(Dr, Vp + j * a.v_s, g, hd);
-        const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd);
-        if (static_cast<unsigned>(j - vis_lo) > static_cast<unsigned>(vis_span)) continue;
-        const float w = __builtin_amdgcn_exp2f(fmaf(s, c2, -lse2)) * (dp - del);
-        for (int e = 0; e < 8; ++e)
-          if (c + e < hd) acc[e] = fmaf(w, to_f32(Kp[j * a.k_s + c + e]), acc[e]);
+  for (int c0 = 0; c0 < hd; c0 += 32) {  // as in the forward
+    float e = kScaled<T> ? kFirstE : 0.f;
+    f32x16 acc[1] = {f32x16{}};
+#pragma unroll 1
+    for (int k0 = w_lo; k0 <= w_hi; k0 += 32) {
+      const T* kr = k0 + l32 <= w_hi ? Kp + (k0 + l32) * a.k_s : nullptr;
+      const T* vr = k0 + l32 <= w_hi ? Vp + (k0 + l32) * a.v_s : nullptr;
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = M::mma(operand_step<T, KR>(kr, ks, g, hd), qreg[ks], s);
+        dp = M::mma(operand_step<T, KR>(vr, ks, g, hd), dreg[ks], dp);
       }
-      for (int e = 0; e < 8; ++e)
-        if (bad && put && c + e < hd) out[c + e] = static_cast<T>(acc[e] * a.scale);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[j], c2, e - lse2)) * (dp[j] - del);
+        dp[j] = seen(k0 + 8 * (j >> 2) + 4 * g + (j & 3)) ? w : 0.f;
+      }
+      if constexpr (kScaled<T>) {
+        float by;
+        if (moved_e(dp, by)) {
+          const float f = __builtin_amdgcn_exp2f(by);
+          e += by;
+          dp *= f;
+          acc[0] *= f;
+        }
+      }
+      V8 w[2];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j >> 3][j & 7] = static_cast<T>(dp[j]);
+      const bool kept = whole_rows(k0);
+      add_columns<T, 1>(acc, Kp, a.k_s, k0, w_hi + 1, c0, w, kept, sees_all(k0), g, hd);
+      if (!kept)
+        add_odd<T, 1>(acc, Kp, a.k_s, k0, odd_rows<T, KS, KR>(Kp, a.k_s, k0, w_hi + 1, 1, 0, g, hd), c0, dp,
+                      seen, g, hd);
+      if (!__any(bad && !all_nan<1, KR>(acc, c0, g, hd))) break;
     }
+    if (bad) store_block<T>(out, acc[0], a.scale * __builtin_amdgcn_exp2f(-e), c0, g, hd);
   }
 }
 
@@ -351,7 +398,8 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
   __shared__ __attribute__((aligned(16))) float dels[2][NT / 64][64];
   __shared__ __attribute__((aligned(16))) T Vw[4][32 * D];
 
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63;
+  int l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const PackedPlan plan(a);
   const int block = blockIdx.x / (a.Hkv * a.parts), in_block = blockIdx.x % (a.Hkv * a.parts);
@@ -363,8 +411,8 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
   if (k0 >= rows) return;
   const int kw0 = k0 + 32 * (wave & 3);
   const int q_off = kSplit ? wave / 4 * (SUB * MQ) : 0;  // this wave's queries in a step
-  const int my_key = kw0 + l32;
-  const bool in = my_key < rows;
+  int my_key = kw0 + l32;
+  bool in = my_key < rows;
   const float c2 = a.scale_log2;
 
   const int last = rows - 1;
@@ -552,12 +600,15 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
     join_groups<TQ * D * 2>(dv, Q0, Q1, dO0, dO1);
     if (!first) return;
   }
+  relane(l32, g);
+  my_key = kw0 + l32;
+  in = my_key < rows;
   const bool whole = a.parts == 1;
   const bool put = in && (my_key < plan.n || (whole && !a.keep_tail));
   T* dkp = static_cast<T*>(a.dk) + hk * a.dk_h + my_key * a.dk_s;
   T* dvp = static_cast<T*>(a.dv) + hk * a.dv_h + my_key * a.dv_s;
   const int64_t at_part = ((static_cast<int64_t>(part) * a.T + my_key) * a.Hkv + hk) * hd;
-  const bool bad_k = row_has_nan<NB>(dk, g, hd), bad_v = row_has_nan<NB>(dv, g, hd);
+  const bool bad_k = put && row_has_nan<NB, KR>(dk, g, hd), bad_v = put && row_has_nan<NB, KR>(dv, g, hd);
   if (put && whole) {
     store_accumulators<T, NB, KR>(dkp, dk, a.scale, g, hd);
     store_accumulators<T, NB, KR>(dvp, dv, 1.f, g, hd);
@@ -565,42 +616,109 @@ __global__ __launch_bounds__(kSplit ? 512 : 256, 2) void packed_dkdv_kernel(Pack
     store_partial<NB, KR>(a.dk_part + at_part, dk, a.scale, g, hd);
     store_partial<NB, KR>(a.dv_part + at_part, dv, 1.f, g, hd);
   }
-  if (__any(bad_k | bad_v)) {  // see row_has_nan; dK, then dV
-    const T* Kr = Kp + clip(my_key) * a.k_s;
-    const T* Vr = Vp + clip(my_key) * a.v_s;
-#pragma unroll 1
-    for (int n = 0; n < 2 * KS; ++n) {
-      const bool second = n >= KS;
-      const int c0 = 16 * (second ? n - KS : n) + 8 * g;
-      float acc[8] = {};
-#pragma unroll 1
-      for (int h = h_first; h < h_first + n_rep; ++h) {
-        const T* Qp = static_cast<const T*>(a.q) + h * a.q_h;
-        const T* Dp = static_cast<const T*>(a.dout) + h * a.do_h;
-        const int64_t at = static_cast<int64_t>(h) * a.T;
-        const T* rows_of = second ? Dp : Qp;
-        const int64_t ld = second ? a.do_s : a.q_s;
-#pragma unroll 1
-        for (int i = w_lo; i <= w_hi; ++i) {
-          const float s = dot_two_rows<T>(Kr, Qp + i * a.q_s, g, hd);
-          const float dp = dot_two_rows<T>(Vr, Dp + i * a.do_s, g, hd);
-          if (static_cast<unsigned>(i - vis_lo) > static_cast<unsigned>(vis_span)) continue;
-          const float p = __builtin_amdgcn_exp2f(fmaf(s, c2, -a.lse2[at + i] - kPShift<T>));
-          const float w = second ? p : p * (dp - a.delta[at + i]) * a.scale;
-          for (int e = 0; e < 8; ++e)
-            if (c0 + e < hd) acc[e] = fmaf(w, to_f32(rows_of[i * ld + c0 + e]), acc[e]);
-        }
-      }
-      T* row = second ? dvp : dkp;
-      float* part_row = (second ? a.dv_part : a.dk_part) + at_part;
-      for (int e = 0; e < 8; ++e)
-        if ((second ? bad_v : bad_k) && put && c0 + e < hd) {
-          if (whole)
-            row[c0 + e] = static_cast<T>(acc[e]);
-          else
-            part_row[c0 + e] = acc[e];
-        }
+  if (__builtin_expect(!__any(bad_k | bad_v), 1)) return;
+
+  // see row_has_nan
+  auto seen = [&](int i) __attribute__((always_inline)) {
+    return static_cast<unsigned>(i - vis_lo) <= static_cast<unsigned>(vis_span);
+  };
+  auto by_all = [&](int i0) __attribute__((always_inline)) { return i0 >= f_lo && i0 + 31 <= f_hi; };
+  auto sees_all = [&](int i0) __attribute__((always_inline)) { return seen(i0) && seen(i0 + 31); };
+  // whether every row sees all of a tile or nothing of it
+  auto whole_rows = [&](int i0) __attribute__((always_inline)) {
+    return !__any(!sees_all(i0) && i0 + 31 >= vis_lo && i0 <= vis_lo + vis_span);
+  };
+  // products of 32 rows of X (those up to `top`) with an operand of the keys
+  auto products = [&](f32x16& c, const T* X, int64_t ld, int i0, int top, auto&& other) __attribute__((always_inline)) {
+    const T* row = i0 + l32 <= top ? X + (i0 + l32) * ld : nullptr;
+    c = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      c = M::mma(operand_step<T, KR>(row, ks, g, hd), other(ks), c);
     }
+  };
+  auto k_operand = [&](int ks) __attribute__((always_inline)) { return kreg[ks]; };
+  auto v_operand = [&](int ks) __attribute__((always_inline)) {
+    return *reinterpret_cast<const V8*>(&Vme[tile_off<D>(l32, 16 * ks + 8 * g)]);
+  };
+  bool found = false;
+  const int t_lo = w_lo > q_lo ? q_lo + ((w_lo - q_lo) & ~(MQ - 1)) : q_lo;
+  const int t_top = below(q_lo + ((w_hi - q_lo) & ~(MQ - 1)) + MQ - 1);
+#pragma unroll 1
+  for (int h = h_first; h < h_first + n_rep && !found; ++h) {
+    const T* Qp = static_cast<const T*>(a.q) + h * a.q_h;
+    const T* Dp = static_cast<const T*>(a.dout) + h * a.do_h;
+    const int64_t at = static_cast<int64_t>(h) * a.T;
+#pragma unroll 1
+    for (int i0 = t_lo; i0 <= t_top && !found; i0 += 32) {
+      if (by_all(i0)) continue;
+      f32x16 dp;
+      products(dp, Dp, a.do_s, i0, t_top, v_operand);
+      bool odd = false;  // a masked P or dS that is not zero
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int i = i0 + 8 * (j >> 2) + 4 * g + (j & 3), r = i < t_top ? i : t_top;
+        const float p = __builtin_amdgcn_exp2f(-INFINITY - a.lse2[at + r]);
+        odd |= !seen(i) && (p != 0.f || p * (dp[j] - a.delta[at + r]) != 0.f);
+      }
+      found = __any(odd) || (odd_rows<T, KS, KR>(Qp, a.q_s, i0, t_top + 1, f_lo, f_hi, g, hd) |
+                             odd_rows<T, KS, KR>(Dp, a.do_s, i0, t_top + 1, f_lo, f_hi, g, hd)) != 0;
+    }
+  }
+  if (__builtin_expect(!found, 1)) return;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // dK, then dV
+    const bool second = pass == 1, bad = second ? bad_v : bad_k;
+    if (!__any(bad)) continue;
+    const int64_t ld = second ? a.do_s : a.q_s;
+    float e = kFirstE, f_e = __builtin_amdgcn_exp2f(kFirstE - kPShift<T>);
+#pragma unroll
+    for (int nt = 0; nt < NB; ++nt) dk[nt] = f32x16{};
+    bool open = true;
+#pragma unroll 1
+    for (int h = h_first; h < h_first + n_rep && open; ++h) {
+      const T* Qp = static_cast<const T*>(a.q) + h * a.q_h;
+      const T* Dp = static_cast<const T*>(a.dout) + h * a.do_h;
+      const T* X = second ? Dp : Qp;
+      const int64_t at = static_cast<int64_t>(h) * a.T;
+#pragma unroll 1
+      for (int i0 = w_lo; i0 <= w_hi && open; i0 += 32) {
+        f32x16 s, dp;
+        products(s, Qp, a.q_s, i0, w_hi, k_operand);
+        products(dp, Dp, a.do_s, i0, w_hi, v_operand);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int i = i0 + 8 * (j >> 2) + 4 * g + (j & 3), r = i < w_hi ? i : w_hi;
+          float p = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -a.lse2[at + r]));
+          if (!second) p *= kScaled<T> ? (dp[j] - a.delta[at + r]) * f_e : dp[j] - a.delta[at + r];
+          s[j] = seen(i) ? p : 0.f;
+        }
+        if constexpr (kScaled<T>) {
+          float by;
+          if (!second && moved_e(s, by)) {
+            const float f = __builtin_amdgcn_exp2f(by);
+            e += by;
+            f_e *= f;
+            s *= f;
+#pragma unroll
+            for (int nt = 0; nt < NB; ++nt) dk[nt] *= f;
+          }
+        }
+        V8 w[2];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j >> 3][j & 7] = static_cast<T>(s[j]);
+        const bool kept = whole_rows(i0);
+        add_columns<T, NB>(dk, X, ld, i0, w_hi + 1, 0, w, kept, sees_all(i0), g, hd);
+        if (!kept)
+          add_odd<T, NB>(dk, X, ld, i0, odd_rows<T, KS, KR>(X, ld, i0, w_hi + 1, 1, 0, g, hd), 0, s,
+                      seen, g, hd);
+        open = __any(bad && !all_nan<NB, KR>(dk, 0, g, hd));
+      }
+    }
+    const float f = second ? __builtin_amdgcn_exp2f(-kPShift<T>)
+                           : a.scale * (kScaled<T> ? __builtin_amdgcn_exp2f(-e) : 1.f);
+    if (bad && whole) store_accumulators<T, NB, KR>(second ? dvp : dkp, dk, f, g, hd);
+    if (bad && !whole) store_partial<NB, KR>((second ? a.dv_part : a.dk_part) + at_part, dk, f, g, hd);
   }
 }
 

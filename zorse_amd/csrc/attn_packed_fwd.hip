@@ -117,7 +117,8 @@ void packed_fwd_kernel(PackedArgs a) {
   const int hd = KR ? a.d : D;
   __shared__ __attribute__((aligned(16))) T K0[TN * D], K1[TN * D], V0[TN * D], V1[TN * D];
 
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63;
+  int l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const PackedPlan plan(a);
   int block, hq;
@@ -128,8 +129,8 @@ void packed_fwd_kernel(PackedArgs a) {
   const int hk = hq / (a.Hq / a.Hkv);
   const int qw0 = q0 + 32 * (wave % QW);
   const int k_off = kSplit ? wave / QW * BN : 0;  // this wave's keys in a step
-  const int my_q = qw0 + l32;
-  const bool in = my_q < rows;
+  int my_q = qw0 + l32;
+  bool in = my_q < rows;
 
   // the wave's and the block's ranges of keys (scalar: their rows are uniform)
   const int last = rows - 1;
@@ -415,47 +416,98 @@ void packed_fwd_kernel(PackedArgs a) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[nt][j] = o[nt][j] * f1 + *at(nt, j) * f2;
   }
+  relane(l32, g);
+  my_q = qw0 + l32;
+  in = my_q < rows;
   const float l_tot = l_i + other_half(l_i);
   // no weight although keys are visible: every score is -inf or NaN, and so is O
   const float inv = l_tot > 0.f ? 1.0f / l_tot : any_key ? NAN : 0.f;
   const bool put = in && (my_q < plan.n || !a.keep_tail);
   T* Op = static_cast<T*>(a.out) + hq * a.o_h + my_q * a.o_s;
   float* lp = a.lse_out + static_cast<int64_t>(hq) * a.T + my_q;
-  const bool bad = row_has_nan<NB>(o, g, hd);
+  const bool bad = put && row_has_nan<NB, KR>(o, g, hd);
   if (put) {
     store_accumulators<T, NB, KR>(Op, o, inv, g, hd);
     if (g == 0) *lp = l_tot > 0.f ? m_ref * a.scale + logf(l_tot) : any_key ? NAN : -INFINITY;
   }
-  if (__any(bad)) {  // see row_has_nan
-    const T* Qr = Qp + clip(my_q) * a.q_s;
-    auto seen = [&](int j) __attribute__((always_inline)) {
-      return static_cast<unsigned>(j - vis_lo) <= static_cast<unsigned>(vis_span);
-    };
-    float m = -INFINITY, l = 0.f;
-#pragma unroll 1
-    for (int j = w_lo; j <= w_hi; ++j) {
-      const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd) * c2;
-      if (!seen(j)) continue;
-      const float m_new = fmaxf(m, s), ref = m_new == -INFINITY ? 0.f : m_new;
-      l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(s - ref);
-      m = m_new;
+  if (__builtin_expect(!__any(bad), 1)) return;
+
+  // see row_has_nan; the products of one 32-key tile
+  auto raw_scores = [&](f32x16& c, int k0, int past) __attribute__((always_inline)) {
+    const T* row = k0 + l32 < past ? Kp + (k0 + l32) * a.k_s : nullptr;
+    c = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      c = M::mma(operand_step<T, KR>(row, ks, g, hd), qreg[ks], c);
     }
-    const float ref = m == -INFINITY ? 0.f : m, w = l > 0.f ? 1.0f / l : any_key ? NAN : 0.f;
-    if (bad && put && g == 0) *lp = l > 0.f ? m / kLog2e + logf(l) : any_key ? NAN : -INFINITY;
+  };
+  auto seen = [&](int j) __attribute__((always_inline)) {
+    return static_cast<unsigned>(j - vis_lo) <= static_cast<unsigned>(vis_span);
+  };
+  auto by_all = [&](int k0) __attribute__((always_inline)) { return k0 >= f_lo && k0 + 31 <= f_hi; };
+  auto sees_all = [&](int k0) __attribute__((always_inline)) { return seen(k0) && seen(k0 + 31); };
+  // whether every row sees all of a tile or nothing of it
+  auto whole_rows = [&](int k0) __attribute__((always_inline)) {
+    return !__any(!sees_all(k0) && k0 + 31 >= vis_lo && k0 <= vis_lo + vis_span);
+  };
+  bool found = false;
+  {
+    // what the wave met: whole 64-key tiles, of its own range or (kSplit) the block's
+    const int t_lo = !kSplit && w_lo > kv_lo ? kv_lo + ((w_lo - kv_lo) & ~(BN - 1)) : kv_lo;
+    int past = kSplit ? kv_lo + n_t * TN : kv_lo + ((w_hi - kv_lo) & ~(BN - 1)) + BN;
+    past = past < plan.n ? past : plan.n;
 #pragma unroll 1
-    for (int n = 0; n < KS; ++n) {  // both halves alike: they exchange sums
-      const int c = 16 * n + 8 * g;
-      float acc[8] = {};
+    for (int k0 = t_lo; k0 < past && !found; k0 += 32) {
+      if (by_all(k0)) continue;
+      f32x16 c;
+      raw_scores(c, k0, past);
+      bool odd = false;  // a masked score that -inf does not hide
+#pragma unroll
+      for (int j = 0; j < 16; ++j) odd |= !seen(k0 + 8 * (j >> 2) + 4 * g + (j & 3)) && is_odd(c[j]);
+      found = __any(odd) || odd_rows<T, KS, KR>(Vp, a.v_s, k0, past, f_lo, f_hi, g, hd) != 0;
+    }
+  }
+  if (__builtin_expect(!found, 1)) return;
+  const bool l_stands = l_tot == l_tot;
+  // 32 columns of the result at a time: few registers, so that the loops before keep theirs
 #pragma unroll 1
-      for (int j = w_lo; j <= w_hi; ++j) {
-        const float s = dot_two_rows<T>(Qr, Kp + j * a.k_s, g, hd) * c2;
-        if (!seen(j)) continue;
-        const float p = __builtin_amdgcn_exp2f(s - ref);
-        for (int e = 0; e < 8; ++e)
-          if (c + e < hd) acc[e] = fmaf(p, to_f32(Vp[j * a.v_s + c + e]), acc[e]);
+  for (int c0 = 0; c0 < hd; c0 += 32) {
+    float m = -INFINITY, l = 0.f;
+    f32x16 acc[1] = {f32x16{}};
+#pragma unroll 1
+    for (int k0 = w_lo; k0 <= w_hi; k0 += 32) {
+      f32x16 c;
+      raw_scores(c, k0, w_hi + 1);
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        c[j] = seen(k0 + 8 * (j >> 2) + 4 * g + (j & 3)) ? c[j] : -INFINITY;
+        mloc = fmaxf(mloc, c[j]);
       }
-      for (int e = 0; e < 8; ++e)
-        if (bad && put && c + e < hd) Op[c + e] = static_cast<T>(acc[e] * w);
+      const float m_new = fmaxf(m, fmaxf(mloc, other_half(mloc)));
+      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c2);
+      const float mc = m_new == -INFINITY ? 0.f : m_new * c2;
+      m = m_new;
+      l *= alpha;
+      acc[0] *= alpha;
+      V8 w[2];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        c[j] = __builtin_amdgcn_exp2f(fmaf(c[j], c2, -mc));
+        l += c[j];
+        w[j >> 3][j & 7] = static_cast<T>(c[j]);
+      }
+      const bool kept = whole_rows(k0);
+      add_columns<T, 1>(acc, Vp, a.v_s, k0, w_hi + 1, c0, w, kept, sees_all(k0), g, hd);
+      if (!kept)
+        add_odd<T, 1>(acc, Vp, a.v_s, k0, odd_rows<T, KS, KR>(Vp, a.v_s, k0, w_hi + 1, 1, 0, g, hd), c0, c,
+                      seen, g, hd);
+      if (!__any(bad && !(all_nan<1, KR>(acc, c0, g, hd) && (l_stands || l != l)))) break;
+    }
+    l += other_half(l);
+    if (bad) {
+      store_block<T>(Op, acc[0], l > 0.f ? 1.0f / l : any_key ? NAN : 0.f, c0, g, hd);
+      if (c0 == 0 && g == 0 && !l_stands) *lp = l > 0.f ? m * a.scale + logf(l) : any_key ? NAN : -INFINITY;
     }
   }
 }
