@@ -175,3 +175,19 @@ def test_differentiated_twice_and_captured(dev):
         got = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
         torch.cuda.synchronize()
+
+
+def test_more_than_2_24_workgroups(dev):
+    """A token of 129 pairs takes a workgroup of 256 threads, and a launch fewer than
+    2^32 of them along an axis."""
+    from zorse_amd import functional as F, kernels as K
+    T, d = (1 << 24) + 5, 258
+    cos, sin = (t.to(dev) for t in _tables(50, d))
+    axes = F.pair_axes_of((d // 2,))
+    q = torch.empty(T, 1, d, device=dev, dtype=torch.bfloat16).normal_()
+    pos = torch.randint(0, 50, (1, T), device=dev)
+    parts = [slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)]
+    want = [K.rope_axes(q[s].clone(), None, cos, sin, pos[:, s].contiguous(), axes)[0] for s in parts]
+    K.rope_axes(q, None, cos, sin, pos, axes, q_out=q)
+    for s, w in zip(parts, want):
+        assert torch.equal(q[s], w)

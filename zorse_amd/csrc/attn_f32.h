@@ -156,17 +156,6 @@ __device__ __forceinline__ void store_row(float* dst, const f32x4 (&x)[N], float
   }
 }
 
-// A launch holds fewer than 2^32 threads along x: workgroup n of any number is
-// (n % kGridX, n / kGridX), those past the last one leave at once.
-constexpr int64_t kGridX = int64_t(1) << 20;
-__device__ __forceinline__ int64_t group_id() {
-  return static_cast<int64_t>(blockIdx.y) * kGridX + blockIdx.x;
-}
-dim3 group_grid(int64_t n) {
-  if (n <= kGridX) return dim3(static_cast<unsigned>(n));
-  return dim3(static_cast<unsigned>(kGridX), static_cast<unsigned>((n + kGridX - 1) / kGridX));
-}
-
 // float4 accesses: head dim and strides multiples of 4, pointers of 16 bytes
 bool vec4_ok(int64_t d, std::initializer_list<int64_t> strides,
              std::initializer_list<const void*> ptrs) {

@@ -43,7 +43,7 @@ template <typename T, int V, bool kInterleaved>
 __global__ __launch_bounds__(256) void rope_axes_kernel(AxesArgs a, PairAxes axes) {
   typedef T TV __attribute__((ext_vector_type(V)));
   const int slot = threadIdx.x / a.lanes;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * a.per_group + slot;
+  const int64_t token = group_id() * a.per_group + slot;
   if (slot >= a.per_group || token >= a.tokens) return;
   const int r = threadIdx.x - slot * a.lanes;
   const int h0 = r / a.n_chunks, i0 = (r - h0 * a.n_chunks) * V;
@@ -123,7 +123,7 @@ static void launch_rope_axes(AxesArgs& a, const PairAxes& axes, bool interleaved
   if (a.at_once > most) a.at_once = most;
   a.lanes = a.at_once * a.n_chunks;
   a.per_group = 256 / a.lanes;
-  const dim3 grid(static_cast<unsigned>((a.tokens + a.per_group - 1) / a.per_group));
+  const dim3 grid = group_grid((a.tokens + a.per_group - 1) / a.per_group);
   if (interleaved)
     hipLaunchKernelGGL((rope_axes_kernel<T, V, true>), grid, dim3(256), 0, s, a, axes);
   else

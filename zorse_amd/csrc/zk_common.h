@@ -96,6 +96,17 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// A launch holds fewer than 2^32 threads along x: workgroup n of any number is
+// (n % kGridX, n / kGridX), those past the last one leave at once.
+constexpr int64_t kGridX = int64_t(1) << 20;
+__device__ __forceinline__ int64_t group_id() {
+  return static_cast<int64_t>(blockIdx.y) * kGridX + blockIdx.x;
+}
+inline dim3 group_grid(int64_t n) {
+  if (n <= kGridX) return dim3(static_cast<unsigned>(n));
+  return dim3(static_cast<unsigned>(kGridX), static_cast<unsigned>((n + kGridX - 1) / kGridX));
+}
+
 // Number of CUs on the current device (cached per device).
 int device_cus();
 
