@@ -672,7 +672,8 @@ typedef struct zk_muon_matrix {
   int64_t rows, cols, ld_grad, ld_out, ld_param, ld_momentum;
   int64_t grad_dtype, out_dtype;
 } zk_muon_matrix;
-/* Bytes of workspace for a list. */
+/* Bytes of workspace for a list.  Without a workspace a call checks all else and launches
+ * nothing: ZK_EWORKSPACE where nothing else is wrong. */
 int64_t zk_muon_workspace(const zk_muon_matrix* list, int64_t n);
 int zk_orthogonalize(const zk_muon_matrix* list, int64_t n, int steps, double a,
                      double b, double c, double eps, void* workspace,

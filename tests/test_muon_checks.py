@@ -65,3 +65,13 @@ def test_wrappers_refuse():
     with pytest.raises(ValueError, match="adjust"):
         K.muon_multi([x], [x], [x], lr=0.1, momentum=0.9, weight_decay=0.0, adjust="none")
     assert K.orthogonalize([]) == []
+
+
+def test_a_call_without_a_workspace_checks_the_rest():
+    row = _row(param=12288, momentum=16384)
+
+    def call(lr=0.1, mu=0.9, n=1):
+        return _abi.lib().zk_muon_multi(ctypes.byref(row), n, 5, 3.4445, -4.775, 2.0315, 1e-7, lr, mu, 0.0, 1,
+                                        0, None, 0, None)
+
+    assert call() == -5 and call(lr=-1.0) == -1 and call(mu=1.0) == -1 and call(n=0) == 0

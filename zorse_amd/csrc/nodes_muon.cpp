@@ -1,5 +1,7 @@
 // The lists of the orthogonal updates on torch's C++ side: checks, tables and the
 // launches through the C ABI.
+#include <array>
+
 #include "nodes.h"
 
 namespace {
@@ -115,59 +117,84 @@ std::vector<Tensor> orthogonalize(const py::object& matrices, const py::object& 
   return result;
 }
 
-// kernels.muon_multi
-void muon_multi(const py::object& params_, const py::object& grads_, const py::object& momenta_,
-                const py::object& lows_, int steps, double a, double b, double c, double eps, double lr,
-                double momentum, double weight_decay, bool nesterov, bool match_rms) {
-  const std::string who = "muon_multi";
-  const std::vector<MaybeTensor> params = list_of(who, params_), grads = list_of(who, grads_),
-                                 momenta = list_of(who, momenta_);
-  std::vector<MaybeTensor> lows(params.size());
-  if (!lows_.is_none()) lows = list_of(who, lows_);
-  if (grads.size() != params.size() || momenta.size() != params.size() || lows.size() != params.size())
-    bad(who + ": the lists differ in length");
-  std::vector<zk_muon_matrix> table;
-  std::vector<Span> spans;
-  for (size_t i = 0; i < params.size(); ++i) {
-    if (!params[i] || !grads[i] || !momenta[i])
-      bad(who + ": tensor " + std::to_string(i) + " is None");
-    const Tensor& p = *params[i];
-    zk_muon_matrix m{};
-    m.ld_param = matrix(who, "param", i, p, p, 1 << ZK_F32, true, spans);
-    one_device(who, p, *params[0]);
-    m.ld_grad = matrix(who, "grad", i, *grads[i], p, kAnyFloat, false, spans);
-    m.ld_momentum = matrix(who, "momentum", i, *momenta[i], p, 1 << ZK_F32, true, spans);
-    m.param = static_cast<float*>(p.data_ptr());
-    m.grad = grads[i]->data_ptr();
-    m.momentum = static_cast<float*>(momenta[i]->data_ptr());
-    m.rows = p.size(0), m.cols = p.size(1);
-    m.grad_dtype = code_of(grads[i]->scalar_type());
-    if (lows[i]) {
-      m.ld_out = matrix(who, "lowp_out", i, *lows[i], p, kAnyFloat, true, spans);
-      m.out = lows[i]->data_ptr();
-      m.out_dtype = code_of(lows[i]->scalar_type());
+// kernels.muon_step: a step whose arguments are checked and whose workspace is there,
+// so that run() refuses nothing.
+class MuonStep {
+ public:
+  MuonStep(const py::object& params_, const py::object& grads_, const py::object& momenta_, const py::object& lows_,
+           int steps, double a, double b, double c, double eps, double lr, double momentum, double weight_decay,
+           bool nesterov, bool match_rms)
+      : steps_(steps), nesterov_(nesterov), adjust_(match_rms ? ZK_MUON_MATCH_RMS : ZK_MUON_ORIGINAL),
+        hyper_{a, b, c, eps, lr, momentum, weight_decay} {
+    const std::string who = "muon_multi";
+    std::vector<MaybeTensor> params = list_of(who, params_), grads = list_of(who, grads_),
+                             momenta = list_of(who, momenta_), lows(params.size());
+    if (!lows_.is_none()) lows = list_of(who, lows_);
+    if (grads.size() != params.size() || momenta.size() != params.size() || lows.size() != params.size())
+      bad(who + ": the lists differ in length");
+    std::vector<Span> spans;
+    for (size_t i = 0; i < params.size(); ++i) {
+      if (!params[i] || !grads[i] || !momenta[i]) bad(who + ": tensor " + std::to_string(i) + " is None");
+      const Tensor& p = *params[i];
+      zk_muon_matrix m{};
+      m.ld_param = matrix(who, "param", i, p, p, 1 << ZK_F32, true, spans);
+      one_device(who, p, *params[0]);
+      m.ld_grad = matrix(who, "grad", i, *grads[i], p, kAnyFloat, false, spans);
+      m.ld_momentum = matrix(who, "momentum", i, *momenta[i], p, 1 << ZK_F32, true, spans);
+      m.param = static_cast<float*>(p.data_ptr());
+      m.grad = grads[i]->data_ptr();
+      m.momentum = static_cast<float*>(momenta[i]->data_ptr());
+      m.rows = p.size(0), m.cols = p.size(1);
+      m.grad_dtype = code_of(grads[i]->scalar_type());
+      if (lows[i]) {
+        m.ld_out = matrix(who, "lowp_out", i, *lows[i], p, kAnyFloat, true, spans);
+        m.out = lows[i]->data_ptr();
+        m.out_dtype = code_of(lows[i]->scalar_type());
+      }
+      if (p.numel() > 0) table_.push_back(m);
     }
-    if (p.numel() > 0) table.push_back(m);
+    no_overlaps(who, spans);
+    for (std::vector<MaybeTensor>* list : {&params, &grads, &momenta, &lows})
+      for (const MaybeTensor& t : *list)
+        if (t) kept_.push_back(*t);
+    const py::gil_scoped_release free_gil;
+    std::optional<c10::DeviceGuard> on;
+    if (!table_.empty()) on.emplace(kept_[0].device());
+    const int status = call(nullptr, 0, nullptr);  // with no workspace: all other checks
+    if (status != ZK_EWORKSPACE) check(status, "zk_muon_multi");
+    if (table_.empty()) return;
+    bytes_ = zk_muon_workspace(table_.data(), static_cast<int64_t>(table_.size()));
+    ws_ = workspace(bytes_, kept_[0]);
   }
-  no_overlaps(who, spans);
-  const int64_t n = static_cast<int64_t>(table.size()), bytes = zk_muon_workspace(table.data(), n);
-  const py::gil_scoped_release free_gil;
-  std::optional<c10::DeviceGuard> on;
-  Tensor ws;
-  zk_stream_t stream = nullptr;
-  if (n > 0) {
-    on.emplace(params[0]->device());
-    ws = workspace(bytes, *params[0]);
-    stream = stream_of(*params[0]);
+
+  void run() {
+    if (table_.empty()) return;
+    const py::gil_scoped_release free_gil;
+    const c10::DeviceGuard on(ws_.device());
+    check(call(ws_.data_ptr(), bytes_, stream_of(ws_)), "zk_muon_multi");
   }
-  check(zk_muon_multi(table.data(), n, steps, a, b, c, eps, lr, momentum, weight_decay, nesterov,
-                      match_rms ? ZK_MUON_MATCH_RMS : ZK_MUON_ORIGINAL, address(ws), bytes, stream),
-        "zk_muon_multi");
-}
+
+ private:
+  int call(void* ws, int64_t bytes, zk_stream_t stream) const {
+    const auto& [a, b, c, eps, lr, momentum, weight_decay] = hyper_;
+    return zk_muon_multi(table_.data(), static_cast<int64_t>(table_.size()), steps_, a, b, c, eps, lr, momentum,
+                         weight_decay, nesterov_, adjust_, ws, bytes, stream);
+  }
+
+  int steps_, nesterov_, adjust_;
+  std::array<double, 7> hyper_;
+  std::vector<zk_muon_matrix> table_;
+  std::vector<Tensor> kept_;
+  Tensor ws_;
+  int64_t bytes_ = 0;
+};
 
 }  // namespace
 
 void bind_muon(py::module_& m) {
   m.def("orthogonalize", &orthogonalize);
-  m.def("muon_multi", &muon_multi);
+  py::class_<MuonStep>(m, "MuonStep")
+      .def(py::init<const py::object&, const py::object&, const py::object&, const py::object&, int, double, double,
+                    double, double, double, double, double, bool, bool>())
+      .def("run", &MuonStep::run);
 }

@@ -996,11 +996,21 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=MUON_COEFFICIENTS, e
     return _abi.nodes().orthogonalize(matrices, outs, dtype, steps, *coefficients, eps)
 
 
-def muon_multi(params, grads, momenta, *, lr: float, momentum: float, weight_decay: float,
-               nesterov: bool = True, adjust: str = "original", steps: int = 5,
-               coefficients=MUON_COEFFICIENTS, eps: float = 1e-7, lowp_outs=None) -> None:
+def muon_step(params, grads, momenta, *, lr: float, momentum: float, weight_decay: float,
+              nesterov: bool = True, adjust: str = "original", steps: int = 5,
+              coefficients=MUON_COEFFICIENTS, eps: float = 1e-7, lowp_outs=None):
+    """muon_multi's step after its checks, nothing launched yet: ``run()``, once and on
+    the same stream, does it and refuses nothing (for a caller that steps other tensors
+    with it)."""
+    if adjust not in ("original", "match_rms_adamw"):
+        raise ValueError(f"muon_multi: adjust is 'original' or 'match_rms_adamw' (got {adjust!r})")
+    return _abi.nodes().MuonStep(params, grads, momenta, lowp_outs, steps, *coefficients, eps, lr, momentum,
+                                 weight_decay, nesterov, adjust == "match_rms_adamw")
+
+
+def muon_multi(params, grads, momenta, **options) -> None:
     """One step of a list of matrices by the orthogonal factors of their momenta
-    (zk_muon_multi), in place:
+    (zk_muon_multi; the options are muon_step's), in place:
         m = momentum m + (1 - momentum) g
         u = (1 - momentum) g + momentum m if nesterov else m
         p = p (1 - lr weight_decay) - lr f orthogonalize(u)
@@ -1009,10 +1019,7 @@ def muon_multi(params, grads, momenta, *, lr: float, momentum: float, weight_dec
     parameters; 2-D tensors with unit column stride.  f: "original",
     sqrt(max(1, rows / cols)), or "match_rms_adamw", 0.2 sqrt(max(rows, cols)).
     What is written may not overlap anything else in the lists."""
-    if adjust not in ("original", "match_rms_adamw"):
-        raise ValueError(f"muon_multi: adjust is 'original' or 'match_rms_adamw' (got {adjust!r})")
-    _abi.nodes().muon_multi(params, grads, momenta, lowp_outs, steps, *coefficients, eps, lr, momentum,
-                            weight_decay, nesterov, adjust == "match_rms_adamw")
+    muon_step(params, grads, momenta, **options).run()
 
 
 def cast_(src: torch.Tensor, dst: torch.Tensor, accumulate: bool = False) -> torch.Tensor:

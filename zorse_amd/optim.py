@@ -385,16 +385,20 @@ class Muon(FusedAdamW):
                 rest[4].append(None if low is None else low[a:a + n])
                 steps.append(st["step"] + 1)
                 at += n
+        # a refused list has not been stepped: both are checked before either is
+        muon = None
         if mats[0]:
-            K.muon_multi(*mats[:3], lowp_outs=mats[3], lr=group["lr"], momentum=group["momentum"],
-                         weight_decay=group["weight_decay"], nesterov=group["nesterov"],
-                         adjust=group["adjust"], steps=group["ns_steps"],
-                         coefficients=group["ns_coefficients"], eps=group["eps"])
+            muon = K.muon_step(*mats[:3], lowp_outs=mats[3], lr=group["lr"], momentum=group["momentum"],
+                               weight_decay=group["weight_decay"], nesterov=group["nesterov"],
+                               adjust=group["adjust"], steps=group["ns_steps"],
+                               coefficients=group["ns_coefficients"], eps=group["eps"])
         if rest[0]:
             lr = group["lr"] if group["adam_lr"] is None else group["adam_lr"]
             b1, b2 = group["adam_betas"]
             K.adamw_multi(*rest[:4], steps, lowp_outs=rest[4], lr=lr, beta1=b1, beta2=b2,
                           eps=group["adam_eps"], weight_decay=group["weight_decay"])
+        if muon is not None:
+            muon.run()
         for st in states:
             st["step"] = st["step"] + 1
         for p in params:
