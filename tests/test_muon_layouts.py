@@ -87,3 +87,19 @@ def test_cpu_parameters_are_refused():
     with pytest.raises(ValueError, match="GPU tensors"):
         opt.step()
     assert opt.state[p]["step"] == 0
+
+
+@pytest.mark.parametrize("name,more", [("momentum_buffer", 3), ("momentum_buffer", -1), ("exp_avg", 4),
+                                       ("exp_avg_sq", -2), ("master", 8)])
+def test_a_state_of_another_size_is_refused(name, more):
+    layer = _layer(torch.bfloat16)
+    p = layer.flat_param
+    opt = optim.Muon([p], matrices=optim.flat_matrices(layer))
+    opt._init_state(p)
+    saved = copy.deepcopy(opt.state_dict())
+    saved["state"][0][name] = torch.ones(saved["state"][0][name].numel() + more)
+    opt.load_state_dict(saved)
+    p.grad = torch.zeros_like(p)
+    with pytest.raises(ValueError, match=name):
+        opt.step()
+    assert opt.state[p]["step"] == 0

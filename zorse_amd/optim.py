@@ -349,6 +349,16 @@ class Muon(FusedAdamW):
                     st[k] = t.to(p.device)
         return st
 
+    @staticmethod
+    def _check_sizes(where: list, p: torch.Tensor, st: dict) -> None:
+        """A loaded state may be of other matrices or another parameter."""
+        n = sum(r * c for _, r, c in where)
+        for name, want in (("momentum_buffer", n), ("exp_avg", p.numel() - n), ("exp_avg_sq", p.numel() - n)):
+            if (st[name].numel() if name in st else 0) != want:
+                raise ValueError(f"Muon: a state's {name} does not have its parameter's {want} elements")
+        if "master" in st and st["master"].numel() != p.numel():
+            raise ValueError(f"Muon: a state's master does not have its parameter's {p.numel()} elements")
+
     def _step_one(self, group: dict, p: torch.Tensor) -> None:
         self._step_list(group, [p])
 
@@ -368,6 +378,7 @@ class Muon(FusedAdamW):
             if master is not None:
                 flat, low = master, flat
             where, others = self._layout(group, p)
+            self._check_sizes(where, p, st)
             at = 0
             for a, r, c in where:
                 cut = slice(a, a + r * c)
