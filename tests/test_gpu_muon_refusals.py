@@ -78,3 +78,30 @@ def test_a_step_checked_before_it_runs(dev):
     K.muon_step([], [], [], **kw).run()
     with pytest.raises(RuntimeError, match="ZK_EINVAL"):
         K.muon_step([p], [g], [m], lr=-1.0, momentum=0.9, weight_decay=0.0)
+
+
+def test_columns_of_one_buffer(dev):
+    """Matrices beside each other share no element, though their spans meet."""
+    from zorse_amd import kernels as K
+    cuts = (0, 30, 70, 71, 100)
+
+    def columns(seed):
+        buf = torch.randn(50, 100, device=dev, generator=torch.Generator(dev).manual_seed(seed))
+        return buf, [buf[:, a:b] for a, b in zip(cuts, cuts[1:])]
+
+    kw = dict(lr=0.1, momentum=0.9, weight_decay=0.1)
+    (pb, ps), (gb, gs), (mb, ms) = (columns(i) for i in range(3))
+    twins = [[t.clone() for t in ts] for ts in (ps, gs, ms)]
+    K.muon_multi(ps, gs, ms, **kw)
+    K.muon_multi(*twins, **kw)
+    for a, b in zip((*ps, *ms), (*twins[0], *twins[2])):
+        assert torch.equal(a, b)
+    # parameter, gradient and momentum in one buffer, and a single row between others
+    buf = torch.randn(50, 100, device=dev)
+    K.muon_multi([buf[:, :30]], [buf[:, 30:60]], [buf[:, 60:90]], **kw)
+    K.orthogonalize([buf[:, :30], buf[3:4, 90:95]], outs=[buf[:, 30:60], buf[9:10, 60:65]])
+    for bad in ([buf[:, :30], buf[:, 29:50]], [buf[:, 20:40], buf[1:, 10:21]], [buf[:, :30], buf[7:8, 25:35]],
+                [buf[:, 80:], buf[:20, :30].as_strided((20, 30), (101, 1), 85)]):
+        grads = [torch.zeros_like(t) for t in bad]
+        with pytest.raises(ValueError, match="overlaps"):
+            K.muon_multi(bad, grads, [torch.zeros_like(t) for t in bad], **kw)

@@ -19,8 +19,8 @@ std::vector<MaybeTensor> list_of(const std::string& who, const py::object& o) {
   return out;
 }
 
-struct Span {
-  uintptr_t begin, end;
+struct Span {  // of a matrix: bytes, and those of a row and between rows
+  uintptr_t begin, end, width, pitch;
   bool written;
 };
 
@@ -40,18 +40,31 @@ int64_t matrix(const std::string& who, const char* name, size_t i, const Tensor&
     bad(at + " needs unit column stride and rows that do not overlap");
   if (rows > 0 && cols > 0) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-    spans.push_back({p, p + ((rows - 1) * ld + cols) * t.element_size(), written});
+    const uintptr_t e = t.element_size();
+    spans.push_back({p, p + ((rows - 1) * ld + cols) * e, cols * e, rows > 1 ? ld * e : 0, written});
   }
   return ld;
 }
 
+// Whether matrices whose spans meet, b's beginning in a's, share bytes: columns of one
+// buffer, rows equally far apart, lie beside each other.
+bool share(const Span& a, const Span& b) {
+  const uintptr_t pitch = a.pitch ? a.pitch : b.pitch;
+  if (pitch == 0 || (a.pitch && b.pitch && a.pitch != b.pitch)) return true;
+  const uintptr_t at = (b.begin - a.begin) % pitch;
+  return at < a.width || at + b.width > pitch;
+}
+
 void no_overlaps(const std::string& who, std::vector<Span>& spans) {
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
-  uintptr_t read = 0, written = 0;  // the ends so far
+  std::vector<Span> open;  // that end behind the current one's beginning
   for (const Span& s : spans) {
-    if (s.begin < written || (s.written && s.begin < read))
-      bad(who + ": a tensor that is written is in the lists twice, or overlaps another");
-    (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span& o) { return o.end <= s.begin; }),
+               open.end());
+    for (const Span& o : open)
+      if ((s.written || o.written) && share(o, s))
+        bad(who + ": a tensor that is written is in the lists twice, or overlaps another");
+    open.push_back(s);
   }
 }
 
