@@ -4,9 +4,10 @@
 //   Bound by the matrix instructions: seven products where five are needed, because
 // each kernel forms S and dP for itself (one kernel for all three would add dQ in
 // fp32 with atomics, in no fixed order).  32 causal heads of 128, 8 key heads, 8192
-// tokens: dQ 750 us (3 products, 1100 TFLOP/s), dK / dV 1040 (4, 1057), their sums
-// 29; documents of 30 to 2500 of 4096 tokens, 32 heads: 74 and 100, where the blocks
-// of the longest document end last.  P and dS are rounded to the storage type as
+// tokens: dQ 755 us (3 products, 1090 TFLOP/s), dK / dV 1045 (4, 1052), their sums
+// 29; documents of 30 to 1209 of 4096 tokens, 32 heads: 74 and 97, where a quarter of the
+// tiles' area is masked, blocks of few tiles wait for their first loads, and those of the
+// longest document end last (matrix units busy 27 % of the time).  P and dS are rounded to the storage type as
 // operands of the products that follow, with fp32 sums; in fp16 scaled first (kScaled).
 #include <type_traits>
 

@@ -4,9 +4,11 @@
 //  * Whole: 64 rows a workgroup, 4 waves, each meets whole tiles of 32 rows.
 //  * Split: 32 rows, 8 waves; the four waves of 16 rows take 16 rows each of tiles of
 //    64, and their partial sums are joined through LDS at the end.
-//   Bound by the matrix instructions (a 16 x 16 x 4 product takes its SIMD 32 cycles),
-// and where a launch has few workgroups by those of the one with the most tiles, of
-// which Split does a quarter at a time.  So Split up to two of Whole's workgroups a CU
+//   Bound by the matrix instructions (a 16 x 16 x 4 product takes its SIMD 32 cycles)
+// in launches that fill the chip; where a launch has few workgroups, by the chain of each
+// tile (loads, LDS, two barriers, products, exponentials) in the one with the most tiles,
+// of which Split does a quarter at a time (1111 tokens in texts of up to 385, 8 heads of
+// 64: the matrix units are busy 8 - 13 % of the time).  So Split up to two of Whole's workgroups a CU
 // (head dim 64, causal, forward and backward in us, Whole against Split: 1024 tokens,
 // 8 heads 78 + 357 against 42 + 153 (one sum a key head); 2048, 16 heads 180 + 526 against 135 + 414, but in
 // sequences of 200 31 + 86 against 31 + 104), Whole past it (4096 tokens, 16 heads of
