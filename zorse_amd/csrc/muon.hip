@@ -349,15 +349,27 @@ void plan_run(const zk_muon_matrix* list, int n, Sides* d) {
 bool scales_of(int steps, double a, double b, double c, float* Sx, float* S, float* R) {
   if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c))) return false;
   double most = 1.0, most_p = 0, most_l = 1.0;
+  // where a z + b z^3 + c z^5 and b l + c l^2, l = z^2, may be largest: at the range's end
+  // and where their derivatives are zero
+  double roots[3] = {c != 0 ? -b / (2 * c) : -1};
+  if (c != 0) {
+    const double half = 0.3 * b / c, q = half * half - 0.2 * a / c;
+    if (q >= 0) roots[1] = -half + sqrt(q), roots[2] = -half - sqrt(q);
+  } else if (b != 0) {
+    roots[1] = -a / (3 * b);
+  }
   for (int k = 0; k < steps; ++k) {
     double next = 0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double z = most * i / 4096, l = z * z, p = b * l + c * l * l;
-      next = fmax(next, fabs(z * (a + p)));
+    const auto at = [&](double l) {
+      if (!(l > 0 && l <= most * most)) return;
+      const double p = b * l + c * l * l;
+      next = fmax(next, fabs(sqrt(l) * (a + p)));
       most_p = fmax(most_p, fabs(p));
-    }
+    };
+    at(most * most);
+    for (const double l : roots) at(l);
     if (!(next < 16.0)) return false;
-    most = next * 1.02;  // between the samples, and roundings
+    most = next * 1.02;  // roundings
     most_l = fmax(most_l, most * most);
   }
   // Sx = 2^h, Sx^2 most_l < 2^31; S = 2^i, S^2 most_l < 2^15.5; R = 2^j
