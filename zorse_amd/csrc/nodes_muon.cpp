@@ -116,13 +116,15 @@ std::vector<Tensor> orthogonalize(const py::object& matrices, const py::object& 
     if (x.numel() > 0) table.push_back(m);
   }
   no_overlaps(who, spans);
-  const int64_t n = static_cast<int64_t>(table.size()), bytes = zk_muon_workspace(table.data(), n);
+  const int64_t n = static_cast<int64_t>(table.size());
   const py::gil_scoped_release free_gil;
   std::optional<c10::DeviceGuard> on;
   Tensor ws;
   zk_stream_t stream = nullptr;
+  int64_t bytes = 0;
   if (n > 0) {
     on.emplace(result[0].device());
+    bytes = zk_muon_workspace(table.data(), n);  // it goes by the device's CUs
     ws = workspace(bytes, result[0]);
     stream = stream_of(result[0]);
   }
