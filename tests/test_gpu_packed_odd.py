@@ -75,6 +75,41 @@ def test_large_finite_values_of_others(dev, d, H):
     _near(got, want, "neighbours", torch.tensor([*range(70), *range(150, 200)]))
 
 
+@pytest.mark.parametrize("dt,H,d", [(BF, 4, 128), (FP, 34, 64), (FP, 4, 72), (BF, 34, 100), (F4, 4, 64)])
+@pytest.mark.parametrize("causal,window", [(True, 50), (True, 200), (False, 0)])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_odd_rows_outside_a_window_and_of_whole_sequences(dev, dt, H, d, causal, window, value):
+    """Odd tokens at both ends of a long sequence, those of a neighbour among its
+    blocks, and single ones: rows that see none of them are as without them."""
+    T, offsets = 420, [0, 301, 310, 400]
+    q, k, v, do = _inputs(T, H, H // 2, d, dt, 24)
+    want, _ = _reference(q, k, v, do, offsets, causal, window, 1 / math.sqrt(d), dt)
+    odd = [*range(3), 299, 300, *range(301, 310), *range(400, T)]
+    if not causal:  # a whole sequence sees its own
+        odd = [*range(301, 310), *range(400, T)]
+    for t in (q, k, v, do):
+        t[odd] = value
+    got = _run(dev, q, k, v, do, offsets, causal, window)
+    sees = [i for i in range(400) if not any(
+        (a <= j < b and a <= i < b) and (not causal or (j <= i and (not window or i - j < window)))
+        for j in odd for a, b in zip(offsets, offsets[1:]))]
+    seen = [j for j in range(400) if not any(
+        (a <= j < b and a <= i < b) and (not causal or (j <= i and (not window or i - j < window)))
+        for i in odd for a, b in zip(offsets, offsets[1:]))]
+    rows = torch.tensor(sees)
+    _near(got[:2], want[:2], "rows", rows)
+    # a key's gradients take the rows that see it: of those that see an odd token too, its
+    # own dv has their P, which is not a number, so keys beside no odd row or key
+    clean = [j for j in seen if all(i in set(sees) for i in range(400) if any(
+        a <= j < b and a <= i < b for a, b in zip(offsets, offsets[1:])) and
+        (not causal or (j <= i and (not window or i - j < window))))]
+    assert len(sees) > 80 and len(clean) > 40
+    for n in (2, 3):
+        _near(got[n:n + 1], want[n:n + 1], "keys", torch.tensor(clean))
+    for x in got:
+        assert not bool(x[400:].any())
+
+
 def _time(fn):
     fn()
     best = math.inf
